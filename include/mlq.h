@@ -412,6 +412,134 @@ MLQ_API mlq_status mlq_peer_close(void* ptr);
 MLQ_API mlq_status mlq_peer_free(void* ptr);
 
 /* ---------------------------------------------------------------------------
+ * Mixture-of-experts layers and the linear with an epilogue
+ *
+ * The feed-forward block of a mixture-of-experts model over the same packed
+ * blocks: a router, the chosen experts' SwiGLU products, and (for a shared
+ * expert or any other product) a linear whose store applies bias,
+ * activation, a scale per row and the residual.  No counterpart in the
+ * reference, whose feed-forward is dense (src/forward.cc:573-581).
+ *
+ * Workspace: these calls keep nothing between calls and allocate nothing.
+ * The caller passes a device buffer of at least the bytes the matching
+ * *_workspace_bytes function returns, 256-byte aligned; its contents need
+ * not be initialised and mean nothing afterwards.  One call at a time may use a
+ * workspace: calls ordered on one stream may share it, calls (or captured
+ * graphs) that may run at the same time need one each.
+ *
+ * x, y, ids, weights and residual are dense row-major device arrays with
+ * the alignment of their type.  y may be residual itself.  y may be x itself
+ * when both have the same width.  Weights may start at any address and have any
+ * row pitch; 16-byte aligned matrices whose row pitch is a multiple of 16
+ * bytes stream fastest.
+ *
+ * All launches use programmatic dependent launch (see the top of this
+ * file): they read x, ids, weights, bias, row_scale and residual and write y only
+ * after the previous kernel on the stream has completed, and may stream
+ * the quantized weights before.  They can be captured into a graph.
+ *
+ * Arithmetic: weights are exact; each row of x (and of an expert's hidden
+ * vector) is carried as 24-bit fixed point against a power of two per
+ * 32-value block; sums are exact integers per block and fp32 across blocks.
+ * Outputs are within ~1e-6 relative L2 of the 64-bit result.  A value of x
+ * that is not finite makes every output that reads it NaN.  Results do not
+ * depend on the other rows of the call or on their order beyond rounding,
+ * and a call repeated gives the same bits.
+ * ------------------------------------------------------------------------- */
+#define MLQ_MOE_MAX_EXPERTS 1024
+#define MLQ_MOE_MAX_TOP_K 64
+
+typedef enum mlq_scoring {
+    MLQ_SCORE_SOFTMAX = 0, /* s = softmax of the row's logits over all experts */
+    MLQ_SCORE_SIGMOID = 1  /* s = 1 / (1 + exp(-logit)) */
+} mlq_scoring;
+
+typedef struct mlq_router {
+    const float* w;     /* device [n_experts][in_features] fp32 (GGUF ffn_gate_inp) */
+    const float* bias;  /* device [n_experts] added to the scores for the choice only, or NULL */
+    int n_experts, in_features, top_k;
+    int scoring;        /* mlq_scoring */
+    int renormalize;    /* 1: divide the chosen scores by their sum */
+    float scale;        /* multiplies the weights */
+} mlq_router;
+
+/* ids[r][0..top_k) = the experts with the largest s (+ bias), descending,
+ * equal ones by the lowest index; weights[r][j] = s of expert ids[r][j] (without
+ * the bias; renormalized, times scale).  An expert whose choice score is
+ * -inf is never chosen (a bias of -inf masks an expert): a slot left without
+ * one gets id -1 and weight 0.  A NaN score counts as the greatest.  Chosen
+ * scores that sum to 0 give weights of 0.  Logits and scores are computed in
+ * 64 bits, so the choice is that of exact arithmetic unless two scores agree
+ * to ~1e-15.  logits: [rows][n_experts] fp32, or NULL. */
+MLQ_API mlq_status mlq_moe_route(const mlq_router* router, const float* x, int rows, int32_t* ids,
+                                 float* weights, float* logits, void* workspace,
+                                 size_t workspace_bytes, mlq_stream stream);
+MLQ_API size_t mlq_moe_route_workspace_bytes(const mlq_router* router, int rows);
+
+/* Stacked experts, as GGUF stores them (ffn_gate_exps, ffn_up_exps,
+ * ffn_down_exps: dims {in, out, n_experts}), so mlq_gguf_upload_rows brings
+ * each stack (or the experts [e0, e1): rows [e0 * out, e1 * out)) to the
+ * device as it is. */
+typedef struct mlq_experts {
+    int fmt;                 /* mlq_format of w_gate and w_up */
+    int fmt_down;            /* mlq_format of w_down */
+    int n_experts;
+    int in_features, hidden, out_features;
+    const void* w_gate;      /* [n_experts][hidden][ceil(in/32)] blocks */
+    const void* w_up;        /* as w_gate */
+    const void* w_down;      /* [n_experts][out_features][ceil(hidden/32)] blocks */
+    size_t block_count;      /* of w_gate, and of w_up */
+    size_t block_count_down; /* of w_down */
+} mlq_experts;
+
+/* y[r] = residual[r] + sum_j weights[r][j] E_ids[r][j](x[r]),
+ * E_e(x) = (silu(x Wg_e^T) * (x Wu_e^T)) Wd_e^T.  ids and weights:
+ * [rows][top_k].  A slot whose id is outside [0, n_experts) adds nothing (-1:
+ * a padded row, or an expert that another GPU holds); a row of only such slots
+ * gives y = residual (0 without one).  The same expert may appear in several
+ * slots.  Up to 32 rows every chosen expert's weights are read once. */
+MLQ_API mlq_status mlq_moe_experts(const mlq_experts* experts, const float* x, int rows, int top_k,
+                                   const int32_t* ids, const float* weights, const float* residual,
+                                   float* y, void* workspace, size_t workspace_bytes,
+                                   mlq_stream stream);
+MLQ_API size_t mlq_moe_experts_workspace_bytes(const mlq_experts* experts, int rows, int top_k);
+
+/* mlq_moe_route, then mlq_moe_experts with its choice: the whole layer.
+ * router->in_features and n_experts are those of experts.  ids and weights
+ * ([rows][router->top_k]) receive the choice. */
+MLQ_API mlq_status mlq_moe_layer(const mlq_router* router, const mlq_experts* experts, const float* x,
+                                 int rows, const float* residual, float* y, int32_t* ids,
+                                 float* weights, void* workspace, size_t workspace_bytes,
+                                 mlq_stream stream);
+MLQ_API size_t mlq_moe_layer_workspace_bytes(const mlq_router* router, const mlq_experts* experts, int rows);
+
+typedef enum mlq_activation {
+    MLQ_ACT_NONE = 0,
+    MLQ_ACT_SILU = 1,      /* v / (1 + exp(-v)) */
+    MLQ_ACT_GELU = 2,      /* v Phi(v) */
+    MLQ_ACT_GELU_TANH = 3, /* 0.5 v (1 + tanh(sqrt(2/pi) (v + 0.044715 v^3))) */
+    MLQ_ACT_RELU = 4,
+    MLQ_ACT_SIGMOID = 5    /* 1 / (1 + exp(-v)) */
+} mlq_activation;
+
+/* What a linear's store does, in this order; NULL leaves a step out. */
+typedef struct mlq_epilogue {
+    const float* bias;      /* device [out_features], added to the product */
+    int activation;         /* mlq_activation */
+    const float* row_scale; /* device [rows], multiplies the activated row (a gate per token) */
+    const float* residual;  /* device [rows][out_features], added last */
+} mlq_epilogue;
+
+/* y[r][o] = residual[r][o] + row_scale[r] * act((x W^T)[r][o] + bias[o]).
+ * Arguments and checks of mlq_linear; any number of rows. */
+MLQ_API mlq_status mlq_linear_epilogue(mlq_format fmt, const void* w, size_t block_count,
+                                       int out_features, int in_features, const float* x, int rows,
+                                       const mlq_epilogue* epilogue, float* y, void* workspace,
+                                       size_t workspace_bytes, mlq_stream stream);
+MLQ_API size_t mlq_linear_epilogue_workspace_bytes(mlq_format fmt, int out_features, int in_features,
+                                                   int rows);
+
+/* ---------------------------------------------------------------------------
  * GGUF ingestion: quantized blocks from a GGUF (v3) file straight to device
  * memory.  Replaces GgufReader::load (src/gguf.cc:396-575),
  * readGgufTensorRaw (src/gguf.cc:614-662) and loadQuantizedTensor

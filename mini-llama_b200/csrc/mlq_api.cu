@@ -692,6 +692,17 @@ mlq_status run_ops(const mlq_linear_op* ops, int n, const float* const* xs, floa
 
 }  // namespace
 
+mlq_status mlq::current_device_facts(DeviceFacts* f) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return fail_cuda("cudaGetDevice", e);
+    mlq_status st = MLQ_OK;
+    DeviceState* ds = device_state(dev, &st);
+    if (!ds) return st;
+    *f = DeviceFacts{ds->sm_count, ds->smem_per_sm, ds->err_flag};
+    return MLQ_OK;
+}
+
 void mlq::set_last_error(const char* msg) { t_last_error = msg ? msg : ""; }
 
 extern "C" {

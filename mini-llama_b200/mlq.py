@@ -523,3 +523,286 @@ def quantize_model(ops, stream=None) -> None:
     """mlq_quantize_model over a list of QuantizeOp."""
     arr = (QuantizeOp * max(1, len(ops)))(*ops)
     check(_convert_lib().mlq_quantize_model(arr, len(ops), _stream_handle(stream)))
+
+
+# ---------------------------------------------------------------------------
+# mixture-of-experts layers and the linear with an epilogue (mlq_moe_*,
+# mlq_linear_epilogue)
+# ---------------------------------------------------------------------------
+SCORINGS = {"softmax": 0, "sigmoid": 1}
+ACTIVATIONS = {None: 0, "none": 0, "silu": 1, "gelu": 2, "gelu_tanh": 3, "relu": 4, "sigmoid": 5}
+MOE_MAX_EXPERTS = 1024
+MOE_MAX_TOP_K = 64
+
+
+class RouterStruct(ctypes.Structure):
+    """struct mlq_router (include/mlq.h)."""
+    _fields_ = [("w", ctypes.c_void_p), ("bias", ctypes.c_void_p), ("n_experts", ctypes.c_int),
+                ("in_features", ctypes.c_int), ("top_k", ctypes.c_int), ("scoring", ctypes.c_int),
+                ("renormalize", ctypes.c_int), ("scale", ctypes.c_float)]
+
+
+class ExpertsStruct(ctypes.Structure):
+    """struct mlq_experts (include/mlq.h)."""
+    _fields_ = [("fmt", ctypes.c_int), ("fmt_down", ctypes.c_int), ("n_experts", ctypes.c_int),
+                ("in_features", ctypes.c_int), ("hidden", ctypes.c_int), ("out_features", ctypes.c_int),
+                ("w_gate", ctypes.c_void_p), ("w_up", ctypes.c_void_p), ("w_down", ctypes.c_void_p),
+                ("block_count", ctypes.c_size_t), ("block_count_down", ctypes.c_size_t)]
+
+
+class EpilogueStruct(ctypes.Structure):
+    """struct mlq_epilogue (include/mlq.h)."""
+    _fields_ = [("bias", ctypes.c_void_p), ("activation", ctypes.c_int), ("row_scale", ctypes.c_void_p),
+                ("residual", ctypes.c_void_p)]
+
+
+def _moe_lib():
+    L = lib()
+    if not getattr(L, "_moe_ready", False):
+        rp, ep, pp = ctypes.POINTER(RouterStruct), ctypes.POINTER(ExpertsStruct), ctypes.POINTER(EpilogueStruct)
+        L.mlq_moe_route.argtypes = [rp, _vp, _i, _vp, _vp, _vp, _vp, _sz, _vp]
+        L.mlq_moe_route_workspace_bytes.argtypes = [rp, _i]
+        L.mlq_moe_experts.argtypes = [ep, _vp, _i, _i, _vp, _vp, _vp, _vp, _vp, _sz, _vp]
+        L.mlq_moe_experts_workspace_bytes.argtypes = [ep, _i, _i]
+        L.mlq_moe_layer.argtypes = [rp, ep, _vp, _i, _vp, _vp, _vp, _vp, _vp, _sz, _vp]
+        L.mlq_moe_layer_workspace_bytes.argtypes = [rp, ep, _i]
+        L.mlq_linear_epilogue.argtypes = [_i, _vp, _sz, _i, _i, _vp, _i, pp, _vp, _vp, _sz, _vp]
+        L.mlq_linear_epilogue_workspace_bytes.argtypes = [_i, _i, _i, _i]
+        for name in ("mlq_moe_route", "mlq_moe_experts", "mlq_moe_layer", "mlq_linear_epilogue"):
+            getattr(L, name).restype = _i
+            getattr(L, name + "_workspace_bytes").restype = _sz
+        L._moe_ready = True
+    return L
+
+
+def _need(t, dtype, shape, device, what: str):
+    """The address of a dense tensor of this dtype, shape and device (None
+    for None); ValueError otherwise: the C ABI takes bare pointers."""
+    if t is None:
+        return None
+    if t.dtype != dtype or tuple(t.shape) != tuple(shape) or t.device != device or not t.is_contiguous():
+        raise ValueError(f"{what}: expected a contiguous {dtype} tensor of shape {tuple(shape)} on {device}, got "
+                         f"{t.dtype} {tuple(t.shape)} on {t.device} with strides {t.stride()}")
+    return t.data_ptr()
+
+
+def _rows_of(x, in_features: int):
+    if x.dim() not in (1, 2) or x.shape[-1] != in_features:
+        raise ValueError(f"x: expected [rows, {in_features}] or [{in_features}], got {tuple(x.shape)}")
+    return 1 if x.dim() == 1 else x.shape[0]
+
+
+def _blocks_need(w, fmt, rows: int, cols: int, device, what: str) -> int:
+    """Address of packed blocks [rows][ceil(cols / 32)] (uint8, any shape)."""
+    import torch
+    name = _fmt_name(fmt)
+    if w is None or w.dtype != torch.uint8 or not w.is_contiguous() or w.device != device:
+        raise ValueError(f"{what}: expected contiguous uint8 blocks on {device}")
+    if w.numel() != weight_bytes(name, rows, cols):
+        raise ValueError(f"{what}: expected {weight_bytes(name, rows, cols)} bytes, got {w.numel()}")
+    return w.data_ptr()
+
+
+class _On:
+    """Makes a tensor's device current for one call (the library runs on the
+    current device); stream: the caller's, or that device's current one."""
+
+    def __init__(self, device, stream):
+        import torch
+        if device.type != "cuda":
+            raise ValueError(f"expected CUDA tensors, got tensors on {device}")
+        self.other = device.index is not None and device.index != torch.cuda.current_device()
+        if self.other:
+            self.guard = torch.cuda.device(device)
+            self.guard.__enter__()
+        self.stream = _stream_handle(stream)
+
+    def done(self):
+        if self.other:
+            self.guard.__exit__(None, None, None)
+
+
+def _workspace(ws, need: int, device):
+    """The caller's workspace, or a fresh one from torch's allocator (which
+    keeps it alive in stream order, and per graph under capture)."""
+    import torch
+    if ws is None:
+        return torch.empty(need, dtype=torch.uint8, device=device)
+    if ws.dtype != torch.uint8 or not ws.is_contiguous() or ws.device != device:
+        raise ValueError(f"workspace: expected a contiguous uint8 tensor on {device}")
+    return ws
+
+
+class Router:
+    """mlq_router: fp32 weights [n_experts, in], an optional bias [n_experts]
+    that takes part in the choice only."""
+
+    def __init__(self, w, top_k: int, bias=None, scoring: str = "softmax", renormalize: bool = True,
+                 scale: float = 1.0):
+        import torch
+        if w.dim() != 2:
+            raise ValueError("router weights: expected [n_experts, in_features]")
+        if scoring not in SCORINGS:
+            raise ValueError(f"unknown scoring {scoring!r}")
+        self.n_experts, self.in_features = w.shape
+        self.top_k, self.device = int(top_k), w.device
+        self._keep = (w, bias)
+        self.struct = RouterStruct(_need(w, torch.float32, w.shape, w.device, "router weights"),
+                                   _need(bias, torch.float32, (self.n_experts,), w.device, "router bias"),
+                                   self.n_experts, self.in_features, self.top_k, SCORINGS[scoring],
+                                   1 if renormalize else 0, float(scale))
+        self.ref = ctypes.byref(self.struct)
+
+
+class Experts:
+    """mlq_experts: stacked packed blocks, w_gate and w_up [n_experts][hidden][in]
+    in `fmt`, w_down [n_experts][out][hidden] in `fmt_down` (default fmt)."""
+
+    def __init__(self, fmt, w_gate, w_up, w_down, n_experts: int, in_features: int, hidden: int, out_features=None,
+                 fmt_down=None):
+        fmt_down = fmt if fmt_down is None else fmt_down
+        out_features = in_features if out_features is None else out_features
+        self.device, self.n_experts, self.in_features, self.out_features = w_gate.device, n_experts, in_features, out_features
+        self._keep = (w_gate, w_up, w_down)
+        self.struct = ExpertsStruct(
+            fmt_id(fmt), fmt_id(fmt_down), n_experts, in_features, hidden, out_features,
+            _blocks_need(w_gate, fmt, n_experts * hidden, in_features, self.device, "w_gate"),
+            _blocks_need(w_up, fmt, n_experts * hidden, in_features, self.device, "w_up"),
+            _blocks_need(w_down, fmt_down, n_experts * out_features, hidden, self.device, "w_down"),
+            n_experts * hidden * blocks_per_row(in_features), n_experts * out_features * blocks_per_row(hidden))
+        self.ref = ctypes.byref(self.struct)
+
+
+def _bytes_or_raise(n: int) -> int:
+    if n == 0:
+        raise MLQError(9, lib().mlq_last_error().decode() or "workspace size: bad arguments")
+    return n
+
+
+def route_workspace_bytes(router: Router, rows: int) -> int:
+    return _bytes_or_raise(_moe_lib().mlq_moe_route_workspace_bytes(router.ref, rows))
+
+
+def experts_workspace_bytes(experts: Experts, rows: int, top_k: int) -> int:
+    return _bytes_or_raise(_moe_lib().mlq_moe_experts_workspace_bytes(experts.ref, rows, top_k))
+
+
+def layer_workspace_bytes(router: Router, experts: Experts, rows: int) -> int:
+    return _bytes_or_raise(_moe_lib().mlq_moe_layer_workspace_bytes(router.ref, experts.ref, rows))
+
+
+def epilogue_workspace_bytes(fmt, out_features: int, in_features: int, rows: int) -> int:
+    return _bytes_or_raise(_moe_lib().mlq_linear_epilogue_workspace_bytes(fmt_id(fmt), out_features, in_features, rows))
+
+
+def moe_route(router: Router, x, ids=None, weights=None, logits=None, workspace=None, stream=None):
+    """mlq_moe_route: (ids int32 [rows, top_k], weights float32 [rows, top_k])
+    of x float32 [rows, in] (or [in]).  logits: float32 [rows, n_experts] to
+    fill, or None.  Without `workspace` one is allocated for the call."""
+    import torch
+    L = _moe_lib()
+    dev = x.device
+    rows = _rows_of(x, router.in_features)
+    xp = _need(x, torch.float32, x.shape, router.device, "x")
+    shape = (rows, router.top_k)
+    if ids is None:
+        ids = torch.empty(shape, dtype=torch.int32, device=dev)
+    if weights is None:
+        weights = torch.empty(shape, dtype=torch.float32, device=dev)
+    ws = _workspace(workspace, 0 if workspace is not None else route_workspace_bytes(router, rows), dev)
+    on = _On(dev, stream)
+    try:
+        check(L.mlq_moe_route(router.ref, xp, rows, _need(ids, torch.int32, shape, dev, "ids"),
+                              _need(weights, torch.float32, shape, dev, "weights"),
+                              _need(logits, torch.float32, (rows, router.n_experts), dev, "logits"),
+                              ws.data_ptr(), ws.numel(), on.stream))
+    finally:
+        on.done()
+    return ids, weights
+
+
+def moe_experts(experts: Experts, x, ids, weights, residual=None, y=None, workspace=None, stream=None):
+    """mlq_moe_experts: y = residual + sum over slots of weights * expert(x),
+    ids int32 / weights float32 [rows, top_k]; ids outside [0, n_experts) add
+    nothing."""
+    import torch
+    L = _moe_lib()
+    dev = x.device
+    rows = _rows_of(x, experts.in_features)
+    xp = _need(x, torch.float32, x.shape, experts.device, "x")
+    top_k = ids.shape[-1]
+    shape = (rows, top_k) if ids.dim() == 2 else (top_k,)
+    yshape = (experts.out_features,) if x.dim() == 1 else (rows, experts.out_features)
+    if y is None:
+        y = torch.empty(yshape, dtype=torch.float32, device=dev)
+    ws = _workspace(workspace, 0 if workspace is not None else experts_workspace_bytes(experts, rows, top_k), dev)
+    on = _On(dev, stream)
+    try:
+        check(L.mlq_moe_experts(experts.ref, xp, rows, top_k, _need(ids, torch.int32, shape, dev, "ids"),
+                                _need(weights, torch.float32, shape, dev, "weights"),
+                                _need(residual, torch.float32, yshape, dev, "residual"),
+                                _need(y, torch.float32, yshape, dev, "y"), ws.data_ptr(), ws.numel(), on.stream))
+    finally:
+        on.done()
+    return y
+
+
+def moe_layer(router: Router, experts: Experts, x, residual=None, y=None, ids=None, weights=None, workspace=None,
+              stream=None):
+    """mlq_moe_layer: the router's choice, then the experts; returns
+    (y, ids, weights)."""
+    import torch
+    L = _moe_lib()
+    dev = x.device
+    rows = _rows_of(x, experts.in_features)
+    xp = _need(x, torch.float32, x.shape, experts.device, "x")
+    if router.device != dev:
+        raise ValueError(f"the router is on {router.device}, x on {dev}")
+    shape = (rows, router.top_k)
+    yshape = (experts.out_features,) if x.dim() == 1 else (rows, experts.out_features)
+    if ids is None:
+        ids = torch.empty(shape, dtype=torch.int32, device=dev)
+    if weights is None:
+        weights = torch.empty(shape, dtype=torch.float32, device=dev)
+    if y is None:
+        y = torch.empty(yshape, dtype=torch.float32, device=dev)
+    ws = _workspace(workspace, 0 if workspace is not None else layer_workspace_bytes(router, experts, rows), dev)
+    on = _On(dev, stream)
+    try:
+        check(L.mlq_moe_layer(router.ref, experts.ref, xp, rows, _need(residual, torch.float32, yshape, dev, "residual"),
+                              _need(y, torch.float32, yshape, dev, "y"), _need(ids, torch.int32, shape, dev, "ids"),
+                              _need(weights, torch.float32, shape, dev, "weights"), ws.data_ptr(), ws.numel(),
+                              on.stream))
+    finally:
+        on.done()
+    return y, ids, weights
+
+
+def linear_epilogue(fmt, w, out_features: int, in_features: int, x, bias=None, activation=None, row_scale=None,
+                    residual=None, y=None, workspace=None, stream=None):
+    """mlq_linear_epilogue: y = residual + row_scale[:, None] * act(x @ W^T + bias);
+    activation: None / "none", "silu", "gelu", "gelu_tanh", "relu", "sigmoid"."""
+    import torch
+    L = _moe_lib()
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"unknown activation {activation!r}")
+    dev = x.device
+    rows = _rows_of(x, in_features)
+    xp = _need(x, torch.float32, x.shape, dev, "x")
+    wp = _blocks_need(w, fmt, out_features, in_features, dev, "w")
+    yshape = (out_features,) if x.dim() == 1 else (rows, out_features)
+    if y is None:
+        y = torch.empty(yshape, dtype=torch.float32, device=dev)
+    ep = EpilogueStruct(_need(bias, torch.float32, (out_features,), dev, "bias"), ACTIVATIONS[activation],
+                        _need(row_scale, torch.float32, (rows,), dev, "row_scale"),
+                        _need(residual, torch.float32, yshape, dev, "residual"))
+    ws = _workspace(workspace,
+                    0 if workspace is not None else epilogue_workspace_bytes(fmt, out_features, in_features, rows), dev)
+    on = _On(dev, stream)
+    try:
+        check(L.mlq_linear_epilogue(fmt_id(fmt), wp, out_features * blocks_per_row(in_features), out_features,
+                                    in_features, xp, rows, ctypes.byref(ep), _need(y, torch.float32, yshape, dev, "y"),
+                                    ws.data_ptr(), ws.numel(), on.stream))
+    finally:
+        on.done()
+    return y
