@@ -439,10 +439,11 @@ MLQ_API mlq_status mlq_peer_free(void* ptr);
  * the quantized weights before.  They can be captured into a graph.
  *
  * Arithmetic: weights are exact; each row of x (and of an expert's hidden
- * vector) is carried as 24-bit fixed point against a power of two per
- * 32-value block; sums are exact integers per block and fp32 across blocks.
- * Outputs are within ~1e-6 relative L2 of the 64-bit result.  A value of x
- * that is not finite makes every output that reads it NaN.  Results do not
+ * vector) is carried, per 32-value block, as 31-bit fixed point or as the sum
+ * of two fp16 values (to 2^-22 of each value) against a power of two; sums
+ * are integers or fp32 per block and fp32 across blocks.  Outputs are within
+ * ~1e-6 relative L2 of the 64-bit result.  A value of x that is not finite
+ * makes every output that reads it NaN.  Results do not
  * depend on the other rows of the call or on their order beyond rounding,
  * and a call repeated gives the same bits.
  * ------------------------------------------------------------------------- */

@@ -3,20 +3,24 @@
 //
 // A call is up to three launches, chained by programmatic dependent launch:
 //   prep   sorts the (row, slot) pairs by expert into segments of at most 32
-//          and slices x into digits;
+//          and slices x;
 //   pair   h = silu(x Wg^T) * (x Wu^T) per segment, sliced in its epilogue;
 //   down   h Wd^T per segment, weighed and summed per row by the CTA that
 //          finishes a row tile last (fixed order), or by a fourth launch
 //          when there are many rows;
 // and two (prep, down in its plain form) for the linear with an epilogue.
 //
-// The streaming kernel.  A unit is a row tile of one matrix against one
-// segment.  Its 8 warps split the tile in 16-row strips and the K axis in
-// interleaved steps of 8 blocks; every warp fetches its own 16 x 8 blocks by
-// TMA into a ring of its own, so the weight stream never waits for another
-// warp; units follow one another in a static order and the ring runs ahead
-// across them.  The K parts of a unit meet in shared memory (fixed order), one
-// barrier per unit.  Two CTAs per SM: one computes while the other drains.
+// The streaming kernel.  One CTA per SM: a producer warp and 8 computing
+// warps.  A unit is a tile of 32, 64 or 128 rows of one matrix against one
+// segment; the computing warps split it in 32-row groups and the K axis in
+// interleaved steps of 8 blocks.  A round is one step of every warp: 256
+// (row, block) squares of 32 whatever the tile, so rounds cost the same and the
+// launch's rounds are dealt out evenly, a contiguous range per CTA.  Each
+// warp has a ring of weight slots of its own that the producer fills by TMA,
+// running ahead across units, so the weight stream does not wait for a unit's
+// end.  The K parts of a unit meet in shared memory in a fixed order; a unit
+// whose rounds fall to several CTAs is added up (in order) by the last of
+// them to finish.
 #include "mlq_imma.cuh"
 #include "mlq_tmap.h"
 
@@ -29,18 +33,24 @@ struct ImmaMaps {
     CUtensorMap m[2];
 };
 
+// Sliced rows of x or h: [row][bprp][128 bytes], a scale and a sum per block.
+struct Sliced {
+    uint8_t* data;
+    float* scale;
+    float* sum;
+};
+
 struct ImmaArgs {
     const uint8_t* w[2];      // stacked matrices [n][out][bpr]; [1]: the up projections (kPair)
     long long row_bytes;      // bytes of a matrix row
     long long total_rows;     // rows of the whole stack
     int out;                  // rows of one matrix
     int bpr, bprp;            // blocks per row, and padded to whole steps
-    int strips;               // 16-row strips of a unit (1, 2, 4 or 8); kPair: 4 (32 gate and 32 up rows)
+    int groups;               // 32-row groups of a unit (1, 2 or 4); kPair: 16 gate and 16 up rows each, 2 or 4
     int tiles;                // row tiles of one matrix
     int slots;                // ring depth of a warp
-    const uint8_t* dig;       // sliced rows of x / h: digits [row][bprp][96]
-    const float* scale;       // [row][bprp]
-    const float* sum;         // [row][bprp]
+    int few;                  // segments of at most this many rows go by digits
+    Sliced few_x, many_x;     // digits / halves (the same arrays for h: a segment has one form)
     // segments (kPair, kDown); kPlain: rows in order, one matrix
     const Segment* segs;
     const int* nseg;
@@ -48,15 +58,17 @@ struct ImmaArgs {
     int top_k, rows;
     // kPair: sliced h by position
     int next_fmt, next_bprp;
-    uint8_t* hdig;
-    float* hscale;
-    float* hsum;
+    Sliced h;
     // kDown: one value per pair, then the weighed sum
     float* part;              // [pair][out]
-    unsigned int* done;       // per row tile, zero before the launch; null: a later launch sums
+    unsigned int* done;       // units finished per row tile, zero before the launch; null: a later launch sums
     const int32_t* ids;
     const float* weights;
     int n_experts;
+    // units that several CTAs share
+    float* split;             // [CTA][head, tail][row of x][row of the tile]
+    unsigned int* split_done; // per CTA, zero before the launch
+    int split_tokens;         // rows of x of a split slot
     // kPlain / kDown
     const float* bias;
     const float* row_scale;
@@ -66,99 +78,108 @@ struct ImmaArgs {
     int* err;
 };
 
-// The accumulators of up to 2 NT rows of x: a matrix instruction's 8 columns
-// are the digits (hi, mid, lo, none) of 2 rows, so lane t holds (hi, mid)
-// (t even) or lo (t odd) of row t / 2 and the two are added once, at the end.
+// The accumulators of up to 2 NT rows of x by digits: an instruction's 8
+// columns are the 4 digits of 2 rows, so lane t holds digits 3 and 2 (t even) or
+// 1 and 0 (t odd) of row t / 2, and the two are added once, at the end.
 template <int F, int NT>
 struct FewRows {
     static constexpr int kSubs = 1;
     uint32_t bo[NT], so[NT];
-    bool on[NT];
-    float acc[NT][2], accm[NT][2];
+    float acc[NT][2][2], accm[F == kQ4_1 ? NT : 1][2][2];
 
     template <class TokenOf>
     __device__ __forceinline__ void init(const ImmaArgs& a, int count, int lane, TokenOf token) {
         const int g = lane >> 2, t = lane & 3;
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
-            const int r = 2 * i + (g >> 2), s = g & 3;
-            on[i] = s < 3 && r < count;
-            bo[i] = (uint32_t)token(r < count ? r : 0) * (uint32_t)a.bprp * kDigitBytes + (s < 3 ? s : 0) * 32 + t * 8;
-            const int rs = 2 * i + (t >> 1);
+            // columns without a row of x repeat the first one's; nothing reads them
+            const int r = 2 * i + (g >> 2), rs = 2 * i + (t >> 1);
+            bo[i] = (uint32_t)token(r < count ? r : 0) * (uint32_t)a.bprp * kSlicedBytes + (g & 3) * 32 + t * 8;
             so[i] = (uint32_t)token(rs < count ? rs : 0) * (uint32_t)a.bprp;
-            acc[i][0] = acc[i][1] = accm[i][0] = accm[i][1] = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                acc[i][j][0] = acc[i][j][1] = 0.0f;
+                if (F == kQ4_1) accm[i][j][0] = accm[i][j][1] = 0.0f;
+            }
         }
     }
 
-    template <bool ALN, class Wait>
-    __device__ __forceinline__ void step(const ImmaArgs& a, int kb, uint32_t r0, uint32_t r1, int lane, Wait wait) {
+    template <bool ALN, class Rows, class Wait>
+    __device__ __forceinline__ void step(const ImmaArgs& a, int kb, int valid, int lane, Wait wait, Rows rows) {
         const int t = lane & 3;
         uint2 b[NT][kChunkBlocks];
-        float s[NT][kChunkBlocks], m[NT][F == kQ4_1 ? kChunkBlocks : 1];
+        float4 s[NT][2], m[F == kQ4_1 ? NT : 1][2];
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
-            const uint8_t* p = a.dig + bo[i] + (size_t)kb * kDigitBytes;
+            const uint8_t* p = a.few_x.data + bo[i] + (size_t)kb * kSlicedBytes;
 #pragma unroll
-            for (int k = 0; k < kChunkBlocks; ++k)
-                b[i][k] = on[i] ? *reinterpret_cast<const uint2*>(p + k * kDigitBytes) : make_uint2(0, 0);
-            const float4* sp = reinterpret_cast<const float4*>(a.scale + so[i] + kb);
-            const float4 s0 = sp[0], s1 = sp[1];
-            s[i][0] = s0.x, s[i][1] = s0.y, s[i][2] = s0.z, s[i][3] = s0.w;
-            s[i][4] = s1.x, s[i][5] = s1.y, s[i][6] = s1.z, s[i][7] = s1.w;
+            for (int k = 0; k < kChunkBlocks; ++k) b[i][k] = *reinterpret_cast<const uint2*>(p + k * kSlicedBytes);
+            const float4* sp = reinterpret_cast<const float4*>(a.few_x.scale + so[i] + kb);
+            s[i][0] = sp[0], s[i][1] = sp[1];
             if (F == kQ4_1) {
-                const float4* mp = reinterpret_cast<const float4*>(a.sum + so[i] + kb);
-                const float4 m0 = mp[0], m1 = mp[1];
-                m[i][0] = m0.x, m[i][1] = m0.y, m[i][2] = m0.z, m[i][3] = m0.w;
-                m[i][4] = m1.x, m[i][5] = m1.y, m[i][6] = m1.z, m[i][7] = m1.w;
+                const float4* mp = reinterpret_cast<const float4*>(a.few_x.sum + so[i] + kb);
+                m[i][0] = mp[0], m[i][1] = mp[1];
             }
         }
         wait();
 #pragma unroll
         for (int p = 0; p < kChunkBlocks / 2; ++p) {
-            BlockA A[2];
-            load_pair<F, ALN>(r0, r1, p, t, A[0], A[1]);
+            if (!ALN && 2 * p >= valid) break;
 #pragma unroll
-            for (int o = 0; o < 2; ++o)
+            for (int j = 0; j < 2; ++j) {
+                RawA A[2];
+                load_pair<F, ALN>(rows(j, 0), rows(j, 1), p, t, A[0], A[1]);
+                if (!ALN && 2 * p + 1 >= valid) A[1].d[0] = A[1].d[1] = A[1].m[0] = A[1].m[1] = 0.0f;
 #pragma unroll
-                for (int i = 0; i < NT; ++i) {
-                    int c[4];
-                    imma_s8(c, A[o].a, b[i][2 * p + o]);
-                    const float sx = s[i][2 * p + o];
-                    acc[i][0] = fmaf(A[o].d[0] * sx, (float)(c[0] * 256 + c[1]), acc[i][0]);
-                    acc[i][1] = fmaf(A[o].d[1] * sx, (float)(c[2] * 256 + c[3]), acc[i][1]);
-                    if (F == kQ4_1) {
-                        accm[i][0] = fmaf(A[o].m[0], m[i][2 * p + o], accm[i][0]);
-                        accm[i][1] = fmaf(A[o].m[1], m[i][2 * p + o], accm[i][1]);
+                for (int o = 0; o < 2; ++o) {
+                    uint32_t op[4];
+                    int8_operand<F>(A[o], op);
+#pragma unroll
+                    for (int i = 0; i < NT; ++i) {
+                        int c[4];
+                        imma_s8(c, op, b[i][2 * p + o]);
+                        const float4 s4 = s[i][p >> 1];
+                        const float sx = p & 1 ? (o ? s4.w : s4.z) : (o ? s4.y : s4.x);
+                        acc[i][j][0] = fmaf(A[o].d[0] * sx, (float)(c[0] * 256 + c[1]), acc[i][j][0]);
+                        acc[i][j][1] = fmaf(A[o].d[1] * sx, (float)(c[2] * 256 + c[3]), acc[i][j][1]);
+                        if (F == kQ4_1) {
+                            const float4 m4 = m[i][p >> 1];
+                            const float mx = p & 1 ? (o ? m4.w : m4.z) : (o ? m4.y : m4.x);
+                            accm[i][j][0] = fmaf(A[o].m[0], mx, accm[i][j][0]);
+                            accm[i][j][1] = fmaf(A[o].m[1], mx, accm[i][j][1]);
+                        }
                     }
                 }
+            }
         }
     }
 
-    // red: [row of x 0..7][weight row 0..15] of this warp
-    __device__ __forceinline__ void store(float* red, int, int lane) {
-        const int g = lane >> 2, t = lane & 3;
-        // an accumulator holds 256 times its first digit plus the second: (hi, mid) is 256 too small, (lo, 0) 256
-        // too large; q4 codes count 16
-        const float f = (t & 1 ? 0.00390625f : 256.0f) * (F == kQ8_0 ? 1.0f : 0.0625f);
+    // put(row of x 0..7, 16-row strip j, row half q, value)
+    template <class Put>
+    __device__ __forceinline__ void store(int, int lane, Put put) {
+        const int t = lane & 3;
+        // digits 3 and 2 count 2^16 times digits 1 and 0; q4 codes count 16
+        const float f = (t & 1 ? 1.0f : 65536.0f) * (F == kQ8_0 ? 1.0f : 0.0625f);
 #pragma unroll
         for (int i = 0; i < NT; ++i)
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                float v = acc[i][q] * f;
-                v += __shfl_xor_sync(0xffffffffu, v, 1);
-                if (F == kQ4_1) v += accm[i][q];
-                if (!(t & 1)) red[(2 * i + (t >> 1)) * 16 + g + 8 * q] = v;
-            }
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    float v = acc[i][j][q] * f;
+                    v += __shfl_xor_sync(0xffffffffu, v, 1);
+                    if (F == kQ4_1) v += accm[i][j][q];
+                    if (!(t & 1)) put(2 * i + (t >> 1), j, q, v);
+                }
     }
 };
 
-// Up to 8 S rows of x: three instructions (hi, mid, lo) whose 8 columns are 8
-// rows of x, so a lane has all digits of rows 2t and 2t + 1.
+// Up to 8 S rows of x by halves: one column per row.
 template <int F, int S>
 struct ManyRows {
     static constexpr int kSubs = S;
     uint32_t bo[S], so[S][2];
-    float acc[S][2][2];  // [.][weight row g / g + 8][row of x]
+    float acc[S][2][2][2];  // [.][strip][row half][row of x 2t, 2t + 1]
 
     template <class TokenOf>
     __device__ __forceinline__ void init(const ImmaArgs& a, int count, int lane, TokenOf token) {
@@ -166,69 +187,79 @@ struct ManyRows {
 #pragma unroll
         for (int i = 0; i < S; ++i) {
             const int r = 8 * i + g;
-            bo[i] = (uint32_t)token(r < count ? r : 0) * (uint32_t)a.bprp * kDigitBytes + t * 8;
+            bo[i] = (uint32_t)token(r < count ? r : 0) * (uint32_t)a.bprp * kSlicedBytes + t * 16;
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                const int rs = 8 * i + 2 * t + q;
-                so[i][q] = (uint32_t)token(rs < count ? rs : 0) * (uint32_t)a.bprp;
-                acc[i][q][0] = acc[i][q][1] = 0.0f;
+            for (int x = 0; x < 2; ++x) {
+                const int rs = 8 * i + 2 * t + x;
+                so[i][x] = (uint32_t)token(rs < count ? rs : 0) * (uint32_t)a.bprp;
             }
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+                acc[i][j][0][0] = acc[i][j][0][1] = acc[i][j][1][0] = acc[i][j][1][1] = 0.0f;
         }
     }
 
-    template <bool ALN, class Wait>
-    __device__ __forceinline__ void step(const ImmaArgs& a, int kb, uint32_t r0, uint32_t r1, int lane, Wait wait) {
+    template <bool ALN, class Rows, class Wait>
+    __device__ __forceinline__ void step(const ImmaArgs& a, int kb, int valid, int lane, Wait wait, Rows rows) {
         const int t = lane & 3;
         wait();
 #pragma unroll
         for (int p = 0; p < kChunkBlocks / 2; ++p) {
-            BlockA A[2];
-            load_pair<F, ALN>(r0, r1, p, t, A[0], A[1]);
+            if (2 * p >= valid) break;
+            RawA A[2][2];  // [strip][block]
 #pragma unroll
-            for (int i = 0; i < S; ++i) {
-                const uint8_t* bp = a.dig + bo[i] + (size_t)(kb + 2 * p) * kDigitBytes;
-                const float2 s0 = *reinterpret_cast<const float2*>(a.scale + so[i][0] + kb + 2 * p);
-                const float2 s1 = *reinterpret_cast<const float2*>(a.scale + so[i][1] + kb + 2 * p);
+            for (int j = 0; j < 2; ++j) load_pair<F, ALN>(rows(j, 0), rows(j, 1), p, t, A[j][0], A[j][1]);
 #pragma unroll
-                for (int o = 0; o < 2; ++o) {
-                    int hi[4], mid[4], lo[4];
-                    imma_s8(hi, A[o].a, *reinterpret_cast<const uint2*>(bp + o * kDigitBytes));
-                    imma_s8(mid, A[o].a, *reinterpret_cast<const uint2*>(bp + o * kDigitBytes + 32));
-                    imma_s8(lo, A[o].a, *reinterpret_cast<const uint2*>(bp + o * kDigitBytes + 64));
-                    const float sx[2] = {o ? s0.y : s0.x, o ? s1.y : s1.x};
+            for (int o = 0; o < 2; ++o) {
+                if (2 * p + o >= valid) break;
+                const int blk = kb + 2 * p + o;
+                uint32_t op[2][8];
+                half_operand<F>(A[0][o], op[0]);
+                half_operand<F>(A[1][o], op[1]);
 #pragma unroll
-                    for (int q = 0; q < 2; ++q)
+                for (int i = 0; i < S; ++i) {
+                    const uint4* bp = reinterpret_cast<const uint4*>(a.many_x.data + bo[i] + (size_t)blk * kSlicedBytes);
+                    const uint4 hi = bp[0], lo = bp[4];
+                    const float s0 = a.many_x.scale[so[i][0] + blk], s1 = a.many_x.scale[so[i][1] + blk];
+                    float m0 = 0.0f, m1 = 0.0f;
+                    if (F == kQ4_1) m0 = a.many_x.sum[so[i][0] + blk], m1 = a.many_x.sum[so[i][1] + blk];
 #pragma unroll
-                        for (int x = 0; x < 2; ++x) {
-                            const float v = fmaf((float)(hi[2 * q + x] * 256 + mid[2 * q + x]), 256.0f,
-                                                 (float)lo[2 * q + x]);
-                            acc[i][q][x] = fmaf(A[o].d[q] * sx[x], v, acc[i][q][x]);
+                    for (int j = 0; j < 2; ++j) {
+                        float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                        hmma_f16(c, op[j], lo.x, lo.y);
+                        hmma_f16(c, op[j] + 4, lo.z, lo.w);
+                        hmma_f16(c, op[j], hi.x, hi.y);
+                        hmma_f16(c, op[j] + 4, hi.z, hi.w);
+                        const RawA& A1 = A[j][o];
+                        acc[i][j][0][0] = fmaf(A1.d[0] * s0, c[0], acc[i][j][0][0]);
+                        acc[i][j][0][1] = fmaf(A1.d[0] * s1, c[1], acc[i][j][0][1]);
+                        acc[i][j][1][0] = fmaf(A1.d[1] * s0, c[2], acc[i][j][1][0]);
+                        acc[i][j][1][1] = fmaf(A1.d[1] * s1, c[3], acc[i][j][1][1]);
+                        if (F == kQ4_1) {
+                            acc[i][j][0][0] = fmaf(A1.m[0], m0, acc[i][j][0][0]);
+                            acc[i][j][0][1] = fmaf(A1.m[0], m1, acc[i][j][0][1]);
+                            acc[i][j][1][0] = fmaf(A1.m[1], m0, acc[i][j][1][0]);
+                            acc[i][j][1][1] = fmaf(A1.m[1], m1, acc[i][j][1][1]);
                         }
-                    if (F == kQ4_1) {
-                        // the block's offset term, in the accumulator's unit (codes count 16)
-                        const float2 m0 = *reinterpret_cast<const float2*>(a.sum + so[i][0] + kb + 2 * p);
-                        const float2 m1 = *reinterpret_cast<const float2*>(a.sum + so[i][1] + kb + 2 * p);
-                        const float mx[2] = {16.0f * (o ? m0.y : m0.x), 16.0f * (o ? m1.y : m1.x)};
-#pragma unroll
-                        for (int q = 0; q < 2; ++q)
-#pragma unroll
-                            for (int x = 0; x < 2; ++x) acc[i][q][x] = fmaf(A[o].m[q], mx[x], acc[i][q][x]);
                     }
                 }
             }
         }
     }
 
-    __device__ __forceinline__ void store(float* red, int sub, int lane) {
-        const int g = lane >> 2, t = lane & 3;
-        const float f = F == kQ8_0 ? 1.0f : 0.0625f;
+    template <class Put>
+    __device__ __forceinline__ void store(int sub, int lane, Put put) {
+        const int t = lane & 3;
 #pragma unroll
         for (int i = 0; i < S; ++i)
             if (i == sub) {
 #pragma unroll
-                for (int q = 0; q < 2; ++q)
+                for (int j = 0; j < 2; ++j)
 #pragma unroll
-                    for (int x = 0; x < 2; ++x) red[(2 * t + x) * 16 + g + 8 * q] = acc[i][q][x] * f;
+                    for (int q = 0; q < 2; ++q) {
+                        put(2 * t, j, q, acc[i][j][q][0]);
+                        put(2 * t + 1, j, q, acc[i][j][q][1]);
+                    }
             }
     }
 };
@@ -246,10 +277,6 @@ __device__ __forceinline__ float activate(float v, int act) {
     }
 }
 
-__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, uint32_t bytes) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-
 // y[r][o] = residual[r][o] + sum_j weights[r][j] part[r k + j][o], slots in
 // order; a slot without an expert adds nothing.
 __device__ __forceinline__ float combine(const ImmaArgs& a, int r, int o) {
@@ -263,193 +290,279 @@ __device__ __forceinline__ float combine(const ImmaArgs& a, int r, int o) {
     return a.residual ? a.residual[at] + v : v;
 }
 
-constexpr int kRedFloats = kImmaWarps * 8 * 16;
+// The barrier of the computing warps.
+__device__ __forceinline__ void compute_sync() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kImmaWarps) : "memory"); }
+
+constexpr int kThreads = 32 * (kImmaWarps + 1);
+constexpr int kRedFloats = kImmaWarps * 8 * 32;  // [warp][row of x][row of the group]
+constexpr int kMaxCtas = 192;                    // CTAs of a launch at most (split slots)
+
+// How a launch's rounds are dealt out: CTA i takes [begin(i), begin(i + 1)).
+// Whole units when that costs no CTA more than 2 rounds (a round takes about
+// 0.8 us of a CTA's share of HBM, adding up a split unit about 2 us).
+struct Deal {
+    long long total;
+    int units, per_unit, ctas;
+    bool whole;
+    __device__ Deal(int units_, int per_unit_, int ctas_) : units(units_), per_unit(per_unit_), ctas(ctas_) {
+        total = (long long)units * per_unit;
+        if (ctas > total) ctas = (int)total;
+        const long long even = ctas ? (total + ctas - 1) / ctas : 0;
+        const long long by_unit = ctas ? (long long)((units + ctas - 1) / ctas) * per_unit : 0;
+        whole = by_unit <= even + 2;
+        if (whole && ctas > units) ctas = units;
+    }
+    __device__ long long begin(int i) const {
+        return whole ? (long long)units * i / ctas * per_unit : total * i / ctas;
+    }
+    // the CTA that has round t (not asked when units are whole)
+    __device__ int owner(long long t) const { return (int)(((t + 1) * ctas - 1) / total); }
+};
 
 template <int F, int MODE, bool ALN>
-__global__ void __launch_bounds__(32 * kImmaWarps, 2)
-    imma_kernel(const __grid_constant__ ImmaMaps maps, const ImmaArgs a) {
+__global__ void __launch_bounds__(kThreads, 1) imma_kernel(const __grid_constant__ ImmaMaps maps, const ImmaArgs a) {
     extern __shared__ __align__(128) uint8_t smem[];
     using S = Slot<F, ALN>;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int strip = warp % a.strips, kw = warp / a.strips, kws = kImmaWarps / a.strips;
+    __shared__ int s_last, s_dead, s_issued[kImmaWarps];
+    const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
+    const int kws = kImmaWarps / a.groups;
     const int steps = (a.bpr + kChunkBlocks - 1) / kChunkBlocks;
-    const uint32_t slots = smem_u32(smem) + (uint32_t)warp * a.slots * S::kBytes;
+    const int per_unit = (steps + kws - 1) / kws;
     float* red = reinterpret_cast<float*>(smem + kImmaWarps * a.slots * S::kBytes);  // two buffers
-    const uint32_t bars = smem_u32(red + 2 * kRedFloats) + warp * a.slots * 8;
-    __shared__ int s_last;
-
-    if (ALN && lane == 0) {
-        for (int i = 0; i < a.slots; ++i) mbar_init(bars + 8 * i, 1);
-        fence_mbar_init();
+    const uint32_t slots0 = smem_u32(smem), bars0 = smem_u32(red + 2 * kRedFloats);
+    // barriers of warp w's slot i: full at bars0 + 16 (w slots + i), empty 8 bytes on
+    if (threadIdx.x == 0) s_dead = 0;
+    for (int i = threadIdx.x; i < kImmaWarps * a.slots; i += kThreads) {
+        mbar_init(bars0 + 16 * i, ALN ? 1 : 32);
+        mbar_init(bars0 + 16 * i + 8, 1);
     }
-    __syncwarp();
+    fence_mbar_init();
 
     // The segments come from prep.  kPair is prep's dependent, so it waits;
     // kDown started after every CTA of kPair had waited for prep, so prep has
     // completed: it reads the segments (past L1) and streams weights at once.
-    if (MODE == kPair) {
-        grid_dependency_wait();
-        launch_dependents();
-    }
+    if (MODE == kPair) grid_dependency_wait();
+    if (MODE != kDown) launch_dependents();
+    __syncthreads();
     const int nseg = MODE == kPlain ? (a.rows + kSegTokens - 1) / kSegTokens : __ldcg(a.nseg);
-    const int units = nseg * a.tiles;
+    const Deal deal(nseg * a.tiles, per_unit, gridDim.x);
+    const bool has_work = (int)blockIdx.x < deal.ctas;
+    const long long t0 = has_work ? deal.begin(blockIdx.x) : 0, t1 = has_work ? deal.begin(blockIdx.x + 1) : 0;
+    // kPair: a segment's tiles follow one another (its rows of x stay near); kDown, kPlain: a tile's segments do
+    auto tile_of = [&](int u) { return MODE == kPair ? u % a.tiles : u / nseg; };
+    auto seg_of = [&](int u) { return MODE == kPair ? u / a.tiles : u % nseg; };
+    const int unit_rows = (MODE == kPair ? 16 : 32) * a.groups;
 
-    // what the ring fetches next: unit pu, K step pc
-    int pu = blockIdx.x, pc = kw, p_slot = 0, in_flight = 0;
-    long long p_row = 0;
-    bool alive = true;  // false once a wait ran out: nothing more is fetched or waited for
-    int lost = 0, lost_slot = 0, lost_phase = 0;
-    auto unit_row = [&](int u) -> long long {
-        const int seg = u % nseg, tile = u / nseg;
-        const int e = MODE == kPlain ? 0 : __ldcg(&a.segs[seg].expert);
-        return (long long)e * a.out + (long long)tile * (MODE == kPair ? 32 : 16 * a.strips) +
-               strip * (MODE == kPair ? 8 : 16);
-    };
-    if (kw >= steps) pu = units;
-    if (pu < units) p_row = unit_row(pu);
-    auto fetch = [&]() {
-        if (pu < units && alive) {
-            const uint32_t dst = slots + p_slot * S::kBytes;
-            if constexpr (ALN) {
-                if (lane == 0) {
-                    const uint32_t bar = bars + 8 * p_slot;
-                    mbar_arrive_expect_tx(bar, S::kBytes);
+    if (warp == kImmaWarps) {
+        // ---- producer ----
+        int issued = 0;  // of the ring of warp `lane` (aligned) or of every ring
+        bool alive = true;
+        int u = t0 < t1 ? (int)(t0 / per_unit) : 0, r = t0 < t1 ? (int)(t0 % per_unit) : 0;
+        long long row0 = 0;
+        bool fresh = true;
+        if constexpr (ALN) {
+            // lane w fills the ring of warp w
+            const int w = lane, grp = w % a.groups, kw = w / a.groups;
+            int slot = 0, phase = 1;
+            if (w < kImmaWarps) {
+                for (long long t = t0; t < t1; ++t) {
+                    if (fresh) {
+                        const int e = MODE == kPlain ? 0 : __ldcg(&a.segs[seg_of(u)].expert);
+                        row0 = (long long)e * a.out + (long long)tile_of(u) * unit_rows + grp * (MODE == kPair ? 16 : 32);
+                        fresh = false;
+                    }
+                    const int c = r * kws + kw;
+                    if (c < steps) {
+                        const uint32_t bar = bars0 + 16 * (w * a.slots + slot);
+                        const uint32_t dst = slots0 + (w * a.slots + slot) * S::kBytes;
+                        if (!mbar_wait(bar + 8, phase)) {
+                            report_error(a.err, 31);
+                            *(volatile int*)&s_dead = 1;
+                        }
+                        if (*(volatile int*)&s_dead) break;
+                        mbar_arrive_expect_tx(bar, S::kBytes);
 #pragma unroll
-                    for (int b = 0; b < S::kBoxes; ++b) {
-                        const int c0 = (pc * chunk_bytes(F) + b * S::kBoxBytes) / 2;
-                        const uint32_t d = dst + b * 16 * S::kBoxBytes;
-                        tma_load_2d(d, &maps.m[0], c0, (int)p_row, bar);
-                        if (MODE == kPair) tma_load_2d(d + 8 * S::kBoxBytes, &maps.m[1], c0, (int)p_row, bar);
+                        for (int b = 0; b < S::kBoxes; ++b) {
+                            const int c0 = (c * chunk_bytes(F) + b * S::kPitch) / 2;
+                            const uint32_t d = dst + b * 32 * S::kPitch;
+                            tma_load_2d(d, &maps.m[0], c0, (int)row0, bar);
+                            if (MODE == kPair) tma_load_2d(d + 16 * S::kPitch, &maps.m[1], c0, (int)row0, bar);
+                        }
+                        ++issued;
+                        if (++slot == a.slots) slot = 0, phase ^= 1;
                     }
+                    if (++r == per_unit) r = 0, ++u, fresh = true;
                 }
-            } else {
-                // two lanes per row, the 16-byte windows that hold its blocks
-                const int r = lane >> 1;
-                const uint8_t* base = MODE == kPair && r >= 8 ? a.w[1] : a.w[0];
-                const long long row = p_row + (MODE == kPair ? (r & 7) : r);
-                const long long off = row * a.row_bytes + (long long)pc * chunk_bytes(F);
-                long long left = a.row_bytes - (long long)pc * chunk_bytes(F);
-                if (left > chunk_bytes(F)) left = chunk_bytes(F);
-                if (row >= a.total_rows) left = 0;
-                const uint8_t* src = base + (left > 0 ? off : 0);
-                const uint8_t* end = src + (left > 0 ? left : 0);
-                const uint8_t* win = reinterpret_cast<const uint8_t*>(reinterpret_cast<uintptr_t>(src) & ~(uintptr_t)15);
-                const uint32_t drow = dst + r * S::kPitch;
-                for (int i = lane & 1; i < (chunk_bytes(F) + 15 + 15) / 16; i += 2) {
-                    const uint8_t* q = win + 16 * i;
-                    long long n = end - q;
-                    n = n < 0 ? 0 : (n > 16 ? 16 : n);
-                    if (q < base && n > 0) {
-                        // the stack's first bytes, when it starts inside a window: nothing before it is read
-                        for (int k = 0; k < 16; ++k)
-                            sts_u8(drow + 16 * i + k, q + k >= base && k < n ? (uint32_t)q[k] : 0u);
+                s_issued[w] = issued;
+            }
+        } else {
+            // lane l copies row l of each warp's slot
+            int count[kImmaWarps] = {};
+            const uint8_t* base = MODE == kPair && lane >= 16 ? a.w[1] : a.w[0];
+            const uint8_t* stack_end = base + a.total_rows * a.row_bytes;
+            for (long long t = t0; t < t1 && alive; ++t) {
+                if (fresh) {
+                    const int e = MODE == kPlain ? 0 : __ldcg(&a.segs[seg_of(u)].expert);
+                    row0 = (long long)e * a.out + (long long)tile_of(u) * unit_rows + (MODE == kPair ? lane & 15 : lane);
+                    fresh = false;
+                }
+#pragma unroll
+                for (int w = 0; w < kImmaWarps; ++w) {
+                    const int c = r * kws + w / a.groups;
+                    if (c >= steps || !alive) continue;
+                    const int slot = count[w] % a.slots;
+                    const uint32_t bar = bars0 + 16 * (w * a.slots + slot);
+                    const bool ok = mbar_wait(bar + 8, ((count[w] / a.slots) & 1) ^ 1);
+                    if (!__all_sync(0xffffffffu, ok)) {
+                        if (lane == 0) report_error(a.err, 31), *(volatile int*)&s_dead = 1;
+                        alive = false;
+                        continue;
+                    }
+                    const long long row = row0 + (w % a.groups) * (MODE == kPair ? 16 : 32);
+                    const uint32_t dst = slots0 + (w * a.slots + slot) * S::kBytes + lane * S::kPitch;
+                    uint32_t bytes = 0;
+                    const uint8_t* win = nullptr;
+                    uint32_t into = dst;
+                    if (row < a.total_rows) {
+                        const uint8_t* src = base + row * a.row_bytes + (long long)c * chunk_bytes(F);
+                        long long left = a.row_bytes - (long long)c * chunk_bytes(F);
+                        if (left > chunk_bytes(F)) left = chunk_bytes(F);
+                        const uintptr_t lo = reinterpret_cast<uintptr_t>(src) & ~(uintptr_t)15;
+                        const uintptr_t hi = (reinterpret_cast<uintptr_t>(src) + left + 15) & ~(uintptr_t)15;
+                        win = reinterpret_cast<const uint8_t*>(lo);
+                        const uint8_t* wend = reinterpret_cast<const uint8_t*>(hi);
+                        // windows that stick out of the stack: its own bytes there one by one, the rest not at all
+                        if (win < base) {
+                            const int skip = (int)(base - win);
+                            for (int k = skip; k < 16 && base + (k - skip) < stack_end; ++k) sts_u8(dst + k, win[k]);
+                            win += 16;
+                            into += 16;
+                        }
+                        if (wend > stack_end && wend > win) {
+                            wend -= 16;
+                            for (int k = 0; wend + k < stack_end; ++k)
+                                sts_u8(into + (uint32_t)(wend - win) + k, wend[k]);
+                        }
+                        bytes = wend > win ? (uint32_t)(wend - win) : 0;
+                    }
+                    if (bytes) {
+                        mbar_arrive_expect_tx(bar, bytes);
+                        bulk_g2s(into, win, bytes, bar);
                     } else {
-                        cp_async_16(drow + 16 * i, n > 0 ? q : win + (win < base ? 16 : 0), (uint32_t)n);
+                        mbar_arrive(bar);
                     }
+                    ++count[w];
                 }
+                if (*(volatile int*)&s_dead) alive = false;
+                if (++r == per_unit) r = 0, ++u, fresh = true;
             }
-            ++in_flight;
-            if (++p_slot == a.slots) p_slot = 0;
-            pc += kws;
-            if (pc >= steps) {
-                pc = kw;
-                pu += gridDim.x;
-                if (pu < units) p_row = unit_row(pu);
-            }
+            if (lane == 0)
+#pragma unroll
+                for (int w = 0; w < kImmaWarps; ++w) s_issued[w] = count[w];
         }
-        if constexpr (!ALN) asm volatile("cp.async.commit_group;" ::: "memory");
-    };
-
-    if (MODE == kPlain) {
-        launch_dependents();
+        __syncwarp();
+        if (MODE != kPair) grid_dependency_wait();
+        if (MODE == kDown) launch_dependents();
+        __syncthreads();
+        return;
     }
-    for (int i = 0; i < a.slots; ++i) fetch();
+
+    // ---- computing warps ----
     if (MODE != kPair) grid_dependency_wait();
     if (MODE == kDown) launch_dependents();
+    const int grp = warp % a.groups, kw = warp / a.groups, g = lane >> 2;
+    const uint32_t bars = bars0 + 16 * warp * a.slots, slots = slots0 + warp * a.slots * S::kBytes;
+    int slot = 0, phase = 0, taken = 0, buf = 0;
+    bool alive = true;
+    int finished_tile = -1, finished = 0;  // kDown: units of one tile whose parts this CTA has written
 
-    int slot = 0, phase = 0, buf = 0;
-    auto stream = [&](auto& acc, int seg_first, int count, int u) {
-        // the rows of x of this segment, in the sliced arrays
+    // kDown: counts them, and the CTA that completes a tile sums it for every row of x
+    auto settle = [&]() {
+        if (MODE != kDown || !a.done || finished == 0) return;
+        compute_sync();
+        if (threadIdx.x == 0) {
+            __threadfence();
+            s_last = atomicAdd(a.done + finished_tile, (unsigned)finished) + finished == (unsigned)nseg;
+            __threadfence();
+        }
+        compute_sync();
+        if (s_last) {
+            for (int i = threadIdx.x; i < unit_rows * a.rows; i += 32 * kImmaWarps) {
+                const int o = finished_tile * unit_rows + i % unit_rows, x = i / unit_rows;
+                if (o < a.out) a.y[(size_t)x * a.out + o] = combine(a, x, o);
+            }
+        }
+        finished = 0;
+    };
+
+    auto run_unit = [&](auto& acc, const Sliced& in, int first, int count, int u, int e, int r0, int r1) {
+        using Acc = typename std::remove_reference<decltype(acc)>::type;
+        (void)in;
+        const int tile = tile_of(u);
         acc.init(a, count, lane, [&](int r) -> int {
-            if (MODE == kPair) return __ldcg(a.order + seg_first + r) / a.top_k;
-            return seg_first + r;
+            if (MODE == kPair) return __ldcg(a.order + first + r) / a.top_k;
+            return first + r;
         });
-        const int g = lane >> 2;
-        const long long off0 = ALN ? 0 : unit_row(u) * a.row_bytes;  // for the byte shift of each row in its window
-        for (int c = kw; c < steps; c += kws) {
+        for (int r = r0; r < r1; ++r) {
+            const int c = r * kws + kw;
+            if (c >= steps) break;
             const uint32_t at = slots + slot * S::kBytes;
-            uint32_t r0, r1;
-            (void)off0;
-            if constexpr (ALN) {
-                r0 = at + g * S::kBoxBytes;
-                r1 = r0 + 8 * S::kBoxBytes;
-            } else {
-                const long long o = off0 + (long long)c * chunk_bytes(F);
-                const uintptr_t w0 = reinterpret_cast<uintptr_t>(a.w[0]) + o;
-                const uintptr_t w1 = MODE == kPair ? reinterpret_cast<uintptr_t>(a.w[1]) + o : w0 + 8 * a.row_bytes;
-                r0 = at + g * S::kPitch + (uint32_t)((w0 + g * a.row_bytes) & 15);
-                r1 = at + (g + 8) * S::kPitch + (uint32_t)((w1 + g * a.row_bytes) & 15);
+            uint32_t shift[2] = {0, 0};
+            if constexpr (!ALN) {
+                // where each row starts in its window
+                const long long off = ((long long)e * a.out + (long long)tile * unit_rows + grp * (MODE == kPair ? 16 : 32)) *
+                                          a.row_bytes +
+                                      (long long)c * chunk_bytes(F);
+                shift[0] = (uint32_t)((reinterpret_cast<uintptr_t>(a.w[0]) + off) & 15);
+                shift[1] = (uint32_t)((reinterpret_cast<uintptr_t>(a.w[MODE == kPair ? 1 : 0]) + off) & 15);
             }
-            acc.template step<ALN>(a, c * kChunkBlocks, r0, r1, lane, [&]() {
-                if constexpr (ALN) {
-                    if (alive && !__all_sync(0xffffffffu, mbar_wait(bars + 8 * slot, phase))) {
+            acc.template step<ALN>(
+                a, c * kChunkBlocks, a.bpr - c * kChunkBlocks, lane,
+                [&]() {
+                    if (alive && !__all_sync(0xffffffffu, mbar_wait(bars + 16 * slot, phase))) {
                         alive = false;
-                        lost = in_flight, lost_slot = slot, lost_phase = phase;
-                        if (lane == 0) report_error(a.err, 30);
+                        if (lane == 0) report_error(a.err, 30), *(volatile int*)&s_dead = 1;
                     }
-                } else {
-                    // fetch() commits one group per step, so at most slots - 1 newer groups are in flight
-                    switch (a.slots) {
-                        case 2: asm volatile("cp.async.wait_group 1;" ::: "memory"); break;
-                        case 3: asm volatile("cp.async.wait_group 2;" ::: "memory"); break;
-                        default: asm volatile("cp.async.wait_group 3;" ::: "memory"); break;
-                    }
-                    __syncwarp();
-                }
-            });
+                },
+                [&](int j, int q) -> uint32_t {
+                    // slot row of strip j's row g + 8 q
+                    const int row = MODE == kPair ? 16 * q + 8 * j + g : 16 * j + 8 * q + g;
+                    if constexpr (ALN) return at + row * S::kPitch;
+                    const int in_matrix = MODE == kPair ? 8 * j + g : row;
+                    return at + row * S::kPitch + ((shift[MODE == kPair ? q : 0] + (uint32_t)(in_matrix * (a.row_bytes & 15))) & 15);
+                });
             __syncwarp();
-            --in_flight;
-            if (++slot == a.slots) {
-                slot = 0;
-                phase ^= 1;
-            }
-            fetch();
+            if (alive) ++taken;
+            if (lane == 0) mbar_arrive(bars + 16 * slot + 8);
+            if (++slot == a.slots) slot = 0, phase ^= 1;
         }
 
-        using Acc = typename std::remove_reference<decltype(acc)>::type;
-        const int tile = u / nseg;
-#pragma unroll 1
-        for (int sub = 0; sub < Acc::kSubs; ++sub) {
-            if (sub * 8 >= count) break;
-            float* rb = red + buf * kRedFloats;
-            buf ^= 1;
-            acc.store(rb + warp * 128, sub, lane);
-            __syncthreads();
-            const int n = count - 8 * sub < 8 ? count - 8 * sub : 8;
+        // one row of x's sums of this unit: get(row of the tile as the slots have it)
+        auto epilogue = [&](int sub, int n, auto get) {
             if (MODE == kPair) {
-                // warp w: row w of x, a block of 32 hidden values, lane l at the K position l of the next product
-                if (warp < n) {
-                    const int el = imma_element(a.next_fmt, tile & 1, lane);
-                    const float* p = rb + (el >> 3) * 128 + warp * 16 + (el & 7);
-                    float gate = 0.0f, up = 0.0f;
-                    for (int k = 0; k < kws; ++k) {
-                        gate += p[k * a.strips * 128];
-                        up += p[k * a.strips * 128 + 8];
-                    }
-                    const float h = tile * 32 + el < a.out ? silu_mul(gate, up) : 0.0f;
-                    const size_t at = (size_t)(seg_first + 8 * sub + warp) * a.next_bprp + tile;
-                    slice_block(h, a.hdig + at * kDigitBytes, a.hscale + at, a.hsum + at, lane);
+                // a warp takes a block of 32 hidden values of one row of x, in the lane order of the next product
+                const int blocks = a.groups / 2;
+                for (int i = warp; i < n * blocks; i += kImmaWarps) {
+                    const int tok = i / blocks, b = tile * blocks + i % blocks;
+                    if (32 * b >= a.out) continue;
+                    const bool few = count <= a.few;
+                    const int el = few ? imma_element(a.next_fmt, b & 1, lane) : half_element(a.next_fmt, b & 1, lane);
+                    const int loc = 32 * (i % blocks) + el;
+                    const int row = (loc >> 4) * 32 + (loc & 15);
+                    const float h = 32 * b + el < a.out ? silu_mul(get(tok, row), get(tok, row + 16)) : 0.0f;
+                    const size_t at = (size_t)(first + 8 * sub + tok) * a.next_bprp + b;
+                    if (few)
+                        slice_digits(h, a.h.data + at * kSlicedBytes, a.h.scale + at, a.h.sum + at, lane);
+                    else
+                        slice_halves(h, a.h.data + at * kSlicedBytes, a.h.scale + at, a.h.sum + at, lane);
                 }
             } else {
-                const int rows = 16 * a.strips;
-                for (int i = threadIdx.x; i < rows * n; i += blockDim.x) {
-                    const int tok = i / rows, row = i % rows;
-                    const int o = tile * rows + row;
+                for (int i = threadIdx.x; i < unit_rows * n; i += 32 * kImmaWarps) {
+                    const int tok = i / unit_rows, row = i % unit_rows;
+                    const int o = tile * unit_rows + row;
                     if (o >= a.out) continue;
-                    float v = 0.0f;
-                    for (int k = 0; k < kws; ++k)
-                        v += rb[(k * a.strips + (row >> 4)) * 128 + tok * 16 + (row & 15)];
-                    const int r = seg_first + 8 * sub + tok;
+                    float v = get(tok, row);
+                    const int r = first + 8 * sub + tok;
                     if (MODE == kDown) {
                         a.part[(size_t)__ldcg(a.order + r) * a.out + o] = v;
                     } else {
@@ -461,71 +574,110 @@ __global__ void __launch_bounds__(32 * kImmaWarps, 2)
                     }
                 }
             }
+        };
+
+        const bool whole = r0 == 0 && r1 == per_unit;
+        const int slot_rows = 32 * a.groups;
+        const size_t split_size = (size_t)a.split_tokens * slot_rows;
+        int a0 = 0, a1 = 0;
+        if (!whole) {
+            a0 = deal.owner((long long)u * per_unit);
+            a1 = deal.owner((long long)u * per_unit + per_unit - 1);
         }
-        if (MODE == kDown && a.done) {
-            // the CTA that finishes a row tile last sums it for every row of x
-            __syncthreads();
+        // a CTA's tail slot holds the unit that starts in its range, its head slot the one that started before
+        float* mine = a.split + ((size_t)2 * blockIdx.x + ((int)blockIdx.x == a0 ? 1 : 0)) * split_size;
+#pragma unroll 1
+        for (int sub = 0; sub < Acc::kSubs; ++sub) {
+            if (sub * 8 >= count) break;
+            const int n = count - 8 * sub < 8 ? count - 8 * sub : 8;
+            float* rb = red + buf * kRedFloats;
+            buf ^= 1;
+            acc.store(sub, lane, [&](int tok, int j, int q, float v) {
+                const int row = MODE == kPair ? 16 * q + 8 * j + g : 16 * j + 8 * q + g;
+                rb[(warp * 8 + tok) * 32 + row] = v;
+            });
+            compute_sync();
+            auto sum_parts = [&](int tok, int row) {
+                float v = 0.0f;
+                for (int k = 0; k < kws; ++k) v += rb[((k * a.groups + (row >> 5)) * 8 + tok) * 32 + (row & 31)];
+                return v;
+            };
+            if (whole) {
+                epilogue(sub, n, sum_parts);
+            } else {
+                for (int i = threadIdx.x; i < slot_rows * n; i += 32 * kImmaWarps)
+                    mine[(size_t)(8 * sub + i / slot_rows) * slot_rows + i % slot_rows] = sum_parts(i / slot_rows, i % slot_rows);
+            }
+        }
+        bool complete = whole;
+        if (!whole) {
+            compute_sync();
             if (threadIdx.x == 0) {
                 __threadfence();
-                s_last = atomicAdd(a.done + tile, 1u) + 1 == (unsigned)nseg;
+                s_last = atomicAdd(a.split_done + a0, 1u) == (unsigned)(a1 - a0);
                 __threadfence();
             }
-            __syncthreads();
-            if (s_last) {
-                const int rows = 16 * a.strips;
-                for (int i = threadIdx.x; i < rows * a.rows; i += blockDim.x) {
-                    const int o = tile * rows + i % rows, r = i / rows;
-                    if (o < a.out) a.y[(size_t)r * a.out + o] = combine(a, r, o);
-                }
-            }
+            compute_sync();
+            complete = s_last;
+            compute_sync();  // s_last may be written again
+            if (complete)
+                for (int sub = 0; sub * 8 < count; ++sub)
+                    epilogue(sub, count - 8 * sub < 8 ? count - 8 * sub : 8, [&](int tok, int row) {
+                        const size_t at = (size_t)(8 * sub + tok) * slot_rows + row;
+                        float v = __ldcg(a.split + ((size_t)2 * a0 + 1) * split_size + at);
+                        for (int i = a0 + 1; i <= a1; ++i) v += __ldcg(a.split + (size_t)2 * i * split_size + at);
+                        return v;
+                    });
+        }
+        if (MODE == kDown && complete) {
+            finished_tile = tile;
+            ++finished;
         }
     };
 
-    for (int u = blockIdx.x; u < units; u += gridDim.x) {
-        const int seg = u % nseg;
-        int first, count;
+    for (long long t = t0; t < t1;) {
+        const int u = (int)(t / per_unit), r0 = (int)(t % per_unit);
+        const int r1 = t1 - t < per_unit - r0 ? r0 + (int)(t1 - t) : per_unit;
+        t += r1 - r0;
+        const int seg = seg_of(u);
+        int first, count, e = 0;
         if (MODE == kPlain) {
             first = seg * kSegTokens;
             count = a.rows - first < kSegTokens ? a.rows - first : kSegTokens;
         } else {
+            e = __ldcg(&a.segs[seg].expert);
             first = __ldcg(&a.segs[seg].start);
             count = __ldcg(&a.segs[seg].count);
         }
-        if (count <= 2) {
+        if (MODE == kDown && tile_of(u) != finished_tile) settle();
+        if (count <= 2 && count <= a.few) {
             FewRows<F, 1> acc;
-            stream(acc, first, count, u);
-        } else if (count <= 4) {
+            run_unit(acc, a.few_x, first, count, u, e, r0, r1);
+        } else if (count <= 4 && count <= a.few) {
             FewRows<F, 2> acc;
-            stream(acc, first, count, u);
+            run_unit(acc, a.few_x, first, count, u, e, r0, r1);
         } else if (count <= 8) {
             ManyRows<F, 1> acc;
-            stream(acc, first, count, u);
+            run_unit(acc, a.many_x, first, count, u, e, r0, r1);
         } else if (count <= 16) {
             ManyRows<F, 2> acc;
-            stream(acc, first, count, u);
+            run_unit(acc, a.many_x, first, count, u, e, r0, r1);
         } else {
             ManyRows<F, 4> acc;
-            stream(acc, first, count, u);
+            run_unit(acc, a.many_x, first, count, u, e, r0, r1);
         }
     }
+    settle();
     if (MODE == kDown && nseg == 0 && a.done) {
         // no row names an expert
         const size_t n = (size_t)a.rows * a.out;
-        for (size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (size_t)gridDim.x * blockDim.x)
+        for (size_t i = (size_t)blockIdx.x * 32 * kImmaWarps + threadIdx.x; i < n; i += (size_t)gridDim.x * 32 * kImmaWarps)
             a.y[i] = a.residual ? a.residual[i] : 0.0f;
     }
+    __syncthreads();  // the producer has issued its last copy
     // after a wait that ran out, copies may still be in flight: each is waited for once more, bounded
-    if constexpr (ALN) {
-        for (; lost > 0; --lost) {
-            mbar_wait(bars + 8 * lost_slot, lost_phase);
-            if (++lost_slot == a.slots) {
-                lost_slot = 0;
-                lost_phase ^= 1;
-            }
-        }
-    } else {
-        asm volatile("cp.async.wait_all;" ::: "memory");
-    }
+    if (*(volatile int*)&s_dead)
+        for (int i = taken; i < s_issued[warp]; ++i) mbar_wait(bars + 16 * (i % a.slots), (i / a.slots) & 1);
 }
 
 // y from the parts of every pair, for calls with many rows.
@@ -540,9 +692,8 @@ __global__ void combine_kernel(const ImmaArgs a) {
 struct PrepArgs {
     const float* x;
     int rows, in, bpr, bprp, fmt;
-    uint8_t* dig;
-    float* scale;
-    float* sum;
+    Sliced few, many;  // data null: that form is not needed
+    unsigned int* split_done;
     // experts only (ids not null)
     const int32_t* ids;
     int pairs, n_experts;
@@ -552,18 +703,19 @@ struct PrepArgs {
     unsigned int* done;
     int tiles;
     // padding blocks of the sliced h
-    float* hscale;
-    float* hsum;
+    Sliced h;
     int h_bpr, h_bprp;
 };
 
-// Pairs by expert (CTA 0), x in digits (one warp per block).  Latency-bound:
+// Pairs by expert (CTA 0), x sliced (one warp per block).  Latency-bound:
 // a decode call's x is a few KB.
 __global__ void __launch_bounds__(256) prep_kernel(const PrepArgs a) {
     launch_dependents();
     grid_dependency_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     int first = blockIdx.x, ctas = gridDim.x;
+    if (blockIdx.x == 0)
+        for (int i = threadIdx.x; i < 2 * kMaxCtas; i += 256) a.split_done[i] = 0;
     if (a.ids) {
         if (blockIdx.x == 0) {
             __shared__ int cnt[MLQ_MOE_MAX_EXPERTS];
@@ -574,8 +726,8 @@ __global__ void __launch_bounds__(256) prep_kernel(const PrepArgs a) {
             const int pad = a.h_bprp - a.h_bpr;
             for (int i = threadIdx.x; i < a.pairs * pad; i += 256) {
                 const size_t at = (size_t)(i / pad) * a.h_bprp + a.h_bpr + i % pad;
-                a.hscale[at] = 0.0f;
-                a.hsum[at] = 0.0f;
+                a.h.scale[at] = 0.0f;
+                a.h.sum[at] = 0.0f;
             }
             __syncthreads();
             for (int p = threadIdx.x; p < a.pairs; p += 256) {
@@ -642,9 +794,15 @@ __global__ void __launch_bounds__(256) prep_kernel(const PrepArgs a) {
     const long long n = (long long)a.rows * a.bprp;
     for (long long i = (long long)first * 8 + warp; i < n; i += (long long)ctas * 8) {
         const int r = (int)(i / a.bprp), b = (int)(i % a.bprp);
-        const int at = b * kQK + imma_element(a.fmt, b & 1, lane);
-        const float v = at < a.in ? a.x[(long long)r * a.in + at] : 0.0f;
-        slice_block(v, a.dig + i * kDigitBytes, a.scale + i, a.sum + i, lane);
+        const float* x = a.x + (long long)r * a.in;
+        if (a.few.data) {
+            const int at = b * kQK + imma_element(a.fmt, b & 1, lane);
+            slice_digits(at < a.in ? x[at] : 0.0f, a.few.data + i * kSlicedBytes, a.few.scale + i, a.few.sum + i, lane);
+        }
+        if (a.many.data) {
+            const int at = b * kQK + half_element(a.fmt, b & 1, lane);
+            slice_halves(at < a.in ? x[at] : 0.0f, a.many.data + i * kSlicedBytes, a.many.scale + i, a.many.sum + i, lane);
+        }
     }
 }
 
@@ -653,13 +811,6 @@ size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 bool aligned_rows(int fmt, const void* w, int bpr) {
     return reinterpret_cast<uintptr_t>(w) % 16 == 0 && (long long)bpr * block_bytes(fmt) % 16 == 0 &&
            encode_fn() != nullptr;
-}
-
-int slot_bytes(int fmt, bool aln) {
-    if (aln) return fmt == kQ8_0 ? Slot<kQ8_0, true>::kBytes : (fmt == kQ4_0 ? Slot<kQ4_0, true>::kBytes
-                                                                             : Slot<kQ4_1, true>::kBytes);
-    return fmt == kQ8_0 ? Slot<kQ8_0, false>::kBytes : (fmt == kQ4_0 ? Slot<kQ4_0, false>::kBytes
-                                                                     : Slot<kQ4_1, false>::kBytes);
 }
 
 template <typename... Params, typename... Args>
@@ -678,60 +829,58 @@ cudaError_t launch_pdl(void (*kernel)(Params...), int grid, int block, size_t sm
     return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
 }
 
+// Ring depth: what the SM's shared memory leaves room for, 2..8.
 template <int F, int MODE, bool ALN>
-cudaError_t launch_one(ImmaArgs a, const ImmaMaps& maps, int grid, size_t smem, cudaStream_t stream) {
+cudaError_t launch_one(ImmaArgs a, int grid, int smem_per_sm, cudaStream_t stream) {
+    using S = Slot<F, ALN>;
     auto k = imma_kernel<F, MODE, ALN>;
-    cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return e;
-    return launch_pdl(k, grid, 32 * kImmaWarps, smem, stream, maps, a);
-}
-
-// Ring depth: what two CTAs per SM leave room for, 2..8 (2..4 without tensor maps).
-template <int MODE>
-cudaError_t launch_imma(int fmt, ImmaArgs a, int sm_count, int smem_per_sm, int max_units, cudaStream_t stream) {
-    const bool aln = aligned_rows(fmt, a.w[0], a.bpr) && (MODE != kPair || aligned_rows(fmt, a.w[1], a.bpr));
-    a.row_bytes = (long long)a.bpr * block_bytes(fmt);
-    const int sb = slot_bytes(fmt, aln);
     const int fixed = 2 * kRedFloats * 4 + 1024 + 256;  // the system's 1 KB per CTA, the static part
-    a.slots = (smem_per_sm / 2 - fixed) / (kImmaWarps * (sb + 8));
-    if (a.slots > (aln ? 8 : 4)) a.slots = aln ? 8 : 4;
+    a.slots = (smem_per_sm - fixed) / (kImmaWarps * (S::kBytes + 16));
+    if (a.slots > 8) a.slots = 8;
     if (a.slots < 2) return cudaErrorInvalidConfiguration;
-    const size_t smem = (size_t)kImmaWarps * a.slots * (sb + 8) + 2 * kRedFloats * 4;
+    const size_t smem = (size_t)kImmaWarps * a.slots * (S::kBytes + 16) + 2 * kRedFloats * 4;
     ImmaMaps maps{};
-    if (aln) {
-        const int box = fmt == kQ8_0 ? 272 : (fmt == kQ4_0 ? 144 : 80);
+    if (ALN) {
         for (int i = 0; i < (MODE == kPair ? 2 : 1); ++i)
             if (!make_map_2d(&maps.m[i], CU_TENSOR_MAP_DATA_TYPE_UINT16, const_cast<uint8_t*>(a.w[i]),
-                             (uint64_t)a.row_bytes / 2, (uint64_t)a.total_rows, (uint64_t)a.row_bytes, box / 2,
-                             MODE == kPair ? 8 : 16, CU_TENSOR_MAP_SWIZZLE_NONE))
+                             (uint64_t)a.row_bytes / 2, (uint64_t)a.total_rows, (uint64_t)a.row_bytes, S::kPitch / 2,
+                             MODE == kPair ? 16 : 32, CU_TENSOR_MAP_SWIZZLE_NONE))
                 return cudaErrorInvalidValue;
     }
-    int grid = 2 * sm_count;
-    if (grid > max_units) grid = max_units;
-    if (grid < 1) grid = 1;
+    cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
+    return launch_pdl(k, grid, kThreads, smem, stream, maps, a);
+}
+
+template <int MODE>
+cudaError_t launch_imma(int fmt, ImmaArgs a, int sm_count, int smem_per_sm, long long max_units, cudaStream_t stream) {
+    const bool aln = aligned_rows(fmt, a.w[0], a.bpr) && (MODE != kPair || aligned_rows(fmt, a.w[1], a.bpr));
+    a.row_bytes = (long long)a.bpr * block_bytes(fmt);
+    const int steps = (a.bpr + kChunkBlocks - 1) / kChunkBlocks, kws = kImmaWarps / a.groups;
+    const long long rounds = max_units * ((steps + kws - 1) / kws);
+    int grid = sm_count < kMaxCtas ? sm_count : kMaxCtas;
+    if (grid > rounds) grid = rounds < 1 ? 1 : (int)rounds;
     switch (fmt) {
         case kQ8_0:
-            return aln ? launch_one<kQ8_0, MODE, true>(a, maps, grid, smem, stream)
-                       : launch_one<kQ8_0, MODE, false>(a, maps, grid, smem, stream);
+            return aln ? launch_one<kQ8_0, MODE, true>(a, grid, smem_per_sm, stream)
+                       : launch_one<kQ8_0, MODE, false>(a, grid, smem_per_sm, stream);
         case kQ4_0:
-            return aln ? launch_one<kQ4_0, MODE, true>(a, maps, grid, smem, stream)
-                       : launch_one<kQ4_0, MODE, false>(a, maps, grid, smem, stream);
+            return aln ? launch_one<kQ4_0, MODE, true>(a, grid, smem_per_sm, stream)
+                       : launch_one<kQ4_0, MODE, false>(a, grid, smem_per_sm, stream);
         default:
-            return aln ? launch_one<kQ4_1, MODE, true>(a, maps, grid, smem, stream)
-                       : launch_one<kQ4_1, MODE, false>(a, maps, grid, smem, stream);
+            return aln ? launch_one<kQ4_1, MODE, true>(a, grid, smem_per_sm, stream)
+                       : launch_one<kQ4_1, MODE, false>(a, grid, smem_per_sm, stream);
     }
 }
 
-// 16-row strips of a unit: no more K parts than there are K steps, then
-// taller units while there are enough of them to spread over the SMs (a
-// taller unit has fewer K parts to add up).
-int choose_strips(int out, int bpr, int nseg, int sm_count) {
+// 32-row groups of a unit: no more K parts than there are K steps, and the
+// tallest tile whose units still give every SM one (a taller unit has fewer
+// K parts to add up and reads its rows of x less often).
+int choose_groups(int out, int bpr, long long nseg, int sm_count, int least) {
     const int steps = (bpr + kChunkBlocks - 1) / kChunkBlocks;
-    int kws = kImmaWarps;
-    while (kws > steps) kws >>= 1;
-    int strips = kImmaWarps / kws;
-    while (strips < 4 && (long long)((out + 32 * strips - 1) / (32 * strips)) * nseg >= 6LL * sm_count) strips *= 2;
-    return strips;
+    int g = 4;
+    while (g > least && kImmaWarps / (g / 2) <= steps && (out + 32 * g - 1) / (32 * g) * nseg < sm_count) g /= 2;
+    return g;
 }
 
 struct Carve {
@@ -742,23 +891,38 @@ struct Carve {
         p += align256(n * sizeof(T));
         return r;
     }
+    Sliced take_sliced(size_t rows, int bprp) {
+        Sliced s;
+        s.data = take<uint8_t>(rows * bprp * kSlicedBytes);
+        s.scale = take<float>(rows * bprp);
+        s.sum = take<float>(rows * bprp);
+        return s;
+    }
 };
 
 size_t sliced_bytes(size_t rows, int bprp) {
-    return align256(rows * bprp * kDigitBytes) + 2 * align256(rows * bprp * sizeof(float));
+    return align256(rows * bprp * kSlicedBytes) + 2 * align256(rows * bprp * sizeof(float));
 }
 
 constexpr int kMaxPairs = 8192;           // pairs of one pass at most
-constexpr size_t kMaxSliced = 1u << 30;   // digit bytes of one pass at most (offsets are 32 bits)
+constexpr size_t kMaxSliced = 1u << 30;   // sliced bytes of one pass at most (offsets are 32 bits)
 constexpr size_t kMaxParts = 1u << 30;    // bytes of the pairs' outputs of one pass at most
 constexpr int kMaxPassRows = 16384;       // rows of one pass of a linear at most
 constexpr int kCombineRows = 32;          // more rows: the sum over slots is a launch of its own
 
+int split_tokens(int rows) { return rows < kSegTokens ? rows : kSegTokens; }
+
+// Two slots per CTA of at most 128 rows, and the counters of two launches.
+size_t split_bytes(int rows) {
+    return align256((size_t)2 * kMaxCtas * split_tokens(rows) * 128 * sizeof(float)) +
+           align256(2 * kMaxCtas * sizeof(unsigned int));
+}
+
 // Rows of x of one pass.
 int experts_pass_rows(const MoeShape& s, int rows, int top_k) {
     long long n = kMaxPairs / top_k;
-    const long long per = (long long)top_k * padded_blocks((s.hidden + kQK - 1) / kQK) * kDigitBytes;
-    const long long perx = (long long)padded_blocks((s.in + kQK - 1) / kQK) * kDigitBytes;
+    const long long per = (long long)top_k * padded_blocks((s.hidden + kQK - 1) / kQK) * kSlicedBytes;
+    const long long perx = (long long)padded_blocks((s.in + kQK - 1) / kQK) * kSlicedBytes;
     const long long cap = (long long)kMaxSliced / (per > perx ? per : perx);
     const long long capp = (long long)kMaxParts / ((long long)top_k * s.out * (long long)sizeof(float));
     if (n > cap) n = cap;
@@ -768,7 +932,7 @@ int experts_pass_rows(const MoeShape& s, int rows, int top_k) {
 }
 
 int linear_pass_rows(int in, int rows) {
-    long long n = (long long)kMaxSliced / ((long long)padded_blocks((in + kQK - 1) / kQK) * kDigitBytes);
+    long long n = (long long)kMaxSliced / ((long long)padded_blocks((in + kQK - 1) / kQK) * kSlicedBytes);
     if (n > kMaxPassRows) n = kMaxPassRows;
     return rows < n ? rows : (int)n;
 }
@@ -778,16 +942,16 @@ int max_segments(int pairs, int n_experts) {
     return full < pairs ? full : pairs;
 }
 
-int down_strips(const MoeShape& s, int rows, int top_k, int sm_count) {
-    const int pairs = rows * top_k;
-    return choose_strips(s.out, (s.hidden + kQK - 1) / kQK, pairs < s.n_experts ? pairs : s.n_experts, sm_count);
+int prep_ctas(long long blocks, int sm_count) {
+    const long long n = (blocks + 7) / 8;
+    return (int)(n < 8LL * sm_count ? n : 8LL * sm_count);
 }
 
 }  // namespace
 
 size_t epilogue_workspace_bytes(int in, int rows) {
-    const int bprp = padded_blocks((in + kQK - 1) / kQK);
-    return sliced_bytes(linear_pass_rows(in, rows), bprp);
+    const int n = linear_pass_rows(in, rows);
+    return sliced_bytes(n, padded_blocks((in + kQK - 1) / kQK)) + split_bytes(n);
 }
 
 cudaError_t launch_linear_epilogue(int fmt, const uint8_t* w, int out, int in, const float* x, int rows,
@@ -801,29 +965,28 @@ cudaError_t launch_linear_epilogue(int fmt, const uint8_t* w, int out, int in, c
         PrepArgs p{};
         p.x = x + (long long)r0 * in;
         p.rows = n, p.in = in, p.bpr = bpr, p.bprp = bprp, p.fmt = fmt;
-        p.dig = c.take<uint8_t>((size_t)n * bprp * kDigitBytes);
-        p.scale = c.take<float>((size_t)n * bprp);
-        p.sum = c.take<float>((size_t)n * bprp);
-        const long long blocks = (long long)n * bprp;
-        cudaError_t e = launch_pdl(prep_kernel, (int)((blocks + 7) / 8 < 8 * sm_count ? (blocks + 7) / 8 : 8 * sm_count),
-                                   256, 0, stream, p);
+        (n <= kFewRows ? p.few : p.many) = c.take_sliced(n, bprp);
+        float* split = c.take<float>((size_t)2 * kMaxCtas * split_tokens(n) * 128);
+        p.split_done = c.take<unsigned int>(2 * kMaxCtas);
+        cudaError_t e = launch_pdl(prep_kernel, prep_ctas((long long)n * bprp, sm_count), 256, 0, stream, p);
         if (e != cudaSuccess) return e;
         ImmaArgs a{};
         a.w[0] = w;
         a.total_rows = out, a.out = out, a.bpr = bpr, a.bprp = bprp;
         const int nseg = (n + kSegTokens - 1) / kSegTokens;
-        a.strips = choose_strips(out, bpr, nseg, sm_count);
-        a.tiles = (out + 16 * a.strips - 1) / (16 * a.strips);
-        a.dig = p.dig, a.scale = p.scale, a.sum = p.sum;
+        a.groups = choose_groups(out, bpr, nseg, sm_count, 1);
+        a.tiles = (out + 32 * a.groups - 1) / (32 * a.groups);
+        a.few = n <= kFewRows ? kFewRows : 0;
+        a.few_x = p.few, a.many_x = p.many;
         a.rows = n;
+        a.split = split, a.split_done = p.split_done, a.split_tokens = split_tokens(n);
         a.bias = ep.bias;
         a.row_scale = ep.row_scale ? ep.row_scale + r0 : nullptr;
         a.residual = ep.residual ? ep.residual + (long long)r0 * out : nullptr;
         a.act = ep.activation;
         a.y = y + (long long)r0 * out;
         a.err = err;
-        const long long units = (long long)nseg * a.tiles;
-        e = launch_imma<kPlain>(fmt, a, sm_count, smem_per_sm, units > INT_MAX ? INT_MAX : (int)units, stream);
+        e = launch_imma<kPlain>(fmt, a, sm_count, smem_per_sm, (long long)nseg * a.tiles, stream);
         if (e != cudaSuccess) return e;
         r0 += n;
     }
@@ -834,8 +997,9 @@ size_t experts_workspace_bytes(const MoeShape& s, int rows, int top_k) {
     const int n = experts_pass_rows(s, rows, top_k), pairs = n * top_k;
     const int bprp = padded_blocks((s.in + kQK - 1) / kQK), hp = padded_blocks((s.hidden + kQK - 1) / kQK);
     return 256 + align256((size_t)max_segments(pairs, s.n_experts) * sizeof(Segment)) +
-           align256((size_t)pairs * sizeof(int)) + align256((size_t)((s.out + 15) / 16) * sizeof(unsigned int)) +
-           sliced_bytes(n, bprp) + sliced_bytes(pairs, hp) + align256((size_t)pairs * s.out * sizeof(float));
+           align256((size_t)pairs * sizeof(int)) + align256((size_t)((s.out + 31) / 32) * sizeof(unsigned int)) +
+           (pairs > kFewRows ? 2 : 1) * sliced_bytes(n, bprp) + sliced_bytes(pairs, hp) +
+           align256((size_t)pairs * s.out * sizeof(float)) + split_bytes(pairs);
 }
 
 cudaError_t launch_experts(const MoeShape& s, const uint8_t* gate, const uint8_t* up, const uint8_t* down,
@@ -848,67 +1012,66 @@ cudaError_t launch_experts(const MoeShape& s, const uint8_t* gate, const uint8_t
     for (int r0 = 0; r0 < rows; r0 += pass) {
         const int n = rows - r0 < pass ? rows - r0 : pass, pairs = n * top_k;
         const int nseg_max = max_segments(pairs, s.n_experts);
-        const int strips = down_strips(s, n, top_k, sm_count);
-        const int tiles = (s.out + 16 * strips - 1) / (16 * strips);
+        const int nseg_likely = pairs < s.n_experts ? pairs : nseg_max;
+        const int groups = choose_groups(s.out, hb, nseg_likely, sm_count, 1);
+        const int tiles = (s.out + 32 * groups - 1) / (32 * groups);
         Carve c{static_cast<uint8_t*>(ws)};
         PrepArgs p{};
         p.nseg = c.take<int>(1);
         p.segs = c.take<Segment>(nseg_max);
         p.order = c.take<int>(pairs);
-        p.done = c.take<unsigned int>((s.out + 15) / 16);
+        p.done = c.take<unsigned int>((s.out + 31) / 32);
         p.tiles = tiles;
         p.x = x + (long long)r0 * s.in;
         p.rows = n, p.in = s.in, p.bpr = bpr, p.bprp = bprp, p.fmt = s.fmt;
-        p.dig = c.take<uint8_t>((size_t)n * bprp * kDigitBytes);
-        p.scale = c.take<float>((size_t)n * bprp);
-        p.sum = c.take<float>((size_t)n * bprp);
+        p.few = c.take_sliced(n, bprp);
+        if (pairs > kFewRows) p.many = c.take_sliced(n, bprp);  // a row may name an expert more than once
         p.ids = ids + (long long)r0 * top_k;
         p.pairs = pairs, p.n_experts = s.n_experts;
-        uint8_t* hdig = c.take<uint8_t>((size_t)pairs * hp * kDigitBytes);
-        p.hscale = c.take<float>((size_t)pairs * hp);
-        p.hsum = c.take<float>((size_t)pairs * hp);
+        p.h = c.take_sliced(pairs, hp);
         p.h_bpr = hb, p.h_bprp = hp;
         float* part = c.take<float>((size_t)pairs * s.out);
-        const long long blocks = (long long)n * bprp;
-        cudaError_t e =
-            launch_pdl(prep_kernel, 1 + (int)((blocks + 7) / 8 < 8 * sm_count ? (blocks + 7) / 8 : 8 * sm_count), 256, 0,
-                       stream, p);
+        float* split = c.take<float>((size_t)2 * kMaxCtas * split_tokens(pairs) * 128);
+        p.split_done = c.take<unsigned int>(2 * kMaxCtas);
+        cudaError_t e = launch_pdl(prep_kernel, 1 + prep_ctas((long long)n * bprp, sm_count), 256, 0, stream, p);
         if (e != cudaSuccess) return e;
 
         ImmaArgs a{};
         a.w[0] = gate, a.w[1] = up;
         a.total_rows = (long long)s.n_experts * s.hidden;
         a.out = s.hidden, a.bpr = bpr, a.bprp = bprp;
-        a.strips = 4;
-        a.tiles = (s.hidden + 31) / 32;
-        a.dig = p.dig, a.scale = p.scale, a.sum = p.sum;
+        a.groups = choose_groups(2 * s.hidden, bpr, nseg_likely, sm_count, 2);
+        a.tiles = (s.hidden + 16 * a.groups - 1) / (16 * a.groups);
+        a.few = kFewRows;
+        a.few_x = p.few, a.many_x = p.many;
         a.segs = p.segs, a.nseg = p.nseg, a.order = p.order;
         a.top_k = top_k, a.rows = n;
         a.next_fmt = s.fmt_down, a.next_bprp = hp;
-        a.hdig = hdig, a.hscale = p.hscale, a.hsum = p.hsum;
+        a.h = p.h;
+        a.split = split, a.split_done = p.split_done, a.split_tokens = split_tokens(pairs);
         a.err = err;
-        long long units = (long long)nseg_max * a.tiles;
-        e = launch_imma<kPair>(s.fmt, a, sm_count, smem_per_sm, units > INT_MAX ? INT_MAX : (int)units, stream);
+        e = launch_imma<kPair>(s.fmt, a, sm_count, smem_per_sm, (long long)nseg_max * a.tiles, stream);
         if (e != cudaSuccess) return e;
 
         ImmaArgs d{};
         d.w[0] = down;
         d.total_rows = (long long)s.n_experts * s.out;
         d.out = s.out, d.bpr = hb, d.bprp = hp;
-        d.strips = strips, d.tiles = tiles;
-        d.dig = hdig, d.scale = p.hscale, d.sum = p.hsum;
+        d.groups = groups, d.tiles = tiles;
+        d.few = kFewRows;
+        d.few_x = p.h, d.many_x = p.h;
         d.segs = p.segs, d.nseg = p.nseg, d.order = p.order;
         d.top_k = top_k, d.rows = n;
         d.part = part;
         d.done = n <= kCombineRows ? p.done : nullptr;
+        d.split = split, d.split_done = p.split_done + kMaxCtas, d.split_tokens = split_tokens(pairs);
         d.ids = p.ids;
         d.weights = weights + (long long)r0 * top_k;
         d.n_experts = s.n_experts;
         d.residual = residual ? residual + (long long)r0 * s.out : nullptr;
         d.y = y + (long long)r0 * s.out;
         d.err = err;
-        units = (long long)nseg_max * tiles;
-        e = launch_imma<kDown>(s.fmt_down, d, sm_count, smem_per_sm, units > INT_MAX ? INT_MAX : (int)units, stream);
+        e = launch_imma<kDown>(s.fmt_down, d, sm_count, smem_per_sm, (long long)nseg_max * tiles, stream);
         if (e != cudaSuccess) return e;
         if (!d.done) {
             const long long vals = (long long)n * s.out;

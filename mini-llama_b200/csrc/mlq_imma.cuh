@@ -3,20 +3,24 @@
 //
 // The mathematics.  A weight block is d * c (+ m) with integer codes c, so
 // the sum over one 32-value block is d * sum_i c_i x_i (+ m * sum_i x_i).
-// Activations are carried as 24-bit block fixed point: for each 32-value
-// block of a row of x a power of two s with
-//     x_i = s * (65536 hi_i + 256 mid_i + lo_i),   hi, mid, lo in [-128, 127],
-// rounded once (|error| <= s / 2 <= 2^-23 max|x_block|, at most one bit more
-// than the rounding of fp32 itself).  The codes meet the three digits in
-// m16n8k32 int8 matrix instructions -- one instruction covers exactly one
-// block of 16 weight rows, and every integer sum in it is exact -- and are
-// folded once per block in fp32 with d * s.
+// c_i is exact in 8 bits, x is cut into pieces whose products with c are
+// exact, and one fp32 fold per block applies d and the block's scale of x:
 //
-// Why this form: weights are read once and need no conversion (q8_0 codes are
-// the operand, q4 codes take 3 instructions per 8 weights), so a warp issues
-// ~30 instructions per 512 weights and the kernel is bound by HBM for up to
-// ~8 rows of x per matrix.  The instruction runs at 1 per 2.2 cycles and SM
-// here (1.05 POP/s measured).
+// * up to 4 rows of x: 4 signed base-256 digits of x_i / s, s a power of two
+//   per 32-value block of a row (31-bit fixed point, error <= 2^-31
+//   max|x_block|).  The codes meet the digits in m16n8k32 int8 matrix
+//   instructions: one covers exactly one block of 16 weight rows, its 8 columns are
+//   the digits of 2 rows of x, and every integer sum is exact.  q8_0 codes are
+//   the operand as they are, q4 codes take 3 instructions per 8 weights.
+// * more rows: x_i / s = hi + lo in fp16 (error <= 2^-22 |x_i|, s a power of
+//   two per block), codes as fp16, 4 m16n8k16 instructions per block and 8 rows
+//   into one fp32 accumulator.  One column per row instead of 4, and a fold
+//   of 2 instructions per value instead of 4, for ~20 conversions per block that
+//   many columns share.
+//
+// Both are bound by HBM while an expert has few rows.  The int8 instruction
+// runs at one per 2.2 cycles and SM here (1.05 POP/s measured), the fp16 one
+// too (0.52 PFLOP/s).
 #pragma once
 
 #include <limits.h>
@@ -26,10 +30,11 @@
 
 namespace mlq {
 
-constexpr int kDigitBytes = 96;    // one sliced block: 3 digits x 32 values
+constexpr int kSlicedBytes = 128;  // one sliced block of x: 4 digits, or hi and lo, of 32 values
 constexpr int kChunkBlocks = 8;    // blocks of one K step of a warp
-constexpr int kImmaWarps = 8;      // warps of a CTA
-constexpr int kSegTokens = 32;     // rows of x (tokens) of a segment at most
+constexpr int kImmaWarps = 8;      // warps of a CTA that compute
+constexpr int kSegTokens = 32;     // rows of x of a segment at most
+constexpr int kFewRows = 4;        // rows of x that go by digits
 
 __host__ __device__ inline int padded_blocks(int bpr) { return (bpr + kChunkBlocks - 1) / kChunkBlocks * kChunkBlocks; }
 
@@ -41,10 +46,10 @@ struct Segment {
     int pad;
 };
 
-// Element of a block at position l (0..31) of the matrix instruction's K
-// axis: l = 16 h + 4 t + j is byte j of operand register h of the lanes
-// t mod 4.  The order follows from reading a block as aligned 32-bit words;
-// q8_0 and q4_0 blocks are 2 mod 4 bytes long, so even and odd blocks differ.
+// Element of a block at position l = 16 h + 4 t + j: byte j of the h-th word
+// of codes that the lanes t mod 4 read (q4: h = 0 the low nibbles, 1 the high).
+// The order follows from reading a block as aligned 32-bit words; q8_0 and
+// q4_0 blocks are 2 mod 4 bytes long, so even and odd blocks differ.
 __device__ __forceinline__ int imma_element(int fmt, int odd, int l) {
     const int h = l >> 4, t = (l >> 2) & 3, j = l & 3;
     if (fmt == kQ8_0) {
@@ -56,39 +61,86 @@ __device__ __forceinline__ int imma_element(int fmt, int odd, int l) {
     return l;
 }
 
-// Slices one block: lane l holds the value at K position l.  Writes 96
-// digit bytes, the scale s and the block's sum.  A block with a value that
-// is not finite gets the scale NaN: every output that reads it is NaN.
-__device__ __forceinline__ void slice_block(float v, uint8_t* dig, float* scale, float* sum, int lane) {
-    float amax = fabsf(v);
-    const bool bad = !(amax <= 3.402823466e38f);
-    for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    const bool any_bad = __any_sync(0xffffffffu, bad);
+// The same for the fp16 form: l = 8 t + i, i the lane's i-th value in operand order.
+__device__ __forceinline__ int half_element(int fmt, int odd, int l) {
+    const int t = l >> 3, i = l & 7;
+    const int h = fmt == kQ8_0 ? i >> 2 : (i >> 1) & 1, j = fmt == kQ8_0 ? i & 3 : 2 * (i & 1) + (i >> 2);
+    return imma_element(fmt, odd, 16 * h + 4 * t + j);
+}
+
+// The power of two 2^k whose product with amax is in (limit / 2, limit], as
+// bits; top: floor(log2 limit).  Clamped so that 2^-k is a normal number.
+__device__ __forceinline__ uint32_t block_scale(float amax, int top, float limit) {
     const int eb = (int)(__float_as_uint(amax) >> 23) & 0xff;
-    int sf = 276 - eb;  // exponent field of 2^(22 - floor(log2 amax))
+    int sf = 254 + top - eb;  // exponent field of 2^(top - floor(log2 amax))
     if (sf > 253) sf = 253;
-    if (amax * __uint_as_float((uint32_t)sf << 23) > 8355711.0f) --sf;  // 127 * 65793: three digits hold it
-    int q = any_bad ? 0 : __float2int_rn(v * __uint_as_float((uint32_t)sf << 23));
+    if (amax * __uint_as_float((uint32_t)sf << 23) > limit) --sf;
+    return (uint32_t)sf << 23;
+}
+
+__device__ __forceinline__ float inverse_scale(uint32_t scale) { return __uint_as_float((254u << 23) - scale); }
+
+// Largest magnitude of a block (lanes hold its values); NaN if one is not finite.
+__device__ __forceinline__ float block_amax(float v) {
+    float amax = fabsf(v);
+    const bool bad = __any_sync(0xffffffffu, !(amax <= 3.402823466e38f));
+    for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    return bad ? __uint_as_float(0x7fc00000u) : amax;
+}
+
+__device__ __forceinline__ float warp_sum(float v) {
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+// Slices a block into digits: lane l holds the value at imma_element l.  A
+// block with a value that is not finite gets the scale NaN: every output that
+// reads it is NaN.
+__device__ __forceinline__ void slice_digits(float v, uint8_t* dig, float* scale, float* sum, int lane) {
+    const float amax = block_amax(v);
+    const bool bad = !(amax == amax);
+    const uint32_t s = block_scale(bad ? 0.0f : amax, 30, 2139062016.0f);  // below 127 * 16843009: four digits hold it
+    const int q = bad ? 0 : __float2int_rn(v * __uint_as_float(s));
     const int d0 = (int)(int8_t)(q & 0xff);
     const int q1 = (q - d0) >> 8;
     const int d1 = (int)(int8_t)(q1 & 0xff);
-    const int d2 = (q1 - d1) >> 8;
+    const int q2 = (q1 - d1) >> 8;
+    const int d2 = (int)(int8_t)(q2 & 0xff);
+    const int d3 = (q2 - d2) >> 8;
+    // 4x4 byte transpose among the 4 lanes of a word: lane j stores digit j (0: the highest) of all four
     const int j = lane & 3;
-    uint32_t w2 = (uint32_t)(d2 & 0xff) << (8 * j), w1 = (uint32_t)(d1 & 0xff) << (8 * j),
-             w0 = (uint32_t)(d0 & 0xff) << (8 * j);
-    for (int o = 1; o <= 2; o <<= 1) {
-        w2 |= __shfl_xor_sync(0xffffffffu, w2, o);
-        w1 |= __shfl_xor_sync(0xffffffffu, w1, o);
-        w0 |= __shfl_xor_sync(0xffffffffu, w0, o);
+    const uint32_t w = (uint32_t)(d3 & 0xff) | (uint32_t)(d2 & 0xff) << 8 | (uint32_t)(d1 & 0xff) << 16 |
+                       (uint32_t)(d0 & 0xff) << 24;
+    uint32_t out = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const uint32_t from = __shfl_sync(0xffffffffu, w, (lane & ~3) + k);
+        out |= ((from >> (8 * j)) & 0xffu) << (8 * k);
     }
     const int h = lane >> 4, t = (lane >> 2) & 3;
-    if (j < 3)  // lane j of each four stores digit j (0: hi, 1: mid, 2: lo)
-        *reinterpret_cast<uint32_t*>(dig + j * 32 + t * 8 + h * 4) = j == 0 ? w2 : (j == 1 ? w1 : w0);
-    const int s = __reduce_add_sync(0xffffffffu, q);  // |s| < 2^28
+    *reinterpret_cast<uint32_t*>(dig + j * 32 + t * 8 + h * 4) = out;
+    const float total = warp_sum(v);
     if (lane == 0) {
-        const float inv = any_bad ? __uint_as_float(0x7fc00000u) : __uint_as_float((uint32_t)(254 - sf) << 23);
-        *scale = inv;
-        *sum = (float)s * inv;
+        *scale = bad ? __uint_as_float(0x7fc00000u) : inverse_scale(s);
+        *sum = total;
+    }
+}
+
+// Slices a block into fp16 hi and lo: lane l holds the value at half_element l.
+__device__ __forceinline__ void slice_halves(float v, uint8_t* out, float* scale, float* sum, int lane) {
+    const float amax = block_amax(v);
+    const bool bad = !(amax == amax);
+    const uint32_t s = block_scale(bad ? 0.0f : amax, 14, 32767.0f);
+    const float q = bad ? 0.0f : v * __uint_as_float(s);
+    const __half hi = __float2half_rn(q);
+    const __half lo = __float2half_rn(q - __half2float(hi));
+    __half* o = reinterpret_cast<__half*>(out);
+    o[lane] = hi;
+    o[32 + lane] = lo;
+    const float total = warp_sum(v);
+    if (lane == 0) {
+        *scale = bad ? __uint_as_float(0x7fc00000u) : inverse_scale(s);
+        *sum = total;
     }
 }
 
@@ -99,36 +151,43 @@ __device__ __forceinline__ void imma_s8(int (&c)[4], const uint32_t (&a)[4], uin
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y), "r"(0));
 }
 
-// Facts of a warp's weight slot (16 rows x 8 blocks in shared memory).
+__device__ __forceinline__ void hmma_f16(float (&c)[4], const uint32_t* a, uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Facts of a warp's weight slot (32 rows x 8 blocks in shared memory).
 // Aligned rows come by 2-D TMA boxes; the row pitch is 4 mod 8 words, so the
 // 8 rows x 4 words that a warp reads at a time touch 32 banks (q4_1 takes two
-// boxes of 4 blocks for that).  Other rows come by 16-byte copies of the
-// aligned window around each row, in a pitch with the same property.
+// boxes of 4 blocks for that).  Other rows come one by one, by 1-D copies of
+// the 16-byte aligned window around each, in a pitch with the same property.
 template <int F, bool ALN>
 struct Slot;
 template <>
 struct Slot<kQ8_0, true> {
-    static constexpr int kBoxes = 1, kBoxBytes = 272, kBytes = 16 * 272;
+    static constexpr int kBoxes = 1, kPitch = 272, kBytes = 32 * 272;
 };
 template <>
 struct Slot<kQ4_0, true> {
-    static constexpr int kBoxes = 1, kBoxBytes = 144, kBytes = 16 * 144;
+    static constexpr int kBoxes = 1, kPitch = 144, kBytes = 32 * 144;
 };
 template <>
 struct Slot<kQ4_1, true> {
-    static constexpr int kBoxes = 2, kBoxBytes = 80, kBytes = 2 * 16 * 80;
+    static constexpr int kBoxes = 2, kPitch = 80, kBytes = 2 * 32 * 80;
 };
 template <>
 struct Slot<kQ8_0, false> {
-    static constexpr int kPitch = 304, kBytes = 16 * 304;
+    static constexpr int kBoxes = 1, kPitch = 304, kBytes = 32 * 304;
 };
 template <>
 struct Slot<kQ4_0, false> {
-    static constexpr int kPitch = 176, kBytes = 16 * 176;
+    static constexpr int kBoxes = 1, kPitch = 176, kBytes = 32 * 176;
 };
 template <>
 struct Slot<kQ4_1, false> {
-    static constexpr int kPitch = 176, kBytes = 16 * 176;
+    static constexpr int kBoxes = 1, kPitch = 176, kBytes = 32 * 176;
 };
 
 __host__ __device__ constexpr int chunk_bytes(int f) { return kChunkBlocks * block_bytes(f); }
@@ -145,53 +204,105 @@ __device__ __forceinline__ uint32_t lds_word(uint32_t a) {
     return lds_any(a);
 }
 
-// One block of 16 weight rows as the matrix instruction's A operand, with
-// the rows' scales (rows g and g + 8 of lane 4 g + t).
-struct BlockA {
-    uint32_t a[4];
+__device__ __forceinline__ float low_half(uint32_t w) {
+    return __low2float(*reinterpret_cast<const __half2*>(&w));
+}
+__device__ __forceinline__ float high_half(uint32_t w) {
+    return __high2float(*reinterpret_cast<const __half2*>(&w));
+}
+
+// One block of 16 weight rows (rows g and g + 8 of lane 4 g + t): the lane's
+// words of codes (q4: one word per row) and the rows' scales.
+struct RawA {
+    uint32_t w[2][2];  // [row][word]
     float d[2], m[2];
 };
 
-// q4 codes as signed bytes 16 * (c - 8): one shift and two masks for 8 codes.
-__device__ __forceinline__ void nibbles(uint32_t v, uint32_t& lo, uint32_t& hi) {
-    lo = ((v << 4) & 0xf0f0f0f0u) ^ 0x80808080u;
-    hi = (v & 0xf0f0f0f0u) ^ 0x80808080u;
-}
-
 // Blocks 2p and 2p + 1 of the slot rows at r0 (row g) and r1 (row g + 8).
 template <int F, bool ALN>
-__device__ __forceinline__ void load_pair(uint32_t r0, uint32_t r1, int p, int t, BlockA& even, BlockA& odd) {
+__device__ __forceinline__ void load_pair(uint32_t r0, uint32_t r1, int p, int t, RawA& even, RawA& odd) {
     const uint32_t r[2] = {r0, r1};
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         if (F == kQ8_0) {
             const uint32_t b = r[i] + 68 * p;
             const uint32_t w0 = lds_word<ALN>(b), w8 = lds_word<ALN>(b + 32);
-            even.a[i] = lds_word<ALN>(b + 4 + 4 * t);
+            even.w[i][0] = lds_word<ALN>(b + 4 + 4 * t);
             const uint32_t e1 = lds_word<ALN>(b + 20 + 4 * t);
-            even.a[2 + i] = t == 3 ? __byte_perm(w0, w8, 0x5432) : e1;
-            odd.a[i] = lds_word<ALN>(b + 36 + 4 * t);
-            odd.a[2 + i] = lds_word<ALN>(b + 52 + 4 * t);
-            even.d[i] = half_bits_to_float(w0 & 0xffffu);
-            odd.d[i] = half_bits_to_float(w8 >> 16);
+            even.w[i][1] = t == 3 ? __byte_perm(w0, w8, 0x5432) : e1;
+            odd.w[i][0] = lds_word<ALN>(b + 36 + 4 * t);
+            odd.w[i][1] = lds_word<ALN>(b + 52 + 4 * t);
+            even.d[i] = low_half(w0);
+            odd.d[i] = high_half(w8);
         } else if (F == kQ4_0) {
             const uint32_t b = r[i] + 36 * p;
             const uint32_t w0 = lds_word<ALN>(b), w4 = lds_word<ALN>(b + 16);
             const uint32_t e = lds_word<ALN>(b + 4 + 4 * t);
-            nibbles(t == 3 ? __byte_perm(w0, w4, 0x5432) : e, even.a[i], even.a[2 + i]);
-            nibbles(lds_word<ALN>(b + 20 + 4 * t), odd.a[i], odd.a[2 + i]);
-            even.d[i] = half_bits_to_float(w0 & 0xffffu);
-            odd.d[i] = half_bits_to_float(w4 >> 16);
+            even.w[i][0] = t == 3 ? __byte_perm(w0, w4, 0x5432) : e;
+            odd.w[i][0] = lds_word<ALN>(b + 20 + 4 * t);
+            even.d[i] = low_half(w0);
+            odd.d[i] = high_half(w4);
         } else {
             // aligned: blocks 0..3 in the first box, 4..7 in the second
-            const uint32_t b = ALN ? r[i] + (p >> 1) * (16 * 80) + (p & 1) * 40 : r[i] + 40 * p;
+            const uint32_t b = ALN ? r[i] + (p >> 1) * (32 * 80) + (p & 1) * 40 : r[i] + 40 * p;
             const uint32_t w0 = lds_word<ALN>(b), w5 = lds_word<ALN>(b + 20);
-            nibbles(lds_word<ALN>(b + 4 + 4 * t), even.a[i], even.a[2 + i]);
-            nibbles(lds_word<ALN>(b + 24 + 4 * t), odd.a[i], odd.a[2 + i]);
-            even.d[i] = half_bits_to_float(w0 & 0xffffu);
-            even.m[i] = fmaf(8.0f, even.d[i], half_bits_to_float(w0 >> 16));  // d c + m = d (c - 8) + (m + 8 d)
-            odd.d[i] = half_bits_to_float(w5 & 0xffffu);
-            odd.m[i] = fmaf(8.0f, odd.d[i], half_bits_to_float(w5 >> 16));
+            even.w[i][0] = lds_word<ALN>(b + 4 + 4 * t);
+            odd.w[i][0] = lds_word<ALN>(b + 24 + 4 * t);
+            even.d[i] = low_half(w0);
+            even.m[i] = fmaf(8.0f, even.d[i], high_half(w0));  // d c + m = d (c - 8) + (m + 8 d)
+            odd.d[i] = low_half(w5);
+            odd.m[i] = fmaf(8.0f, odd.d[i], high_half(w5));
+        }
+    }
+}
+
+// The A operand of the int8 instruction.  q4 codes as signed bytes
+// 16 * (c - 8): one shift and two masks for 8 codes.
+template <int F>
+__device__ __forceinline__ void int8_operand(const RawA& r, uint32_t (&a)[4]) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        if (F == kQ8_0) {
+            a[i] = r.w[i][0];
+            a[2 + i] = r.w[i][1];
+        } else {
+            a[i] = ((r.w[i][0] << 4) & 0xf0f0f0f0u) ^ 0x80808080u;
+            a[2 + i] = (r.w[i][0] & 0xf0f0f0f0u) ^ 0x80808080u;
+        }
+    }
+}
+
+__device__ __forceinline__ uint32_t hsub2_bits(uint32_t a, uint32_t b) {
+    const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+__device__ __forceinline__ uint32_t hfma2_bits(uint32_t a, uint32_t b, uint32_t c) {
+    const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b),
+                              *reinterpret_cast<const __half2*>(&c));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+// The A operands of the two fp16 instructions: the code is put under the
+// exponent of 1024 (1024 + c is exact in fp16) and the offset subtracted.
+template <int F>
+__device__ __forceinline__ void half_operand(const RawA& r, uint32_t (&a)[8]) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        if (F == kQ8_0) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const uint32_t u = r.w[i][h] ^ 0x80808080u;  // c + 128
+                a[4 * h + i] = hsub2_bits(__byte_perm(u, 0x64646464u, 0x4140), 0x64806480u);  // - 1152
+                a[4 * h + 2 + i] = hsub2_bits(__byte_perm(u, 0x64646464u, 0x4342), 0x64806480u);
+            }
+        } else {
+            const uint32_t v = r.w[i][0], v8 = v >> 8;
+            // low nibbles: 1024 + c - 1032; high ones: (1024 + 16 c) / 16 - 72
+            a[i] = hsub2_bits((v & 0x000f000fu) | 0x64006400u, 0x64086408u);
+            a[2 + i] = hfma2_bits((v & 0x00f000f0u) | 0x64006400u, 0x2c002c00u, 0xd480d480u);
+            a[4 + i] = hsub2_bits((v8 & 0x000f000fu) | 0x64006400u, 0x64086408u);
+            a[6 + i] = hfma2_bits((v8 & 0x00f000f0u) | 0x64006400u, 0x2c002c00u, 0xd480d480u);
         }
     }
 }

@@ -3,12 +3,16 @@ with an epilogue, with elementwise error bounds of the library's arithmetic
 (test infrastructure).
 
 The bounds follow the arithmetic in include/mlq.h, not a measurement:
-* a value of x in a block with largest magnitude A is off by at most half a
-  step of the 24-bit fixed point, A / 8355711 < 1.01 * 2^-23 A;
-* integer sums of a block are exact; the fp32 steps round by 2^-24 relative
-  each: per block one conversion of the integer sum, one product and one sum,
-  then a few for the parts of the K axis -- counted as (blocks + 16) roundings
-  of the sum of magnitudes (each sum's partial values stay below it)."""
+* a value x in a block with largest magnitude A is carried either as 31-bit
+  fixed point (half a step: below 1.01 * 2^-31 A) or as two fp16 values (each
+  rounding 2^-11 relative: 2^-22 |x|, and at most 2^-39 A where the second is
+  subnormal); the sum of both bounds covers either;
+* integer sums of a block are exact.  The fp32 steps round by 2^-24 relative
+  each: per block one conversion of the integer sum, one product and one sum, then a
+  few for the parts of the K axis -- counted as (blocks + 16) roundings of the sum
+  of magnitudes (each sum's partial values stay below it).  The fp16 form's sums
+  are made by the matrix unit, which may truncate: 4 instructions per
+  block, 2^-22 of that block's magnitudes each, 16 roundings more in all."""
 from __future__ import annotations
 
 import math
@@ -75,9 +79,9 @@ def product(x, fmt, blocks, out, dx=None):
     """x W^T in float64 and its bound; dx: an elementwise error of x already there."""
     w, mag = dequantize64(fmt, blocks, out, x.shape[1])
     xa = np.abs(x) + (0 if dx is None else dx)
-    step = 1.01 * 2.0 ** -23 * block_max(xa)
+    step = 2.0 ** -22 * xa + 1.01 * 2.0 ** -31 * block_max(xa)
     nb = (x.shape[1] + 31) // 32
-    bound = step @ np.abs(w).T + (nb + 16) * EPS * ((xa + step) @ mag.T)
+    bound = step @ np.abs(w).T + (nb + 32) * EPS * ((xa + step) @ mag.T)
     if dx is not None:
         bound = bound + dx @ np.abs(w).T
     return x @ w.T, bound
