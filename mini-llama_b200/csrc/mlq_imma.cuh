@@ -68,6 +68,9 @@ __device__ __forceinline__ int half_element(int fmt, int odd, int l) {
     return imma_element(fmt, odd, 16 * h + 4 * t + j);
 }
 
+// Where block b of a row sliced into digits starts (see slice_digits).
+__host__ __device__ constexpr int digit_block(int b) { return (b >> 1) * 2 * kSlicedBytes + (b & 1) * 8; }
+
 // The power of two 2^k whose product with amax is in (limit / 2, limit], as
 // bits; top: floor(log2 limit).  Clamped so that 2^-k is a normal number.
 __device__ __forceinline__ uint32_t block_scale(float amax, int top, float limit) {
@@ -93,8 +96,9 @@ __device__ __forceinline__ float warp_sum(float v) {
     return v;
 }
 
-// Slices a block into digits: lane l holds the value at imma_element l.  A
-// block with a value that is not finite gets the scale NaN: every output that
+// Slices a block into digits: lane l holds the value at imma_element l.  Two
+// blocks share 256 bytes, [digit][t][block of the pair][word h]; dig is the
+// pair's start plus 8 bytes for the odd block (digit_block).  A block with a value that is not finite gets the scale NaN: every output that
 // reads it is NaN.
 __device__ __forceinline__ void slice_digits(float v, uint8_t* dig, float* scale, float* sum, int lane) {
     const float amax = block_amax(v);
@@ -118,7 +122,7 @@ __device__ __forceinline__ void slice_digits(float v, uint8_t* dig, float* scale
         out |= ((from >> (8 * j)) & 0xffu) << (8 * k);
     }
     const int h = lane >> 4, t = (lane >> 2) & 3;
-    *reinterpret_cast<uint32_t*>(dig + j * 32 + t * 8 + h * 4) = out;
+    *reinterpret_cast<uint32_t*>(dig + j * 64 + t * 16 + h * 4) = out;
     const float total = warp_sum(v);
     if (lane == 0) {
         *scale = bad ? __uint_as_float(0x7fc00000u) : inverse_scale(s);

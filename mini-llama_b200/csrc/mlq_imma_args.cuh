@@ -1,0 +1,98 @@
+// mlq_imma_args.cuh -- what the launches of mlq_imma.cu share.
+#pragma once
+
+#include "mlq_imma.cuh"
+
+namespace mlq {
+
+enum Mode { kPlain = 0, kPair = 1, kDown = 2 };
+
+struct ImmaMaps {
+    CUtensorMap m[2];
+};
+
+// Sliced rows of x or h: [row][bprp][128 bytes], a scale and a sum per block.
+struct Sliced {
+    uint8_t* data;
+    float* scale;
+    float* sum;
+};
+
+struct ImmaArgs {
+    const uint8_t* w[2];      // stacked matrices [n][out][bpr]; [1]: the up projections (kPair)
+    long long row_bytes;      // bytes of a matrix row
+    long long total_rows;     // rows of the whole stack
+    int out;                  // rows of one matrix
+    int bpr, bprp;            // blocks per row, and padded to whole steps
+    int groups;               // 32-row groups of a unit (1, 2 or 4); kPair: 16 gate and 16 up rows each, 2 or 4
+    int tiles;                // row tiles of one matrix
+    int slots;                // ring depth of a warp
+    int few;                  // segments of at most this many rows go by digits
+    Sliced few_x, many_x;     // digits / halves (the same arrays for h: a segment has one form)
+    // segments (kPair, kDown); kPlain: rows in order, one matrix
+    const Segment* segs;
+    const int* nseg;
+    const int* order;         // expert-sorted position -> pair
+    int top_k, rows;
+    // kPair: sliced h by position
+    int next_fmt, next_bprp;
+    Sliced h;
+    // kDown: one value per pair, then the weighed sum
+    float* part;              // [pair][out]
+    unsigned int* done;       // units finished per row tile, zero before the launch; null: a later launch sums
+    const int32_t* ids;
+    const float* weights;
+    int n_experts;
+    // units that several CTAs share
+    float* split;             // [CTA][head, tail][row of x][row of the tile]
+    unsigned int* split_done; // per CTA, zero before the launch
+    int split_tokens;         // rows of x of a split slot
+    // kPlain / kDown
+    const float* bias;
+    const float* row_scale;
+    const float* residual;
+    float* y;
+    int act;
+    int* err;
+};
+
+constexpr int kMaxCtas = 192; // CTAs of a launch at most (split slots)
+
+// y[r][o] = residual[r][o] + sum_j weights[r][j] part[r k + j][o], slots in
+// order; a slot without an expert adds nothing.
+__device__ __forceinline__ float combine(const ImmaArgs& a, int r, int o) {
+    float v = 0.0f;
+    for (int j = 0; j < a.top_k; ++j) {
+        const int p = r * a.top_k + j;
+        const int e = a.ids[p];
+        if (e >= 0 && e < a.n_experts) v = fmaf(a.weights[p], __ldcg(a.part + (size_t)p * a.out + o), v);
+    }
+    const size_t at = (size_t)r * a.out + o;
+    return a.residual ? a.residual[at] + v : v;
+}
+
+template <typename... Params, typename... Args>
+inline cudaError_t launch_pdl(void (*kernel)(Params...), int grid, int block, size_t smem, cudaStream_t stream,
+                       Args&&... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(block);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
+}
+
+// One streaming launch (mlq_imma_{plain,pair,down}.cu).  max_units: an upper bound of its units.
+cudaError_t launch_imma_plain(int fmt, const ImmaArgs& a, int sm_count, int smem_per_sm, long long max_units,
+                              cudaStream_t stream);
+cudaError_t launch_imma_pair(int fmt, const ImmaArgs& a, int sm_count, int smem_per_sm, long long max_units,
+                             cudaStream_t stream);
+cudaError_t launch_imma_down(int fmt, const ImmaArgs& a, int sm_count, int smem_per_sm, long long max_units,
+                             cudaStream_t stream);
+
+}  // namespace mlq
