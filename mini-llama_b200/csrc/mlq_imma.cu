@@ -5,7 +5,7 @@
 //   prep   sorts the (row, slot) pairs by expert into segments of at most 32
 //          and slices x;
 //   pair   h = silu(x Wg^T) * (x Wu^T) per segment, sliced in its epilogue;
-//   down   h Wd^T per segment, weighed and summed per row by the CTA that
+//   down   h Wd^T per segment, weighed and summed per row by the team that
 //          finishes a row tile last (fixed order), or by a fourth launch
 //          when there are many rows;
 // and two (prep, down in its plain form) for the linear with an epilogue.
@@ -26,7 +26,9 @@ __global__ void combine_kernel(const ImmaArgs a) {
 struct PrepArgs {
     const float* x;
     int rows, in, bpr, bprp, fmt;
-    Sliced few, many;  // data null: that form is not needed
+    Sliced sliced;
+    bool few;    // as digits, else as halves
+    int seg_cap; // rows of a segment at most
     unsigned int* split_done;
     // experts only (ids not null)
     const int32_t* ids;
@@ -49,7 +51,7 @@ __global__ void __launch_bounds__(256) prep_kernel(const PrepArgs a) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     int first = blockIdx.x, ctas = gridDim.x;
     if (blockIdx.x == 0)
-        for (int i = threadIdx.x; i < 2 * kMaxCtas; i += 256) a.split_done[i] = 0;
+        for (int i = threadIdx.x; i < 2 * kMaxTeams; i += 256) a.split_done[i] = 0;
     if (a.ids) {
         if (blockIdx.x == 0) {
             __shared__ int cnt[MLQ_MOE_MAX_EXPERTS];
@@ -76,7 +78,7 @@ __global__ void __launch_bounds__(256) prep_kernel(const PrepArgs a) {
                 const int e = threadIdx.x * kPer + i;
                 n[i] = e < a.n_experts ? cnt[e] : 0;
                 np += n[i];
-                ns += (n[i] + kSegTokens - 1) / kSegTokens;
+                ns += (n[i] + a.seg_cap - 1) / a.seg_cap;
             }
             int ip = np, is = ns;
             for (int o = 1; o < 32; o <<= 1) {
@@ -90,8 +92,8 @@ __global__ void __launch_bounds__(256) prep_kernel(const PrepArgs a) {
             for (int i = 0; i < kPer; ++i) {
                 const int e = threadIdx.x * kPer + i;
                 if (e < a.n_experts) cnt[e] = op;
-                for (int k = 0; k < n[i]; k += kSegTokens)
-                    a.segs[os++] = Segment{e, op + k, n[i] - k < kSegTokens ? n[i] - k : kSegTokens, 0};
+                for (int k = 0; k < n[i]; k += a.seg_cap)
+                    a.segs[os++] = Segment{e, op + k, n[i] - k < a.seg_cap ? n[i] - k : a.seg_cap, 0};
                 op += n[i];
             }
             if (threadIdx.x == 255) *a.nseg = os;
@@ -129,27 +131,28 @@ __global__ void __launch_bounds__(256) prep_kernel(const PrepArgs a) {
     for (long long i = (long long)first * 8 + warp; i < n; i += (long long)ctas * 8) {
         const int r = (int)(i / a.bprp), b = (int)(i % a.bprp);
         const float* x = a.x + (long long)r * a.in;
-        if (a.few.data) {
+        if (a.few) {
             const int at = b * kQK + imma_element(a.fmt, b & 1, lane);
-            slice_digits(at < a.in ? x[at] : 0.0f, a.few.data + (i - b) * kSlicedBytes + digit_block(b), a.few.scale + i, a.few.sum + i, lane);
-        }
-        if (a.many.data) {
+            slice_digits(at < a.in ? x[at] : 0.0f, a.sliced.data + (i - b) * kSlicedBytes + digit_block(b),
+                         a.sliced.scale + i, a.sliced.sum + i, lane);
+        } else {
             const int at = b * kQK + half_element(a.fmt, b & 1, lane);
-            slice_halves(at < a.in ? x[at] : 0.0f, a.many.data + i * kSlicedBytes, a.many.scale + i, a.many.sum + i, lane);
+            slice_halves(at < a.in ? x[at] : 0.0f, a.sliced.data + i * kSlicedBytes, a.sliced.scale + i, a.sliced.sum + i,
+                         lane);
         }
     }
 }
 
 size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 
-// 32-row groups of a unit: no more K parts than there are K steps, and the
-// tallest tile whose units still give every SM one (a taller unit has fewer
+// 16-row strips of a unit: no more K parts than there are K steps, and the
+// tallest tile whose units still give every team one (a taller unit has fewer
 // K parts to add up and reads its rows of x less often).
-int choose_groups(int out, int bpr, long long nseg, int sm_count, int least) {
+int choose_strips(int out, int bpr, long long nseg, int sm_count, int least) {
     const int steps = (bpr + kChunkBlocks - 1) / kChunkBlocks;
-    int g = 4;
-    while (g > least && kImmaWarps / (g / 2) <= steps && (out + 32 * g - 1) / (32 * g) * nseg < sm_count) g /= 2;
-    return g;
+    int n = 8;
+    while (n > least && kImmaWarps / (n / 2) <= steps && (out + 16 * n - 1) / (16 * n) * nseg < 2 * sm_count) n /= 2;
+    return n;
 }
 
 struct Carve {
@@ -181,10 +184,10 @@ constexpr int kCombineRows = 32;          // more rows: the sum over slots is a 
 
 int split_tokens(int rows) { return rows < kSegTokens ? rows : kSegTokens; }
 
-// Two slots per CTA of at most 128 rows, and the counters of two launches.
+// Two slots per team of at most 128 rows, and the counters of two launches.
 size_t split_bytes(int rows) {
-    return align256((size_t)2 * kMaxCtas * split_tokens(rows) * 128 * sizeof(float)) +
-           align256(2 * kMaxCtas * sizeof(unsigned int));
+    return align256((size_t)2 * kMaxTeams * split_tokens(rows) * 128 * sizeof(float)) +
+           align256(2 * kMaxTeams * sizeof(unsigned int));
 }
 
 // Rows of x of one pass.
@@ -206,10 +209,16 @@ int linear_pass_rows(int in, int rows) {
     return rows < n ? rows : (int)n;
 }
 
-int max_segments(int pairs, int n_experts) {
-    const int full = pairs / kSegTokens + (pairs < n_experts ? pairs : n_experts);
+int max_segments(int pairs, int n_experts, int cap) {
+    const int full = pairs / cap + (pairs < n_experts ? pairs : n_experts);
     return full < pairs ? full : pairs;
 }
+
+// Whether a call's rows of x go by digits, in segments of at most 4: while an
+// expert has about two rows its weights' way from HBM takes longer than any
+// work on them; an expert with more rows has several segments, whose weights
+// come from L2 after the first.
+bool few_rows(int pairs, int n_experts) { return pairs <= 2 * n_experts || pairs <= kFewRows; }
 
 int prep_ctas(long long blocks, int sm_count) {
     const long long n = (blocks + 7) / 8;
@@ -234,19 +243,21 @@ cudaError_t launch_linear_epilogue(int fmt, const uint8_t* w, int out, int in, c
         PrepArgs p{};
         p.x = x + (long long)r0 * in;
         p.rows = n, p.in = in, p.bpr = bpr, p.bprp = bprp, p.fmt = fmt;
-        (n <= kFewRows ? p.few : p.many) = c.take_sliced(n, bprp);
-        float* split = c.take<float>((size_t)2 * kMaxCtas * split_tokens(n) * 128);
-        p.split_done = c.take<unsigned int>(2 * kMaxCtas);
+        p.few = n <= kFewRows;
+        p.sliced = c.take_sliced(n, bprp);
+        float* split = c.take<float>((size_t)2 * kMaxTeams * split_tokens(n) * 128);
+        p.split_done = c.take<unsigned int>(2 * kMaxTeams);
         cudaError_t e = launch_pdl(prep_kernel, prep_ctas((long long)n * bprp, sm_count), 256, 0, stream, p);
         if (e != cudaSuccess) return e;
         ImmaArgs a{};
         a.w[0] = w;
         a.total_rows = out, a.out = out, a.bpr = bpr, a.bprp = bprp;
-        const int nseg = (n + kSegTokens - 1) / kSegTokens;
-        a.groups = choose_groups(out, bpr, nseg, sm_count, 1);
-        a.tiles = (out + 32 * a.groups - 1) / (32 * a.groups);
-        a.few = n <= kFewRows ? kFewRows : 0;
-        a.few_x = p.few, a.many_x = p.many;
+        a.few = p.few;
+        a.seg_cap = p.few ? kFewRows : kSegTokens;
+        const int nseg = (n + a.seg_cap - 1) / a.seg_cap;
+        a.strips = choose_strips(out, bpr, nseg, sm_count, 1);
+        a.tiles = (out + 16 * a.strips - 1) / (16 * a.strips);
+        a.x = p.sliced;
         a.rows = n;
         a.split = split, a.split_done = p.split_done, a.split_tokens = split_tokens(n);
         a.bias = ep.bias;
@@ -265,9 +276,9 @@ cudaError_t launch_linear_epilogue(int fmt, const uint8_t* w, int out, int in, c
 size_t experts_workspace_bytes(const MoeShape& s, int rows, int top_k) {
     const int n = experts_pass_rows(s, rows, top_k), pairs = n * top_k;
     const int bprp = padded_blocks((s.in + kQK - 1) / kQK), hp = padded_blocks((s.hidden + kQK - 1) / kQK);
-    return 256 + align256((size_t)max_segments(pairs, s.n_experts) * sizeof(Segment)) +
-           align256((size_t)pairs * sizeof(int)) + align256((size_t)((s.out + 31) / 32) * sizeof(unsigned int)) +
-           (pairs > kFewRows ? 2 : 1) * sliced_bytes(n, bprp) + sliced_bytes(pairs, hp) +
+    return 256 + align256((size_t)max_segments(pairs, s.n_experts, few_rows(pairs, s.n_experts) ? kFewRows : kSegTokens) * sizeof(Segment)) +
+           align256((size_t)pairs * sizeof(int)) + align256((size_t)((s.out + 15) / 16) * sizeof(unsigned int)) +
+           sliced_bytes(n, bprp) + sliced_bytes(pairs, hp) +
            align256((size_t)pairs * s.out * sizeof(float)) + split_bytes(pairs);
 }
 
@@ -280,28 +291,30 @@ cudaError_t launch_experts(const MoeShape& s, const uint8_t* gate, const uint8_t
     const int hb = (s.hidden + kQK - 1) / kQK, hp = padded_blocks(hb);
     for (int r0 = 0; r0 < rows; r0 += pass) {
         const int n = rows - r0 < pass ? rows - r0 : pass, pairs = n * top_k;
-        const int nseg_max = max_segments(pairs, s.n_experts);
+        const bool few = few_rows(pairs, s.n_experts);
+        const int cap = few ? kFewRows : kSegTokens;
+        const int nseg_max = max_segments(pairs, s.n_experts, cap);
         const int nseg_likely = pairs < s.n_experts ? pairs : nseg_max;
-        const int groups = choose_groups(s.out, hb, nseg_likely, sm_count, 1);
-        const int tiles = (s.out + 32 * groups - 1) / (32 * groups);
+        const int strips = choose_strips(s.out, hb, nseg_likely, sm_count, 1);
+        const int tiles = (s.out + 16 * strips - 1) / (16 * strips);
         Carve c{static_cast<uint8_t*>(ws)};
         PrepArgs p{};
         p.nseg = c.take<int>(1);
         p.segs = c.take<Segment>(nseg_max);
         p.order = c.take<int>(pairs);
-        p.done = c.take<unsigned int>((s.out + 31) / 32);
+        p.done = c.take<unsigned int>((s.out + 15) / 16);
         p.tiles = tiles;
         p.x = x + (long long)r0 * s.in;
         p.rows = n, p.in = s.in, p.bpr = bpr, p.bprp = bprp, p.fmt = s.fmt;
-        p.few = c.take_sliced(n, bprp);
-        if (pairs > kFewRows) p.many = c.take_sliced(n, bprp);  // a row may name an expert more than once
+        p.few = few, p.seg_cap = cap;
+        p.sliced = c.take_sliced(n, bprp);
         p.ids = ids + (long long)r0 * top_k;
         p.pairs = pairs, p.n_experts = s.n_experts;
         p.h = c.take_sliced(pairs, hp);
         p.h_bpr = hb, p.h_bprp = hp;
         float* part = c.take<float>((size_t)pairs * s.out);
-        float* split = c.take<float>((size_t)2 * kMaxCtas * split_tokens(pairs) * 128);
-        p.split_done = c.take<unsigned int>(2 * kMaxCtas);
+        float* split = c.take<float>((size_t)2 * kMaxTeams * split_tokens(pairs) * 128);
+        p.split_done = c.take<unsigned int>(2 * kMaxTeams);
         cudaError_t e = launch_pdl(prep_kernel, 1 + prep_ctas((long long)n * bprp, sm_count), 256, 0, stream, p);
         if (e != cudaSuccess) return e;
 
@@ -309,10 +322,10 @@ cudaError_t launch_experts(const MoeShape& s, const uint8_t* gate, const uint8_t
         a.w[0] = gate, a.w[1] = up;
         a.total_rows = (long long)s.n_experts * s.hidden;
         a.out = s.hidden, a.bpr = bpr, a.bprp = bprp;
-        a.groups = choose_groups(2 * s.hidden, bpr, nseg_likely, sm_count, 2);
-        a.tiles = (s.hidden + 16 * a.groups - 1) / (16 * a.groups);
-        a.few = kFewRows;
-        a.few_x = p.few, a.many_x = p.many;
+        a.strips = choose_strips(2 * s.hidden, bpr, nseg_likely, sm_count, 4);
+        a.tiles = (s.hidden + 8 * a.strips - 1) / (8 * a.strips);
+        a.few = few, a.seg_cap = cap;
+        a.x = p.sliced;
         a.segs = p.segs, a.nseg = p.nseg, a.order = p.order;
         a.top_k = top_k, a.rows = n;
         a.next_fmt = s.fmt_down, a.next_bprp = hp;
@@ -326,14 +339,14 @@ cudaError_t launch_experts(const MoeShape& s, const uint8_t* gate, const uint8_t
         d.w[0] = down;
         d.total_rows = (long long)s.n_experts * s.out;
         d.out = s.out, d.bpr = hb, d.bprp = hp;
-        d.groups = groups, d.tiles = tiles;
-        d.few = kFewRows;
-        d.few_x = p.h, d.many_x = p.h;
+        d.strips = strips, d.tiles = tiles;
+        d.few = few, d.seg_cap = cap;
+        d.x = p.h;
         d.segs = p.segs, d.nseg = p.nseg, d.order = p.order;
         d.top_k = top_k, d.rows = n;
         d.part = part;
         d.done = n <= kCombineRows ? p.done : nullptr;
-        d.split = split, d.split_done = p.split_done + kMaxCtas, d.split_tokens = split_tokens(pairs);
+        d.split = split, d.split_done = p.split_done + kMaxTeams, d.split_tokens = split_tokens(pairs);
         d.ids = p.ids;
         d.weights = weights + (long long)r0 * top_k;
         d.n_experts = s.n_experts;

@@ -162,7 +162,7 @@ __device__ __forceinline__ void hmma_f16(float (&c)[4], const uint32_t* a, uint3
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Facts of a warp's weight slot (32 rows x 8 blocks in shared memory).
+// Facts of a warp's weight slot (16 rows x 8 blocks in shared memory).
 // Aligned rows come by 2-D TMA boxes; the row pitch is 4 mod 8 words, so the
 // 8 rows x 4 words that a warp reads at a time touch 32 banks (q4_1 takes two
 // boxes of 4 blocks for that).  Other rows come one by one, by 1-D copies of
@@ -171,27 +171,27 @@ template <int F, bool ALN>
 struct Slot;
 template <>
 struct Slot<kQ8_0, true> {
-    static constexpr int kBoxes = 1, kPitch = 272, kBytes = 32 * 272;
+    static constexpr int kBoxes = 1, kPitch = 272, kBytes = 16 * 272;
 };
 template <>
 struct Slot<kQ4_0, true> {
-    static constexpr int kBoxes = 1, kPitch = 144, kBytes = 32 * 144;
+    static constexpr int kBoxes = 1, kPitch = 144, kBytes = 16 * 144;
 };
 template <>
 struct Slot<kQ4_1, true> {
-    static constexpr int kBoxes = 2, kPitch = 80, kBytes = 2 * 32 * 80;
+    static constexpr int kBoxes = 2, kPitch = 80, kBytes = 2 * 16 * 80;
 };
 template <>
 struct Slot<kQ8_0, false> {
-    static constexpr int kBoxes = 1, kPitch = 304, kBytes = 32 * 304;
+    static constexpr int kBoxes = 1, kPitch = 304, kBytes = 16 * 304;
 };
 template <>
 struct Slot<kQ4_0, false> {
-    static constexpr int kBoxes = 1, kPitch = 176, kBytes = 32 * 176;
+    static constexpr int kBoxes = 1, kPitch = 176, kBytes = 16 * 176;
 };
 template <>
 struct Slot<kQ4_1, false> {
-    static constexpr int kBoxes = 1, kPitch = 176, kBytes = 32 * 176;
+    static constexpr int kBoxes = 1, kPitch = 176, kBytes = 16 * 176;
 };
 
 __host__ __device__ constexpr int chunk_bytes(int f) { return kChunkBlocks * block_bytes(f); }
@@ -248,7 +248,7 @@ __device__ __forceinline__ void load_pair(uint32_t r0, uint32_t r1, int p, int t
             odd.d[i] = high_half(w4);
         } else {
             // aligned: blocks 0..3 in the first box, 4..7 in the second
-            const uint32_t b = ALN ? r[i] + (p >> 1) * (32 * 80) + (p & 1) * 40 : r[i] + 40 * p;
+            const uint32_t b = ALN ? r[i] + (p >> 1) * (16 * 80) + (p & 1) * 40 : r[i] + 40 * p;
             const uint32_t w0 = lds_word<ALN>(b), w5 = lds_word<ALN>(b + 20);
             even.w[i][0] = lds_word<ALN>(b + 4 + 4 * t);
             odd.w[i][0] = lds_word<ALN>(b + 24 + 4 * t);

@@ -24,11 +24,12 @@ struct ImmaArgs {
     long long total_rows;     // rows of the whole stack
     int out;                  // rows of one matrix
     int bpr, bprp;            // blocks per row, and padded to whole steps
-    int groups;               // 32-row groups of a unit (1, 2 or 4); kPair: 16 gate and 16 up rows each, 2 or 4
+    int strips;               // 16-row strips of a unit (1, 2, 4 or 8); kPair: 8 gate and 8 up rows each, 4 or 8
     int tiles;                // row tiles of one matrix
     int slots;                // ring depth of a warp
-    int few;                  // segments of at most this many rows go by digits
-    Sliced few_x, many_x;     // digits / halves (the same arrays for h: a segment has one form)
+    bool few;                 // the launch's rows of x are digits (else halves)
+    int seg_cap;              // rows of x of a segment at most
+    Sliced x;                 // rows of x or h
     // segments (kPair, kDown); kPlain: rows in order, one matrix
     const Segment* segs;
     const int* nseg;
@@ -43,9 +44,9 @@ struct ImmaArgs {
     const int32_t* ids;
     const float* weights;
     int n_experts;
-    // units that several CTAs share
-    float* split;             // [CTA][head, tail][row of x][row of the tile]
-    unsigned int* split_done; // per CTA, zero before the launch
+    // units that several teams share
+    float* split;             // [team][head, tail][row of x][row of the tile]
+    unsigned int* split_done; // per team, zero before the launch
     int split_tokens;         // rows of x of a split slot
     // kPlain / kDown
     const float* bias;
@@ -56,7 +57,7 @@ struct ImmaArgs {
     int* err;
 };
 
-constexpr int kMaxCtas = 192; // CTAs of a launch at most (split slots)
+constexpr int kMaxTeams = 320;  // teams of a launch at most (split slots)
 
 // y[r][o] = residual[r][o] + sum_j weights[r][j] part[r k + j][o], slots in
 // order; a slot without an expert adds nothing.
