@@ -196,16 +196,20 @@ struct Slot<kQ4_1, false> {
 
 __host__ __device__ constexpr int chunk_bytes(int f) { return kChunkBlocks * block_bytes(f); }
 
-// Four bytes at any byte address of shared memory.
-__device__ __forceinline__ uint32_t lds_any(uint32_t a) {
-    const uint32_t lo = lds_u32(a & ~3u), hi = lds_u32((a & ~3u) + 4);
-    return __funnelshift_r(lo, hi, 8 * (a & 3));
-}
-
-template <bool ALN>
+// The word OFF bytes after `a` in shared memory; a is 4-byte aligned where ALN.
+template <bool ALN, int OFF>
 __device__ __forceinline__ uint32_t lds_word(uint32_t a) {
-    if (ALN) return lds_u32(a);
-    return lds_any(a);
+    uint32_t lo;
+    if constexpr (ALN) {
+        asm volatile("ld.shared.u32 %0, [%1+%2];" : "=r"(lo) : "r"(a), "n"(OFF));
+        return lo;
+    } else {
+        uint32_t hi;
+        const uint32_t w = a & ~3u;
+        asm volatile("ld.shared.u32 %0, [%1+%2];" : "=r"(lo) : "r"(w), "n"(OFF));
+        asm volatile("ld.shared.u32 %0, [%1+%2];" : "=r"(hi) : "r"(w), "n"(OFF + 4));
+        return __funnelshift_r(lo, hi, 8 * (a & 3));
+    }
 }
 
 __device__ __forceinline__ float low_half(uint32_t w) {
@@ -222,36 +226,45 @@ struct RawA {
     float d[2], m[2];
 };
 
-// Blocks 2p and 2p + 1 of the slot rows at r0 (row g) and r1 (row g + 8).
-template <int F, bool ALN>
-__device__ __forceinline__ void load_pair(uint32_t r0, uint32_t r1, int p, int t, RawA& even, RawA& odd) {
-    const uint32_t r[2] = {r0, r1};
+// Where a lane finds its rows' blocks: rows g and g + 8 of its slot.
+struct RowBase {
+    uint32_t row[2];   // the row
+    uint32_t word[2];  // the row + 4 t
+    uint32_t pick;     // byte selection: lanes t = 3 join a word from two (q8_0 and q4_0 even blocks)
+};
+
+__device__ __forceinline__ RowBase row_base(uint32_t r0, uint32_t r1, int t) {
+    return RowBase{{r0, r1}, {r0 + 4 * t, r1 + 4 * t}, t == 3 ? 0x5432u : 0x7654u};
+}
+
+// Blocks 2 P and 2 P + 1 of the lane's rows.
+template <int F, bool ALN, int P>
+__device__ __forceinline__ void load_pair(const RowBase& r, RawA& even, RawA& odd) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        if (F == kQ8_0) {
-            const uint32_t b = r[i] + 68 * p;
-            const uint32_t w0 = lds_word<ALN>(b), w8 = lds_word<ALN>(b + 32);
-            even.w[i][0] = lds_word<ALN>(b + 4 + 4 * t);
-            const uint32_t e1 = lds_word<ALN>(b + 20 + 4 * t);
-            even.w[i][1] = t == 3 ? __byte_perm(w0, w8, 0x5432) : e1;
-            odd.w[i][0] = lds_word<ALN>(b + 36 + 4 * t);
-            odd.w[i][1] = lds_word<ALN>(b + 52 + 4 * t);
+        if constexpr (F == kQ8_0) {
+            constexpr int b = 68 * P;
+            const uint32_t w0 = lds_word<ALN, b>(r.row[i]), w8 = lds_word<ALN, b + 32>(r.row[i]);
+            even.w[i][0] = lds_word<ALN, b + 4>(r.word[i]);
+            // the last word: bytes of words 0 and 8 (what lane 3 has loaded), the others theirs
+            even.w[i][1] = __byte_perm(w0, lds_word<ALN, b + 20>(r.word[i]), r.pick);
+            odd.w[i][0] = lds_word<ALN, b + 36>(r.word[i]);
+            odd.w[i][1] = lds_word<ALN, b + 52>(r.word[i]);
             even.d[i] = low_half(w0);
             odd.d[i] = high_half(w8);
-        } else if (F == kQ4_0) {
-            const uint32_t b = r[i] + 36 * p;
-            const uint32_t w0 = lds_word<ALN>(b), w4 = lds_word<ALN>(b + 16);
-            const uint32_t e = lds_word<ALN>(b + 4 + 4 * t);
-            even.w[i][0] = t == 3 ? __byte_perm(w0, w4, 0x5432) : e;
-            odd.w[i][0] = lds_word<ALN>(b + 20 + 4 * t);
+        } else if constexpr (F == kQ4_0) {
+            constexpr int b = 36 * P;
+            const uint32_t w0 = lds_word<ALN, b>(r.row[i]), w4 = lds_word<ALN, b + 16>(r.row[i]);
+            even.w[i][0] = __byte_perm(w0, lds_word<ALN, b + 4>(r.word[i]), r.pick);
+            odd.w[i][0] = lds_word<ALN, b + 20>(r.word[i]);
             even.d[i] = low_half(w0);
             odd.d[i] = high_half(w4);
         } else {
             // aligned: blocks 0..3 in the first box, 4..7 in the second
-            const uint32_t b = ALN ? r[i] + (p >> 1) * (16 * 80) + (p & 1) * 40 : r[i] + 40 * p;
-            const uint32_t w0 = lds_word<ALN>(b), w5 = lds_word<ALN>(b + 20);
-            even.w[i][0] = lds_word<ALN>(b + 4 + 4 * t);
-            odd.w[i][0] = lds_word<ALN>(b + 24 + 4 * t);
+            constexpr int b = ALN ? (P >> 1) * (16 * 80) + (P & 1) * 40 : 40 * P;
+            const uint32_t w0 = lds_word<ALN, b>(r.row[i]), w5 = lds_word<ALN, b + 20>(r.row[i]);
+            even.w[i][0] = lds_word<ALN, b + 4>(r.word[i]);
+            odd.w[i][0] = lds_word<ALN, b + 24>(r.word[i]);
             even.d[i] = low_half(w0);
             even.m[i] = fmaf(8.0f, even.d[i], high_half(w0));  // d c + m = d (c - 8) + (m + 8 d)
             odd.d[i] = low_half(w5);

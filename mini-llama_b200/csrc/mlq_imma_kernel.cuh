@@ -22,6 +22,15 @@
 namespace mlq {
 namespace {
 
+// f(integral_constant 0), .., f(integral_constant N - 1)
+template <int N, int I = 0, class Fn>
+__device__ __forceinline__ void static_for(Fn f) {
+    if constexpr (I < N) {
+        f(std::integral_constant<int, I>{});
+        static_for<N, I + 1>(f);
+    }
+}
+
 // The sliced rows of x that a unit reads.
 struct XView {
     const uint8_t* data;
@@ -35,54 +44,63 @@ struct XView {
 // 1 and 0 (t odd) of row t / 2, and the two are added once, at the end.
 template <int F, int NT>
 struct FewRows {
-    uint32_t bo[NT], so[NT];
-    uint4 b[NT][2][2];  // [.][half of a K step][pair of blocks]
+    const uint4* xp[NT];  // x of the K step
+    const float4* sp[NT];
+    ptrdiff_t to_sum;     // from a scale to the block's sum
+    uint4 b[NT][2][2];    // [.][half of a K step][pair of blocks]
     float4 s[NT][2], m[F == kQ4_1 ? NT : 1][2];
     float acc[NT][2], accm[F == kQ4_1 ? NT : 1][2];
 
     template <class TokenOf>
-    __device__ __forceinline__ void init(const XView& a, int count, int lane, TokenOf token) {
+    __device__ __forceinline__ void init(const XView& a, int count, int block, int lane, TokenOf token) {
         const int g = lane >> 2, t = lane & 3;
+        to_sum = reinterpret_cast<const float4*>(a.sum) - reinterpret_cast<const float4*>(a.scale);
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
             // columns without a row of x repeat the first one's; nothing reads them
             const int r = 2 * i + (g >> 2), rs = 2 * i + (t >> 1);
-            bo[i] = (uint32_t)token(r < count ? r : 0) * a.bprp * kSlicedBytes + (g & 3) * 64 + t * 16;
-            so[i] = (uint32_t)token(rs < count ? rs : 0) * a.bprp;
+            xp[i] = reinterpret_cast<const uint4*>(
+                a.data + ((size_t)token(r < count ? r : 0) * a.bprp + block) * kSlicedBytes + (g & 3) * 64 + t * 16);
+            sp[i] = reinterpret_cast<const float4*>(a.scale + (size_t)token(rs < count ? rs : 0) * a.bprp + block);
             acc[i][0] = acc[i][1] = 0.0f;
             if (F == kQ4_1) accm[i][0] = accm[i][1] = 0.0f;
         }
+        load_x(0);
     }
 
-    // Half h of the x registers: the four blocks from kb.
-    __device__ __forceinline__ void load_x(const XView& a, int kb, int h) {
+    // Half h of the x registers: four blocks of the K step.
+    __device__ __forceinline__ void load_x(int h) {
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
-            const uint4* x = reinterpret_cast<const uint4*>(a.data + bo[i] + (size_t)kb * kSlicedBytes);
-            b[i][h][0] = x[0], b[i][h][1] = x[16];
-            s[i][h] = *reinterpret_cast<const float4*>(a.scale + so[i] + kb);
-            if (F == kQ4_1) m[i][h] = *reinterpret_cast<const float4*>(a.sum + so[i] + kb);
+            b[i][h][0] = xp[i][32 * h], b[i][h][1] = xp[i][32 * h + 16];
+            s[i][h] = sp[i][h];
+            if (F == kQ4_1) m[i][h] = sp[i][h + to_sum];
         }
     }
 
-    __device__ __forceinline__ void prime(const XView& a, int kb) { load_x(a, kb, 0); }
-
-    // One K step of 8 blocks from kb: while four are multiplied, the next four (of this step, then of the next one
-    // at kb_next) are fetched.
+    // One K step of 8 blocks: while four are multiplied, the next four (of this step, then of the next one, `ahead`
+    // blocks on) are fetched.
     template <bool ALN, class Wait>
-    __device__ __forceinline__ void step(const XView& a, int kb, int kb_next, int valid, uint32_t r0, uint32_t r1,
-                                         int lane, Wait wait) {
-        const int t = lane & 3;
+    __device__ __forceinline__ void step(int ahead, int valid, uint32_t r0, uint32_t r1, int lane, Wait wait) {
+        const RowBase rows = row_base(r0, r1, lane & 3);
+        static_for<2>([&](auto hc) {
+            constexpr int h = decltype(hc)::value;
+            if (h == 0) {
+                load_x(1);
+                wait();
+            } else {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            load_x(a, h ? kb_next : kb + 4, h ^ 1);
-            if (h == 0) wait();
-#pragma unroll
-            for (int p2 = 0; p2 < 2; ++p2) {
-                const int p = 2 * h + p2;
-                if (!ALN && 2 * p >= valid) continue;
+                for (int i = 0; i < NT; ++i) {
+                    xp[i] += ahead * (kSlicedBytes / 16);
+                    sp[i] += ahead / 4;
+                }
+                load_x(0);
+            }
+            static_for<2>([&](auto pc) {
+                constexpr int p2 = decltype(pc)::value, p = 2 * h + p2;
+                if (!ALN && 2 * p >= valid) return;
                 RawA A[2];
-                load_pair<F, ALN>(r0, r1, p, t, A[0], A[1]);
+                load_pair<F, ALN, p>(rows, A[0], A[1]);
                 if (!ALN && 2 * p + 1 >= valid) A[1].d[0] = A[1].d[1] = A[1].m[0] = A[1].m[1] = 0.0f;
 #pragma unroll
                 for (int o = 0; o < 2; ++o) {
@@ -105,8 +123,8 @@ struct FewRows {
                         }
                     }
                 }
-            }
-        }
+            });
+        });
     }
 
     // red: [row of x][weight row 0..15] of this warp
@@ -130,56 +148,58 @@ struct FewRows {
 template <int F, int S>
 struct ManyRows {
     static constexpr int kG = S < 2 ? S : 2;  // groups of 8 rows per buffer
-    uint32_t bo[S], so[S][2];
+    const uint8_t* data;
+    const float* scale;
+    ptrdiff_t to_sum;
+    uint32_t bo[S], so[S][2];  // of the block that is multiplied
     uint4 hi[2][kG], lo[2][kG];
     float s[2][kG][2], m[2][kG][2];
     float acc[S][2][2];  // [.][row half][row of x 2t, 2t + 1]
 
     template <class TokenOf>
-    __device__ __forceinline__ void init(const XView& a, int count, int lane, TokenOf token) {
+    __device__ __forceinline__ void init(const XView& a, int count, int block, int lane, TokenOf token) {
         const int g = lane >> 2, t = lane & 3;
+        data = a.data, scale = a.scale, to_sum = a.sum - a.scale;
 #pragma unroll
         for (int i = 0; i < S; ++i) {
             const int r = 8 * i + g;
-            bo[i] = (uint32_t)token(r < count ? r : 0) * a.bprp * kSlicedBytes + t * 16;
+            bo[i] = ((uint32_t)token(r < count ? r : 0) * a.bprp + block) * kSlicedBytes + t * 16;
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
                 const int rs = 8 * i + 2 * t + x;
-                so[i][x] = (uint32_t)token(rs < count ? rs : 0) * a.bprp;
+                so[i][x] = (uint32_t)token(rs < count ? rs : 0) * a.bprp + block;
             }
             acc[i][0][0] = acc[i][0][1] = acc[i][1][0] = acc[i][1][1] = 0.0f;
         }
+        load_x(0, 0, 0);
     }
 
-    // Buffer q: x of rows 8 kG gr .. of block blk.
-    __device__ __forceinline__ void load_x(const XView& a, int blk, int gr, int q) {
+    // Buffer q: x of rows 8 kG gr .., `on` blocks on.
+    __device__ __forceinline__ void load_x(int on, int gr, int q) {
 #pragma unroll
         for (int k = 0; k < kG; ++k) {
             const int i = gr * kG + k;
-            const uint4* x = reinterpret_cast<const uint4*>(a.data + bo[i] + (size_t)blk * kSlicedBytes);
+            const uint4* x = reinterpret_cast<const uint4*>(data + bo[i] + on * kSlicedBytes);
             hi[q][k] = x[0], lo[q][k] = x[4];
 #pragma unroll
             for (int x2 = 0; x2 < 2; ++x2) {
-                s[q][k][x2] = a.scale[so[i][x2] + blk];
-                if (F == kQ4_1) m[q][k][x2] = a.sum[so[i][x2] + blk];
+                s[q][k][x2] = scale[so[i][x2] + on];
+                if (F == kQ4_1) m[q][k][x2] = scale[so[i][x2] + on + to_sum];
             }
         }
     }
 
-    __device__ __forceinline__ void prime(const XView& a, int kb) { load_x(a, kb, 0, 0); }
-
-    // One K step of 8 blocks from kb: while up to 16 rows of a block are multiplied, the next ones (then the next
-    // block's, then the next step's) are fetched.
+    // One K step of 8 blocks: while up to 16 rows of a block are multiplied, the next ones (then the next block's, then
+    // the next step's, `ahead` blocks on) are fetched.
     template <bool ALN, class Wait>
-    __device__ __forceinline__ void step(const XView& a, int kb, int kb_next, int valid, uint32_t r0, uint32_t r1,
-                                         int lane, Wait wait) {
-        const int t = lane & 3;
-#pragma unroll
-        for (int p = 0; p < kChunkBlocks / 2; ++p) {
-            if (2 * p >= valid) break;
-            if (p == 0) wait();
+    __device__ __forceinline__ void step(int ahead, int valid, uint32_t r0, uint32_t r1, int lane, Wait wait) {
+        const RowBase rows = row_base(r0, r1, lane & 3);
+        wait();
+        static_for<kChunkBlocks / 2>([&](auto pc) {
+            constexpr int p = decltype(pc)::value;
+            if (2 * p >= valid) return;
             RawA A[2];
-            load_pair<F, ALN>(r0, r1, p, t, A[0], A[1]);
+            load_pair<F, ALN, p>(rows, A[0], A[1]);
 #pragma unroll
             for (int o = 0; o < 2; ++o) {
                 const int n = 2 * p + o;
@@ -190,9 +210,9 @@ struct ManyRows {
                 for (int gr = 0; gr < S / kG; ++gr) {
                     const int q = (n * (S / kG) + gr) & 1;
                     if (gr + 1 < S / kG)
-                        load_x(a, kb + n, gr + 1, q ^ 1);
+                        load_x(n, gr + 1, q ^ 1);
                     else
-                        load_x(a, n + 1 < kChunkBlocks && n + 1 < valid ? kb + n + 1 : kb_next, 0, q ^ 1);
+                        load_x(n + 1 < kChunkBlocks && n + 1 < valid ? n + 1 : ahead, 0, q ^ 1);
 #pragma unroll
                     for (int k = 0; k < kG; ++k) {
                         const int i = gr * kG + k;
@@ -211,6 +231,11 @@ struct ManyRows {
                     }
                 }
             }
+        });
+#pragma unroll
+        for (int i = 0; i < S; ++i) {
+            bo[i] += ahead * kSlicedBytes;
+            so[i][0] += ahead, so[i][1] += ahead;
         }
     }
 
@@ -314,17 +339,17 @@ __device__ __forceinline__ WarpState unit_sums(const UnitArgs u, WarpState st) {
     using S = Slot<F, ALN>;
     constexpr uint32_t kStage = kImmaWarps * S::kBytes;
     const int lane = threadIdx.x & 31, g = lane >> 2;
+    int c = u.c0;
     Acc acc;
-    acc.init(u.x, u.count, lane, [&](int r) -> int {
+    acc.init(u.x, u.count, (c < u.c_end ? c : 0) * kChunkBlocks, lane, [&](int r) -> int {
         if (MODE == kPair) return __ldcg(u.order + u.first + r) / u.top_k;
         return u.first + r;
     });
-    int c = u.c0;
-    if (c < u.c_end) acc.prime(u.x, c * kChunkBlocks);
     for (int r = 0; r < u.rounds; ++r, c += u.kws) {
-        const int cn = c + u.kws < u.c_end ? c + u.kws : c;  // the step after this one
+        const uint32_t full = u.full + 16 * st.stage;
         auto wait = [&]() {
-            if (st.alive && !__all_sync(0xffffffffu, mbar_wait(u.full + 16 * st.stage, st.phase))) {
+            if (__all_sync(0xffffffffu, mbar_try_wait(full, st.phase)) || !st.alive) return;
+            if (!__all_sync(0xffffffffu, mbar_wait(full, st.phase))) {
                 st.alive = false;
                 if (lane == 0) report_error(u.err, 30), *u.dead = 1;
             }
@@ -335,16 +360,16 @@ __device__ __forceinline__ WarpState unit_sums(const UnitArgs u, WarpState st) {
                 row0 += (u.window0 + (uint32_t)c * u.window_step) & 15;
                 row1 += (u.window1 + (uint32_t)c * u.window_step) & 15;
             }
-            acc.template step<ALN>(u.x, c * kChunkBlocks, cn * kChunkBlocks, u.blocks - c * kChunkBlocks, row0, row1, lane,
-                                   wait);
+            const int ahead = c + u.kws < u.c_end ? u.kws * kChunkBlocks : 0;  // to the step after this one
+            acc.template step<ALN>(ahead, u.blocks - c * kChunkBlocks, row0, row1, lane, wait);
         } else {
             wait();
         }
         __syncwarp();
-        if (st.alive) ++st.taken;
-        if (lane == 0) mbar_arrive(u.full + 16 * st.stage + 8);
+        if (lane == 0) mbar_arrive(full + 8);
         if (++st.stage == u.stages) st.stage = 0, st.phase ^= 1;
     }
+    if (st.alive) st.taken += u.rounds;
     acc.store(u.red, lane);
     return st;
 }
