@@ -275,6 +275,11 @@ __device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
 constexpr int kTeams = 2;
 constexpr int kThreads = 32 * kTeams * (kImmaWarps + 2);  // computing warps, then two producer warps per team
 constexpr int kTeamThreads = 32 * kImmaWarps;
+// Registers: the launch has 96 per thread (65536 / 640, in eights); the
+// producers keep 32 and the computing warps take what that frees.
+constexpr int kLaunchRegs = 96, kProducerRegs = 32, kComputeRegs = 112;
+static_assert((2 * kTeams * kProducerRegs + kTeams * kImmaWarps * kComputeRegs) * 32 <= kThreads * kLaunchRegs,
+              "the shares must not exceed the launch's registers, or setmaxnreg would wait for ever");
 constexpr int kRedFloats = kImmaWarps * kSegTokens * 16;  // [warp][row of x][row of the strip]
 
 // The barrier of a team's computing warps.
@@ -423,6 +428,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int unit_rows = (MODE == kPair ? 8 : 16) * a.strips;
 
     if (producer) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kProducerRegs));
         const int half = cta_warp & 1;
         bool fresh = true;
         int row0 = 0, stage = 0, phase = 1, n = 0;
@@ -511,6 +517,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
 
     // ---- computing warps ----
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kComputeRegs));
     if (MODE != kPair) grid_dependency_wait();
     if (MODE == kDown) launch_dependents();
     const int warp = cta_warp % kImmaWarps, tid = threadIdx.x % kTeamThreads;
@@ -708,6 +715,14 @@ cudaError_t launch_one(ImmaArgs a, int grid, int smem_per_sm, cudaStream_t strea
                              MODE == kPair ? 8 : 16, CU_TENSOR_MAP_SWIZZLE_NONE))
                 return cudaErrorInvalidValue;
     }
+    // once per kernel: its shared memory, and that it was built with the registers its split counts on
+    static const cudaError_t ready = [&] {
+        cudaFuncAttributes fa{};
+        cudaError_t e = cudaFuncGetAttributes(&fa, k);
+        if (e == cudaSuccess && fa.numRegs < kLaunchRegs) e = cudaErrorInvalidConfiguration;
+        return e;
+    }();
+    if (ready != cudaSuccess) return ready;
     cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
     return launch_pdl(k, grid, kThreads, smem, stream, maps, a);
