@@ -5,9 +5,8 @@
 //   prep   sorts the (row, slot) pairs by expert into segments of at most 32
 //          and slices x;
 //   pair   h = silu(x Wg^T) * (x Wu^T) per segment, sliced in its epilogue;
-//   down   h Wd^T per segment, weighed and summed per row by the team that
-//          finishes a row tile last (fixed order), or by a fourth launch
-//          when there are many rows;
+//   down   h Wd^T, weighed and summed per row over the segments of a tile in
+//          order, or, with many rows, by a fourth launch over the slots;
 // and two (prep, down in its plain form) for the linear with an epilogue.
 #include "mlq_imma_args.cuh"
 
@@ -36,8 +35,6 @@ struct PrepArgs {
     Segment* segs;
     int* nseg;
     int* order;
-    unsigned int* done;
-    int tiles;
     // padding blocks of the sliced h
     Sliced h;
     int h_bpr, h_bprp;
@@ -58,7 +55,6 @@ __global__ void __launch_bounds__(256) prep_kernel(const PrepArgs a) {
             __shared__ int wsum[2][8];
             __shared__ unsigned char in_warp[8][MLQ_MOE_MAX_EXPERTS];
             for (int e = threadIdx.x; e < a.n_experts; e += 256) cnt[e] = 0;
-            for (int i = threadIdx.x; i < a.tiles; i += 256) a.done[i] = 0;
             const int pad = a.h_bprp - a.h_bpr;
             for (int i = threadIdx.x; i < a.pairs * pad; i += 256) {
                 const size_t at = (size_t)(i / pad) * a.h_bprp + a.h_bpr + i % pad;
@@ -145,14 +141,32 @@ __global__ void __launch_bounds__(256) prep_kernel(const PrepArgs a) {
 
 size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 
-// 16-row strips of a unit: no more K parts than there are K steps, and the
-// tallest tile whose units still give every team one (a taller unit has fewer
-// K parts to add up and reads its rows of x less often).
-int choose_strips(int out, int bpr, long long nseg, int sm_count, int least) {
+// About how many rounds the busiest team has (see Deal): `units` of `per`
+// rounds, each with an end that takes `end` rounds' time.
+double deal_cost(long long units, long long per, double end, int teams) {
+    const long long each = units / teams, rest = units % teams;
+    double c = each * (per + end);
+    if (rest) {
+        const double split = (double)((rest * per + teams - 1) / teams) + 4;
+        c += end + (split < per ? split : per);
+    }
+    return c;
+}
+
+// 16-row strips of a unit (at least `least`): the K axis is then split in 8 /
+// strips parts.  all_segs: a unit meets every segment.
+int choose_strips(int out, int bpr, int nseg, bool all_segs, int sm_count, int least) {
     const int steps = (bpr + kChunkBlocks - 1) / kChunkBlocks;
-    int n = 8;
-    while (n > least && kImmaWarps / (n / 2) <= steps && (out + 16 * n - 1) / (16 * n) * nseg < 2 * sm_count) n /= 2;
-    return n;
+    int best = kImmaWarps;
+    double best_cost = 1e300;
+    for (int n = kImmaWarps; n >= least; n /= 2) {
+        const int kws = kImmaWarps / n;
+        const long long per = (steps + kws - 1) / kws, tiles = (out + 16 * n - 1) / (16 * n);
+        const double c = all_segs ? deal_cost(tiles, per * nseg, 0.5 * nseg + 0.5, 2 * sm_count)
+                                  : deal_cost(tiles * nseg, per, 0.7, 2 * sm_count);
+        if (c < best_cost) best_cost = c, best = n;
+    }
+    return best;
 }
 
 struct Carve {
@@ -255,11 +269,11 @@ cudaError_t launch_linear_epilogue(int fmt, const uint8_t* w, int out, int in, c
         a.few = p.few;
         a.seg_cap = p.few ? kFewRows : kSegTokens;
         const int nseg = (n + a.seg_cap - 1) / a.seg_cap;
-        a.strips = choose_strips(out, bpr, nseg, sm_count, 1);
+        a.strips = choose_strips(out, bpr, nseg, false, sm_count, 1);
         a.tiles = (out + 16 * a.strips - 1) / (16 * a.strips);
         a.x = p.sliced;
         a.rows = n;
-        a.split = split, a.split_done = p.split_done, a.split_tokens = split_tokens(n);
+        a.split = split, a.split_done = p.split_done, a.split_size = (size_t)split_tokens(n) * 16 * a.strips;
         a.bias = ep.bias;
         a.row_scale = ep.row_scale ? ep.row_scale + r0 : nullptr;
         a.residual = ep.residual ? ep.residual + (long long)r0 * out : nullptr;
@@ -274,12 +288,18 @@ cudaError_t launch_linear_epilogue(int fmt, const uint8_t* w, int out, int in, c
 }
 
 size_t experts_workspace_bytes(const MoeShape& s, int rows, int top_k) {
-    const int n = experts_pass_rows(s, rows, top_k), pairs = n * top_k;
+    const int pass = experts_pass_rows(s, rows, top_k);
     const int bprp = padded_blocks((s.in + kQK - 1) / kQK), hp = padded_blocks((s.hidden + kQK - 1) / kQK);
-    return 256 + align256((size_t)max_segments(pairs, s.n_experts, few_rows(pairs, s.n_experts) ? kFewRows : kSegTokens) * sizeof(Segment)) +
-           align256((size_t)pairs * sizeof(int)) + align256((size_t)((s.out + 15) / 16) * sizeof(unsigned int)) +
-           sliced_bytes(n, bprp) + sliced_bytes(pairs, hp) +
-           align256((size_t)pairs * s.out * sizeof(float)) + split_bytes(pairs);
+    auto bytes = [&](int n) {
+        const int pairs = n * top_k, cap = few_rows(pairs, s.n_experts) ? kFewRows : kSegTokens;
+        return 256 + align256((size_t)max_segments(pairs, s.n_experts, cap) * sizeof(Segment)) +
+               align256((size_t)pairs * sizeof(int)) + sliced_bytes(n, bprp) + sliced_bytes(pairs, hp) +
+               (n <= kCombineRows ? 0 : align256((size_t)pairs * s.out * sizeof(float))) + split_bytes(pairs);
+    };
+    // the last pass may be smaller, and take another form
+    const int last = rows % pass;
+    const size_t whole = bytes(pass), rest = last ? bytes(last) : 0;
+    return whole > rest ? whole : rest;
 }
 
 cudaError_t launch_experts(const MoeShape& s, const uint8_t* gate, const uint8_t* up, const uint8_t* down,
@@ -295,15 +315,13 @@ cudaError_t launch_experts(const MoeShape& s, const uint8_t* gate, const uint8_t
         const int cap = few ? kFewRows : kSegTokens;
         const int nseg_max = max_segments(pairs, s.n_experts, cap);
         const int nseg_likely = pairs < s.n_experts ? pairs : nseg_max;
-        const int strips = choose_strips(s.out, hb, nseg_likely, sm_count, 1);
+        const int strips = choose_strips(s.out, hb, nseg_likely, n <= kCombineRows, sm_count, 1);
         const int tiles = (s.out + 16 * strips - 1) / (16 * strips);
         Carve c{static_cast<uint8_t*>(ws)};
         PrepArgs p{};
         p.nseg = c.take<int>(1);
         p.segs = c.take<Segment>(nseg_max);
         p.order = c.take<int>(pairs);
-        p.done = c.take<unsigned int>((s.out + 15) / 16);
-        p.tiles = tiles;
         p.x = x + (long long)r0 * s.in;
         p.rows = n, p.in = s.in, p.bpr = bpr, p.bprp = bprp, p.fmt = s.fmt;
         p.few = few, p.seg_cap = cap;
@@ -312,7 +330,7 @@ cudaError_t launch_experts(const MoeShape& s, const uint8_t* gate, const uint8_t
         p.pairs = pairs, p.n_experts = s.n_experts;
         p.h = c.take_sliced(pairs, hp);
         p.h_bpr = hb, p.h_bprp = hp;
-        float* part = c.take<float>((size_t)pairs * s.out);
+        float* part = c.take<float>(n <= kCombineRows ? 0 : (size_t)pairs * s.out);
         float* split = c.take<float>((size_t)2 * kMaxTeams * split_tokens(pairs) * 128);
         p.split_done = c.take<unsigned int>(2 * kMaxTeams);
         cudaError_t e = launch_pdl(prep_kernel, 1 + prep_ctas((long long)n * bprp, sm_count), 256, 0, stream, p);
@@ -322,7 +340,7 @@ cudaError_t launch_experts(const MoeShape& s, const uint8_t* gate, const uint8_t
         a.w[0] = gate, a.w[1] = up;
         a.total_rows = (long long)s.n_experts * s.hidden;
         a.out = s.hidden, a.bpr = bpr, a.bprp = bprp;
-        a.strips = choose_strips(2 * s.hidden, bpr, nseg_likely, sm_count, 4);
+        a.strips = choose_strips(2 * s.hidden, bpr, nseg_likely, false, sm_count, 4);
         a.tiles = (s.hidden + 8 * a.strips - 1) / (8 * a.strips);
         a.few = few, a.seg_cap = cap;
         a.x = p.sliced;
@@ -330,7 +348,7 @@ cudaError_t launch_experts(const MoeShape& s, const uint8_t* gate, const uint8_t
         a.top_k = top_k, a.rows = n;
         a.next_fmt = s.fmt_down, a.next_bprp = hp;
         a.h = p.h;
-        a.split = split, a.split_done = p.split_done, a.split_tokens = split_tokens(pairs);
+        a.split = split, a.split_done = p.split_done, a.split_size = (size_t)split_tokens(pairs) * 16 * a.strips;
         a.err = err;
         e = launch_imma_pair(s.fmt, a, sm_count, smem_per_sm, (long long)nseg_max * a.tiles, stream);
         if (e != cudaSuccess) return e;
@@ -344,9 +362,9 @@ cudaError_t launch_experts(const MoeShape& s, const uint8_t* gate, const uint8_t
         d.x = p.h;
         d.segs = p.segs, d.nseg = p.nseg, d.order = p.order;
         d.top_k = top_k, d.rows = n;
-        d.part = part;
-        d.done = n <= kCombineRows ? p.done : nullptr;
-        d.split = split, d.split_done = p.split_done + kMaxTeams, d.split_tokens = split_tokens(pairs);
+        d.part = n <= kCombineRows ? nullptr : part;
+        d.split = split, d.split_done = p.split_done + kMaxTeams;
+        d.split_size = (size_t)split_tokens(pairs) * 16 * strips;
         d.ids = p.ids;
         d.weights = weights + (long long)r0 * top_k;
         d.n_experts = s.n_experts;
@@ -355,7 +373,7 @@ cudaError_t launch_experts(const MoeShape& s, const uint8_t* gate, const uint8_t
         d.err = err;
         e = launch_imma_down(s.fmt_down, d, sm_count, smem_per_sm, (long long)nseg_max * tiles, stream);
         if (e != cudaSuccess) return e;
-        if (!d.done) {
+        if (d.part) {
             const long long vals = (long long)n * s.out;
             e = launch_pdl(combine_kernel, (int)((vals + 255) / 256 < 16 * sm_count ? (vals + 255) / 256 : 16 * sm_count),
                            256, 0, stream, d);

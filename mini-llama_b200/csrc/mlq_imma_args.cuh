@@ -38,16 +38,15 @@ struct ImmaArgs {
     // kPair: sliced h by position
     int next_fmt, next_bprp;
     Sliced h;
-    // kDown: one value per pair, then the weighed sum
+    // kDown: one value per pair for a later launch to sum; null: a unit meets every segment and is summed at once
     float* part;              // [pair][out]
-    unsigned int* done;       // units finished per row tile, zero before the launch; null: a later launch sums
     const int32_t* ids;
     const float* weights;
     int n_experts;
     // units that several teams share
-    float* split;             // [team][head, tail][row of x][row of the tile]
+    float* split;             // [team][head, tail][split_size]: row of x, row of the tile
     unsigned int* split_done; // per team, zero before the launch
-    int split_tokens;         // rows of x of a split slot
+    size_t split_size;
     // kPlain / kDown
     const float* bias;
     const float* row_scale;

@@ -287,32 +287,52 @@ __device__ __forceinline__ void team_sync(int team) {
     asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "n"(kTeamThreads) : "memory");
 }
 
-// How a launch's rounds are dealt out: team i takes [begin(i), begin(i + 1)).
-// Whole units when that costs no team more than 2 rounds (a round takes about
-// 0.8 us of a team's share of HBM, adding up a split unit about 2 us).
+// How a launch's units, of `per` rounds each, are dealt out.  Every team takes
+// `each` whole units; the units left over are spread by rounds, a contiguous
+// range per team, when that saves more than the adding up costs (about 2 us
+// for whoever finishes a shared unit, where a round takes about 0.8 us of a
+// team's share of HBM), else one unit each to as many teams.
 struct Deal {
-    long long total;
-    int units, per_unit, teams;
-    bool whole;
-    __device__ __forceinline__ Deal(int units_, int per_unit_, int teams_)
-        : units(units_), per_unit(per_unit_), teams(teams_) {
-        total = (long long)units * per_unit;
-        if (teams > total) teams = (int)total;
-        const long long even = teams ? (total + teams - 1) / teams : 0;
-        const long long by_unit = teams ? (long long)((units + teams - 1) / teams) * per_unit : 0;
-        whole = by_unit <= even + 2;
-        if (whole && teams > units) teams = units;
+    int teams, per, each, rest;  // rest: units left over
+    long long rounds;            // theirs, dealt by rounds to the first `sharers` teams; 0: dealt whole
+    int sharers;                 // each has a round at least: who shares a unit follows from its ends
+    __device__ __forceinline__ Deal(int units, int per_, int teams_) : teams(teams_), per(per_) {
+        each = units / teams;
+        rest = units - each * teams;
+        const long long all = (long long)rest * per;
+        rounds = (all + teams - 1) / teams + 4 < per ? all : 0;
+        sharers = rounds < teams ? (int)rounds : teams;
     }
-    __device__ __forceinline__ long long begin(int i) const {
-        return whole ? (long long)units * i / teams * per_unit : total * i / teams;
-    }
-    // the team that has round t (not asked when units are whole)
-    __device__ __forceinline__ int owner(long long t) const { return (int)(((t + 1) * teams - 1) / total); }
+    // first round (among the left-over units') of team i, and the team that has round t
+    __device__ __forceinline__ long long begin(int i) const { return i < sharers ? rounds * i / sharers : rounds; }
+    __device__ __forceinline__ int owner(long long t) const { return (int)(((t + 1) * sharers - 1) / rounds); }
 };
 
-// A team's place in the launch: unit (tile, segment), round in the unit, rounds left.
-struct Place {
-    int tile, seg, round, left;
+// A team's work, piece by piece: rounds [r0, r1) of unit u.
+struct Work {
+    int u, r0, r1, n;    // the piece, and how many there were
+    long long t, t_end;  // rounds of left-over units still to come
+    int left;            // whole units still to come
+    __device__ __forceinline__ Work(const Deal& d, int id) : u(0), r0(0), r1(0), n(0) {
+        left = d.each + (d.rounds == 0 && id < d.rest ? 1 : 0);
+        t = d.rounds ? d.begin(id) : 0;
+        t_end = d.rounds ? d.begin(id + 1) : 0;
+    }
+    // whole units lie `teams` apart, so that the teams work on neighbours
+    __device__ __forceinline__ bool next(const Deal& d, int id) {
+        if (left > 0) {
+            u = n * d.teams + id, r0 = 0, r1 = d.per;
+            --left, ++n;
+            return true;
+        }
+        if (t >= t_end) return false;
+        const int k = (int)(t / d.per);
+        u = d.each * d.teams + k;
+        r0 = (int)(t - (long long)k * d.per);
+        r1 = t_end - t < d.per - r0 ? r0 + (int)(t_end - t) : d.per;
+        t += r1 - r0;
+        return true;
+    }
 };
 
 // A computing warp's place in its team's ring.
@@ -390,18 +410,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int team = producer ? (cta_warp - kTeams * kImmaWarps) >> 1 : cta_warp / kImmaWarps;
     const int kws = kImmaWarps / a.strips;
     const int steps = (a.bpr + kChunkBlocks - 1) / kChunkBlocks;
-    const int per_unit = (steps + kws - 1) / kws;
-    // shared memory: weight stages [team][stage][warp], sums [team], the stages' barriers [team][stage] (full, empty)
+    const int per_seg = (steps + kws - 1) / kws;  // rounds of a tile against a segment
+    // shared memory: weight stages [team][stage][warp], sums [team], (all_segs) y [team], the stages' barriers [team][stage] (full, empty)
     constexpr uint32_t kStage = kImmaWarps * S::kBytes;
     const uint32_t red0 = kTeams * a.slots * kStage;
-    const uint32_t bars = smem_u32(smem) + red0 + kTeams * kRedFloats * 4 + 16 * team * a.slots;
+    const uint32_t y_floats = MODE == kDown && !a.part ? a.rows * 16 * a.strips : 0;
+    const uint32_t bars0 = smem_u32(smem) + red0 + kTeams * (kRedFloats + y_floats) * 4;
+    const uint32_t bars = bars0 + 16 * team * a.slots;
     const uint32_t ring = smem_u32(smem) + team * a.slots * kStage;
     if (threadIdx.x == 0) {
         s_dead = 0;
-        const uint32_t all = smem_u32(smem) + red0 + kTeams * kRedFloats * 4;
         for (int i = 0; i < kTeams * a.slots; ++i) {
-            mbar_init(all + 16 * i, ALN ? 1 : 64);
-            mbar_init(all + 16 * i + 8, kImmaWarps);
+            mbar_init(bars0 + 16 * i, ALN ? 1 : 64);
+            mbar_init(bars0 + 16 * i + 8, kImmaWarps);
         }
         fence_mbar_init();
     }
@@ -413,99 +434,101 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (MODE != kDown) launch_dependents();
     __syncthreads();
     const int nseg = MODE == kPlain ? (a.rows + a.seg_cap - 1) / a.seg_cap : __ldcg(a.nseg);
-    // A tile's segments follow one another: segments with more rows take
-    // longer, so each team gets a mix, and the teams that share a tile are few.
-    Place at{0, 0, 0, 0};
+    // kDown with few rows (a.part null): a unit is a tile against every segment; otherwise against one, and the
+    // segments of a tile are neighbours.
+    const bool all_segs = MODE == kDown && !a.part;
     const int id = kTeams * blockIdx.x + team;
-    {
-        const Deal deal(nseg * a.tiles, per_unit, kTeams * gridDim.x);
-        if (id < deal.teams) {
-            const long long t0 = deal.begin(id);
-            const int u = (int)(t0 / per_unit);
-            at = Place{u / nseg, u % nseg, (int)(t0 % per_unit), (int)(deal.begin(id + 1) - t0)};
-        }
-    }
+    const Deal deal(all_segs ? (nseg ? a.tiles : 0) : nseg * a.tiles, all_segs ? nseg * per_seg : per_seg,
+                    kTeams * gridDim.x);
+    Work work(deal, id);
     const int unit_rows = (MODE == kPair ? 8 : 16) * a.strips;
 
     if (producer) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kProducerRegs));
         const int half = cta_warp & 1;
-        bool fresh = true;
-        int row0 = 0, stage = 0, phase = 1, n = 0;
-        for (; at.left > 0; --at.left, ++n) {
-            // tensor maps: the team's two producers take stages in turn (lane w fetches warp w's slot; issuing a box
-            // takes ~70 cycles); 16-byte windows: each takes the slots of four warps of every stage
-            const bool mine = !ALN || (n & 1) == half;
-            if (mine) {
-                if (fresh) {
-                    const int e = MODE == kPlain ? 0 : __ldcg(&a.segs[at.seg].expert);
-                    row0 = e * a.out + at.tile * unit_rows;
-                    fresh = false;
-                }
-                const uint32_t full = bars + 16 * stage, dst = ring + stage * kStage;
-                if (!__all_sync(0xffffffffu, mbar_wait(full + 8, phase))) {
-                    if (lane == 0) report_error(a.err, 31), *(volatile int*)&s_dead = 1;
-                    break;
-                }
-                if (__any_sync(0xffffffffu, *(volatile int*)&s_dead)) break;
-                if constexpr (ALN) {
-                    const int active = steps - at.round * kws < kws ? steps - at.round * kws : kws;  // K parts of this round
-                    if (lane == 0) mbar_arrive_expect_tx(full, active * a.strips * S::kBytes);
-                    __syncwarp();
-                    const int kw = lane / a.strips, c = at.round * kws + kw;
-                    if (kw < active) {
-                        const int row = row0 + (lane % a.strips) * (MODE == kPair ? 8 : 16);
-#pragma unroll
-                        for (int b = 0; b < S::kBoxes; ++b) {
-                            const int c0 = (c * chunk_bytes(F) + b * S::kPitch) / 2;
-                            const uint32_t d = dst + lane * S::kBytes + b * 16 * S::kPitch;
-                            tma_load_2d(d, &maps.m[0], c0, row, full);
-                            if (MODE == kPair) tma_load_2d(d + 8 * S::kPitch, &maps.m[1], c0, row, full);
-                        }
+        int stage = 0, phase = 1, n = 0;
+        bool alive = true;
+        while (alive && work.next(deal, id)) {
+            int seg = all_segs ? work.r0 / per_seg : work.u % nseg, round = all_segs ? work.r0 % per_seg : work.r0;
+            const int tile = all_segs ? work.u : work.u / nseg;
+            int row0 = 0;
+            bool fresh = true;
+            for (int r = work.r0; r < work.r1; ++r, ++n) {
+                // tensor maps: the team's two producers take stages in turn (lane w fetches warp w's slot; issuing a box
+                // takes ~70 cycles); 16-byte windows: each takes the slots of four warps of every stage
+                const bool mine = !ALN || (n & 1) == half;
+                if (mine) {
+                    if (fresh) {
+                        const int e = MODE == kPlain ? 0 : __ldcg(&a.segs[seg].expert);
+                        row0 = e * a.out + tile * unit_rows;
+                        fresh = false;
                     }
-                    __syncwarp();
-                } else {
-                    // lanes 2r, 2r + 1: the windows that hold row r's blocks
-                    const int r = lane >> 1, sub = lane & 1;
-                    const uint8_t* base = MODE == kPair && r >= 8 ? a.w[1] : a.w[0];
-                    bool stored = false;
+                    const uint32_t full = bars + 16 * stage, dst = ring + stage * kStage;
+                    if (!__all_sync(0xffffffffu, mbar_wait(full + 8, phase))) {
+                        if (lane == 0) report_error(a.err, 31), *(volatile int*)&s_dead = 1;
+                        alive = false;
+                        break;
+                    }
+                    if (__any_sync(0xffffffffu, *(volatile int*)&s_dead)) {
+                        alive = false;
+                        break;
+                    }
+                    if constexpr (ALN) {
+                        const int active = steps - round * kws < kws ? steps - round * kws : kws;  // K parts of this round
+                        if (lane == 0) mbar_arrive_expect_tx(full, active * a.strips * S::kBytes);
+                        __syncwarp();
+                        const int kw = lane / a.strips, c = round * kws + kw;
+                        if (kw < active) {
+                            const int row = row0 + (lane % a.strips) * (MODE == kPair ? 8 : 16);
 #pragma unroll
-                    for (int k = 0; k < kImmaWarps / 2; ++k) {
-                        const int w = kImmaWarps / 2 * half + k, c = at.round * kws + w / a.strips;
-                        const long long row =
-                            row0 + (w % a.strips) * (MODE == kPair ? 8 : 16) + (MODE == kPair ? (r & 7) : r);
-                        if (c >= steps || row >= a.total_rows) continue;
-                        long long left = a.row_bytes - (long long)c * chunk_bytes(F);
-                        if (left > chunk_bytes(F)) left = chunk_bytes(F);
-                        const uint8_t* src = base + row * a.row_bytes + (long long)c * chunk_bytes(F);
-                        const uint8_t* end = src + left;
-                        const uint8_t* q =
-                            reinterpret_cast<const uint8_t*>(reinterpret_cast<uintptr_t>(src) & ~(uintptr_t)15) + 16 * sub;
-                        uint32_t to = dst + w * S::kBytes + r * S::kPitch + 16 * sub;
-#pragma unroll
-                        for (int i = 0; i < (chunk_bytes(F) + 15 + 31) / 32; ++i, q += 32, to += 32) {
-                            if (q >= end) break;
-                            if (q < base) {  // the stack starts inside this window: only its own bytes are read
-                                for (int b = (int)(base - q); b < 16 && q + b < end; ++b) sts_u8(to + b, q[b]);
-                                stored = true;
-                            } else {
-                                const long long m = end - q;
-                                cp_async_16(to, q, m < 16 ? (uint32_t)m : 16u);
+                            for (int b = 0; b < S::kBoxes; ++b) {
+                                const int c0 = (c * chunk_bytes(F) + b * S::kPitch) / 2;
+                                const uint32_t d = dst + lane * S::kBytes + b * 16 * S::kPitch;
+                                tma_load_2d(d, &maps.m[0], c0, row, full);
+                                if (MODE == kPair) tma_load_2d(d + 8 * S::kPitch, &maps.m[1], c0, row, full);
                             }
                         }
-                    }
-                    if (stored) {  // plain stores are ordered by a plain arrival
-                        asm volatile("cp.async.wait_all;" ::: "memory");
-                        mbar_arrive(full);
+                        __syncwarp();
                     } else {
-                        cp_async_arrive(full);
+                        // lanes 2r, 2r + 1: the windows that hold row r's blocks
+                        const int r = lane >> 1, sub = lane & 1;
+                        const uint8_t* base = MODE == kPair && r >= 8 ? a.w[1] : a.w[0];
+                        bool stored = false;
+#pragma unroll
+                        for (int k = 0; k < kImmaWarps / 2; ++k) {
+                            const int w = kImmaWarps / 2 * half + k, c = round * kws + w / a.strips;
+                            const long long row =
+                                row0 + (w % a.strips) * (MODE == kPair ? 8 : 16) + (MODE == kPair ? (r & 7) : r);
+                            if (c >= steps || row >= a.total_rows) continue;
+                            long long left = a.row_bytes - (long long)c * chunk_bytes(F);
+                            if (left > chunk_bytes(F)) left = chunk_bytes(F);
+                            const uint8_t* src = base + row * a.row_bytes + (long long)c * chunk_bytes(F);
+                            const uint8_t* end = src + left;
+                            const uint8_t* q =
+                                reinterpret_cast<const uint8_t*>(reinterpret_cast<uintptr_t>(src) & ~(uintptr_t)15) + 16 * sub;
+                            uint32_t to = dst + w * S::kBytes + r * S::kPitch + 16 * sub;
+#pragma unroll
+                            for (int i = 0; i < (chunk_bytes(F) + 15 + 31) / 32; ++i, q += 32, to += 32) {
+                                if (q >= end) break;
+                                if (q < base) {  // the stack starts inside this window: only its own bytes are read
+                                    for (int b = (int)(base - q); b < 16 && q + b < end; ++b) sts_u8(to + b, q[b]);
+                                    stored = true;
+                                } else {
+                                    const long long m = end - q;
+                                    cp_async_16(to, q, m < 16 ? (uint32_t)m : 16u);
+                                }
+                            }
+                        }
+                        if (stored) {  // plain stores are ordered by a plain arrival
+                            asm volatile("cp.async.wait_all;" ::: "memory");
+                            mbar_arrive(full);
+                        } else {
+                            cp_async_arrive(full);
+                        }
                     }
                 }
-            }
-            if (++stage == a.slots) stage = 0, phase ^= 1;
-            if (++at.round == per_unit) {
-                at.round = 0, fresh = true;
-                if (++at.seg == nseg) at.seg = 0, ++at.tile;
+                if (++stage == a.slots) stage = 0, phase ^= 1;
+                if (++round == per_seg) round = 0, ++seg, fresh = true;
             }
         }
         if (!ALN) asm volatile("cp.async.wait_all;" ::: "memory");
@@ -526,161 +549,177 @@ __global__ void __launch_bounds__(kThreads, 1)
     WarpState st{0, 0, 0, true};
     int half = 0;
     bool wide = false;  // the last unit's sums took the whole buffer
-    int finished_tile = -1, finished = 0;  // kDown: units of one tile whose parts this team has written
+    float* ysum = reinterpret_cast<float*>(smem + red0) + kTeams * kRedFloats + team * y_floats;  // all_segs: [row][row of the tile]
 
-    // kDown: counts them, and the team that completes a tile sums it for every row of x
-    auto settle = [&]() {
-        if (MODE != kDown || !a.done || finished == 0) return;
+    // Units that several teams share.  A team's tail slot holds the piece of the unit that starts in its range, its head
+    // slot that of the unit that started before.
+    auto slot_of = [&](int t, bool tail) { return a.split + ((size_t)2 * t + (tail ? 1 : 0)) * a.split_size; };
+    int j0 = 0, j1 = 0;  // the teams that share the piece's unit
+    auto join = [&](int n, auto value) -> int {
+        const long long t = (long long)(work.u - deal.each * deal.teams) * deal.per;
+        j0 = deal.owner(t), j1 = deal.owner(t + deal.per - 1);
+        float* mine = slot_of(id, id == j0);
+        for (int i = tid; i < n; i += kTeamThreads) mine[i] = value(i);
         team_sync(team);
         if (tid == 0) {
             __threadfence();
-            s_last[team] = atomicAdd(a.done + finished_tile, (unsigned)finished) + finished == (unsigned)nseg;
+            s_last[team] = atomicAdd(a.split_done + j0, 1u) == (unsigned)(j1 - j0);
             __threadfence();
         }
         team_sync(team);
-        if (s_last[team]) {
-            for (int i = tid; i < unit_rows * a.rows; i += kTeamThreads) {
-                const int o = finished_tile * unit_rows + i % unit_rows, x = i / unit_rows;
-                if (o < a.out) a.y[(size_t)x * a.out + o] = combine(a, x, o);
-            }
-        }
-        finished = 0;
+        return s_last[team];
+    };
+    auto joined = [&](int i) {
+        float v = __ldcg(slot_of(j0, true) + i);
+#pragma unroll 4
+        for (int t = j0 + 1; t <= j1; ++t) v += __ldcg(slot_of(t, false) + i);
+        return v;
     };
 
-    while (at.left > 0) {
-        const int tile = at.tile, r0 = at.round, r1 = at.left < per_unit - r0 ? r0 + at.left : per_unit;
-        int first, count, e = 0;
-        if (MODE == kPlain) {
-            first = at.seg * a.seg_cap;
-            count = a.rows - first < a.seg_cap ? a.rows - first : a.seg_cap;
-        } else {
-            e = __ldcg(&a.segs[at.seg].expert);
-            first = __ldcg(&a.segs[at.seg].start);
-            count = __ldcg(&a.segs[at.seg].count);
-        }
-        if (MODE == kDown && tile != finished_tile) settle();
-        // sums of up to 16 rows of x alternate between the buffer's halves; more take it all
-        const int tokens = count <= 16 ? 16 : 32;
-        if (wide || count > 16) team_sync(team);
-        wide = count > 16;
-        float* rb = red + (wide ? 0 : half * (kRedFloats / 2));
-        half ^= 1;
-        UnitArgs u{};
-        u.x = XView{a.x.data, a.x.scale, a.x.sum, (uint32_t)a.bprp};
-        u.order = a.order, u.top_k = a.top_k;
-        u.red = rb + warp * tokens * 16;
-        u.full = bars, u.slots = ring + warp * S::kBytes, u.stages = a.slots;
-        u.first = first, u.count = count;
-        u.c0 = r0 * kws + kw, u.kws = kws, u.rounds = r1 - r0, u.blocks = a.bpr;
-        u.c_end = r1 * kws < steps ? r1 * kws : steps;
-        u.err = a.err, u.dead = &s_dead;
-        if constexpr (!ALN) {
-            const long long off =
-                ((long long)e * a.out + (long long)tile * unit_rows + strip * (MODE == kPair ? 8 : 16) + (lane >> 2)) * a.row_bytes;
-            u.window0 = (uint32_t)(reinterpret_cast<uintptr_t>(a.w[0]) + off) & 15;
-            u.window1 = (uint32_t)(reinterpret_cast<uintptr_t>(a.w[MODE == kPair ? 1 : 0]) + off +
-                                   (MODE == kPair ? 0 : 8 * a.row_bytes)) & 15;
-            u.window_step = chunk_bytes(F) & 15;
-        }
-        if constexpr (FEW) {
-            if (count <= 2)
-                st = unit_sums<FewRows<F, 1>, F, MODE, ALN>(u, st);
-            else
-                st = unit_sums<FewRows<F, 2>, F, MODE, ALN>(u, st);
-        } else {
-            if (count <= 8)
-                st = unit_sums<ManyRows<F, 1>, F, MODE, ALN>(u, st);
-            else if (count <= 16)
-                st = unit_sums<ManyRows<F, 2>, F, MODE, ALN>(u, st);
-            else
-                st = unit_sums<ManyRows<F, 4>, F, MODE, ALN>(u, st);
-        }
-        team_sync(team);
-        auto sum_parts = [&](int tok, int row) {
-            float v = 0.0f;
-            for (int k = 0; k < kws; ++k) v += rb[((k * a.strips + (row >> 4)) * tokens + tok) * 16 + (row & 15)];
-            return v;
-        };
-
-        // the unit's results: get(row of x of the segment, row of the tile as the slots have it)
-        auto epilogue = [&](auto get) {
-            if (MODE == kPair) {
-                // a warp takes a block of 32 hidden values of one row of x, in the lane order of the next product
-                const int blocks = a.strips / 4;
-                for (int i = warp; i < count * blocks; i += kImmaWarps) {
-                    const int tok = i / blocks, b = tile * blocks + i % blocks;
-                    if (32 * b >= a.out) continue;
-                    const int el = FEW ? imma_element(a.next_fmt, b & 1, lane) : half_element(a.next_fmt, b & 1, lane);
-                    const int loc = 32 * (i % blocks) + el;
-                    const int row = (loc >> 3) * 16 + (loc & 7);
-                    const float h = 32 * b + el < a.out ? silu_mul(get(tok, row), get(tok, row + 8)) : 0.0f;
-                    const size_t to = (size_t)(first + tok) * a.next_bprp + b;
-                    if (FEW)
-                        slice_digits(h, a.h.data + (to - b) * kSlicedBytes + digit_block(b), a.h.scale + to, a.h.sum + to, lane);
-                    else
-                        slice_halves(h, a.h.data + to * kSlicedBytes, a.h.scale + to, a.h.sum + to, lane);
-                }
+    while (work.next(deal, id)) {
+        const bool whole = work.r1 - work.r0 == deal.per;
+        const int tile = all_segs ? work.u : work.u / nseg;
+        if (all_segs)
+            for (int i = tid; i < (int)y_floats; i += kTeamThreads) ysum[i] = 0.0f;
+        int seg = all_segs ? work.r0 / per_seg : work.u % nseg;
+        for (int done = work.r0; done < work.r1; ++seg) {
+            const int base = all_segs ? seg * per_seg : 0;
+            const int r0 = done - base, r1 = work.r1 - base < per_seg ? work.r1 - base : per_seg;
+            done = base + r1;
+            int first, count, e = 0;
+            if (MODE == kPlain) {
+                first = seg * a.seg_cap;
+                count = a.rows - first < a.seg_cap ? a.rows - first : a.seg_cap;
             } else {
-                for (int i = tid; i < unit_rows * count; i += kTeamThreads) {
-                    const int tok = i / unit_rows, row = i % unit_rows;
-                    const int o = tile * unit_rows + row;
-                    if (o >= a.out) continue;
-                    float v = get(tok, row);
-                    const int r = first + tok;
-                    if (MODE == kDown) {
-                        a.part[(size_t)__ldcg(a.order + r) * a.out + o] = v;
-                    } else {
-                        if (a.bias) v += a.bias[o];
-                        v = activate(v, a.act);
-                        if (a.row_scale) v *= a.row_scale[r];
-                        const size_t to = (size_t)r * a.out + o;
-                        a.y[to] = a.residual ? a.residual[to] + v : v;
+                e = __ldcg(&a.segs[seg].expert);
+                first = __ldcg(&a.segs[seg].start);
+                count = __ldcg(&a.segs[seg].count);
+            }
+            // sums of up to 16 rows of x alternate between the buffer's halves; more take it all
+            const int tokens = count <= 16 ? 16 : 32;
+            if (wide || count > 16) team_sync(team);
+            wide = count > 16;
+            float* rb = red + (wide ? 0 : half * (kRedFloats / 2));
+            half ^= 1;
+            UnitArgs u{};
+            u.x = XView{a.x.data, a.x.scale, a.x.sum, (uint32_t)a.bprp};
+            u.order = a.order, u.top_k = a.top_k;
+            u.red = rb + warp * tokens * 16;
+            u.full = bars, u.slots = ring + warp * S::kBytes, u.stages = a.slots;
+            u.first = first, u.count = count;
+            u.c0 = r0 * kws + kw, u.kws = kws, u.rounds = r1 - r0, u.blocks = a.bpr;
+            u.c_end = r1 * kws < steps ? r1 * kws : steps;
+            u.err = a.err, u.dead = &s_dead;
+            if constexpr (!ALN) {
+                const long long off =
+                    ((long long)e * a.out + (long long)tile * unit_rows + strip * (MODE == kPair ? 8 : 16) + (lane >> 2)) * a.row_bytes;
+                u.window0 = (uint32_t)(reinterpret_cast<uintptr_t>(a.w[0]) + off) & 15;
+                u.window1 = (uint32_t)(reinterpret_cast<uintptr_t>(a.w[MODE == kPair ? 1 : 0]) + off +
+                                       (MODE == kPair ? 0 : 8 * a.row_bytes)) & 15;
+                u.window_step = chunk_bytes(F) & 15;
+            }
+            if constexpr (FEW) {
+                if (count <= 2)
+                    st = unit_sums<FewRows<F, 1>, F, MODE, ALN>(u, st);
+                else
+                    st = unit_sums<FewRows<F, 2>, F, MODE, ALN>(u, st);
+            } else {
+                if (count <= 8)
+                    st = unit_sums<ManyRows<F, 1>, F, MODE, ALN>(u, st);
+                else if (count <= 16)
+                    st = unit_sums<ManyRows<F, 2>, F, MODE, ALN>(u, st);
+                else
+                    st = unit_sums<ManyRows<F, 4>, F, MODE, ALN>(u, st);
+            }
+            team_sync(team);
+            auto sum_parts = [&](int tok, int row) {
+                float v = 0.0f;
+                for (int k = 0; k < kws; ++k) v += rb[((k * a.strips + (row >> 4)) * tokens + tok) * 16 + (row & 15)];
+                return v;
+            };
+
+            if (all_segs) {
+                // a thread takes a row of the tile and every second row of x, so that no other adds to its sums
+                for (int i = tid; i < 2 * unit_rows; i += kTeamThreads) {
+                    const int row = i % unit_rows, odd = i / unit_rows;
+                    for (int tok = 0; tok < count; ++tok) {
+                        const int pair = __ldcg(a.order + first + tok), x = pair / a.top_k;
+                        if ((x & 1) != odd) continue;
+                        float* to = ysum + x * unit_rows + row;
+                        *to = fmaf(a.weights[pair], sum_parts(tok, row), *to);
                     }
                 }
+                continue;
             }
-        };
 
-        bool complete = true;
-        if (r0 == 0 && r1 == per_unit) {
-            epilogue(sum_parts);
-        } else {
-            // a unit that several teams share: each leaves its sums, the last adds them up in order.  A team's tail slot
-            // holds the unit that starts in its range, its head slot the one that started before.
-            const Deal deal(nseg * a.tiles, per_unit, kTeams * gridDim.x);
-            const long long t = ((long long)tile * nseg + at.seg) * per_unit;
-            const int a0 = deal.owner(t), a1 = deal.owner(t + per_unit - 1);
-            const int slot_rows = 16 * a.strips;
-            const size_t split_size = (size_t)a.split_tokens * slot_rows;
-            float* mine = a.split + ((size_t)2 * id + (id == a0 ? 1 : 0)) * split_size;
-            for (int i = tid; i < slot_rows * count; i += kTeamThreads)
-                mine[(size_t)(i / slot_rows) * slot_rows + i % slot_rows] = sum_parts(i / slot_rows, i % slot_rows);
-            team_sync(team);
-            if (tid == 0) {
-                __threadfence();
-                s_last[team] = atomicAdd(a.split_done + a0, 1u) == (unsigned)(a1 - a0);
-                __threadfence();
+            // the unit's results: get(row of x of the segment, row of the tile as the slots have it)
+            auto epilogue = [&](auto get) {
+                if (MODE == kPair) {
+                    // a warp takes a block of 32 hidden values of one row of x, in the lane order of the next product
+                    const int blocks = a.strips / 4;
+                    for (int i = warp; i < count * blocks; i += kImmaWarps) {
+                        const int tok = i / blocks, b = tile * blocks + i % blocks;
+                        if (32 * b >= a.out) continue;
+                        const int el = FEW ? imma_element(a.next_fmt, b & 1, lane) : half_element(a.next_fmt, b & 1, lane);
+                        const int loc = 32 * (i % blocks) + el;
+                        const int row = (loc >> 3) * 16 + (loc & 7);
+                        const float h = 32 * b + el < a.out ? silu_mul(get(tok, row), get(tok, row + 8)) : 0.0f;
+                        const size_t to = (size_t)(first + tok) * a.next_bprp + b;
+                        if (FEW)
+                            slice_digits(h, a.h.data + (to - b) * kSlicedBytes + digit_block(b), a.h.scale + to, a.h.sum + to, lane);
+                        else
+                            slice_halves(h, a.h.data + to * kSlicedBytes, a.h.scale + to, a.h.sum + to, lane);
+                    }
+                } else {
+                    for (int i = tid; i < unit_rows * count; i += kTeamThreads) {
+                        const int tok = i / unit_rows, row = i % unit_rows;
+                        const int o = tile * unit_rows + row;
+                        if (o >= a.out) continue;
+                        float v = get(tok, row);
+                        const int r = first + tok;
+                        if (MODE == kDown) {
+                            a.part[(size_t)__ldcg(a.order + r) * a.out + o] = v;
+                        } else {
+                            if (a.bias) v += a.bias[o];
+                            v = activate(v, a.act);
+                            if (a.row_scale) v *= a.row_scale[r];
+                            const size_t to = (size_t)r * a.out + o;
+                            a.y[to] = a.residual ? a.residual[to] + v : v;
+                        }
+                    }
+                }
+            };
+            if (whole) {
+                epilogue(sum_parts);
+            } else {
+                // leave the sums of this piece; whoever comes last adds the pieces up in order, in its buffer
+                const int slot_rows = 16 * a.strips, n = slot_rows * count;
+                const int last = join(n, [&](int i) { return sum_parts(i / slot_rows, i % slot_rows); });
+                if (last) {
+                    for (int i = tid; i < n; i += kTeamThreads) rb[i] = joined(i);
+                    team_sync(team);
+                    epilogue([&](int tok, int row) { return rb[tok * slot_rows + row]; });
+                }
+                team_sync(team);  // s_last and, where this was the last piece, rb may be written again
             }
+        }
+        if (all_segs) {
             team_sync(team);
-            complete = s_last[team];
-            team_sync(team);  // s_last may be written again
-            if (complete)
-                epilogue([&](int tok, int row) {
-                    const size_t in = (size_t)tok * slot_rows + row;
-                    float v = __ldcg(a.split + ((size_t)2 * a0 + 1) * split_size + in);
-                    for (int i = a0 + 1; i <= a1; ++i) v += __ldcg(a.split + (size_t)2 * i * split_size + in);
-                    return v;
-                });
+            const int n = a.rows * unit_rows;
+            bool last = true;
+            if (!whole) last = join(n, [&](int i) { return ysum[i]; });
+            if (last)
+                for (int i = tid; i < n; i += kTeamThreads) {
+                    const int o = tile * unit_rows + i % unit_rows;
+                    if (o >= a.out) continue;
+                    const float v = whole ? ysum[i] : joined(i);
+                    const size_t to = (size_t)(i / unit_rows) * a.out + o;
+                    a.y[to] = a.residual ? a.residual[to] + v : v;
+                }
+            team_sync(team);  // ysum and s_last may be written again
         }
-        if (MODE == kDown && complete) {
-            finished_tile = tile;
-            ++finished;
-        }
-        at.left -= r1 - r0;
-        at.round = 0;
-        if (++at.seg == nseg) at.seg = 0, ++at.tile;
     }
-    settle();
-    if (MODE == kDown && nseg == 0 && a.done) {
+    if (all_segs && nseg == 0) {
         // no row names an expert
         const size_t n = (size_t)a.rows * a.out;
         for (size_t i = (size_t)id * kTeamThreads + tid; i < n; i += (size_t)kTeams * gridDim.x * kTeamThreads)
@@ -702,11 +741,12 @@ template <int F, int MODE, bool FEW, bool ALN>
 cudaError_t launch_one(ImmaArgs a, int grid, int smem_per_sm, cudaStream_t stream) {
     using S = Slot<F, ALN>;
     auto k = imma_kernel<F, MODE, FEW, ALN>;
-    const int fixed = kTeams * kRedFloats * 4 + 1024 + 256;  // the system's 1 KB per CTA, the static part
+    const int sums = kTeams * (kRedFloats + (MODE == kDown && !a.part ? a.rows * 16 * a.strips : 0)) * 4;
+    const int fixed = sums + 1024 + 256;  // the system's 1 KB per CTA, the static part
     a.slots = (smem_per_sm - fixed) / (kTeams * (kImmaWarps * S::kBytes + 16));
     if (a.slots > 8) a.slots = 8;
     if (a.slots < 2) return cudaErrorInvalidConfiguration;
-    const size_t smem = (size_t)kTeams * a.slots * (kImmaWarps * S::kBytes + 16) + kTeams * kRedFloats * 4;
+    const size_t smem = (size_t)kTeams * a.slots * (kImmaWarps * S::kBytes + 16) + sums;
     ImmaMaps maps{};
     if (ALN) {
         for (int i = 0; i < (MODE == kPair ? 2 : 1); ++i)
