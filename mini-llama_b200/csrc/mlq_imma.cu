@@ -129,7 +129,7 @@ __global__ void __launch_bounds__(256) prep_kernel(const PrepArgs a) {
         const float* x = a.x + (long long)r * a.in;
         if (a.few) {
             const int at = b * kQK + imma_element(a.fmt, b & 1, lane);
-            slice_digits(at < a.in ? x[at] : 0.0f, a.sliced.data + (i - b) * kSlicedBytes + digit_block(b),
+            slice_digits(at < a.in ? x[at] : 0.0f, digit_weight(a.fmt, lane), a.sliced.data + (i - b) * kSlicedBytes + digit_block(b),
                          a.sliced.scale + i, a.sliced.sum + i, lane);
         } else {
             const int at = b * kQK + half_element(a.fmt, b & 1, lane);

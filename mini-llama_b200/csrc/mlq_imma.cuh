@@ -11,7 +11,10 @@
 //   max|x_block|).  The codes meet the digits in m16n8k32 int8 matrix
 //   instructions: one covers exactly one block of 16 weight rows, its 8 columns are
 //   the digits of 2 rows of x, and every integer sum is exact.  q8_0 codes are
-//   the operand as they are, q4 codes take 3 instructions per 8 weights.
+//   the operand as they are.  q4 codes are unsigned bytes, c from the low nibble
+//   and 16 c from the high one (one mask each); the values of x that meet low
+//   nibbles are carried 16-fold instead, and q4_0's offset of 8 is taken off by
+//   the block's sum of x, in the fold.
 // * more rows: x_i / s = hi + lo in fp16 (error <= 2^-22 |x_i|, s a power of
 //   two per block), codes as fp16, 4 m16n8k16 instructions per block and 8 rows
 //   into one fp32 accumulator.  One column per row instead of 4, and a fold
@@ -96,11 +99,17 @@ __device__ __forceinline__ float warp_sum(float v) {
     return v;
 }
 
-// Slices a block into digits: lane l holds the value at imma_element l.  Two
+// What the value at position l of a sliced q4 block is multiplied with: low
+// nibbles (the first 16 positions) meet 16 x, high ones, which count 16, x.
+__device__ __forceinline__ float digit_weight(int fmt, int l) { return fmt != kQ8_0 && l < 16 ? 16.0f : 1.0f; }
+
+// Slices a block into digits: lane l holds the value at imma_element l, times
+// `weight` in the digits (digit_weight).  Two
 // blocks share 256 bytes, [digit][t][block of the pair][word h]; dig is the
 // pair's start plus 8 bytes for the odd block (digit_block).  A block with a value that is not finite gets the scale NaN: every output that
 // reads it is NaN.
-__device__ __forceinline__ void slice_digits(float v, uint8_t* dig, float* scale, float* sum, int lane) {
+__device__ __forceinline__ void slice_digits(float x, float weight, uint8_t* dig, float* scale, float* sum, int lane) {
+    const float v = x * weight;
     const float amax = block_amax(v);
     const bool bad = !(amax == amax);
     const uint32_t s = block_scale(bad ? 0.0f : amax, 30, 2139062016.0f);  // below 127 * 16843009: four digits hold it
@@ -123,7 +132,7 @@ __device__ __forceinline__ void slice_digits(float v, uint8_t* dig, float* scale
     }
     const int h = lane >> 4, t = (lane >> 2) & 3;
     *reinterpret_cast<uint32_t*>(dig + j * 64 + t * 16 + h * 4) = out;
-    const float total = warp_sum(v);
+    const float total = warp_sum(x);
     if (lane == 0) {
         *scale = bad ? __uint_as_float(0x7fc00000u) : inverse_scale(s);
         *sum = total;
@@ -148,11 +157,19 @@ __device__ __forceinline__ void slice_halves(float v, uint8_t* out, float* scale
     }
 }
 
-__device__ __forceinline__ void imma_s8(int (&c)[4], const uint32_t (&a)[4], uint2 b) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
-        : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y), "r"(0));
+// D = A B for 16 rows x 32 codes, signed (q8_0) or unsigned (q4), and digits.
+template <int F>
+__device__ __forceinline__ void imma(int (&c)[4], const uint32_t (&a)[4], uint2 b) {
+    if constexpr (F == kQ8_0)
+        asm volatile(
+            "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+            : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y), "r"(0));
+    else
+        asm volatile(
+            "mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+            : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y), "r"(0));
 }
 
 __device__ __forceinline__ void hmma_f16(float (&c)[4], const uint32_t* a, uint32_t b0, uint32_t b1) {
@@ -266,26 +283,20 @@ __device__ __forceinline__ void load_pair(const RowBase& r, RawA& even, RawA& od
             even.w[i][0] = lds_word<ALN, b + 4>(r.word[i]);
             odd.w[i][0] = lds_word<ALN, b + 24>(r.word[i]);
             even.d[i] = low_half(w0);
-            even.m[i] = fmaf(8.0f, even.d[i], high_half(w0));  // d c + m = d (c - 8) + (m + 8 d)
+            even.m[i] = high_half(w0);
             odd.d[i] = low_half(w5);
-            odd.m[i] = fmaf(8.0f, odd.d[i], high_half(w5));
+            odd.m[i] = high_half(w5);
         }
     }
 }
 
-// The A operand of the int8 instruction.  q4 codes as signed bytes
-// 16 * (c - 8): one shift and two masks for 8 codes.
+// The A operand of the int8 instruction.
 template <int F>
 __device__ __forceinline__ void int8_operand(const RawA& r, uint32_t (&a)[4]) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        if (F == kQ8_0) {
-            a[i] = r.w[i][0];
-            a[2 + i] = r.w[i][1];
-        } else {
-            a[i] = ((r.w[i][0] << 4) & 0xf0f0f0f0u) ^ 0x80808080u;
-            a[2 + i] = (r.w[i][0] & 0xf0f0f0f0u) ^ 0x80808080u;
-        }
+        a[i] = F == kQ8_0 ? r.w[i][0] : r.w[i][0] & 0x0f0f0f0fu;
+        a[2 + i] = F == kQ8_0 ? r.w[i][1] : r.w[i][0] & 0xf0f0f0f0u;
     }
 }
 
@@ -315,11 +326,13 @@ __device__ __forceinline__ void half_operand(const RawA& r, uint32_t (&a)[8]) {
             }
         } else {
             const uint32_t v = r.w[i][0], v8 = v >> 8;
-            // low nibbles: 1024 + c - 1032; high ones: (1024 + 16 c) / 16 - 72
-            a[i] = hsub2_bits((v & 0x000f000fu) | 0x64006400u, 0x64086408u);
-            a[2 + i] = hfma2_bits((v & 0x00f000f0u) | 0x64006400u, 0x2c002c00u, 0xd480d480u);
-            a[4 + i] = hsub2_bits((v8 & 0x000f000fu) | 0x64006400u, 0x64086408u);
-            a[6 + i] = hfma2_bits((v8 & 0x00f000f0u) | 0x64006400u, 0x2c002c00u, 0xd480d480u);
+            // low nibbles: 1024 + c - 1032 (q4_1, whose codes have no offset: - 1024); high ones: (1024 + 16 c) / 16 - 72
+            // (- 64)
+            constexpr uint32_t lo = F == kQ4_0 ? 0x64086408u : 0x64006400u, hi = F == kQ4_0 ? 0xd480d480u : 0xd400d400u;
+            a[i] = hsub2_bits((v & 0x000f000fu) | 0x64006400u, lo);
+            a[2 + i] = hfma2_bits((v & 0x00f000f0u) | 0x64006400u, 0x2c002c00u, hi);
+            a[4 + i] = hsub2_bits((v8 & 0x000f000fu) | 0x64006400u, lo);
+            a[6 + i] = hfma2_bits((v8 & 0x00f000f0u) | 0x64006400u, 0x2c002c00u, hi);
         }
     }
 }

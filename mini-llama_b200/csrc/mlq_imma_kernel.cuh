@@ -48,7 +48,7 @@ struct FewRows {
     const float4* sp[NT];
     ptrdiff_t to_sum;     // from a scale to the block's sum
     uint4 b[NT][2][2];    // [.][half of a K step][pair of blocks]
-    float4 s[NT][2], m[F == kQ4_1 ? NT : 1][2];
+    float4 s[NT][2], m[F != kQ8_0 ? NT : 1][2];  // scales; sums of x
     float acc[NT][2], accm[F == kQ4_1 ? NT : 1][2];
 
     template <class TokenOf>
@@ -74,7 +74,7 @@ struct FewRows {
         for (int i = 0; i < NT; ++i) {
             b[i][h][0] = xp[i][32 * h], b[i][h][1] = xp[i][32 * h + 16];
             s[i][h] = sp[i][h];
-            if (F == kQ4_1) m[i][h] = sp[i][h + to_sum];
+            if (F != kQ8_0) m[i][h] = sp[i][h + to_sum];
         }
     }
 
@@ -83,6 +83,7 @@ struct FewRows {
     template <bool ALN, class Wait>
     __device__ __forceinline__ void step(int ahead, int valid, uint32_t r0, uint32_t r1, int lane, Wait wait) {
         const RowBase rows = row_base(r0, r1, lane & 3);
+        const float offset = lane & 1 ? 0.0f : -8.0f * 16.0f / 65536.0f;
         static_for<2>([&](auto hc) {
             constexpr int h = decltype(hc)::value;
             if (h == 0) {
@@ -112,14 +113,19 @@ struct FewRows {
                         const float4 s4 = s[i][h];
                         const float sx = p2 ? (o ? s4.w : s4.z) : (o ? s4.y : s4.x);
                         int c[4];
-                        imma_s8(c, op, o ? make_uint2(x.z, x.w) : make_uint2(x.x, x.y));
-                        acc[i][0] = fmaf(A[o].d[0] * sx, (float)(c[0] * 256 + c[1]), acc[i][0]);
-                        acc[i][1] = fmaf(A[o].d[1] * sx, (float)(c[2] * 256 + c[3]), acc[i][1]);
-                        if (F == kQ4_1) {
+                        imma<F>(c, op, o ? make_uint2(x.z, x.w) : make_uint2(x.x, x.y));
+                        const float v[2] = {(float)(c[0] * 256 + c[1]), (float)(c[2] * 256 + c[3])};
+                        float mx = 0.0f;
+                        if (F != kQ8_0) {
                             const float4 m4 = m[i][h];
-                            const float mx = p2 ? (o ? m4.w : m4.z) : (o ? m4.y : m4.x);
-                            accm[i][0] = fmaf(A[o].m[0], mx, accm[i][0]);
-                            accm[i][1] = fmaf(A[o].m[1], mx, accm[i][1]);
+                            mx = p2 ? (o ? m4.w : m4.z) : (o ? m4.y : m4.x);
+                        }
+#pragma unroll
+                        for (int q = 0; q < 2; ++q) {
+                            // q4_0: sum of (c - 8) x, in the unit of digits 3 and 2 (see store); lanes of digits 1, 0 take none
+                            const float u = F == kQ4_0 ? fmaf(v[q], sx, mx * offset) : v[q] * sx;
+                            acc[i][q] = fmaf(A[o].d[q], u, acc[i][q]);
+                            if (F == kQ4_1) accm[i][q] = fmaf(A[o].m[q], mx, accm[i][q]);
                         }
                     }
                 }
@@ -666,7 +672,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         const float h = 32 * b + el < a.out ? silu_mul(get(tok, row), get(tok, row + 8)) : 0.0f;
                         const size_t to = (size_t)(first + tok) * a.next_bprp + b;
                         if (FEW)
-                            slice_digits(h, a.h.data + (to - b) * kSlicedBytes + digit_block(b), a.h.scale + to, a.h.sum + to, lane);
+                            slice_digits(h, digit_weight(a.next_fmt, lane), a.h.data + (to - b) * kSlicedBytes + digit_block(b), a.h.scale + to, a.h.sum + to, lane);
                         else
                             slice_halves(h, a.h.data + to * kSlicedBytes, a.h.scale + to, a.h.sum + to, lane);
                     }

@@ -4,13 +4,15 @@ with an epilogue, with elementwise error bounds of the library's arithmetic
 
 The bounds follow the arithmetic in include/mlq.h, not a measurement:
 * a value x in a block with largest magnitude A is carried either as 31-bit
-  fixed point (half a step: below 1.01 * 2^-31 A) or as two fp16 values (each
+  fixed point (half a step: below 1.01 * 2^-31 A; for q4 the block holds 16-fold
+  values too, so 2^-27 A) or as two fp16 values (each
   rounding 2^-11 relative: 2^-22 |x|, and at most 2^-39 A where the second is
   subnormal); the sum of both bounds covers either;
 * integer sums of a block are exact.  The fp32 steps round by 2^-24 relative
   each: per block one conversion of the integer sum, one product and one sum, then a
-  few for the parts of the K axis -- counted as (blocks + 16) roundings of the sum
-  of magnitudes (each sum's partial values stay below it).  The fp16 form's sums
+  few for the parts of the K axis, and 5 in a block's sum of x (q4) -- counted as
+  (blocks + 16) roundings of the sum of magnitudes (each sum's partial values stay
+  below it).  The fp16 form's sums
   are made by the matrix unit, which may truncate: 4 instructions per
   block, 2^-22 of that block's magnitudes each, 16 roundings more in all."""
 from __future__ import annotations
@@ -58,11 +60,11 @@ def dequantize64(fmt, blocks, rows, cols):
         code = np.concatenate((code & 15, code >> 4), 1).astype(np.float64)
         if fmt == "q4_0":
             w = (code - 8) * d
-            mag = np.abs(w)
+            mag = (code + 8) * np.abs(d)  # summed as c x and 8 x apart
         else:
             m = raw[:, 2:4].copy().view(np.float16).astype(np.float64)
             w = code * d + m
-            mag = np.abs((code - 8) * d) + np.abs(m + 8 * d)  # summed as d (c - 8) and m + 8 d apart
+            mag = code * np.abs(d) + np.abs(m)  # summed as d c x and m x apart
     return w.reshape(rows, nb * 32)[:, :cols], mag.reshape(rows, nb * 32)[:, :cols]
 
 
@@ -79,7 +81,7 @@ def product(x, fmt, blocks, out, dx=None):
     """x W^T in float64 and its bound; dx: an elementwise error of x already there."""
     w, mag = dequantize64(fmt, blocks, out, x.shape[1])
     xa = np.abs(x) + (0 if dx is None else dx)
-    step = 2.0 ** -22 * xa + 1.01 * 2.0 ** -31 * block_max(xa)
+    step = 2.0 ** -22 * xa + 1.01 * 2.0 ** -27 * block_max(xa)
     nb = (x.shape[1] + 31) // 32
     bound = step @ np.abs(w).T + (nb + 32) * EPS * ((xa + step) @ mag.T)
     if dx is not None:
