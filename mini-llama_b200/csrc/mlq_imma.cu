@@ -55,11 +55,12 @@ __global__ void __launch_bounds__(256) prep_kernel(const PrepArgs a) {
             __shared__ int wsum[2][8];
             __shared__ unsigned char in_warp[8][MLQ_MOE_MAX_EXPERTS];
             for (int e = threadIdx.x; e < a.n_experts; e += 256) cnt[e] = 0;
-            const int pad = a.h_bprp - a.h_bpr;
+            const int pad = a.few ? a.h_bprp - a.h_bpr : 0;  // halves past a row's end are not read
             for (int i = threadIdx.x; i < a.pairs * pad; i += 256) {
-                const size_t at = (size_t)(i / pad) * a.h_bprp + a.h_bpr + i % pad;
-                a.h.scale[at] = 0.0f;
-                a.h.sum[at] = 0.0f;
+                const int b = a.h_bpr + i % pad;
+                float* at = reinterpret_cast<float*>(a.h.data + ((size_t)(i / pad) * (a.h_bprp / kChunkBlocks) + b / kChunkBlocks) *
+                                                                    kRecordBytes + kRecordScales) + b % kChunkBlocks;
+                at[0] = at[kChunkBlocks] = 0.0f;
             }
             __syncthreads();
             for (int p = threadIdx.x; p < a.pairs; p += 256) {
@@ -129,8 +130,8 @@ __global__ void __launch_bounds__(256) prep_kernel(const PrepArgs a) {
         const float* x = a.x + (long long)r * a.in;
         if (a.few) {
             const int at = b * kQK + imma_element(a.fmt, b & 1, lane);
-            slice_digits(at < a.in ? x[at] : 0.0f, digit_weight(a.fmt, lane), a.sliced.data + (i - b) * kSlicedBytes + digit_block(b),
-                         a.sliced.scale + i, a.sliced.sum + i, lane);
+            slice_digits(at < a.in ? x[at] : 0.0f, digit_weight(a.fmt, lane),
+                         a.sliced.data + (size_t)r * (a.bprp / kChunkBlocks) * kRecordBytes, b, lane);
         } else {
             const int at = b * kQK + half_element(a.fmt, b & 1, lane);
             slice_halves(at < a.in ? x[at] : 0.0f, a.sliced.data + i * kSlicedBytes, a.sliced.scale + i, a.sliced.sum + i,
@@ -177,8 +178,13 @@ struct Carve {
         p += align256(n * sizeof(T));
         return r;
     }
-    Sliced take_sliced(size_t rows, int bprp) {
-        Sliced s;
+    // records (few rows) or data, scales and sums apart
+    Sliced take_sliced(size_t rows, int bprp, bool few) {
+        Sliced s{};
+        if (few) {
+            s.data = take<uint8_t>(rows * (bprp / kChunkBlocks) * kRecordBytes);
+            return s;
+        }
         s.data = take<uint8_t>(rows * bprp * kSlicedBytes);
         s.scale = take<float>(rows * bprp);
         s.sum = take<float>(rows * bprp);
@@ -197,6 +203,9 @@ constexpr int kMaxPassRows = 16384;       // rows of one pass of a linear at mos
 constexpr int kCombineRows = 32;          // more rows: the sum over slots is a launch of its own
 
 int split_tokens(int rows) { return rows < kSegTokens ? rows : kSegTokens; }
+
+// Rows of x of a segment at most in the form of few rows.
+int few_cap(int rows) { return rows < kFewRows ? (rows < 3 ? rows : kFewRows) : kFewRows; }
 
 // Two slots per team of at most 128 rows, and the counters of two launches.
 size_t split_bytes(int rows) {
@@ -258,7 +267,7 @@ cudaError_t launch_linear_epilogue(int fmt, const uint8_t* w, int out, int in, c
         p.x = x + (long long)r0 * in;
         p.rows = n, p.in = in, p.bpr = bpr, p.bprp = bprp, p.fmt = fmt;
         p.few = n <= kFewRows;
-        p.sliced = c.take_sliced(n, bprp);
+        p.sliced = c.take_sliced(n, bprp, p.few);
         float* split = c.take<float>((size_t)2 * kMaxTeams * split_tokens(n) * 128);
         p.split_done = c.take<unsigned int>(2 * kMaxTeams);
         cudaError_t e = launch_pdl(prep_kernel, prep_ctas((long long)n * bprp, sm_count), 256, 0, stream, p);
@@ -267,9 +276,9 @@ cudaError_t launch_linear_epilogue(int fmt, const uint8_t* w, int out, int in, c
         a.w[0] = w;
         a.total_rows = out, a.out = out, a.bpr = bpr, a.bprp = bprp;
         a.few = p.few;
-        a.seg_cap = p.few ? kFewRows : kSegTokens;
+        a.seg_cap = p.few ? few_cap(n) : kSegTokens;
         const int nseg = (n + a.seg_cap - 1) / a.seg_cap;
-        a.strips = choose_strips(out, bpr, nseg, false, sm_count, 1);
+        a.strips = choose_strips(out, bpr, nseg, false, sm_count, p.few ? a.seg_cap : 1);
         a.tiles = (out + 16 * a.strips - 1) / (16 * a.strips);
         a.x = p.sliced;
         a.rows = n;
@@ -291,7 +300,7 @@ size_t experts_workspace_bytes(const MoeShape& s, int rows, int top_k) {
     const int pass = experts_pass_rows(s, rows, top_k);
     const int bprp = padded_blocks((s.in + kQK - 1) / kQK), hp = padded_blocks((s.hidden + kQK - 1) / kQK);
     auto bytes = [&](int n) {
-        const int pairs = n * top_k, cap = few_rows(pairs, s.n_experts) ? kFewRows : kSegTokens;
+        const int pairs = n * top_k, cap = few_rows(pairs, s.n_experts) ? few_cap(n) : kSegTokens;
         return 256 + align256((size_t)max_segments(pairs, s.n_experts, cap) * sizeof(Segment)) +
                align256((size_t)pairs * sizeof(int)) + sliced_bytes(n, bprp) + sliced_bytes(pairs, hp) +
                (n <= kCombineRows ? 0 : align256((size_t)pairs * s.out * sizeof(float))) + split_bytes(pairs);
@@ -312,10 +321,10 @@ cudaError_t launch_experts(const MoeShape& s, const uint8_t* gate, const uint8_t
     for (int r0 = 0; r0 < rows; r0 += pass) {
         const int n = rows - r0 < pass ? rows - r0 : pass, pairs = n * top_k;
         const bool few = few_rows(pairs, s.n_experts);
-        const int cap = few ? kFewRows : kSegTokens;
+        const int cap = few ? few_cap(n) : kSegTokens;
         const int nseg_max = max_segments(pairs, s.n_experts, cap);
         const int nseg_likely = pairs < s.n_experts ? pairs : nseg_max;
-        const int strips = choose_strips(s.out, hb, nseg_likely, n <= kCombineRows, sm_count, 1);
+        const int strips = choose_strips(s.out, hb, nseg_likely, n <= kCombineRows, sm_count, few ? cap : 1);
         const int tiles = (s.out + 16 * strips - 1) / (16 * strips);
         Carve c{static_cast<uint8_t*>(ws)};
         PrepArgs p{};
@@ -325,10 +334,10 @@ cudaError_t launch_experts(const MoeShape& s, const uint8_t* gate, const uint8_t
         p.x = x + (long long)r0 * s.in;
         p.rows = n, p.in = s.in, p.bpr = bpr, p.bprp = bprp, p.fmt = s.fmt;
         p.few = few, p.seg_cap = cap;
-        p.sliced = c.take_sliced(n, bprp);
+        p.sliced = c.take_sliced(n, bprp, p.few);
         p.ids = ids + (long long)r0 * top_k;
         p.pairs = pairs, p.n_experts = s.n_experts;
-        p.h = c.take_sliced(pairs, hp);
+        p.h = c.take_sliced(pairs, hp, few);
         p.h_bpr = hb, p.h_bprp = hp;
         float* part = c.take<float>(n <= kCombineRows ? 0 : (size_t)pairs * s.out);
         float* split = c.take<float>((size_t)2 * kMaxTeams * split_tokens(pairs) * 128);

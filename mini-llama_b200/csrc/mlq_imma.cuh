@@ -71,8 +71,16 @@ __device__ __forceinline__ int half_element(int fmt, int odd, int l) {
     return imma_element(fmt, odd, 16 * h + 4 * t + j);
 }
 
-// Where block b of a row sliced into digits starts (see slice_digits).
-__host__ __device__ constexpr int digit_block(int b) { return (b >> 1) * 2 * kSlicedBytes + (b & 1) * 8; }
+// A row sliced into digits is a sequence of records, one per K step: 8 blocks
+// of digits, their scales, their sums of x.  One bulk copy brings a record to
+// shared memory.
+constexpr int kRecordBytes = kChunkBlocks * (kSlicedBytes + 8);
+constexpr int kRecordScales = kChunkBlocks * kSlicedBytes, kRecordSums = kRecordScales + kChunkBlocks * 4;
+
+// Where block b of a row's records has its digits (see slice_digits).
+__host__ __device__ constexpr int digit_block(int b) {
+    return (b / kChunkBlocks) * kRecordBytes + (b % kChunkBlocks / 2) * 2 * kSlicedBytes + (b & 1) * 8;
+}
 
 // The power of two 2^k whose product with amax is in (limit / 2, limit], as
 // bits; top: floor(log2 limit).  Clamped so that 2^-k is a normal number.
@@ -105,10 +113,10 @@ __device__ __forceinline__ float digit_weight(int fmt, int l) { return fmt != kQ
 
 // Slices a block into digits: lane l holds the value at imma_element l, times
 // `weight` in the digits (digit_weight).  Two
-// blocks share 256 bytes, [digit][t][block of the pair][word h]; dig is the
-// pair's start plus 8 bytes for the odd block (digit_block).  A block with a value that is not finite gets the scale NaN: every output that
+// blocks share 256 bytes, [digit][t][block of the pair][word h].  A block with a value that is not finite gets the scale NaN: every output that
 // reads it is NaN.
-__device__ __forceinline__ void slice_digits(float x, float weight, uint8_t* dig, float* scale, float* sum, int lane) {
+// row: the row's first record, b the block.
+__device__ __forceinline__ void slice_digits(float x, float weight, uint8_t* row, int b, int lane) {
     const float v = x * weight;
     const float amax = block_amax(v);
     const bool bad = !(amax == amax);
@@ -131,11 +139,12 @@ __device__ __forceinline__ void slice_digits(float x, float weight, uint8_t* dig
         out |= ((from >> (8 * j)) & 0xffu) << (8 * k);
     }
     const int h = lane >> 4, t = (lane >> 2) & 3;
-    *reinterpret_cast<uint32_t*>(dig + j * 64 + t * 16 + h * 4) = out;
+    *reinterpret_cast<uint32_t*>(row + digit_block(b) + j * 64 + t * 16 + h * 4) = out;
     const float total = warp_sum(x);
     if (lane == 0) {
-        *scale = bad ? __uint_as_float(0x7fc00000u) : inverse_scale(s);
-        *sum = total;
+        float* at = reinterpret_cast<float*>(row + (b / kChunkBlocks) * kRecordBytes + kRecordScales) + b % kChunkBlocks;
+        at[0] = bad ? __uint_as_float(0x7fc00000u) : inverse_scale(s);
+        at[kChunkBlocks] = total;
     }
 }
 
@@ -227,6 +236,22 @@ __device__ __forceinline__ uint32_t lds_word(uint32_t a) {
         asm volatile("ld.shared.u32 %0, [%1+%2];" : "=r"(hi) : "r"(w), "n"(OFF + 4));
         return __funnelshift_r(lo, hi, 8 * (a & 3));
     }
+}
+
+template <int OFF>
+__device__ __forceinline__ uint4 lds_u4_at(uint32_t a) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4+%5];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "r"(a), "n"(OFF));
+    return v;
+}
+
+template <int OFF>
+__device__ __forceinline__ float2 lds_f2_at(uint32_t a) {
+    float2 v;
+    asm volatile("ld.shared.v2.f32 {%0,%1}, [%2+%3];" : "=f"(v.x), "=f"(v.y) : "r"(a), "n"(OFF));
+    return v;
 }
 
 __device__ __forceinline__ float low_half(uint32_t w) {

@@ -44,92 +44,61 @@ struct XView {
 // 1 and 0 (t odd) of row t / 2, and the two are added once, at the end.
 template <int F, int NT>
 struct FewRows {
-    const uint4* xp[NT];  // x of the K step
-    const float4* sp[NT];
-    ptrdiff_t to_sum;     // from a scale to the block's sum
-    uint4 b[NT][2][2];    // [.][half of a K step][pair of blocks]
-    float4 s[NT][2], m[F != kQ8_0 ? NT : 1][2];  // scales; sums of x
+    uint32_t xo[NT], so[NT];  // a lane's digits and scales in the step's records
     float acc[NT][2], accm[F == kQ4_1 ? NT : 1][2];
 
-    template <class TokenOf>
-    __device__ __forceinline__ void init(const XView& a, int count, int block, int lane, TokenOf token) {
+    __device__ __forceinline__ void init(int count, int lane) {
         const int g = lane >> 2, t = lane & 3;
-        to_sum = reinterpret_cast<const float4*>(a.sum) - reinterpret_cast<const float4*>(a.scale);
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
             // columns without a row of x repeat the first one's; nothing reads them
             const int r = 2 * i + (g >> 2), rs = 2 * i + (t >> 1);
-            xp[i] = reinterpret_cast<const uint4*>(
-                a.data + ((size_t)token(r < count ? r : 0) * a.bprp + block) * kSlicedBytes + (g & 3) * 64 + t * 16);
-            sp[i] = reinterpret_cast<const float4*>(a.scale + (size_t)token(rs < count ? rs : 0) * a.bprp + block);
+            xo[i] = (r < count ? r : 0) * kRecordBytes + (g & 3) * 64 + t * 16;
+            so[i] = (rs < count ? rs : 0) * kRecordBytes + kRecordScales;
             acc[i][0] = acc[i][1] = 0.0f;
             if (F == kQ4_1) accm[i][0] = accm[i][1] = 0.0f;
         }
-        load_x(0);
     }
 
-    // Half h of the x registers: four blocks of the K step.
-    __device__ __forceinline__ void load_x(int h) {
-#pragma unroll
-        for (int i = 0; i < NT; ++i) {
-            b[i][h][0] = xp[i][32 * h], b[i][h][1] = xp[i][32 * h + 16];
-            s[i][h] = sp[i][h];
-            if (F != kQ8_0) m[i][h] = sp[i][h + to_sum];
-        }
-    }
-
-    // One K step of 8 blocks: while four are multiplied, the next four (of this step, then of the next one, `ahead`
-    // blocks on) are fetched.
-    template <bool ALN, class Wait>
-    __device__ __forceinline__ void step(int ahead, int valid, uint32_t r0, uint32_t r1, int lane, Wait wait) {
+    // One K step of 8 blocks; x: the records of the segment's rows.
+    template <bool ALN>
+    __device__ __forceinline__ void step(uint32_t x, int valid, uint32_t r0, uint32_t r1, int lane) {
         const RowBase rows = row_base(r0, r1, lane & 3);
         const float offset = lane & 1 ? 0.0f : -8.0f * 16.0f / 65536.0f;
-        static_for<2>([&](auto hc) {
-            constexpr int h = decltype(hc)::value;
-            if (h == 0) {
-                load_x(1);
-                wait();
-            } else {
+        static_for<kChunkBlocks / 2>([&](auto pc) {
+            constexpr int p = decltype(pc)::value;
+            if (!ALN && 2 * p >= valid) return;
+            uint4 b[NT];
+            float2 s[NT], m[NT];
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+                b[i] = lds_u4_at<256 * p>(x + xo[i]);
+                s[i] = lds_f2_at<8 * p>(x + so[i]);
+                if (F != kQ8_0) m[i] = lds_f2_at<8 * p + 4 * kChunkBlocks>(x + so[i]);
+            }
+            RawA A[2];
+            load_pair<F, ALN, p>(rows, A[0], A[1]);
+            if (!ALN && 2 * p + 1 >= valid) A[1].d[0] = A[1].d[1] = A[1].m[0] = A[1].m[1] = 0.0f;
+#pragma unroll
+            for (int o = 0; o < 2; ++o) {
+                uint32_t op[4];
+                int8_operand<F>(A[o], op);
 #pragma unroll
                 for (int i = 0; i < NT; ++i) {
-                    xp[i] += ahead * (kSlicedBytes / 16);
-                    sp[i] += ahead / 4;
-                }
-                load_x(0);
-            }
-            static_for<2>([&](auto pc) {
-                constexpr int p2 = decltype(pc)::value, p = 2 * h + p2;
-                if (!ALN && 2 * p >= valid) return;
-                RawA A[2];
-                load_pair<F, ALN, p>(rows, A[0], A[1]);
-                if (!ALN && 2 * p + 1 >= valid) A[1].d[0] = A[1].d[1] = A[1].m[0] = A[1].m[1] = 0.0f;
+                    const float sx = o ? s[i].y : s[i].x;
+                    const float mx = F == kQ8_0 ? 0.0f : (o ? m[i].y : m[i].x);
+                    int c[4];
+                    imma<F>(c, op, o ? make_uint2(b[i].z, b[i].w) : make_uint2(b[i].x, b[i].y));
+                    const float v[2] = {(float)(c[0] * 256 + c[1]), (float)(c[2] * 256 + c[3])};
 #pragma unroll
-                for (int o = 0; o < 2; ++o) {
-                    uint32_t op[4];
-                    int8_operand<F>(A[o], op);
-#pragma unroll
-                    for (int i = 0; i < NT; ++i) {
-                        const uint4 x = b[i][h][p2];
-                        const float4 s4 = s[i][h];
-                        const float sx = p2 ? (o ? s4.w : s4.z) : (o ? s4.y : s4.x);
-                        int c[4];
-                        imma<F>(c, op, o ? make_uint2(x.z, x.w) : make_uint2(x.x, x.y));
-                        const float v[2] = {(float)(c[0] * 256 + c[1]), (float)(c[2] * 256 + c[3])};
-                        float mx = 0.0f;
-                        if (F != kQ8_0) {
-                            const float4 m4 = m[i][h];
-                            mx = p2 ? (o ? m4.w : m4.z) : (o ? m4.y : m4.x);
-                        }
-#pragma unroll
-                        for (int q = 0; q < 2; ++q) {
-                            // q4_0: sum of (c - 8) x, in the unit of digits 3 and 2 (see store); lanes of digits 1, 0 take none
-                            const float u = F == kQ4_0 ? fmaf(v[q], sx, mx * offset) : v[q] * sx;
-                            acc[i][q] = fmaf(A[o].d[q], u, acc[i][q]);
-                            if (F == kQ4_1) accm[i][q] = fmaf(A[o].m[q], mx, accm[i][q]);
-                        }
+                    for (int q = 0; q < 2; ++q) {
+                        // q4_0: sum of (c - 8) x, in the unit of digits 3 and 2 (see store); lanes of digits 1, 0 take none
+                        const float u = F == kQ4_0 ? fmaf(v[q], sx, mx * offset) : v[q] * sx;
+                        acc[i][q] = fmaf(A[o].d[q], u, acc[i][q]);
+                        if (F == kQ4_1) accm[i][q] = fmaf(A[o].m[q], mx, accm[i][q]);
                     }
                 }
-            });
+            }
         });
     }
 
@@ -197,10 +166,9 @@ struct ManyRows {
 
     // One K step of 8 blocks: while up to 16 rows of a block are multiplied, the next ones (then the next block's, then
     // the next step's, `ahead` blocks on) are fetched.
-    template <bool ALN, class Wait>
-    __device__ __forceinline__ void step(int ahead, int valid, uint32_t r0, uint32_t r1, int lane, Wait wait) {
+    template <bool ALN>
+    __device__ __forceinline__ void step(int ahead, int valid, uint32_t r0, uint32_t r1, int lane) {
         const RowBase rows = row_base(r0, r1, lane & 3);
-        wait();
         static_for<kChunkBlocks / 2>([&](auto pc) {
             constexpr int p = decltype(pc)::value;
             if (2 * p >= valid) return;
@@ -279,6 +247,8 @@ __device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
 }
 
 constexpr int kTeams = 2;
+// Records of a round: (K parts) x (rows of x of a segment) <= 8, see choose_strips.
+constexpr int kXStage = 8 * kRecordBytes;
 constexpr int kThreads = 32 * kTeams * (kImmaWarps + 2);  // computing warps, then two producer warps per team
 constexpr int kTeamThreads = 32 * kImmaWarps;
 // Registers: the launch has 96 per thread (65536 / 640, in eights); the
@@ -341,6 +311,16 @@ struct Work {
     }
 };
 
+// What a producer fetches next: round `round` of a tile against a segment, into `stage`.
+struct Cursor {
+    Work work;
+    int r, tile, seg, round, row0, first, count, stage, phase, n;  // r: round of the piece; n: rounds so far
+    bool on, fresh;
+    __device__ __forceinline__ explicit Cursor(const Work& w)
+        : work(w), r(0), tile(0), seg(0), round(0), row0(0), first(0), count(0), stage(0), phase(1), n(0), on(false),
+          fresh(true) {}
+};
+
 // A computing warp's place in its team's ring.
 struct WarpState {
     int stage, phase, taken;
@@ -350,10 +330,11 @@ struct WarpState {
 // What a computing warp needs for its part of a unit (by value: the function
 // below has registers of its own).
 struct UnitArgs {
-    XView x;
+    XView x;                 // halves
     const int* order;        // kPair: position -> pair
     float* red;              // this warp's sums
     uint32_t full, slots;    // barrier of stage 0 (16 bytes each: full, empty), this warp's slot of stage 0
+    uint32_t stage_bytes, to_x;  // from the slot to the records of this warp's K part
     int stages;
     int top_k, first, count;
     int c0, c_end, kws;      // K steps: c0, c0 + kws, .. below c_end
@@ -365,36 +346,39 @@ struct UnitArgs {
 
 // The rounds of one unit: this warp's strip against the segment's rows of x,
 // its sums to u.red.  A function of its own for each form of x.
-template <class Acc, int F, int MODE, bool ALN>
+template <class Acc, int F, int MODE, bool FEW, bool ALN>
 __device__ __forceinline__ WarpState unit_sums(const UnitArgs u, WarpState st) {
     using S = Slot<F, ALN>;
-    constexpr uint32_t kStage = kImmaWarps * S::kBytes;
     const int lane = threadIdx.x & 31, g = lane >> 2;
     int c = u.c0;
     Acc acc;
-    acc.init(u.x, u.count, (c < u.c_end ? c : 0) * kChunkBlocks, lane, [&](int r) -> int {
-        if (MODE == kPair) return __ldcg(u.order + u.first + r) / u.top_k;
-        return u.first + r;
-    });
+    if constexpr (FEW)
+        acc.init(u.count, lane);
+    else
+        acc.init(u.x, u.count, (c < u.c_end ? c : 0) * kChunkBlocks, lane, [&](int r) -> int {
+            if (MODE == kPair) return __ldcg(u.order + u.first + r) / u.top_k;
+            return u.first + r;
+        });
     for (int r = 0; r < u.rounds; ++r, c += u.kws) {
-        const uint32_t full = u.full + 16 * st.stage;
-        auto wait = [&]() {
-            if (__all_sync(0xffffffffu, mbar_try_wait(full, st.phase)) || !st.alive) return;
-            if (!__all_sync(0xffffffffu, mbar_wait(full, st.phase))) {
-                st.alive = false;
-                if (lane == 0) report_error(u.err, 30), *u.dead = 1;
-            }
-        };
+        const uint32_t full = u.full + 16 * st.stage, at = u.slots + st.stage * u.stage_bytes;
+        if (!__all_sync(0xffffffffu, mbar_try_wait(full, st.phase)) && st.alive &&
+            !__all_sync(0xffffffffu, mbar_wait(full, st.phase))) {
+            st.alive = false;
+            if (lane == 0) report_error(u.err, 30), *u.dead = 1;
+        }
         if (c < u.c_end) {
-            uint32_t row0 = u.slots + st.stage * kStage + g * S::kPitch, row1 = row0 + 8 * S::kPitch;
+            uint32_t row0 = at + g * S::kPitch, row1 = row0 + 8 * S::kPitch;
             if constexpr (!ALN) {
                 row0 += (u.window0 + (uint32_t)c * u.window_step) & 15;
                 row1 += (u.window1 + (uint32_t)c * u.window_step) & 15;
             }
-            const int ahead = c + u.kws < u.c_end ? u.kws * kChunkBlocks : 0;  // to the step after this one
-            acc.template step<ALN>(ahead, u.blocks - c * kChunkBlocks, row0, row1, lane, wait);
-        } else {
-            wait();
+            const int valid = u.blocks - c * kChunkBlocks;
+            if constexpr (FEW) {
+                acc.template step<ALN>(at + u.to_x, valid, row0, row1, lane);
+            } else {
+                const int ahead = c + u.kws < u.c_end ? u.kws * kChunkBlocks : 0;  // to the step after this one
+                acc.template step<ALN>(ahead, valid, row0, row1, lane);
+            }
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(full + 8);
@@ -417,8 +401,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int kws = kImmaWarps / a.strips;
     const int steps = (a.bpr + kChunkBlocks - 1) / kChunkBlocks;
     const int per_seg = (steps + kws - 1) / kws;  // rounds of a tile against a segment
-    // shared memory: weight stages [team][stage][warp], sums [team], (all_segs) y [team], the stages' barriers [team][stage] (full, empty)
-    constexpr uint32_t kStage = kImmaWarps * S::kBytes;
+    // shared memory: stages [team][stage] of the warps' weights and the rounds' records of x, sums [team], (all_segs) y [team], the stages' barriers [team][stage] (full, empty)
+    constexpr uint32_t kStage = kImmaWarps * S::kBytes + (FEW ? kXStage : 0);
     const uint32_t red0 = kTeams * a.slots * kStage;
     const uint32_t y_floats = MODE == kDown && !a.part ? a.rows * 16 * a.strips : 0;
     const uint32_t bars0 = smem_u32(smem) + red0 + kTeams * (kRedFloats + y_floats) * 4;
@@ -452,94 +436,131 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (producer) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kProducerRegs));
         const int half = cta_warp & 1;
-        int stage = 0, phase = 1, n = 0;
-        bool alive = true;
-        while (alive && work.next(deal, id)) {
-            int seg = all_segs ? work.r0 / per_seg : work.u % nseg, round = all_segs ? work.r0 % per_seg : work.r0;
-            const int tile = all_segs ? work.u : work.u / nseg;
-            int row0 = 0;
-            bool fresh = true;
-            for (int r = work.r0; r < work.r1; ++r, ++n) {
-                // tensor maps: the team's two producers take stages in turn (lane w fetches warp w's slot; issuing a box
-                // takes ~70 cycles); 16-byte windows: each takes the slots of four warps of every stage
-                const bool mine = !ALN || (n & 1) == half;
-                if (mine) {
-                    if (fresh) {
-                        const int e = MODE == kPlain ? 0 : __ldcg(&a.segs[seg].expert);
-                        row0 = e * a.out + tile * unit_rows;
-                        fresh = false;
-                    }
-                    const uint32_t full = bars + 16 * stage, dst = ring + stage * kStage;
-                    if (!__all_sync(0xffffffffu, mbar_wait(full + 8, phase))) {
-                        if (lane == 0) report_error(a.err, 31), *(volatile int*)&s_dead = 1;
-                        alive = false;
-                        break;
-                    }
-                    if (__any_sync(0xffffffffu, *(volatile int*)&s_dead)) {
-                        alive = false;
-                        break;
-                    }
-                    if constexpr (ALN) {
-                        const int active = steps - round * kws < kws ? steps - round * kws : kws;  // K parts of this round
-                        if (lane == 0) mbar_arrive_expect_tx(full, active * a.strips * S::kBytes);
-                        __syncwarp();
-                        const int kw = lane / a.strips, c = round * kws + kw;
-                        if (kw < active) {
-                            const int row = row0 + (lane % a.strips) * (MODE == kPair ? 8 : 16);
+        // Tensor maps: the team's two producers take stages in turn (issuing a box takes ~70 cycles).  16-byte windows:
+        // each takes the slots of four warps of every stage, the first one also x.
+        Cursor cur(work);
+        auto next_piece = [&](Cursor& c) {
+            c.on = c.work.next(deal, id);
+            if (!c.on) return;
+            c.r = c.work.r0;
+            c.tile = all_segs ? c.work.u : c.work.u / nseg;
+            c.seg = all_segs ? c.work.r0 / per_seg : c.work.u % nseg;
+            c.round = all_segs ? c.work.r0 % per_seg : c.work.r0;
+            c.fresh = true;
+        };
+        auto advance = [&](Cursor& c) {
+            ++c.n;
+            if (++c.stage == a.slots) c.stage = 0, c.phase ^= 1;
+            if (++c.round == per_seg) c.round = 0, ++c.seg, c.fresh = true;
+            if (++c.r == c.work.r1) next_piece(c);
+        };
+        auto mine = [&](const Cursor& c) { return !ALN || (c.n & 1) == half; };
+        // the segment's matrix and rows of x
+        auto refresh = [&](Cursor& c) {
+            if (!c.fresh) return;
+            c.fresh = false;
+            const int e = MODE == kPlain ? 0 : __ldcg(&a.segs[c.seg].expert);
+            c.row0 = e * a.out + c.tile * unit_rows;
+            if (FEW) {
+                c.first = MODE == kPlain ? c.seg * a.seg_cap : __ldcg(&a.segs[c.seg].start);
+                c.count = MODE == kPlain ? (a.rows - c.first < a.seg_cap ? a.rows - c.first : a.seg_cap)
+                                         : __ldcg(&a.segs[c.seg].count);
+            }
+        };
+        auto active = [&](const Cursor& c) { return min(steps - c.round * kws, kws); };  // K parts of the round
+        auto fetch_weights = [&](Cursor& c) {
+            const uint32_t full = bars + 16 * c.stage, dst = ring + c.stage * kStage;
+            if constexpr (ALN) {
+                if (lane == 0)
+                    mbar_arrive_expect_tx(full, active(c) * (a.strips * S::kBytes + (FEW ? c.count * kRecordBytes : 0)));
+                __syncwarp();
+                const int kw = lane / a.strips;
+                if (kw < active(c)) {
+                    const int row = c.row0 + (lane % a.strips) * (MODE == kPair ? 8 : 16);
 #pragma unroll
-                            for (int b = 0; b < S::kBoxes; ++b) {
-                                const int c0 = (c * chunk_bytes(F) + b * S::kPitch) / 2;
-                                const uint32_t d = dst + lane * S::kBytes + b * 16 * S::kPitch;
-                                tma_load_2d(d, &maps.m[0], c0, row, full);
-                                if (MODE == kPair) tma_load_2d(d + 8 * S::kPitch, &maps.m[1], c0, row, full);
-                            }
-                        }
-                        __syncwarp();
-                    } else {
-                        // lanes 2r, 2r + 1: the windows that hold row r's blocks
-                        const int r = lane >> 1, sub = lane & 1;
-                        const uint8_t* base = MODE == kPair && r >= 8 ? a.w[1] : a.w[0];
-                        bool stored = false;
+                    for (int b = 0; b < S::kBoxes; ++b) {
+                        const int c0 = ((c.round * kws + kw) * chunk_bytes(F) + b * S::kPitch) / 2;
+                        const uint32_t d = dst + lane * S::kBytes + b * 16 * S::kPitch;
+                        tma_load_2d(d, &maps.m[0], c0, row, full);
+                        if (MODE == kPair) tma_load_2d(d + 8 * S::kPitch, &maps.m[1], c0, row, full);
+                    }
+                }
+                __syncwarp();
+            } else {
+                if (FEW && half == 0 && lane == 0) mbar_expect_tx(full, active(c) * c.count * kRecordBytes);
+                // lanes 2r, 2r + 1: the windows that hold row r's blocks
+                const int r = lane >> 1, sub = lane & 1;
+                const uint8_t* base = MODE == kPair && r >= 8 ? a.w[1] : a.w[0];
+                bool stored = false;
+#pragma unroll 1
+                for (int k = 0; k < kImmaWarps / 2; ++k) {
+                    const int w = kImmaWarps / 2 * half + k, step = c.round * kws + w / a.strips;
+                    const long long row =
+                        c.row0 + (w % a.strips) * (MODE == kPair ? 8 : 16) + (MODE == kPair ? (r & 7) : r);
+                    if (step >= steps || row >= a.total_rows) continue;
+                    long long left = a.row_bytes - (long long)step * chunk_bytes(F);
+                    if (left > chunk_bytes(F)) left = chunk_bytes(F);
+                    const uint8_t* src = base + row * a.row_bytes + (long long)step * chunk_bytes(F);
+                    const uint8_t* end = src + left;
+                    const uint8_t* q =
+                        reinterpret_cast<const uint8_t*>(reinterpret_cast<uintptr_t>(src) & ~(uintptr_t)15) + 16 * sub;
+                    uint32_t to = dst + w * S::kBytes + r * S::kPitch + 16 * sub;
 #pragma unroll
-                        for (int k = 0; k < kImmaWarps / 2; ++k) {
-                            const int w = kImmaWarps / 2 * half + k, c = round * kws + w / a.strips;
-                            const long long row =
-                                row0 + (w % a.strips) * (MODE == kPair ? 8 : 16) + (MODE == kPair ? (r & 7) : r);
-                            if (c >= steps || row >= a.total_rows) continue;
-                            long long left = a.row_bytes - (long long)c * chunk_bytes(F);
-                            if (left > chunk_bytes(F)) left = chunk_bytes(F);
-                            const uint8_t* src = base + row * a.row_bytes + (long long)c * chunk_bytes(F);
-                            const uint8_t* end = src + left;
-                            const uint8_t* q =
-                                reinterpret_cast<const uint8_t*>(reinterpret_cast<uintptr_t>(src) & ~(uintptr_t)15) + 16 * sub;
-                            uint32_t to = dst + w * S::kBytes + r * S::kPitch + 16 * sub;
-#pragma unroll
-                            for (int i = 0; i < (chunk_bytes(F) + 15 + 31) / 32; ++i, q += 32, to += 32) {
-                                if (q >= end) break;
-                                if (q < base) {  // the stack starts inside this window: only its own bytes are read
-                                    for (int b = (int)(base - q); b < 16 && q + b < end; ++b) sts_u8(to + b, q[b]);
-                                    stored = true;
-                                } else {
-                                    const long long m = end - q;
-                                    cp_async_16(to, q, m < 16 ? (uint32_t)m : 16u);
-                                }
-                            }
-                        }
-                        if (stored) {  // plain stores are ordered by a plain arrival
-                            asm volatile("cp.async.wait_all;" ::: "memory");
-                            mbar_arrive(full);
+                    for (int i = 0; i < (chunk_bytes(F) + 15 + 31) / 32; ++i, q += 32, to += 32) {
+                        if (q >= end) break;
+                        if (q < base) {  // the stack starts inside this window: only its own bytes are read
+                            for (int b = (int)(base - q); b < 16 && q + b < end; ++b) sts_u8(to + b, q[b]);
+                            stored = true;
                         } else {
-                            cp_async_arrive(full);
+                            const long long m = end - q;
+                            cp_async_16(to, q, m < 16 ? (uint32_t)m : 16u);
                         }
                     }
                 }
-                if (++stage == a.slots) stage = 0, phase ^= 1;
-                if (++round == per_seg) round = 0, ++seg, fresh = true;
+                __syncwarp();  // the bytes of x are expected before anyone arrives for good
+                if (stored) {  // plain stores are ordered by a plain arrival
+                    asm volatile("cp.async.wait_all;" ::: "memory");
+                    mbar_arrive(full);
+                } else {
+                    cp_async_arrive(full);
+                }
             }
+        };
+        // lane (K part, row of x): its record
+        auto fetch_x = [&](Cursor& c) {
+            if (!FEW || (!ALN && half)) return;
+            const int kw = lane / a.seg_cap, r = lane % a.seg_cap;
+            if (kw < active(c) && r < c.count) {
+                const int row = MODE == kPair ? __ldcg(a.order + c.first + r) / a.top_k : c.first + r;
+                bulk_g2s(ring + c.stage * kStage + kImmaWarps * S::kBytes + lane * kRecordBytes,
+                         a.x.data + ((size_t)row * (a.bprp / kChunkBlocks) + c.round * kws + kw) * kRecordBytes, kRecordBytes,
+                         bars + 16 * c.stage);
+            }
+            __syncwarp();
+        };
+        next_piece(cur);
+        if (MODE != kPair) {
+            // the ring's first weights are on their way while the launch before this one writes x
+            Cursor xs = cur;
+            for (int i = 0; i < a.slots && cur.on; ++i, advance(cur))
+                if (mine(cur)) refresh(cur), fetch_weights(cur);
+            grid_dependency_wait();
+            for (; xs.on && xs.n < cur.n; advance(xs))
+                if (mine(xs)) refresh(xs), fetch_x(xs);
+        }
+        for (; cur.on; advance(cur)) {
+            if (!mine(cur)) continue;
+            refresh(cur);
+            if (!__all_sync(0xffffffffu, mbar_wait(bars + 16 * cur.stage + 8, cur.phase))) {
+                if (lane == 0) report_error(a.err, 31), *(volatile int*)&s_dead = 1;
+                break;
+            }
+            if (__any_sync(0xffffffffu, *(volatile int*)&s_dead)) break;
+            fetch_weights(cur);
+            fetch_x(cur);
         }
         if (!ALN) asm volatile("cp.async.wait_all;" ::: "memory");
-        if (lane == 0) s_issued[team][half] = ALN ? n : 0;
-        if (MODE != kPair) grid_dependency_wait();
+        if (lane == 0) s_issued[team][half] = ALN ? cur.n : 0;
         if (MODE == kDown) launch_dependents();
         __syncthreads();
         return;
@@ -611,7 +632,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             u.x = XView{a.x.data, a.x.scale, a.x.sum, (uint32_t)a.bprp};
             u.order = a.order, u.top_k = a.top_k;
             u.red = rb + warp * tokens * 16;
-            u.full = bars, u.slots = ring + warp * S::kBytes, u.stages = a.slots;
+            u.full = bars, u.slots = ring + warp * S::kBytes, u.stages = a.slots, u.stage_bytes = kStage;
+            u.to_x = (kImmaWarps - warp) * S::kBytes + kw * a.seg_cap * kRecordBytes;
             u.first = first, u.count = count;
             u.c0 = r0 * kws + kw, u.kws = kws, u.rounds = r1 - r0, u.blocks = a.bpr;
             u.c_end = r1 * kws < steps ? r1 * kws : steps;
@@ -626,16 +648,16 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             if constexpr (FEW) {
                 if (count <= 2)
-                    st = unit_sums<FewRows<F, 1>, F, MODE, ALN>(u, st);
+                    st = unit_sums<FewRows<F, 1>, F, MODE, FEW, ALN>(u, st);
                 else
-                    st = unit_sums<FewRows<F, 2>, F, MODE, ALN>(u, st);
+                    st = unit_sums<FewRows<F, 2>, F, MODE, FEW, ALN>(u, st);
             } else {
                 if (count <= 8)
-                    st = unit_sums<ManyRows<F, 1>, F, MODE, ALN>(u, st);
+                    st = unit_sums<ManyRows<F, 1>, F, MODE, FEW, ALN>(u, st);
                 else if (count <= 16)
-                    st = unit_sums<ManyRows<F, 2>, F, MODE, ALN>(u, st);
+                    st = unit_sums<ManyRows<F, 2>, F, MODE, FEW, ALN>(u, st);
                 else
-                    st = unit_sums<ManyRows<F, 4>, F, MODE, ALN>(u, st);
+                    st = unit_sums<ManyRows<F, 4>, F, MODE, FEW, ALN>(u, st);
             }
             team_sync(team);
             auto sum_parts = [&](int tok, int row) {
@@ -672,7 +694,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                         const float h = 32 * b + el < a.out ? silu_mul(get(tok, row), get(tok, row + 8)) : 0.0f;
                         const size_t to = (size_t)(first + tok) * a.next_bprp + b;
                         if (FEW)
-                            slice_digits(h, digit_weight(a.next_fmt, lane), a.h.data + (to - b) * kSlicedBytes + digit_block(b), a.h.scale + to, a.h.sum + to, lane);
+                            slice_digits(h, digit_weight(a.next_fmt, lane),
+                                         a.h.data + (size_t)(first + tok) * (a.next_bprp / kChunkBlocks) * kRecordBytes, b, lane);
                         else
                             slice_halves(h, a.h.data + to * kSlicedBytes, a.h.scale + to, a.h.sum + to, lane);
                     }
@@ -749,10 +772,11 @@ cudaError_t launch_one(ImmaArgs a, int grid, int smem_per_sm, cudaStream_t strea
     auto k = imma_kernel<F, MODE, FEW, ALN>;
     const int sums = kTeams * (kRedFloats + (MODE == kDown && !a.part ? a.rows * 16 * a.strips : 0)) * 4;
     const int fixed = sums + 1024 + 256;  // the system's 1 KB per CTA, the static part
-    a.slots = (smem_per_sm - fixed) / (kTeams * (kImmaWarps * S::kBytes + 16));
+    constexpr int stage = kImmaWarps * S::kBytes + (FEW ? kXStage : 0);
+    a.slots = (smem_per_sm - fixed) / (kTeams * (stage + 16));
     if (a.slots > 8) a.slots = 8;
     if (a.slots < 2) return cudaErrorInvalidConfiguration;
-    const size_t smem = (size_t)kTeams * a.slots * (kImmaWarps * S::kBytes + 16) + sums;
+    const size_t smem = (size_t)kTeams * a.slots * (stage + 16) + sums;
     ImmaMaps maps{};
     if (ALN) {
         for (int i = 0; i < (MODE == kPair ? 2 : 1); ++i)
