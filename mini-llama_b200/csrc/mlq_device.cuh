@@ -64,8 +64,9 @@ __device__ __forceinline__ float silu_mul(float g, float u) {
 // mlq_device_error().  Codes: 1 = pipeline "full" wait, 2 = "empty" wait,
 // 3 = drain wait, 4 = peer flag wait, 5 = consumer rendezvous, 6 = x-tile
 // "empty" wait, 7 = resident x tiles ready wait, 8 = staged x copy wait,
-// 12-16 = GEMM waits, 20-26 = batched-decode GEMM waits, 30 = weight wait of
-// the experts' products and of the linear with an epilogue.
+// 12-16 = GEMM waits, 20-26 = batched-decode GEMM waits, 30-33 = waits of the
+// experts' products and of the linear with an epilogue (few rows: data, free
+// stage; many rows: the same).
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ void report_error(int* err, int code) {
     if (err) atomicCAS(err, 0, code);

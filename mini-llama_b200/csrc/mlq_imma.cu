@@ -25,9 +25,9 @@ __global__ void combine_kernel(const ImmaArgs a) {
 struct PrepArgs {
     const float* x;
     int rows, in, bpr, bprp, fmt;
-    Sliced sliced;
-    bool few;    // as digits, else as halves
-    int seg_cap; // rows of a segment at most
+    uint8_t* sliced;  // records
+    bool few;         // of digits, else of halves
+    int seg_cap;      // rows of a segment at most
     unsigned int* split_done;
     // experts only (ids not null)
     const int32_t* ids;
@@ -36,7 +36,7 @@ struct PrepArgs {
     int* nseg;
     int* order;
     // padding blocks of the sliced h
-    Sliced h;
+    uint8_t* h;
     int h_bpr, h_bprp;
 };
 
@@ -58,7 +58,7 @@ __global__ void __launch_bounds__(256) prep_kernel(const PrepArgs a) {
             const int pad = a.few ? a.h_bprp - a.h_bpr : 0;  // halves past a row's end are not read
             for (int i = threadIdx.x; i < a.pairs * pad; i += 256) {
                 const int b = a.h_bpr + i % pad;
-                float* at = reinterpret_cast<float*>(a.h.data + ((size_t)(i / pad) * (a.h_bprp / kChunkBlocks) + b / kChunkBlocks) *
+                float* at = reinterpret_cast<float*>(a.h + ((size_t)(i / pad) * (a.h_bprp / kChunkBlocks) + b / kChunkBlocks) *
                                                                     kRecordBytes + kRecordScales) + b % kChunkBlocks;
                 at[0] = at[kChunkBlocks] = 0.0f;
             }
@@ -128,15 +128,13 @@ __global__ void __launch_bounds__(256) prep_kernel(const PrepArgs a) {
     for (long long i = (long long)first * 8 + warp; i < n; i += (long long)ctas * 8) {
         const int r = (int)(i / a.bprp), b = (int)(i % a.bprp);
         const float* x = a.x + (long long)r * a.in;
-        if (a.few) {
-            const int at = b * kQK + imma_element(a.fmt, b & 1, lane);
-            slice_digits(at < a.in ? x[at] : 0.0f, digit_weight(a.fmt, lane),
-                         a.sliced.data + (size_t)r * (a.bprp / kChunkBlocks) * kRecordBytes, b, lane);
-        } else {
-            const int at = b * kQK + half_element(a.fmt, b & 1, lane);
-            slice_halves(at < a.in ? x[at] : 0.0f, a.sliced.data + i * kSlicedBytes, a.sliced.scale + i, a.sliced.sum + i,
-                         lane);
-        }
+        uint8_t* row = a.sliced + (size_t)r * (a.bprp / kChunkBlocks) * kRecordBytes;
+        const int at = b * kQK + (a.few ? imma_element(a.fmt, b & 1, lane) : half_element(a.fmt, b & 1, lane));
+        const float v = at < a.in ? x[at] : 0.0f;
+        if (a.few)
+            slice_digits(v, digit_weight(a.fmt, lane), row, b, lane);
+        else
+            slice_halves(v, row, b, lane);
     }
 }
 
@@ -178,23 +176,10 @@ struct Carve {
         p += align256(n * sizeof(T));
         return r;
     }
-    // records (few rows) or data, scales and sums apart
-    Sliced take_sliced(size_t rows, int bprp, bool few) {
-        Sliced s{};
-        if (few) {
-            s.data = take<uint8_t>(rows * (bprp / kChunkBlocks) * kRecordBytes);
-            return s;
-        }
-        s.data = take<uint8_t>(rows * bprp * kSlicedBytes);
-        s.scale = take<float>(rows * bprp);
-        s.sum = take<float>(rows * bprp);
-        return s;
-    }
+    uint8_t* take_sliced(size_t rows, int bprp) { return take<uint8_t>(rows * (bprp / kChunkBlocks) * kRecordBytes); }
 };
 
-size_t sliced_bytes(size_t rows, int bprp) {
-    return align256(rows * bprp * kSlicedBytes) + 2 * align256(rows * bprp * sizeof(float));
-}
+size_t sliced_bytes(size_t rows, int bprp) { return align256(rows * (bprp / kChunkBlocks) * kRecordBytes); }
 
 constexpr int kMaxPairs = 8192;           // pairs of one pass at most
 constexpr size_t kMaxSliced = 1u << 30;   // sliced bytes of one pass at most (offsets are 32 bits)
@@ -202,22 +187,37 @@ constexpr size_t kMaxParts = 1u << 30;    // bytes of the pairs' outputs of one 
 constexpr int kMaxPassRows = 16384;       // rows of one pass of a linear at most
 constexpr int kCombineRows = 32;          // more rows: the sum over slots is a launch of its own
 
-int split_tokens(int rows) { return rows < kSegTokens ? rows : kSegTokens; }
-
 // Rows of x of a segment at most in the form of few rows.
-int few_cap(int rows) { return rows < kFewRows ? (rows < 3 ? rows : kFewRows) : kFewRows; }
+int few_cap(int rows) { return rows < 3 ? rows : kFewRows; }
 
-// Two slots per team of at most 128 rows, and the counters of two launches.
-size_t split_bytes(int rows) {
-    return align256((size_t)2 * kMaxTeams * split_tokens(rows) * 128 * sizeof(float)) +
+// And in that of many: with two stages of 256 q8_0 rows that are not aligned,
+// shared memory has room for 16.
+int many_cap(int fmt, const void* w0, const void* w1, int in) {
+    const int bpr = (in + kQK - 1) / kQK;
+    const long long pitch = (long long)bpr * block_bytes(fmt);
+    const bool aligned = reinterpret_cast<uintptr_t>(w0) % 16 == 0 && reinterpret_cast<uintptr_t>(w1) % 16 == 0 && pitch % 16 == 0;
+    return fmt == kQ8_0 && !aligned ? kSegTokens / 2 : kSegTokens;
+}
+
+// Floats of a slot for a shared unit's sums: rows of x x rows of the tile.  n:
+// rows of the call (a unit of few rows that meets every segment has them all).
+size_t split_floats(bool few, int n, int strips) {
+    if (!few) return (size_t)kSegTokens * 256;
+    return (size_t)(n <= kCombineRows && n > kFewRows ? n : kFewRows) * 16 * strips;
+}
+
+// Two slots per team at most, and the counters of two launches.
+size_t split_count(bool few) { return few ? 2 * kMaxTeams : kMaxTeams; }
+size_t split_bytes(bool few, int n) {
+    return align256(split_floats(few, n, kImmaWarps) * split_count(few) * sizeof(float)) +
            align256(2 * kMaxTeams * sizeof(unsigned int));
 }
 
 // Rows of x of one pass.
 int experts_pass_rows(const MoeShape& s, int rows, int top_k) {
     long long n = kMaxPairs / top_k;
-    const long long per = (long long)top_k * padded_blocks((s.hidden + kQK - 1) / kQK) * kSlicedBytes;
-    const long long perx = (long long)padded_blocks((s.in + kQK - 1) / kQK) * kSlicedBytes;
+    const long long per = (long long)top_k * padded_blocks((s.hidden + kQK - 1) / kQK) * (kSlicedBytes + 8);
+    const long long perx = (long long)padded_blocks((s.in + kQK - 1) / kQK) * (kSlicedBytes + 8);
     const long long cap = (long long)kMaxSliced / (per > perx ? per : perx);
     const long long capp = (long long)kMaxParts / ((long long)top_k * s.out * (long long)sizeof(float));
     if (n > cap) n = cap;
@@ -227,7 +227,7 @@ int experts_pass_rows(const MoeShape& s, int rows, int top_k) {
 }
 
 int linear_pass_rows(int in, int rows) {
-    long long n = (long long)kMaxSliced / ((long long)padded_blocks((in + kQK - 1) / kQK) * kSlicedBytes);
+    long long n = (long long)kMaxSliced / ((long long)padded_blocks((in + kQK - 1) / kQK) * (kSlicedBytes + 8));
     if (n > kMaxPassRows) n = kMaxPassRows;
     return rows < n ? rows : (int)n;
 }
@@ -252,7 +252,7 @@ int prep_ctas(long long blocks, int sm_count) {
 
 size_t epilogue_workspace_bytes(int in, int rows) {
     const int n = linear_pass_rows(in, rows);
-    return sliced_bytes(n, padded_blocks((in + kQK - 1) / kQK)) + split_bytes(n);
+    return sliced_bytes(n, padded_blocks((in + kQK - 1) / kQK)) + split_bytes(n <= kFewRows, n);
 }
 
 cudaError_t launch_linear_epilogue(int fmt, const uint8_t* w, int out, int in, const float* x, int rows,
@@ -267,29 +267,28 @@ cudaError_t launch_linear_epilogue(int fmt, const uint8_t* w, int out, int in, c
         p.x = x + (long long)r0 * in;
         p.rows = n, p.in = in, p.bpr = bpr, p.bprp = bprp, p.fmt = fmt;
         p.few = n <= kFewRows;
-        p.sliced = c.take_sliced(n, bprp, p.few);
-        float* split = c.take<float>((size_t)2 * kMaxTeams * split_tokens(n) * 128);
+        p.sliced = c.take_sliced(n, bprp);
+        float* split = c.take<float>(split_floats(p.few, n, kImmaWarps) * split_count(p.few));
         p.split_done = c.take<unsigned int>(2 * kMaxTeams);
         cudaError_t e = launch_pdl(prep_kernel, prep_ctas((long long)n * bprp, sm_count), 256, 0, stream, p);
         if (e != cudaSuccess) return e;
         ImmaArgs a{};
         a.w[0] = w;
         a.total_rows = out, a.out = out, a.bpr = bpr, a.bprp = bprp;
-        a.few = p.few;
-        a.seg_cap = p.few ? few_cap(n) : kSegTokens;
+        a.seg_cap = p.few ? few_cap(n) : many_cap(fmt, w, w, in);
         const int nseg = (n + a.seg_cap - 1) / a.seg_cap;
-        a.strips = choose_strips(out, bpr, nseg, false, sm_count, p.few ? a.seg_cap : 1);
+        a.strips = p.few ? choose_strips(out, bpr, nseg, false, sm_count, a.seg_cap) : 16;
         a.tiles = (out + 16 * a.strips - 1) / (16 * a.strips);
         a.x = p.sliced;
         a.rows = n;
-        a.split = split, a.split_done = p.split_done, a.split_size = (size_t)split_tokens(n) * 16 * a.strips;
+        a.split = split, a.split_done = p.split_done, a.split_size = split_floats(p.few, n, a.strips);
         a.bias = ep.bias;
         a.row_scale = ep.row_scale ? ep.row_scale + r0 : nullptr;
         a.residual = ep.residual ? ep.residual + (long long)r0 * out : nullptr;
         a.act = ep.activation;
         a.y = y + (long long)r0 * out;
         a.err = err;
-        e = launch_imma_plain(fmt, a, sm_count, smem_per_sm, (long long)nseg * a.tiles, stream);
+        e = (p.few ? launch_few_plain : launch_many_plain)(fmt, a, sm_count, smem_per_sm, (long long)nseg * a.tiles, stream);
         if (e != cudaSuccess) return e;
         r0 += n;
     }
@@ -300,10 +299,12 @@ size_t experts_workspace_bytes(const MoeShape& s, int rows, int top_k) {
     const int pass = experts_pass_rows(s, rows, top_k);
     const int bprp = padded_blocks((s.in + kQK - 1) / kQK), hp = padded_blocks((s.hidden + kQK - 1) / kQK);
     auto bytes = [&](int n) {
-        const int pairs = n * top_k, cap = few_rows(pairs, s.n_experts) ? few_cap(n) : kSegTokens;
+        const int pairs = n * top_k;
+        const bool few = few_rows(pairs, s.n_experts);
+        const int cap = few ? few_cap(n) : kSegTokens / 2;
         return 256 + align256((size_t)max_segments(pairs, s.n_experts, cap) * sizeof(Segment)) +
                align256((size_t)pairs * sizeof(int)) + sliced_bytes(n, bprp) + sliced_bytes(pairs, hp) +
-               (n <= kCombineRows ? 0 : align256((size_t)pairs * s.out * sizeof(float))) + split_bytes(pairs);
+               (few && n <= kCombineRows ? 0 : align256((size_t)pairs * s.out * sizeof(float))) + split_bytes(few, n);
     };
     // the last pass may be smaller, and take another form
     const int last = rows % pass;
@@ -321,10 +322,15 @@ cudaError_t launch_experts(const MoeShape& s, const uint8_t* gate, const uint8_t
     for (int r0 = 0; r0 < rows; r0 += pass) {
         const int n = rows - r0 < pass ? rows - r0 : pass, pairs = n * top_k;
         const bool few = few_rows(pairs, s.n_experts);
-        const int cap = few ? few_cap(n) : kSegTokens;
+        int cap = few_cap(n);
+        if (!few) {
+            const int c0 = many_cap(s.fmt, gate, up, s.in), c1 = many_cap(s.fmt_down, down, down, s.hidden);
+            cap = c0 < c1 ? c0 : c1;
+        }
+        const bool at_once = few && n <= kCombineRows;  // the down product meets all segments of a tile in one unit
         const int nseg_max = max_segments(pairs, s.n_experts, cap);
         const int nseg_likely = pairs < s.n_experts ? pairs : nseg_max;
-        const int strips = choose_strips(s.out, hb, nseg_likely, n <= kCombineRows, sm_count, few ? cap : 1);
+        const int strips = few ? choose_strips(s.out, hb, nseg_likely, at_once, sm_count, cap) : 16;
         const int tiles = (s.out + 16 * strips - 1) / (16 * strips);
         Carve c{static_cast<uint8_t*>(ws)};
         PrepArgs p{};
@@ -334,13 +340,13 @@ cudaError_t launch_experts(const MoeShape& s, const uint8_t* gate, const uint8_t
         p.x = x + (long long)r0 * s.in;
         p.rows = n, p.in = s.in, p.bpr = bpr, p.bprp = bprp, p.fmt = s.fmt;
         p.few = few, p.seg_cap = cap;
-        p.sliced = c.take_sliced(n, bprp, p.few);
+        p.sliced = c.take_sliced(n, bprp);
         p.ids = ids + (long long)r0 * top_k;
         p.pairs = pairs, p.n_experts = s.n_experts;
-        p.h = c.take_sliced(pairs, hp, few);
+        p.h = c.take_sliced(pairs, hp);
         p.h_bpr = hb, p.h_bprp = hp;
-        float* part = c.take<float>(n <= kCombineRows ? 0 : (size_t)pairs * s.out);
-        float* split = c.take<float>((size_t)2 * kMaxTeams * split_tokens(pairs) * 128);
+        float* part = c.take<float>(at_once ? 0 : (size_t)pairs * s.out);
+        float* split = c.take<float>(split_floats(few, n, kImmaWarps) * split_count(few));
         p.split_done = c.take<unsigned int>(2 * kMaxTeams);
         cudaError_t e = launch_pdl(prep_kernel, 1 + prep_ctas((long long)n * bprp, sm_count), 256, 0, stream, p);
         if (e != cudaSuccess) return e;
@@ -349,17 +355,17 @@ cudaError_t launch_experts(const MoeShape& s, const uint8_t* gate, const uint8_t
         a.w[0] = gate, a.w[1] = up;
         a.total_rows = (long long)s.n_experts * s.hidden;
         a.out = s.hidden, a.bpr = bpr, a.bprp = bprp;
-        a.strips = choose_strips(2 * s.hidden, bpr, nseg_likely, false, sm_count, 4);
+        a.strips = few ? choose_strips(2 * s.hidden, bpr, nseg_likely, false, sm_count, 4) : 16;
         a.tiles = (s.hidden + 8 * a.strips - 1) / (8 * a.strips);
-        a.few = few, a.seg_cap = cap;
+        a.seg_cap = cap;
         a.x = p.sliced;
         a.segs = p.segs, a.nseg = p.nseg, a.order = p.order;
         a.top_k = top_k, a.rows = n;
         a.next_fmt = s.fmt_down, a.next_bprp = hp;
         a.h = p.h;
-        a.split = split, a.split_done = p.split_done, a.split_size = (size_t)split_tokens(pairs) * 16 * a.strips;
+        a.split = split, a.split_done = p.split_done, a.split_size = split_floats(few, n, a.strips);
         a.err = err;
-        e = launch_imma_pair(s.fmt, a, sm_count, smem_per_sm, (long long)nseg_max * a.tiles, stream);
+        e = (few ? launch_few_pair : launch_many_pair)(s.fmt, a, sm_count, smem_per_sm, (long long)nseg_max * a.tiles, stream);
         if (e != cudaSuccess) return e;
 
         ImmaArgs d{};
@@ -367,20 +373,20 @@ cudaError_t launch_experts(const MoeShape& s, const uint8_t* gate, const uint8_t
         d.total_rows = (long long)s.n_experts * s.out;
         d.out = s.out, d.bpr = hb, d.bprp = hp;
         d.strips = strips, d.tiles = tiles;
-        d.few = few, d.seg_cap = cap;
+        d.seg_cap = cap;
         d.x = p.h;
         d.segs = p.segs, d.nseg = p.nseg, d.order = p.order;
         d.top_k = top_k, d.rows = n;
-        d.part = n <= kCombineRows ? nullptr : part;
+        d.part = at_once ? nullptr : part;
         d.split = split, d.split_done = p.split_done + kMaxTeams;
-        d.split_size = (size_t)split_tokens(pairs) * 16 * strips;
+        d.split_size = split_floats(few, n, strips);
         d.ids = p.ids;
         d.weights = weights + (long long)r0 * top_k;
         d.n_experts = s.n_experts;
         d.residual = residual ? residual + (long long)r0 * s.out : nullptr;
         d.y = y + (long long)r0 * s.out;
         d.err = err;
-        e = launch_imma_down(s.fmt_down, d, sm_count, smem_per_sm, (long long)nseg_max * tiles, stream);
+        e = (few ? launch_few_down : launch_many_down)(s.fmt_down, d, sm_count, smem_per_sm, (long long)nseg_max * tiles, stream);
         if (e != cudaSuccess) return e;
         if (d.part) {
             const long long vals = (long long)n * s.out;

@@ -71,8 +71,8 @@ __device__ __forceinline__ int half_element(int fmt, int odd, int l) {
     return imma_element(fmt, odd, 16 * h + 4 * t + j);
 }
 
-// A row sliced into digits is a sequence of records, one per K step: 8 blocks
-// of digits, their scales, their sums of x.  One bulk copy brings a record to
+// A sliced row of x is a sequence of records, one per K step: 8 blocks of
+// digits (or halves), their scales, their sums of x.  One bulk copy brings a record to
 // shared memory.
 constexpr int kRecordBytes = kChunkBlocks * (kSlicedBytes + 8);
 constexpr int kRecordScales = kChunkBlocks * kSlicedBytes, kRecordSums = kRecordScales + kChunkBlocks * 4;
@@ -148,21 +148,28 @@ __device__ __forceinline__ void slice_digits(float x, float weight, uint8_t* row
     }
 }
 
-// Slices a block into fp16 hi and lo: lane l holds the value at half_element l.
-__device__ __forceinline__ void slice_halves(float v, uint8_t* out, float* scale, float* sum, int lane) {
+// Where block b of a row's records has its halves: [hi, lo][t][value].
+__host__ __device__ constexpr int half_block(int b) {
+    return (b / kChunkBlocks) * kRecordBytes + (b % kChunkBlocks) * kSlicedBytes;
+}
+
+// Slices a block into fp16 hi and lo: lane l holds the value at half_element
+// l of block b; row: the row's first record.
+__device__ __forceinline__ void slice_halves(float v, uint8_t* row, int b, int lane) {
     const float amax = block_amax(v);
     const bool bad = !(amax == amax);
     const uint32_t s = block_scale(bad ? 0.0f : amax, 14, 32767.0f);
     const float q = bad ? 0.0f : v * __uint_as_float(s);
     const __half hi = __float2half_rn(q);
     const __half lo = __float2half_rn(q - __half2float(hi));
-    __half* o = reinterpret_cast<__half*>(out);
+    __half* o = reinterpret_cast<__half*>(row + half_block(b));
     o[lane] = hi;
     o[32 + lane] = lo;
     const float total = warp_sum(v);
     if (lane == 0) {
-        *scale = bad ? __uint_as_float(0x7fc00000u) : inverse_scale(s);
-        *sum = total;
+        float* at = reinterpret_cast<float*>(row + (b / kChunkBlocks) * kRecordBytes + kRecordScales) + b % kChunkBlocks;
+        at[0] = bad ? __uint_as_float(0x7fc00000u) : inverse_scale(s);
+        at[kChunkBlocks] = total;
     }
 }
 
@@ -244,6 +251,13 @@ __device__ __forceinline__ uint4 lds_u4_at(uint32_t a) {
     asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4+%5];"
                  : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
                  : "r"(a), "n"(OFF));
+    return v;
+}
+
+template <int OFF>
+__device__ __forceinline__ float lds_f1_at(uint32_t a) {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1+%2];" : "=f"(v) : "r"(a), "n"(OFF));
     return v;
 }
 

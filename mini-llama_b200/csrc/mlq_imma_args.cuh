@@ -11,13 +11,6 @@ struct ImmaMaps {
     CUtensorMap m[2];
 };
 
-// Sliced rows of x or h: [row][bprp][128 bytes], a scale and a sum per block.
-struct Sliced {
-    uint8_t* data;
-    float* scale;
-    float* sum;
-};
-
 struct ImmaArgs {
     const uint8_t* w[2];      // stacked matrices [n][out][bpr]; [1]: the up projections (kPair)
     long long row_bytes;      // bytes of a matrix row
@@ -27,9 +20,8 @@ struct ImmaArgs {
     int strips;               // 16-row strips of a unit (1, 2, 4 or 8); kPair: 8 gate and 8 up rows each, 4 or 8
     int tiles;                // row tiles of one matrix
     int slots;                // ring depth of a warp
-    bool few;                 // the launch's rows of x are digits (else halves)
     int seg_cap;              // rows of x of a segment at most
-    Sliced x;                 // rows of x or h
+    const uint8_t* x;         // records of the rows of x or h
     // segments (kPair, kDown); kPlain: rows in order, one matrix
     const Segment* segs;
     const int* nseg;
@@ -37,7 +29,7 @@ struct ImmaArgs {
     int top_k, rows;
     // kPair: sliced h by position
     int next_fmt, next_bprp;
-    Sliced h;
+    uint8_t* h;
     // kDown: one value per pair for a later launch to sum; null: a unit meets every segment and is summed at once
     float* part;              // [pair][out]
     const int32_t* ids;
@@ -87,12 +79,15 @@ inline cudaError_t launch_pdl(void (*kernel)(Params...), int grid, int block, si
     return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
 }
 
-// One streaming launch (mlq_imma_{plain,pair,down}.cu).  max_units: an upper bound of its units.
-cudaError_t launch_imma_plain(int fmt, const ImmaArgs& a, int sm_count, int smem_per_sm, long long max_units,
-                              cudaStream_t stream);
-cudaError_t launch_imma_pair(int fmt, const ImmaArgs& a, int sm_count, int smem_per_sm, long long max_units,
-                             cudaStream_t stream);
-cudaError_t launch_imma_down(int fmt, const ImmaArgs& a, int sm_count, int smem_per_sm, long long max_units,
-                             cudaStream_t stream);
+// One streaming launch (mlq_imma_{few,many}_{plain,pair,down}.cu).
+// max_units: an upper bound of its units.
+#define MLQ_IMMA_LAUNCH(name)                                                                                    \
+    cudaError_t name(int fmt, const ImmaArgs& a, int sm_count, int smem_per_sm, long long max_units, cudaStream_t stream)
+MLQ_IMMA_LAUNCH(launch_few_plain);
+MLQ_IMMA_LAUNCH(launch_few_pair);
+MLQ_IMMA_LAUNCH(launch_few_down);
+MLQ_IMMA_LAUNCH(launch_many_plain);
+MLQ_IMMA_LAUNCH(launch_many_pair);
+MLQ_IMMA_LAUNCH(launch_many_down);
 
 }  // namespace mlq

@@ -1,5 +1,5 @@
-// mlq_imma_kernel.cuh -- the streaming kernel of the experts' products and of
-// the linear with an epilogue (mathematics and operand layout:
+// mlq_imma_few.cuh -- the streaming kernel for few rows of x per matrix
+// (digits, int8 matrix instructions; mathematics and operand layout:
 // mlq_imma.cuh; the launches around it: mlq_imma.cu).
 //
 // One CTA per SM: two teams of 8 computing warps, and two producer warps for
@@ -9,35 +9,15 @@
 // (row, block) squares of 16 x 8 whatever the tile, so rounds cost the same
 // and the launch's rounds are dealt out evenly, a contiguous range per team.
 // The producers fill a ring of stages (one round each) by TMA, running
-// ahead across units, so the weight stream waits for no unit's end, and one team computes while the other is at one.  The K parts of a unit
-// meet in shared memory in a fixed order; a unit whose rounds fall to several
+// ahead across units, so the weight stream waits for no unit's end, and one
+// team computes while the other is at one.  The K parts of a unit meet in shared memory in a fixed order; a unit whose rounds fall to several
 // teams is added up (in order) by the last of them to finish.
 #pragma once
 
-#include <type_traits>
-
-#include "mlq_imma_args.cuh"
-#include "mlq_tmap.h"
+#include "mlq_imma_common.cuh"
 
 namespace mlq {
 namespace {
-
-// f(integral_constant 0), .., f(integral_constant N - 1)
-template <int N, int I = 0, class Fn>
-__device__ __forceinline__ void static_for(Fn f) {
-    if constexpr (I < N) {
-        f(std::integral_constant<int, I>{});
-        static_for<N, I + 1>(f);
-    }
-}
-
-// The sliced rows of x that a unit reads.
-struct XView {
-    const uint8_t* data;
-    const float* scale;
-    const float* sum;
-    uint32_t bprp;
-};
 
 // The accumulators of up to 2 NT rows of x by digits: an instruction's 8
 // columns are the 4 digits of 2 rows, so lane t holds digits 3 and 2 (t even) or
@@ -119,133 +99,6 @@ struct FewRows {
     }
 };
 
-// Up to 8 S rows of x by halves: one column per row.
-template <int F, int S>
-struct ManyRows {
-    static constexpr int kG = S < 2 ? S : 2;  // groups of 8 rows per buffer
-    const uint8_t* data;
-    const float* scale;
-    ptrdiff_t to_sum;
-    uint32_t bo[S], so[S][2];  // of the block that is multiplied
-    uint4 hi[2][kG], lo[2][kG];
-    float s[2][kG][2], m[2][kG][2];
-    float acc[S][2][2];  // [.][row half][row of x 2t, 2t + 1]
-
-    template <class TokenOf>
-    __device__ __forceinline__ void init(const XView& a, int count, int block, int lane, TokenOf token) {
-        const int g = lane >> 2, t = lane & 3;
-        data = a.data, scale = a.scale, to_sum = a.sum - a.scale;
-#pragma unroll
-        for (int i = 0; i < S; ++i) {
-            const int r = 8 * i + g;
-            bo[i] = ((uint32_t)token(r < count ? r : 0) * a.bprp + block) * kSlicedBytes + t * 16;
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                const int rs = 8 * i + 2 * t + x;
-                so[i][x] = (uint32_t)token(rs < count ? rs : 0) * a.bprp + block;
-            }
-            acc[i][0][0] = acc[i][0][1] = acc[i][1][0] = acc[i][1][1] = 0.0f;
-        }
-        load_x(0, 0, 0);
-    }
-
-    // Buffer q: x of rows 8 kG gr .., `on` blocks on.
-    __device__ __forceinline__ void load_x(int on, int gr, int q) {
-#pragma unroll
-        for (int k = 0; k < kG; ++k) {
-            const int i = gr * kG + k;
-            const uint4* x = reinterpret_cast<const uint4*>(data + bo[i] + on * kSlicedBytes);
-            hi[q][k] = x[0], lo[q][k] = x[4];
-#pragma unroll
-            for (int x2 = 0; x2 < 2; ++x2) {
-                s[q][k][x2] = scale[so[i][x2] + on];
-                if (F == kQ4_1) m[q][k][x2] = scale[so[i][x2] + on + to_sum];
-            }
-        }
-    }
-
-    // One K step of 8 blocks: while up to 16 rows of a block are multiplied, the next ones (then the next block's, then
-    // the next step's, `ahead` blocks on) are fetched.
-    template <bool ALN>
-    __device__ __forceinline__ void step(int ahead, int valid, uint32_t r0, uint32_t r1, int lane) {
-        const RowBase rows = row_base(r0, r1, lane & 3);
-        static_for<kChunkBlocks / 2>([&](auto pc) {
-            constexpr int p = decltype(pc)::value;
-            if (2 * p >= valid) return;
-            RawA A[2];
-            load_pair<F, ALN, p>(rows, A[0], A[1]);
-#pragma unroll
-            for (int o = 0; o < 2; ++o) {
-                const int n = 2 * p + o;
-                if (n >= valid) break;
-                uint32_t op[8];
-                half_operand<F>(A[o], op);
-#pragma unroll
-                for (int gr = 0; gr < S / kG; ++gr) {
-                    const int q = (n * (S / kG) + gr) & 1;
-                    if (gr + 1 < S / kG)
-                        load_x(n, gr + 1, q ^ 1);
-                    else
-                        load_x(n + 1 < kChunkBlocks && n + 1 < valid ? n + 1 : ahead, 0, q ^ 1);
-#pragma unroll
-                    for (int k = 0; k < kG; ++k) {
-                        const int i = gr * kG + k;
-                        float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                        hmma_f16(c, op, lo[q][k].x, lo[q][k].y);
-                        hmma_f16(c, op + 4, lo[q][k].z, lo[q][k].w);
-                        hmma_f16(c, op, hi[q][k].x, hi[q][k].y);
-                        hmma_f16(c, op + 4, hi[q][k].z, hi[q][k].w);
-#pragma unroll
-                        for (int r = 0; r < 2; ++r)
-#pragma unroll
-                            for (int x = 0; x < 2; ++x) {
-                                acc[i][r][x] = fmaf(A[o].d[r] * s[q][k][x], c[2 * r + x], acc[i][r][x]);
-                                if (F == kQ4_1) acc[i][r][x] = fmaf(A[o].m[r], m[q][k][x], acc[i][r][x]);
-                            }
-                    }
-                }
-            }
-        });
-#pragma unroll
-        for (int i = 0; i < S; ++i) {
-            bo[i] += ahead * kSlicedBytes;
-            so[i][0] += ahead, so[i][1] += ahead;
-        }
-    }
-
-    __device__ __forceinline__ void store(float* red, int lane) {
-        const int g = lane >> 2, t = lane & 3;
-#pragma unroll
-        for (int i = 0; i < S; ++i)
-#pragma unroll
-            for (int q = 0; q < 2; ++q)
-#pragma unroll
-                for (int x = 0; x < 2; ++x) red[(8 * i + 2 * t + x) * 16 + 8 * q + g] = acc[i][q][x];
-    }
-};
-
-__device__ __forceinline__ float activate(float v, int act) {
-    switch (act) {
-        case MLQ_ACT_SILU: return v / (1.0f + expf(-v));
-        // v * Phi(v), by the complementary error function: no cancellation for negative v
-        case MLQ_ACT_GELU: return 0.5f * v * erfcf(-0.70710678118654752f * v);
-        // 0.5 (1 + tanh u) = 1 / (1 + exp(-2 u)), u = sqrt(2 / pi) (v + 0.044715 v^3)
-        case MLQ_ACT_GELU_TANH: return v / (1.0f + expf(-1.5957691216057308f * v * (1.0f + 0.044715f * v * v)));
-        case MLQ_ACT_RELU: return v < 0.0f ? 0.0f : v;
-        case MLQ_ACT_SIGMOID: return 1.0f / (1.0f + expf(-v));
-        default: return v;
-    }
-}
-
-__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, uint32_t bytes) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-
-// This thread's arrival at an mbarrier once its copies so far have landed.
-__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
-    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
-}
-
 constexpr int kTeams = 2;
 // Records of a round: (K parts) x (rows of x of a segment) <= 8, see choose_strips.
 constexpr int kXStage = 8 * kRecordBytes;
@@ -256,60 +109,13 @@ constexpr int kTeamThreads = 32 * kImmaWarps;
 constexpr int kLaunchRegs = 96, kProducerRegs = 32, kComputeRegs = 112;
 static_assert((2 * kTeams * kProducerRegs + kTeams * kImmaWarps * kComputeRegs) * 32 <= kThreads * kLaunchRegs,
               "the shares must not exceed the launch's registers, or setmaxnreg would wait for ever");
-constexpr int kRedFloats = kImmaWarps * kSegTokens * 16;  // [warp][row of x][row of the strip]
+constexpr int kRedFloats = kImmaWarps * kFewRows * 16;  // [warp][row of x][row of the strip]
+constexpr int kJoinRounds = 4;  // adding up a shared unit: ~2.5 us; a round takes ~0.8 us of a team's share of HBM
 
 // The barrier of a team's computing warps.
 __device__ __forceinline__ void team_sync(int team) {
     asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "n"(kTeamThreads) : "memory");
 }
-
-// How a launch's units, of `per` rounds each, are dealt out.  Every team takes
-// `each` whole units; the units left over are spread by rounds, a contiguous
-// range per team, when that saves more than the adding up costs (about 2 us
-// for whoever finishes a shared unit, where a round takes about 0.8 us of a
-// team's share of HBM), else one unit each to as many teams.
-struct Deal {
-    int teams, per, each, rest;  // rest: units left over
-    long long rounds;            // theirs, dealt by rounds to the first `sharers` teams; 0: dealt whole
-    int sharers;                 // each has a round at least: who shares a unit follows from its ends
-    __device__ __forceinline__ Deal(int units, int per_, int teams_) : teams(teams_), per(per_) {
-        each = units / teams;
-        rest = units - each * teams;
-        const long long all = (long long)rest * per;
-        rounds = (all + teams - 1) / teams + 4 < per ? all : 0;
-        sharers = rounds < teams ? (int)rounds : teams;
-    }
-    // first round (among the left-over units') of team i, and the team that has round t
-    __device__ __forceinline__ long long begin(int i) const { return i < sharers ? rounds * i / sharers : rounds; }
-    __device__ __forceinline__ int owner(long long t) const { return (int)(((t + 1) * sharers - 1) / rounds); }
-};
-
-// A team's work, piece by piece: rounds [r0, r1) of unit u.
-struct Work {
-    int u, r0, r1, n;    // the piece, and how many there were
-    long long t, t_end;  // rounds of left-over units still to come
-    int left;            // whole units still to come
-    __device__ __forceinline__ Work(const Deal& d, int id) : u(0), r0(0), r1(0), n(0) {
-        left = d.each + (d.rounds == 0 && id < d.rest ? 1 : 0);
-        t = d.rounds ? d.begin(id) : 0;
-        t_end = d.rounds ? d.begin(id + 1) : 0;
-    }
-    // whole units lie `teams` apart, so that the teams work on neighbours
-    __device__ __forceinline__ bool next(const Deal& d, int id) {
-        if (left > 0) {
-            u = n * d.teams + id, r0 = 0, r1 = d.per;
-            --left, ++n;
-            return true;
-        }
-        if (t >= t_end) return false;
-        const int k = (int)(t / d.per);
-        u = d.each * d.teams + k;
-        r0 = (int)(t - (long long)k * d.per);
-        r1 = t_end - t < d.per - r0 ? r0 + (int)(t_end - t) : d.per;
-        t += r1 - r0;
-        return true;
-    }
-};
 
 // What a producer fetches next: round `round` of a tile against a segment, into `stage`.
 struct Cursor {
@@ -330,13 +136,11 @@ struct WarpState {
 // What a computing warp needs for its part of a unit (by value: the function
 // below has registers of its own).
 struct UnitArgs {
-    XView x;                 // halves
-    const int* order;        // kPair: position -> pair
     float* red;              // this warp's sums
     uint32_t full, slots;    // barrier of stage 0 (16 bytes each: full, empty), this warp's slot of stage 0
     uint32_t stage_bytes, to_x;  // from the slot to the records of this warp's K part
     int stages;
-    int top_k, first, count;
+    int count;
     int c0, c_end, kws;      // K steps: c0, c0 + kws, .. below c_end
     int rounds, blocks;      // rounds of this part, blocks of a row
     uint32_t window0, window1, window_step;  // rows that are not aligned: where row g (g + 8) starts in its window
@@ -346,19 +150,13 @@ struct UnitArgs {
 
 // The rounds of one unit: this warp's strip against the segment's rows of x,
 // its sums to u.red.  A function of its own for each form of x.
-template <class Acc, int F, int MODE, bool FEW, bool ALN>
+template <class Acc, int F, bool ALN>
 __device__ __forceinline__ WarpState unit_sums(const UnitArgs u, WarpState st) {
     using S = Slot<F, ALN>;
     const int lane = threadIdx.x & 31, g = lane >> 2;
     int c = u.c0;
     Acc acc;
-    if constexpr (FEW)
-        acc.init(u.count, lane);
-    else
-        acc.init(u.x, u.count, (c < u.c_end ? c : 0) * kChunkBlocks, lane, [&](int r) -> int {
-            if (MODE == kPair) return __ldcg(u.order + u.first + r) / u.top_k;
-            return u.first + r;
-        });
+    acc.init(u.count, lane);
     for (int r = 0; r < u.rounds; ++r, c += u.kws) {
         const uint32_t full = u.full + 16 * st.stage, at = u.slots + st.stage * u.stage_bytes;
         if (!__all_sync(0xffffffffu, mbar_try_wait(full, st.phase)) && st.alive &&
@@ -373,12 +171,7 @@ __device__ __forceinline__ WarpState unit_sums(const UnitArgs u, WarpState st) {
                 row1 += (u.window1 + (uint32_t)c * u.window_step) & 15;
             }
             const int valid = u.blocks - c * kChunkBlocks;
-            if constexpr (FEW) {
-                acc.template step<ALN>(at + u.to_x, valid, row0, row1, lane);
-            } else {
-                const int ahead = c + u.kws < u.c_end ? u.kws * kChunkBlocks : 0;  // to the step after this one
-                acc.template step<ALN>(ahead, valid, row0, row1, lane);
-            }
+            acc.template step<ALN>(at + u.to_x, valid, row0, row1, lane);
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(full + 8);
@@ -389,9 +182,9 @@ __device__ __forceinline__ WarpState unit_sums(const UnitArgs u, WarpState st) {
     return st;
 }
 
-template <int F, int MODE, bool FEW, bool ALN>
+template <int F, int MODE, bool ALN>
 __global__ void __launch_bounds__(kThreads, 1)
-    imma_kernel(const __grid_constant__ ImmaMaps maps, const __grid_constant__ ImmaArgs a) {
+    imma_few_kernel(const __grid_constant__ ImmaMaps maps, const __grid_constant__ ImmaArgs a) {
     extern __shared__ __align__(128) uint8_t smem[];
     using S = Slot<F, ALN>;
     __shared__ int s_last[kTeams], s_dead, s_issued[kTeams][2];
@@ -402,10 +195,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int steps = (a.bpr + kChunkBlocks - 1) / kChunkBlocks;
     const int per_seg = (steps + kws - 1) / kws;  // rounds of a tile against a segment
     // shared memory: stages [team][stage] of the warps' weights and the rounds' records of x, sums [team], (all_segs) y [team], the stages' barriers [team][stage] (full, empty)
-    constexpr uint32_t kStage = kImmaWarps * S::kBytes + (FEW ? kXStage : 0);
+    constexpr uint32_t kStage = kImmaWarps * S::kBytes + kXStage;
     const uint32_t red0 = kTeams * a.slots * kStage;
     const uint32_t y_floats = MODE == kDown && !a.part ? a.rows * 16 * a.strips : 0;
-    const uint32_t bars0 = smem_u32(smem) + red0 + kTeams * (kRedFloats + y_floats) * 4;
+    const uint32_t bars0 = smem_u32(smem) + red0 + kTeams * (2 * kRedFloats + y_floats) * 4;
     const uint32_t bars = bars0 + 16 * team * a.slots;
     const uint32_t ring = smem_u32(smem) + team * a.slots * kStage;
     if (threadIdx.x == 0) {
@@ -429,7 +222,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const bool all_segs = MODE == kDown && !a.part;
     const int id = kTeams * blockIdx.x + team;
     const Deal deal(all_segs ? (nseg ? a.tiles : 0) : nseg * a.tiles, all_segs ? nseg * per_seg : per_seg,
-                    kTeams * gridDim.x);
+                    kTeams * gridDim.x, kJoinRounds);
     Work work(deal, id);
     const int unit_rows = (MODE == kPair ? 8 : 16) * a.strips;
 
@@ -461,18 +254,16 @@ __global__ void __launch_bounds__(kThreads, 1)
             c.fresh = false;
             const int e = MODE == kPlain ? 0 : __ldcg(&a.segs[c.seg].expert);
             c.row0 = e * a.out + c.tile * unit_rows;
-            if (FEW) {
-                c.first = MODE == kPlain ? c.seg * a.seg_cap : __ldcg(&a.segs[c.seg].start);
-                c.count = MODE == kPlain ? (a.rows - c.first < a.seg_cap ? a.rows - c.first : a.seg_cap)
-                                         : __ldcg(&a.segs[c.seg].count);
-            }
+            c.first = MODE == kPlain ? c.seg * a.seg_cap : __ldcg(&a.segs[c.seg].start);
+            c.count = MODE == kPlain ? (a.rows - c.first < a.seg_cap ? a.rows - c.first : a.seg_cap)
+                                     : __ldcg(&a.segs[c.seg].count);
         };
         auto active = [&](const Cursor& c) { return min(steps - c.round * kws, kws); };  // K parts of the round
         auto fetch_weights = [&](Cursor& c) {
             const uint32_t full = bars + 16 * c.stage, dst = ring + c.stage * kStage;
             if constexpr (ALN) {
                 if (lane == 0)
-                    mbar_arrive_expect_tx(full, active(c) * (a.strips * S::kBytes + (FEW ? c.count * kRecordBytes : 0)));
+                    mbar_arrive_expect_tx(full, active(c) * (a.strips * S::kBytes + c.count * kRecordBytes));
                 __syncwarp();
                 const int kw = lane / a.strips;
                 if (kw < active(c)) {
@@ -487,7 +278,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 __syncwarp();
             } else {
-                if (FEW && half == 0 && lane == 0) mbar_expect_tx(full, active(c) * c.count * kRecordBytes);
+                if (half == 0 && lane == 0) mbar_expect_tx(full, active(c) * c.count * kRecordBytes);
                 // lanes 2r, 2r + 1: the windows that hold row r's blocks
                 const int r = lane >> 1, sub = lane & 1;
                 const uint8_t* base = MODE == kPair && r >= 8 ? a.w[1] : a.w[0];
@@ -528,12 +319,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         };
         // lane (K part, row of x): its record
         auto fetch_x = [&](Cursor& c) {
-            if (!FEW || (!ALN && half)) return;
+            if (!ALN && half) return;
             const int kw = lane / a.seg_cap, r = lane % a.seg_cap;
             if (kw < active(c) && r < c.count) {
                 const int row = MODE == kPair ? __ldcg(a.order + c.first + r) / a.top_k : c.first + r;
                 bulk_g2s(ring + c.stage * kStage + kImmaWarps * S::kBytes + lane * kRecordBytes,
-                         a.x.data + ((size_t)row * (a.bprp / kChunkBlocks) + c.round * kws + kw) * kRecordBytes, kRecordBytes,
+                         a.x + ((size_t)row * (a.bprp / kChunkBlocks) + c.round * kws + kw) * kRecordBytes, kRecordBytes,
                          bars + 16 * c.stage);
             }
             __syncwarp();
@@ -572,11 +363,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (MODE == kDown) launch_dependents();
     const int warp = cta_warp % kImmaWarps, tid = threadIdx.x % kTeamThreads;
     const int strip = warp % a.strips, kw = warp / a.strips;
-    float* red = reinterpret_cast<float*>(smem + red0) + team * kRedFloats;
+    float* red = reinterpret_cast<float*>(smem + red0) + team * 2 * kRedFloats;
     WarpState st{0, 0, 0, true};
     int half = 0;
-    bool wide = false;  // the last unit's sums took the whole buffer
-    float* ysum = reinterpret_cast<float*>(smem + red0) + kTeams * kRedFloats + team * y_floats;  // all_segs: [row][row of the tile]
+    float* ysum = reinterpret_cast<float*>(smem + red0) + kTeams * 2 * kRedFloats + team * y_floats;  // all_segs: [row][row of the tile]
 
     // Units that several teams share.  A team's tail slot holds the piece of the unit that starts in its range, its head
     // slot that of the unit that started before.
@@ -622,19 +412,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                 first = __ldcg(&a.segs[seg].start);
                 count = __ldcg(&a.segs[seg].count);
             }
-            // sums of up to 16 rows of x alternate between the buffer's halves; more take it all
-            const int tokens = count <= 16 ? 16 : 32;
-            if (wide || count > 16) team_sync(team);
-            wide = count > 16;
-            float* rb = red + (wide ? 0 : half * (kRedFloats / 2));
+            float* rb = red + half * kRedFloats;  // the buffers alternate
             half ^= 1;
             UnitArgs u{};
-            u.x = XView{a.x.data, a.x.scale, a.x.sum, (uint32_t)a.bprp};
-            u.order = a.order, u.top_k = a.top_k;
-            u.red = rb + warp * tokens * 16;
+            u.red = rb + warp * kFewRows * 16;
             u.full = bars, u.slots = ring + warp * S::kBytes, u.stages = a.slots, u.stage_bytes = kStage;
             u.to_x = (kImmaWarps - warp) * S::kBytes + kw * a.seg_cap * kRecordBytes;
-            u.first = first, u.count = count;
+            u.count = count;
             u.c0 = r0 * kws + kw, u.kws = kws, u.rounds = r1 - r0, u.blocks = a.bpr;
             u.c_end = r1 * kws < steps ? r1 * kws : steps;
             u.err = a.err, u.dead = &s_dead;
@@ -646,23 +430,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                                        (MODE == kPair ? 0 : 8 * a.row_bytes)) & 15;
                 u.window_step = chunk_bytes(F) & 15;
             }
-            if constexpr (FEW) {
-                if (count <= 2)
-                    st = unit_sums<FewRows<F, 1>, F, MODE, FEW, ALN>(u, st);
-                else
-                    st = unit_sums<FewRows<F, 2>, F, MODE, FEW, ALN>(u, st);
-            } else {
-                if (count <= 8)
-                    st = unit_sums<ManyRows<F, 1>, F, MODE, FEW, ALN>(u, st);
-                else if (count <= 16)
-                    st = unit_sums<ManyRows<F, 2>, F, MODE, FEW, ALN>(u, st);
-                else
-                    st = unit_sums<ManyRows<F, 4>, F, MODE, FEW, ALN>(u, st);
-            }
+            if (count <= 2)
+                st = unit_sums<FewRows<F, 1>, F, ALN>(u, st);
+            else
+                st = unit_sums<FewRows<F, 2>, F, ALN>(u, st);
             team_sync(team);
             auto sum_parts = [&](int tok, int row) {
                 float v = 0.0f;
-                for (int k = 0; k < kws; ++k) v += rb[((k * a.strips + (row >> 4)) * tokens + tok) * 16 + (row & 15)];
+                for (int k = 0; k < kws; ++k) v += rb[((k * a.strips + (row >> 4)) * kFewRows + tok) * 16 + (row & 15)];
                 return v;
             };
 
@@ -688,16 +463,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                     for (int i = warp; i < count * blocks; i += kImmaWarps) {
                         const int tok = i / blocks, b = tile * blocks + i % blocks;
                         if (32 * b >= a.out) continue;
-                        const int el = FEW ? imma_element(a.next_fmt, b & 1, lane) : half_element(a.next_fmt, b & 1, lane);
+                        const int el = imma_element(a.next_fmt, b & 1, lane);
                         const int loc = 32 * (i % blocks) + el;
                         const int row = (loc >> 3) * 16 + (loc & 7);
                         const float h = 32 * b + el < a.out ? silu_mul(get(tok, row), get(tok, row + 8)) : 0.0f;
-                        const size_t to = (size_t)(first + tok) * a.next_bprp + b;
-                        if (FEW)
-                            slice_digits(h, digit_weight(a.next_fmt, lane),
-                                         a.h.data + (size_t)(first + tok) * (a.next_bprp / kChunkBlocks) * kRecordBytes, b, lane);
-                        else
-                            slice_halves(h, a.h.data + to * kSlicedBytes, a.h.scale + to, a.h.sum + to, lane);
+                        slice_digits(h, digit_weight(a.next_fmt, lane),
+                                     a.h + (size_t)(first + tok) * (a.next_bprp / kChunkBlocks) * kRecordBytes, b, lane);
                     }
                 } else {
                     for (int i = tid; i < unit_rows * count; i += kTeamThreads) {
@@ -760,64 +531,43 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int i = st.taken; i < s_issued[team][i & 1]; ++i) mbar_wait(bars + 16 * (i % a.slots), (i / a.slots) & 1);
 }
 
-bool aligned_rows(int fmt, const void* w, int bpr) {
-    return reinterpret_cast<uintptr_t>(w) % 16 == 0 && (long long)bpr * block_bytes(fmt) % 16 == 0 &&
-           encode_fn() != nullptr;
-}
-
 // Ring depth: what the SM's shared memory leaves room for, 2..8 stages.
-template <int F, int MODE, bool FEW, bool ALN>
+template <int F, int MODE, bool ALN>
 cudaError_t launch_one(ImmaArgs a, int grid, int smem_per_sm, cudaStream_t stream) {
     using S = Slot<F, ALN>;
-    auto k = imma_kernel<F, MODE, FEW, ALN>;
-    const int sums = kTeams * (kRedFloats + (MODE == kDown && !a.part ? a.rows * 16 * a.strips : 0)) * 4;
+    auto k = imma_few_kernel<F, MODE, ALN>;
+    const int sums = kTeams * (2 * kRedFloats + (MODE == kDown && !a.part ? a.rows * 16 * a.strips : 0)) * 4;
     const int fixed = sums + 1024 + 256;  // the system's 1 KB per CTA, the static part
-    constexpr int stage = kImmaWarps * S::kBytes + (FEW ? kXStage : 0);
+    constexpr int stage = kImmaWarps * S::kBytes + kXStage;
     a.slots = (smem_per_sm - fixed) / (kTeams * (stage + 16));
     if (a.slots > 8) a.slots = 8;
     if (a.slots < 2) return cudaErrorInvalidConfiguration;
     const size_t smem = (size_t)kTeams * a.slots * (stage + 16) + sums;
     ImmaMaps maps{};
-    if (ALN) {
-        for (int i = 0; i < (MODE == kPair ? 2 : 1); ++i)
-            if (!make_map_2d(&maps.m[i], CU_TENSOR_MAP_DATA_TYPE_UINT16, const_cast<uint8_t*>(a.w[i]),
-                             (uint64_t)a.row_bytes / 2, (uint64_t)a.total_rows, (uint64_t)a.row_bytes, S::kPitch / 2,
-                             MODE == kPair ? 8 : 16, CU_TENSOR_MAP_SWIZZLE_NONE))
-                return cudaErrorInvalidValue;
-    }
-    // once per kernel: its shared memory, and that it was built with the registers its split counts on
-    static const cudaError_t ready = [&] {
-        cudaFuncAttributes fa{};
-        cudaError_t e = cudaFuncGetAttributes(&fa, k);
-        if (e == cudaSuccess && fa.numRegs < kLaunchRegs) e = cudaErrorInvalidConfiguration;
-        return e;
-    }();
-    if (ready != cudaSuccess) return ready;
-    cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (ALN && !make_weight_maps(&maps, a, MODE == kPair, S::kPitch)) return cudaErrorInvalidValue;
+    cudaError_t e = ready_kernel(k, smem, kLaunchRegs);
     if (e != cudaSuccess) return e;
     return launch_pdl(k, grid, kThreads, smem, stream, maps, a);
 }
 
 template <int MODE>
-cudaError_t launch_imma(int fmt, ImmaArgs a, int sm_count, int smem_per_sm, long long max_units, cudaStream_t stream) {
+cudaError_t launch_few(int fmt, ImmaArgs a, int sm_count, int smem_per_sm, long long max_units, cudaStream_t stream) {
     const bool aln = aligned_rows(fmt, a.w[0], a.bpr) && (MODE != kPair || aligned_rows(fmt, a.w[1], a.bpr));
     a.row_bytes = (long long)a.bpr * block_bytes(fmt);
     const int steps = (a.bpr + kChunkBlocks - 1) / kChunkBlocks, kws = kImmaWarps / a.strips;
     const long long rounds = max_units * ((steps + kws - 1) / kws);
     int grid = sm_count < kMaxTeams / kTeams ? sm_count : kMaxTeams / kTeams;
     if (grid > rounds) grid = rounds < 1 ? 1 : (int)rounds;
-    auto run = [&](auto f) {
-        constexpr int F = decltype(f)::value;
-        if (a.few)
-            return aln ? launch_one<F, MODE, true, true>(a, grid, smem_per_sm, stream)
-                       : launch_one<F, MODE, true, false>(a, grid, smem_per_sm, stream);
-        return aln ? launch_one<F, MODE, false, true>(a, grid, smem_per_sm, stream)
-                   : launch_one<F, MODE, false, false>(a, grid, smem_per_sm, stream);
-    };
     switch (fmt) {
-        case kQ8_0: return run(std::integral_constant<int, kQ8_0>{});
-        case kQ4_0: return run(std::integral_constant<int, kQ4_0>{});
-        default: return run(std::integral_constant<int, kQ4_1>{});
+        case kQ8_0:
+            return aln ? launch_one<kQ8_0, MODE, true>(a, grid, smem_per_sm, stream)
+                       : launch_one<kQ8_0, MODE, false>(a, grid, smem_per_sm, stream);
+        case kQ4_0:
+            return aln ? launch_one<kQ4_0, MODE, true>(a, grid, smem_per_sm, stream)
+                       : launch_one<kQ4_0, MODE, false>(a, grid, smem_per_sm, stream);
+        default:
+            return aln ? launch_one<kQ4_1, MODE, true>(a, grid, smem_per_sm, stream)
+                       : launch_one<kQ4_1, MODE, false>(a, grid, smem_per_sm, stream);
     }
 }
 
