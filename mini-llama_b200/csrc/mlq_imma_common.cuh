@@ -2,6 +2,7 @@
 // asynchronous copies, and how work is dealt out.
 #pragma once
 
+#include <atomic>
 #include <type_traits>
 
 #include "mlq_imma_args.cuh"
@@ -104,18 +105,27 @@ inline bool make_weight_maps(ImmaMaps* maps, const ImmaArgs& a, bool pair, int b
     return true;
 }
 
-// A kernel may use `smem` bytes, and was built with the registers that its
-// split between producers and computing warps counts on (fewer, and the
-// computing warps would wait for more for ever).
+// Once per kernel and device (`done`: a bit per device): the kernel may use
+// all the shared memory there is, and was built with the registers that its split
+// between producers and computing warps counts on (with fewer, the computing
+// warps would wait for more for ever).
 template <class Kernel>
-cudaError_t ready_kernel(Kernel k, size_t smem, int regs) {
+cudaError_t ready_kernel(Kernel k, int regs, std::atomic<uint64_t>& done) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = 1ull << (dev & 63);
+    if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
     cudaFuncAttributes fa{};
-    cudaError_t e = cudaFuncGetAttributes(&fa, k);
+    e = cudaFuncGetAttributes(&fa, k);
     if (e != cudaSuccess) return e;
     if (fa.numRegs < regs) return cudaErrorInvalidConfiguration;
-    return (size_t)fa.maxDynamicSharedSizeBytes >= smem
-               ? cudaSuccess
-               : cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    int most = 0;
+    e = cudaDeviceGetAttribute(&most, cudaDevAttrMaxSharedMemoryPerBlockOptin, dev);
+    if (e == cudaSuccess)
+        e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, most - (int)fa.sharedSizeBytes);
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+    return e;
 }
 
 }  // namespace

@@ -545,7 +545,8 @@ cudaError_t launch_one(ImmaArgs a, int grid, int smem_per_sm, cudaStream_t strea
     const size_t smem = (size_t)kTeams * a.slots * (stage + 16) + sums;
     ImmaMaps maps{};
     if (ALN && !make_weight_maps(&maps, a, MODE == kPair, S::kPitch)) return cudaErrorInvalidValue;
-    cudaError_t e = ready_kernel(k, smem, kLaunchRegs);
+    static std::atomic<uint64_t> done{0};
+    cudaError_t e = ready_kernel(k, kLaunchRegs, done);
     if (e != cudaSuccess) return e;
     return launch_pdl(k, grid, kThreads, smem, stream, maps, a);
 }

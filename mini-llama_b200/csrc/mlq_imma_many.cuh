@@ -411,7 +411,8 @@ cudaError_t launch_one(ImmaArgs a, int grid, int smem_per_sm, cudaStream_t strea
     const size_t smem = (size_t)a.slots * (stage + 16) + kSumFloats * 4;
     ImmaMaps maps{};
     if (ALN && !make_weight_maps(&maps, a, MODE == kPair, S::kPitch)) return cudaErrorInvalidValue;
-    cudaError_t e = ready_kernel(k, smem, kManyLaunchRegs);
+    static std::atomic<uint64_t> done{0};
+    cudaError_t e = ready_kernel(k, kManyLaunchRegs, done);
     if (e != cudaSuccess) return e;
     return launch_pdl(k, grid, kManyThreads, smem, stream, maps, a);
 }

@@ -265,7 +265,9 @@ __global__ void __launch_bounds__(32 * kTopkWarps) route_topk_kernel(const Route
 }
 
 constexpr int kPassRows = 4096;
-constexpr int kTileRows = 128;  // rows from which the tiled logits are faster
+// rows x experts from which the tiled logits are faster (K = 3584: 127 x 256 takes 33 us there and 150 us tiled, where a
+// tile's K steps take that long however few the tiles; 2048 x 256 takes ~600 us there and ~300 us tiled)
+constexpr long long kTileWork = 280 * 1024;
 
 template <typename... Params, typename... Args>
 cudaError_t launch_pdl(void (*kernel)(Params...), dim3 grid, int block, size_t smem, cudaStream_t stream, Args&&... args) {
@@ -307,15 +309,18 @@ cudaError_t launch_route(const mlq_router& r, const float* x, int rows, int32_t*
         cudaError_t e;
         if (a.rows == 1)
             e = launch_pdl(route_logits_kernel<2, 1>, dim3(up(a.n_experts, 2)), 256, 0, stream, a, vec);
-        else if (a.rows < kTileRows)
+        else if ((long long)a.rows * a.n_experts < kTileWork)
             e = launch_pdl(route_logits_kernel<4, 4>, dim3(up(a.n_experts, 4), up(a.rows, 4)), 256, 0, stream, a, vec);
         else
             e = launch_pdl(route_tile_kernel, dim3(up(a.rows, kTile), up(a.n_experts, kTile)), 256, 0, stream, a, vec);
         if (e != cudaSuccess) return e;
+        // at most 64 KB (1024 experts); the default limit of 48 KB is raised only for calls that need it
         const size_t smem = (size_t)kTopkWarps * 2 * a.n_experts * sizeof(double);
-        e = cudaFuncSetAttribute(route_topk_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 (int)(kTopkWarps * 2 * MLQ_MOE_MAX_EXPERTS * sizeof(double)));
-        if (e != cudaSuccess) return e;
+        if (smem > 48 * 1024) {
+            e = cudaFuncSetAttribute(route_topk_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     (int)(kTopkWarps * 2 * MLQ_MOE_MAX_EXPERTS * sizeof(double)));
+            if (e != cudaSuccess) return e;
+        }
         e = launch_pdl(route_topk_kernel, dim3(up(a.rows, kTopkWarps)), 32 * kTopkWarps, smem, stream, a);
         if (e != cudaSuccess) return e;
     }

@@ -575,62 +575,76 @@ def _moe_lib():
     return L
 
 
+_torch = None
+
+
+def _the_torch():
+    """torch, imported on first use (a decode step's calls cost microseconds,
+    an import statement in each of them some tenths)."""
+    global _torch
+    if _torch is None:
+        import torch
+        _torch = torch
+    return _torch
+
+
 def _need(t, dtype, shape, device, what: str):
     """The address of a dense tensor of this dtype, shape and device (None
     for None); ValueError otherwise: the C ABI takes bare pointers."""
     if t is None:
         return None
-    if t.dtype != dtype or tuple(t.shape) != tuple(shape) or t.device != device or not t.is_contiguous():
+    if t.dtype is not dtype or t.shape != shape or t.device != device or not t.is_contiguous():
         raise ValueError(f"{what}: expected a contiguous {dtype} tensor of shape {tuple(shape)} on {device}, got "
                          f"{t.dtype} {tuple(t.shape)} on {t.device} with strides {t.stride()}")
     return t.data_ptr()
 
 
 def _rows_of(x, in_features: int):
-    if x.dim() not in (1, 2) or x.shape[-1] != in_features:
-        raise ValueError(f"x: expected [rows, {in_features}] or [{in_features}], got {tuple(x.shape)}")
-    return 1 if x.dim() == 1 else x.shape[0]
+    shape = x.shape
+    if len(shape) not in (1, 2) or shape[-1] != in_features:
+        raise ValueError(f"x: expected [rows, {in_features}] or [{in_features}], got {tuple(shape)}")
+    return 1 if len(shape) == 1 else shape[0]
 
 
 def _blocks_need(w, fmt, rows: int, cols: int, device, what: str) -> int:
     """Address of packed blocks [rows][ceil(cols / 32)] (uint8, any shape)."""
-    import torch
-    name = _fmt_name(fmt)
-    if w is None or w.dtype != torch.uint8 or not w.is_contiguous() or w.device != device:
+    if w is None or w.dtype is not _the_torch().uint8 or not w.is_contiguous() or w.device != device:
         raise ValueError(f"{what}: expected contiguous uint8 blocks on {device}")
-    if w.numel() != weight_bytes(name, rows, cols):
-        raise ValueError(f"{what}: expected {weight_bytes(name, rows, cols)} bytes, got {w.numel()}")
+    if w.numel() != weight_bytes(_fmt_name(fmt), rows, cols):
+        raise ValueError(f"{what}: expected {weight_bytes(_fmt_name(fmt), rows, cols)} bytes, got {w.numel()}")
     return w.data_ptr()
 
 
-class _On:
-    """Makes a tensor's device current for one call (the library runs on the
+def _on_device(device, stream, fn, *args) -> None:
+    """fn(*args, stream handle) with `device` current (the library runs on the
     current device); stream: the caller's, or that device's current one."""
+    torch = _the_torch()
+    if device.type != "cuda":
+        raise ValueError(f"expected CUDA tensors, got tensors on {device}")
+    if stream is None:
+        # the handle alone: a Stream object costs 3 us, as much as two launches
+        stream = torch._C._cuda_getCurrentRawStream(device.index)
+    elif not isinstance(stream, int):
+        stream = stream.cuda_stream
+    if torch.cuda.current_device() != device.index:
+        with torch.cuda.device(device):
+            status = fn(*args, stream)
+    else:
+        status = fn(*args, stream)
+    if status:
+        check(status)
 
-    def __init__(self, device, stream):
-        import torch
-        if device.type != "cuda":
-            raise ValueError(f"expected CUDA tensors, got tensors on {device}")
-        self.other = device.index is not None and device.index != torch.cuda.current_device()
-        if self.other:
-            self.guard = torch.cuda.device(device)
-            self.guard.__enter__()
-        self.stream = _stream_handle(stream)
 
-    def done(self):
-        if self.other:
-            self.guard.__exit__(None, None, None)
-
-
-def _workspace(ws, need: int, device):
-    """The caller's workspace, or a fresh one from torch's allocator (which
-    keeps it alive in stream order, and per graph under capture)."""
-    import torch
+def _workspace(ws, need, device):
+    """(address, bytes) of the caller's workspace, or of a fresh one of need()
+    bytes from torch's allocator (which keeps it alive in stream order, and
+    per graph under capture), and the tensor."""
+    uint8 = _the_torch().uint8
     if ws is None:
-        return torch.empty(need, dtype=torch.uint8, device=device)
-    if ws.dtype != torch.uint8 or not ws.is_contiguous() or ws.device != device:
+        ws = _the_torch().empty(need(), dtype=uint8, device=device)
+    elif ws.dtype is not uint8 or ws.device != device or not ws.is_contiguous():
         raise ValueError(f"workspace: expected a contiguous uint8 tensor on {device}")
-    return ws
+    return ws.data_ptr(), ws.numel(), ws
 
 
 class Router:
@@ -639,7 +653,7 @@ class Router:
 
     def __init__(self, w, top_k: int, bias=None, scoring: str = "softmax", renormalize: bool = True,
                  scale: float = 1.0):
-        import torch
+        torch = _the_torch()
         if w.dim() != 2:
             raise ValueError("router weights: expected [n_experts, in_features]")
         if scoring not in SCORINGS:
@@ -699,25 +713,19 @@ def moe_route(router: Router, x, ids=None, weights=None, logits=None, workspace=
     """mlq_moe_route: (ids int32 [rows, top_k], weights float32 [rows, top_k])
     of x float32 [rows, in] (or [in]).  logits: float32 [rows, n_experts] to
     fill, or None.  Without `workspace` one is allocated for the call."""
-    import torch
-    L = _moe_lib()
-    dev = x.device
+    torch = _the_torch()
+    dev, f32 = router.device, torch.float32
     rows = _rows_of(x, router.in_features)
-    xp = _need(x, torch.float32, x.shape, router.device, "x")
+    xp = _need(x, f32, x.shape, dev, "x")
     shape = (rows, router.top_k)
     if ids is None:
-        ids = torch.empty(shape, dtype=torch.int32, device=dev)
+        ids = x.new_empty(shape, dtype=torch.int32)
     if weights is None:
-        weights = torch.empty(shape, dtype=torch.float32, device=dev)
-    ws = _workspace(workspace, 0 if workspace is not None else route_workspace_bytes(router, rows), dev)
-    on = _On(dev, stream)
-    try:
-        check(L.mlq_moe_route(router.ref, xp, rows, _need(ids, torch.int32, shape, dev, "ids"),
-                              _need(weights, torch.float32, shape, dev, "weights"),
-                              _need(logits, torch.float32, (rows, router.n_experts), dev, "logits"),
-                              ws.data_ptr(), ws.numel(), on.stream))
-    finally:
-        on.done()
+        weights = x.new_empty(shape)
+    ws, nws, _keep = _workspace(workspace, lambda: route_workspace_bytes(router, rows), dev)
+    _on_device(dev, stream, _moe_lib().mlq_moe_route, router.ref, xp, rows, _need(ids, torch.int32, shape, dev, "ids"),
+               _need(weights, f32, shape, dev, "weights"),
+               _need(logits, f32, (rows, router.n_experts), dev, "logits"), ws, nws)
     return ids, weights
 
 
@@ -725,25 +733,19 @@ def moe_experts(experts: Experts, x, ids, weights, residual=None, y=None, worksp
     """mlq_moe_experts: y = residual + sum over slots of weights * expert(x),
     ids int32 / weights float32 [rows, top_k]; ids outside [0, n_experts) add
     nothing."""
-    import torch
-    L = _moe_lib()
-    dev = x.device
+    torch = _the_torch()
+    dev, f32 = experts.device, torch.float32
     rows = _rows_of(x, experts.in_features)
-    xp = _need(x, torch.float32, x.shape, experts.device, "x")
+    xp = _need(x, f32, x.shape, dev, "x")
     top_k = ids.shape[-1]
     shape = (rows, top_k) if ids.dim() == 2 else (top_k,)
-    yshape = (experts.out_features,) if x.dim() == 1 else (rows, experts.out_features)
+    yshape = (*x.shape[:-1], experts.out_features)
     if y is None:
-        y = torch.empty(yshape, dtype=torch.float32, device=dev)
-    ws = _workspace(workspace, 0 if workspace is not None else experts_workspace_bytes(experts, rows, top_k), dev)
-    on = _On(dev, stream)
-    try:
-        check(L.mlq_moe_experts(experts.ref, xp, rows, top_k, _need(ids, torch.int32, shape, dev, "ids"),
-                                _need(weights, torch.float32, shape, dev, "weights"),
-                                _need(residual, torch.float32, yshape, dev, "residual"),
-                                _need(y, torch.float32, yshape, dev, "y"), ws.data_ptr(), ws.numel(), on.stream))
-    finally:
-        on.done()
+        y = x.new_empty(yshape)
+    ws, nws, _keep = _workspace(workspace, lambda: experts_workspace_bytes(experts, rows, top_k), dev)
+    _on_device(dev, stream, _moe_lib().mlq_moe_experts, experts.ref, xp, rows, top_k,
+               _need(ids, torch.int32, shape, dev, "ids"), _need(weights, f32, shape, dev, "weights"),
+               _need(residual, f32, yshape, dev, "residual"), _need(y, f32, yshape, dev, "y"), ws, nws)
     return y
 
 
@@ -751,30 +753,24 @@ def moe_layer(router: Router, experts: Experts, x, residual=None, y=None, ids=No
               stream=None):
     """mlq_moe_layer: the router's choice, then the experts; returns
     (y, ids, weights)."""
-    import torch
-    L = _moe_lib()
-    dev = x.device
+    torch = _the_torch()
+    dev, f32 = experts.device, torch.float32
     rows = _rows_of(x, experts.in_features)
-    xp = _need(x, torch.float32, x.shape, experts.device, "x")
+    xp = _need(x, f32, x.shape, dev, "x")
     if router.device != dev:
-        raise ValueError(f"the router is on {router.device}, x on {dev}")
+        raise ValueError(f"the router is on {router.device}, the experts on {dev}")
     shape = (rows, router.top_k)
-    yshape = (experts.out_features,) if x.dim() == 1 else (rows, experts.out_features)
+    yshape = (*x.shape[:-1], experts.out_features)
     if ids is None:
-        ids = torch.empty(shape, dtype=torch.int32, device=dev)
+        ids = x.new_empty(shape, dtype=torch.int32)
     if weights is None:
-        weights = torch.empty(shape, dtype=torch.float32, device=dev)
+        weights = x.new_empty(shape)
     if y is None:
-        y = torch.empty(yshape, dtype=torch.float32, device=dev)
-    ws = _workspace(workspace, 0 if workspace is not None else layer_workspace_bytes(router, experts, rows), dev)
-    on = _On(dev, stream)
-    try:
-        check(L.mlq_moe_layer(router.ref, experts.ref, xp, rows, _need(residual, torch.float32, yshape, dev, "residual"),
-                              _need(y, torch.float32, yshape, dev, "y"), _need(ids, torch.int32, shape, dev, "ids"),
-                              _need(weights, torch.float32, shape, dev, "weights"), ws.data_ptr(), ws.numel(),
-                              on.stream))
-    finally:
-        on.done()
+        y = x.new_empty(yshape)
+    ws, nws, _keep = _workspace(workspace, lambda: layer_workspace_bytes(router, experts, rows), dev)
+    _on_device(dev, stream, _moe_lib().mlq_moe_layer, router.ref, experts.ref, xp, rows,
+               _need(residual, f32, yshape, dev, "residual"), _need(y, f32, yshape, dev, "y"),
+               _need(ids, torch.int32, shape, dev, "ids"), _need(weights, f32, shape, dev, "weights"), ws, nws)
     return y, ids, weights
 
 
@@ -782,27 +778,20 @@ def linear_epilogue(fmt, w, out_features: int, in_features: int, x, bias=None, a
                     residual=None, y=None, workspace=None, stream=None):
     """mlq_linear_epilogue: y = residual + row_scale[:, None] * act(x @ W^T + bias);
     activation: None / "none", "silu", "gelu", "gelu_tanh", "relu", "sigmoid"."""
-    import torch
-    L = _moe_lib()
-    if activation not in ACTIVATIONS:
+    torch = _the_torch()
+    act = ACTIVATIONS.get(activation)
+    if act is None:
         raise ValueError(f"unknown activation {activation!r}")
-    dev = x.device
+    dev, f32 = x.device, torch.float32
     rows = _rows_of(x, in_features)
-    xp = _need(x, torch.float32, x.shape, dev, "x")
+    xp = _need(x, f32, x.shape, dev, "x")
     wp = _blocks_need(w, fmt, out_features, in_features, dev, "w")
-    yshape = (out_features,) if x.dim() == 1 else (rows, out_features)
+    yshape = (*x.shape[:-1], out_features)
     if y is None:
-        y = torch.empty(yshape, dtype=torch.float32, device=dev)
-    ep = EpilogueStruct(_need(bias, torch.float32, (out_features,), dev, "bias"), ACTIVATIONS[activation],
-                        _need(row_scale, torch.float32, (rows,), dev, "row_scale"),
-                        _need(residual, torch.float32, yshape, dev, "residual"))
-    ws = _workspace(workspace,
-                    0 if workspace is not None else epilogue_workspace_bytes(fmt, out_features, in_features, rows), dev)
-    on = _On(dev, stream)
-    try:
-        check(L.mlq_linear_epilogue(fmt_id(fmt), wp, out_features * blocks_per_row(in_features), out_features,
-                                    in_features, xp, rows, ctypes.byref(ep), _need(y, torch.float32, yshape, dev, "y"),
-                                    ws.data_ptr(), ws.numel(), on.stream))
-    finally:
-        on.done()
+        y = x.new_empty(yshape)
+    ep = EpilogueStruct(_need(bias, f32, (out_features,), dev, "bias"), act,
+                        _need(row_scale, f32, (rows,), dev, "row_scale"), _need(residual, f32, yshape, dev, "residual"))
+    ws, nws, _keep = _workspace(workspace, lambda: epilogue_workspace_bytes(fmt, out_features, in_features, rows), dev)
+    _on_device(dev, stream, _moe_lib().mlq_linear_epilogue, fmt_id(fmt), wp, out_features * blocks_per_row(in_features),
+               out_features, in_features, xp, rows, ctypes.byref(ep), _need(y, f32, yshape, dev, "y"), ws, nws)
     return y
