@@ -469,9 +469,13 @@ typedef struct mlq_router {
  * the bias; renormalized, times scale).  An expert whose choice score is
  * -inf is never chosen (a bias of -inf masks an expert): a slot left without
  * one gets id -1 and weight 0.  A NaN score counts as the greatest.  Chosen
- * scores that sum to 0 give weights of 0.  Logits and scores are computed in
- * 64 bits, so the choice is that of exact arithmetic unless two scores agree
- * to ~1e-15.  logits: [rows][n_experts] fp32, or NULL. */
+ * scores that sum to 0 give weights of 0.  The choice is that of 64-bit
+ * arithmetic: exact unless two scores agree to ~1e-15.  Calls of many rows (from
+ * rows x n_experts x in_features = 2^26 on) compute x W^T from 31-bit fixed point with
+ * exact sums; a row whose choice that leaves open is computed again in 64 bits, and so is
+ * one whose logits could be off by more than 2^-15 (an element 1000 times the rest;
+ * ordinary rows: 1e-7 at worst, ~1e-9 seen).  logits: [rows][n_experts]
+ * fp32, or NULL. */
 MLQ_API mlq_status mlq_moe_route(const mlq_router* router, const float* x, int rows, int32_t* ids,
                                  float* weights, float* logits, void* workspace,
                                  size_t workspace_bytes, mlq_stream stream);

@@ -66,7 +66,8 @@ __device__ __forceinline__ float silu_mul(float g, float u) {
 // "empty" wait, 7 = resident x tiles ready wait, 8 = staged x copy wait,
 // 12-16 = GEMM waits, 20-26 = batched-decode GEMM waits, 30-33 = waits of the
 // experts' products and of the linear with an epilogue (few rows: data, free
-// stage; many rows: the same).
+// stage; many rows: the same), 34-36 = waits of the router's products (free
+// stage, data, products done).
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ void report_error(int* err, int code) {
     if (err) atomicCAS(err, 0, code);

@@ -233,9 +233,9 @@ cudaError_t launch_linear_epilogue(int fmt, const uint8_t* w, int out, int in, c
                                    cudaStream_t stream);
 
 // The router (mlq_route.cu).
-size_t route_workspace_bytes(int n_experts, int rows);
+size_t route_workspace_bytes(int n_experts, int in, int rows);
 cudaError_t launch_route(const mlq_router& r, const float* x, int rows, int32_t* ids, float* weights, float* logits,
-                         void* ws, cudaStream_t stream);
+                         void* ws, int* err, cudaStream_t stream);
 
 // Quantize fp32 [rows][cols] -> blocks, reference rules (mlq_convert.cu).
 cudaError_t launch_quantize(int fmt, const float* src, long long rows, int cols, uint8_t* blocks,

@@ -87,7 +87,10 @@ mlq::MoeShape shape_of(const mlq_experts& m) {
 
 mlq_status run_route(const char* who, const mlq_router& r, const float* x, int rows, int32_t* ids, float* weights,
                      float* logits, void* ws, mlq_stream stream) {
-    cudaError_t e = mlq::launch_route(r, x, rows, ids, weights, logits, ws, stream);
+    mlq::DeviceFacts f{};
+    mlq_status st = mlq::current_device_facts(&f);
+    if (st != MLQ_OK) return st;
+    cudaError_t e = mlq::launch_route(r, x, rows, ids, weights, logits, ws, f.err, stream);
     return e == cudaSuccess ? MLQ_OK : fail_cuda(std::string(who) + " launch", e);
 }
 
@@ -112,7 +115,7 @@ extern "C" {
 MLQ_API size_t mlq_moe_route_workspace_bytes(const mlq_router* router, int rows) {
     try {
         if (check_router("mlq_moe_route_workspace_bytes", router) != MLQ_OK || rows <= 0) return 0;
-        return mlq::route_workspace_bytes(router->n_experts, rows);
+        return mlq::route_workspace_bytes(router->n_experts, router->in_features, rows);
     } catch (...) {
         return 0;
     }
@@ -126,7 +129,7 @@ MLQ_API mlq_status mlq_moe_route(const mlq_router* router, const float* x, int r
         if (st == MLQ_OK) st = check_rows(who, rows, router->top_k);
         if (st != MLQ_OK) return st;
         if (!x || !ids || !weights) return fail(MLQ_ERR_NULL, std::string(who) + ": null input/output pointer");
-        st = check_workspace(who, workspace, workspace_bytes, mlq::route_workspace_bytes(router->n_experts, rows));
+        st = check_workspace(who, workspace, workspace_bytes, mlq::route_workspace_bytes(router->n_experts, router->in_features, rows));
         if (st != MLQ_OK) return st;
         return run_route(who, *router, x, rows, ids, weights, logits, workspace, stream);
     } catch (...) {
@@ -171,7 +174,7 @@ MLQ_API size_t mlq_moe_layer_workspace_bytes(const mlq_router* router, const mlq
     try {
         if (!valid_router(router) || check_experts("mlq_moe_layer_workspace_bytes", experts) != MLQ_OK || rows <= 0)
             return 0;
-        return mlq::route_workspace_bytes(router->n_experts, rows) +
+        return mlq::route_workspace_bytes(router->n_experts, router->in_features, rows) +
                mlq::experts_workspace_bytes(shape_of(*experts), rows, router->top_k);
     } catch (...) {
         return 0;
@@ -190,7 +193,7 @@ MLQ_API mlq_status mlq_moe_layer(const mlq_router* router, const mlq_experts* ex
         if (router->n_experts != experts->n_experts || router->in_features != experts->in_features)
             return fail(MLQ_ERR_SHAPE, std::string(who) + ": router and experts differ in n_experts or in_features");
         if (!x || !ids || !weights || !y) return fail(MLQ_ERR_NULL, std::string(who) + ": null input/output pointer");
-        const size_t rb = mlq::route_workspace_bytes(router->n_experts, rows);
+        const size_t rb = mlq::route_workspace_bytes(router->n_experts, router->in_features, rows);
         st = check_workspace(who, workspace, workspace_bytes,
                              rb + mlq::experts_workspace_bytes(shape_of(*experts), rows, router->top_k));
         if (st != MLQ_OK) return st;

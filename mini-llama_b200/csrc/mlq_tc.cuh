@@ -43,6 +43,16 @@ __device__ __forceinline__ void mma_f16kind(uint32_t tmem_d, uint64_t adesc, uin
         : "memory");
 }
 
+// D (+)= A * B^T, one kind::i8 MMA (int8 operands, int32 sums).
+__device__ __forceinline__ void mma_i8kind(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                           uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
 // D (+)= A * B^T with A in tensor memory (address a_tmem: its first
 // column; lane = row of A, 32-bit columns = consecutive K pairs for 16-bit
 // types) and B in shared memory.

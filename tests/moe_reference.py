@@ -154,6 +154,18 @@ def epilogue(x, fmt, blocks, out, bias=None, act="none", row_scale=None, residua
     return y, b + 1e-37
 
 
+def digits_bound(x, w):
+    """How far a logit of 31-bit fixed point digits can be from the exact one.
+    A row's unit is a power of two below 2 amax / 2139062016 (the largest magnitude
+    becomes more than half of that); every value is off by half a unit at
+    most, which meets the other side's magnitudes; of the 16 products of
+    digits three are left out: at most 2 * 2^14 * 2^8 + 2^14 units of both per
+    element, and the product of both halves."""
+    x, w = np.abs(x.astype(np.float64)), np.abs(w.astype(np.float64))
+    ux, uw = x.max(1)[:, None] * 2 / 2139062016, w.max(1)[None] * 2 / 2139062016
+    return 0.5 * ux * w.sum(1) + 0.5 * uw * x.sum(1)[:, None] + x.shape[1] * ux * uw * (2.0 ** 23 + 2.0 ** 14 + 0.25)
+
+
 def route(x, w, top_k, bias=None, scoring="softmax", renormalize=True, scale=1.0):
     logits = x.astype(np.float64) @ w.astype(np.float64).T
     if scoring == "softmax":

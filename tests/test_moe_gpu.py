@@ -388,6 +388,109 @@ def test_route_values_that_are_not_finite(pkg):
     assert ids3[0, 0] == 3 and wt3.isfinite().all() and 5 not in ids3[0].tolist()
 
 
+# many rows: logits by digits, uncertain rows again in 64 bits.  From 64 Mi products
+# (rows x in x experts) and 32 rows on
+# (rows, in, experts, top_k, scoring, bias, renormalize, scale)
+BIG_ROUTES = [
+    (64, 4096, 256, 8, "softmax", False, False, 1.0), (33, 4097, 1024, 64, "sigmoid", True, True, 2.5),
+    (300, 2049, 130, 6, "softmax", True, True, 1.0), (2100, 1024, 40, 2, "softmax", False, True, 1.0),
+    (1025, 8192, 8, 8, "softmax", False, True, 1.0), (4096, 1030, 192, 4, "sigmoid", False, False, 1.0),
+    (129, 17000, 33, 3, "sigmoid", True, True, 1.0), (2048, 36, 1000, 1, "softmax", True, True, 16.0), (1024, 4096, 16, 16, "sigmoid", False, True, 1.0),
+]
+
+
+def big_route(pkg, x, w, k, b, scoring, renorm, scale):
+    """Runs the router and checks choice, weights and logits of finite rows."""
+    r = pkg.mlq.Router(dev(w), k, bias=None if b is None else dev(b), scoring=scoring, renormalize=renorm, scale=scale)
+    rows = x.shape[0]
+    logits = torch.empty(rows, w.shape[0], device="cuda")
+    ids, wt = pkg.mlq.moe_route(r, dev(x), logits=logits)
+    want_ids, want_w, want_l = ref.route(x, w, k, b, scoring, renorm, scale)
+    assert np.array_equal(ids.cpu().numpy(), want_ids)
+    # a row whose bound is above 2^-15 is computed in 64 bits: then only the rounding to fp32 is left (half a step:
+    # 2^-24 of the value, but 2^-150 where the value is below fp32's smallest normal one, 2^-126)
+    bound = np.minimum(ref.digits_bound(x, w), 2.0 ** -15)
+    assert (np.abs(logits.cpu().numpy() - want_l) <= bound + 1.01 * ref.EPS * np.abs(want_l) + 2.0 ** -150 + 2.0 ** -50 * (
+        np.abs(x).astype(np.float64) @ np.abs(w.T).astype(np.float64))).all()
+    # a score is off by a factor of at most exp(2 d) (softmax: its own logit and the sum), the sum of the chosen again
+    rel = np.expm1(4 * bound.max(1))[:, None] + 1.01 * ref.EPS
+    assert (np.abs(wt.cpu().numpy() - want_w) <= rel * want_w + 2.0 ** -150).all()
+    return r, ids, wt
+
+
+@pytest.mark.parametrize("c", BIG_ROUTES, ids=lambda c: "-".join(map(str, c)))
+def test_route_many_rows(pkg, c):
+    rows, cin, n, k, scoring, bias, renorm, scale = c
+    rng = np.random.default_rng(rows + cin)
+    x = rng.standard_normal((rows, cin)).astype(np.float32)
+    w = (rng.standard_normal((n, cin)) / np.sqrt(cin)).astype(np.float32)
+    b = (0.1 * rng.standard_normal(n)).astype(np.float32) if bias else None
+    r, ids, wt = big_route(pkg, x, w, k, b, scoring, renorm, scale)
+    # a workspace of exactly the stated size, filled with ones' bits; again from a graph: the same bits
+    size = pkg.mlq.route_workspace_bytes(r, rows)
+    ws = torch.full((size + 256,), 255, dtype=torch.uint8, device="cuda")
+    xd = dev(x)
+    ids2, wt2 = pkg.mlq.moe_route(r, xd, workspace=ws[:size])
+    assert torch.equal(ids, ids2) and torch.equal(wt, wt2) and (ws[size:] == 255).all()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        pkg.mlq.moe_route(r, xd, ids=ids2, weights=wt2, workspace=ws[:size])
+    ids2.fill_(-7), wt2.fill_(-7)
+    g.replay(), g.replay()
+    assert torch.equal(ids, ids2) and torch.equal(wt, wt2)
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_route_many_rows_ties_outliers_masks(pkg, scoring):
+    """Equal experts (the lowest index), experts one fp32 step apart, rows of zeros, rows with
+    an outlier of 1e5 and rows near the ends of fp32's range; then with masked experts."""
+    rng = np.random.default_rng(12)
+    rows, cin, n = 1100, 1000, 80
+    x = rng.integers(-3, 4, (rows, cin)).astype(np.float32)
+    w = (rng.integers(-1, 2, (11, cin)) / 64).astype(np.float32)[rng.integers(0, 11, n)]
+    w[40:] = rng.standard_normal((n - 40, cin)).astype(np.float32) / 32
+    w[50] = w[49]
+    w[50, 3] = np.nextafter(w[50, 3], np.float32(9))
+    x[5] = 0
+    x[6, 10] = 1e5
+    x[7] *= np.float32(1e-38)
+    x[8] *= np.float32(1e30)
+    x[8, 1:] = 0
+    big_route(pkg, x, w, 9, None, scoring, True, 1.0)
+    b = np.zeros(n, np.float32)
+    b[5:] = -np.inf
+    for open_experts in (3, 0):
+        b[open_experts:] = -np.inf
+        r = pkg.mlq.Router(dev(w), 4, bias=dev(b), scoring=scoring)
+        ids, wt = pkg.mlq.moe_route(r, dev(x))
+        want_ids, _, _ = ref.route(x, w, 4, b, scoring)
+        assert np.array_equal(ids.cpu().numpy(), want_ids) and (wt[ids < 0] == 0).all()
+
+
+def test_route_many_rows_not_finite(pkg):
+    """NaN or infinite rows of x take the first experts or infinite logits' order, as in
+    few rows; the other rows keep their bits.  An infinite weight makes every row uncertain."""
+    rng = np.random.default_rng(13)
+    x = rng.standard_normal((720, 1536)).astype(np.float32)
+    w = rng.standard_normal((66, 1536)).astype(np.float32)
+    r = pkg.mlq.Router(dev(w), 4, scoring="sigmoid")
+    ids, wt = pkg.mlq.moe_route(r, dev(x))
+    y = x.copy()
+    y[100, 5], y[300, 7], y[519, 0] = np.nan, np.inf, -np.inf
+    ids2, wt2 = pkg.mlq.moe_route(r, dev(y))
+    same = [k for k in range(720) if k not in (100, 300, 519)]
+    assert torch.equal(ids[same], ids2[same]) and torch.equal(wt[same], wt2[same])
+    for k in (100, 300, 519):  # one row alone is computed in 64 bits
+        one, onew = pkg.mlq.moe_route(r, dev(y[k:k + 1]))
+        assert torch.equal(one[0], ids2[k]) and torch.equal(onew[0].isnan(), wt2[k].isnan())
+    assert ids2[100].tolist() == [0, 1, 2, 3] and wt2[100].isnan().all()
+    big = w.copy()
+    big[7, 3] = np.inf
+    ids3, wt3 = pkg.mlq.moe_route(pkg.mlq.Router(dev(big), 4, scoring="sigmoid"), dev(x))
+    want, want_w, _ = ref.route(x, big, 4, None, "sigmoid")  # a logit of inf scores 1, as any above 37 does in 64 bits
+    assert np.array_equal(ids3.cpu().numpy(), want) and (np.abs(wt3.cpu().numpy() - want_w) <= 1.01 * ref.EPS * want_w).all()
+
+
 # ---------------------------------------------------------------------------
 # the whole layer, and a block of a model
 # ---------------------------------------------------------------------------
