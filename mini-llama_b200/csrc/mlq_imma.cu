@@ -237,11 +237,12 @@ int max_segments(int pairs, int n_experts, int cap) {
     return full < pairs ? full : pairs;
 }
 
-// Whether a call's rows of x go by digits, in segments of at most 4: while an
-// expert has about two rows its weights' way from HBM takes longer than any
-// work on them; an expert with more rows has several segments, whose weights
-// come from L2 after the first.
-bool few_rows(int pairs, int n_experts) { return pairs <= 2 * n_experts || pairs <= kFewRows; }
+// Whether a call's rows of x go by digits, in segments of at most 4: an
+// expert with more rows has several segments, whose weights come from L2 after the
+// first.  60 experts of 3584 x 2560, q4_0 (q8_0), us by digits and by halves: 2 rows
+// per expert 224 and 300 (302 and 338), 4 rows 281 and 364 (343 and 400), 6 rows
+// 388 and 399 (457 and 430), 12 rows 698 and 592 (802 and 604).
+bool few_rows(int pairs, int n_experts) { return pairs <= 5 * n_experts; }
 
 int prep_ctas(long long blocks, int sm_count) {
     const long long n = (blocks + 7) / 8;
