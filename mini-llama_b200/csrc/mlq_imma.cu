@@ -1,9 +1,9 @@
 // mlq_imma.cu -- the experts' products and the linear with an epilogue
 // (mathematics and operand layout: mlq_imma.cuh).
 //
-// A call is up to three launches, chained by programmatic dependent launch:
-//   prep   sorts the (row, slot) pairs by expert into segments of at most 32
-//          and slices x;
+// A call is three to five launches, chained by programmatic dependent launch:
+//   prep   sorts the (row, slot) pairs by expert into segments and slices x (many
+//          rows: slices in a launch of its own, by sorted position);
 //   pair   h = silu(x Wg^T) * (x Wu^T) per segment, sliced in its epilogue;
 //   down   h Wd^T, weighed and summed per row over the segments of a tile in
 //          order, or, with many rows, by a fourth launch over the slots;
@@ -26,12 +26,12 @@ struct PrepArgs {
     const float* x;
     int rows, in, bpr, bprp, fmt;
     uint8_t* sliced;  // records
-    bool few;         // of digits, else of halves
     int seg_cap;      // rows of a segment at most
     unsigned int* split_done;
     // experts only (ids not null)
     const int32_t* ids;
     int pairs, n_experts;
+    int positions;    // many rows: of order, an expert's first one a multiple of 8 (the others: -1); else 0
     Segment* segs;
     int* nseg;
     int* order;
@@ -55,7 +55,9 @@ __global__ void __launch_bounds__(256) prep_kernel(const PrepArgs a) {
             __shared__ int wsum[2][8];
             __shared__ unsigned char in_warp[8][MLQ_MOE_MAX_EXPERTS];
             for (int e = threadIdx.x; e < a.n_experts; e += 256) cnt[e] = 0;
-            const int pad = a.few ? a.h_bprp - a.h_bpr : 0;  // halves past a row's end are not read
+            const int pad = a.h ? a.h_bprp - a.h_bpr : 0;
+            for (int i = threadIdx.x; i < a.positions; i += 256) a.order[i] = -1;
+            const int align = a.positions ? 8 : 1;
             for (int i = threadIdx.x; i < a.pairs * pad; i += 256) {
                 const int b = a.h_bpr + i % pad;
                 float* at = reinterpret_cast<float*>(a.h + ((size_t)(i / pad) * (a.h_bprp / kChunkBlocks) + b / kChunkBlocks) *
@@ -74,7 +76,7 @@ __global__ void __launch_bounds__(256) prep_kernel(const PrepArgs a) {
             for (int i = 0; i < kPer; ++i) {
                 const int e = threadIdx.x * kPer + i;
                 n[i] = e < a.n_experts ? cnt[e] : 0;
-                np += n[i];
+                np += (n[i] + align - 1) / align * align;
                 ns += (n[i] + a.seg_cap - 1) / a.seg_cap;
             }
             int ip = np, is = ns;
@@ -89,9 +91,12 @@ __global__ void __launch_bounds__(256) prep_kernel(const PrepArgs a) {
             for (int i = 0; i < kPer; ++i) {
                 const int e = threadIdx.x * kPer + i;
                 if (e < a.n_experts) cnt[e] = op;
-                for (int k = 0; k < n[i]; k += a.seg_cap)
-                    a.segs[os++] = Segment{e, op + k, n[i] - k < a.seg_cap ? n[i] - k : a.seg_cap, 0};
-                op += n[i];
+                // many rows: segments of one length, not a full one and a rest
+                const int parts = (n[i] + a.seg_cap - 1) / a.seg_cap;
+                const int each = a.positions && parts ? ((n[i] + parts - 1) / parts + 15) / 16 * 16 : a.seg_cap;
+                for (int k = 0; k < parts; ++k)
+                    a.segs[os++] = Segment{e, op + k * each, min(n[i] - k * each, each), 0};
+                op += (n[i] + align - 1) / align * align;
             }
             if (threadIdx.x == 255) *a.nseg = os;
             __syncthreads();
@@ -129,12 +134,41 @@ __global__ void __launch_bounds__(256) prep_kernel(const PrepArgs a) {
         const int r = (int)(i / a.bprp), b = (int)(i % a.bprp);
         const float* x = a.x + (long long)r * a.in;
         uint8_t* row = a.sliced + (size_t)r * (a.bprp / kChunkBlocks) * kRecordBytes;
-        const int at = b * kQK + (a.few ? imma_element(a.fmt, b & 1, lane) : half_element(a.fmt, b & 1, lane));
-        const float v = at < a.in ? x[at] : 0.0f;
-        if (a.few)
-            slice_digits(v, digit_weight(a.fmt, lane), row, b, lane);
-        else
-            slice_halves(v, row, b, lane);
+        const int at = b * kQK + imma_element(a.fmt, b & 1, lane);
+        slice_digits(at < a.in ? x[at] : 0.0f, digit_weight(a.fmt, lane), row, b, lane);
+    }
+}
+
+struct HalvesArgs {
+    const float* x;
+    const int* order;  // position -> pair; null: positions are rows
+    int positions, top_k, in, groups, fmt;
+    uint8_t* halves;   // [position][groups][hi, lo][64]
+    float* scales;     // [groups][pitch]
+    int pitch;
+    unsigned int* split_done;
+};
+
+// x by position for many rows: a warp per 64 values.
+__global__ void __launch_bounds__(256) halves_kernel(const HalvesArgs a) {
+    launch_dependents();
+    grid_dependency_wait();
+    const int lane = threadIdx.x & 31;
+    if (blockIdx.x == 0)
+        for (int i = threadIdx.x; i < 2 * kMaxTeams; i += 256) a.split_done[i] = 0;
+    const long long n = (long long)a.positions * a.groups, step = (long long)gridDim.x * 8;
+    for (long long i = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); i < n; i += step) {
+        const int pos = (int)(i / a.groups), g = (int)(i % a.groups);
+        const int pair = a.order ? a.order[pos] : pos;
+        if (pair < 0) continue;
+        const float* x = a.x + (long long)(a.order ? pair / a.top_k : pair) * a.in;
+        float v[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const int p = 2 * lane + k, at = 64 * g + (p & 32) + tile_element(a.fmt, p & 31);
+            v[k] = at < a.in ? x[at] : 0.0f;
+        }
+        slice_64(v[0], v[1], a.halves + (size_t)i * 256, a.scales + (size_t)g * a.pitch + pos, lane);
     }
 }
 
@@ -190,19 +224,29 @@ constexpr int kCombineRows = 32;          // more rows: the sum over slots is a 
 // Rows of x of a segment at most in the form of few rows.
 int few_cap(int rows) { return rows < 3 ? rows : kFewRows; }
 
-// And in that of many: with two stages of 256 q8_0 rows that are not aligned,
-// shared memory has room for 16.
-int many_cap(int fmt, const void* w0, const void* w1, int in) {
-    const int bpr = (in + kQK - 1) / kQK;
-    const long long pitch = (long long)bpr * block_bytes(fmt);
-    const bool aligned = reinterpret_cast<uintptr_t>(w0) % 16 == 0 && reinterpret_cast<uintptr_t>(w1) % 16 == 0 && pitch % 16 == 0;
-    return fmt == kQ8_0 && !aligned ? kSegTokens / 2 : kSegTokens;
+// And in that of many: half as many again as an expert has on average, so
+// that most experts are one segment.
+int many_cap(int pairs, int n_experts) {
+    const int n = (pairs / n_experts * 3 / 2 + 8 + 31) / 32 * 32;
+    return n < kSegTokens ? n : kSegTokens;
+}
+
+// Positions of `pairs` pairs when every expert starts at a multiple of 8.
+int many_positions(int pairs, int n_experts) { return (pairs + 7 * (pairs < n_experts ? pairs : n_experts) + 7) / 8 * 8; }
+
+int groups_of(int in) { return (in + 63) / 64; }
+
+// A copy of 16 scales may start at the last position.
+int scale_pitch(int positions) { return (positions + 7) / 8 * 8 + kSegTokens; }
+
+size_t halves_bytes(int positions, int groups) {
+    return align256((size_t)positions * groups * 256) + align256((size_t)groups * scale_pitch(positions) * sizeof(float));
 }
 
 // Floats of a slot for a shared unit's sums: rows of x x rows of the tile.  n:
 // rows of the call (a unit of few rows that meets every segment has them all).
 size_t split_floats(bool few, int n, int strips) {
-    if (!few) return (size_t)kSegTokens * 256;
+    if (!few) return (size_t)kSegTokens * 128;
     return (size_t)(n <= kCombineRows && n > kFewRows ? n : kFewRows) * 16 * strips;
 }
 
@@ -216,8 +260,9 @@ size_t split_bytes(bool few, int n) {
 // Rows of x of one pass.
 int experts_pass_rows(const MoeShape& s, int rows, int top_k) {
     long long n = kMaxPairs / top_k;
+    // many rows: x too is by pair
     const long long per = (long long)top_k * padded_blocks((s.hidden + kQK - 1) / kQK) * (kSlicedBytes + 8);
-    const long long perx = (long long)padded_blocks((s.in + kQK - 1) / kQK) * (kSlicedBytes + 8);
+    const long long perx = (long long)top_k * padded_blocks((s.in + kQK - 1) / kQK) * (kSlicedBytes + 8);
     const long long cap = (long long)kMaxSliced / (per > perx ? per : perx);
     const long long capp = (long long)kMaxParts / ((long long)top_k * s.out * (long long)sizeof(float));
     if (n > cap) n = cap;
@@ -249,11 +294,29 @@ int prep_ctas(long long blocks, int sm_count) {
     return (int)(n < 8LL * sm_count ? n : 8LL * sm_count);
 }
 
+// x of `positions` rows (or positions of `order`, to be set) as halves.
+HalvesArgs halves_args(Carve& c, const float* x, int positions, int in, int fmt) {
+    HalvesArgs h{};
+    h.x = x, h.positions = positions, h.in = in, h.fmt = fmt;
+    h.groups = groups_of(in), h.pitch = scale_pitch(positions);
+    h.halves = c.take<uint8_t>((size_t)positions * h.groups * 256);
+    h.scales = c.take<float>((size_t)h.groups * h.pitch);
+    return h;
+}
+
+void set_halves(ImmaArgs& a, const HalvesArgs& h) {
+    a.x = h.halves, a.xs = h.scales, a.xs_pitch = h.pitch, a.x_rows = h.positions, a.groups = h.groups;
+}
+
 }  // namespace
 
 size_t epilogue_workspace_bytes(int in, int rows) {
     const int n = linear_pass_rows(in, rows);
-    return sliced_bytes(n, padded_blocks((in + kQK - 1) / kQK)) + split_bytes(n <= kFewRows, n);
+    // more rows never need less
+    const size_t few = sliced_bytes(n < kFewRows ? n : kFewRows, padded_blocks((in + kQK - 1) / kQK)) +
+                       split_bytes(true, n < kFewRows ? n : kFewRows);
+    const size_t many = n <= kFewRows ? 0 : halves_bytes(n, groups_of(in)) + split_bytes(false, n);
+    return few > many ? few : many;
 }
 
 cudaError_t launch_linear_epilogue(int fmt, const uint8_t* w, int out, int in, const float* x, int rows,
@@ -267,29 +330,43 @@ cudaError_t launch_linear_epilogue(int fmt, const uint8_t* w, int out, int in, c
         PrepArgs p{};
         p.x = x + (long long)r0 * in;
         p.rows = n, p.in = in, p.bpr = bpr, p.bprp = bprp, p.fmt = fmt;
-        p.few = n <= kFewRows;
-        p.sliced = c.take_sliced(n, bprp);
-        float* split = c.take<float>(split_floats(p.few, n, kImmaWarps) * split_count(p.few));
-        p.split_done = c.take<unsigned int>(2 * kMaxTeams);
-        cudaError_t e = launch_pdl(prep_kernel, prep_ctas((long long)n * bprp, sm_count), 256, 0, stream, p);
+        const bool few = n <= kFewRows;
+        HalvesArgs hv{};
+        float* split;
+        cudaError_t e;
+        if (few) {
+            p.sliced = c.take_sliced(n, bprp);
+            split = c.take<float>(split_floats(few, n, kImmaWarps) * split_count(few));
+            p.split_done = c.take<unsigned int>(2 * kMaxTeams);
+            e = launch_pdl(prep_kernel, prep_ctas((long long)n * bprp, sm_count), 256, 0, stream, p);
+        } else {
+            hv = halves_args(c, p.x, n, in, fmt);
+            split = c.take<float>(split_floats(few, n, kImmaWarps) * split_count(few));
+            p.split_done = hv.split_done = c.take<unsigned int>(2 * kMaxTeams);
+            e = launch_pdl(halves_kernel, prep_ctas((long long)n * hv.groups, sm_count), 256, 0, stream, hv);
+        }
         if (e != cudaSuccess) return e;
         ImmaArgs a{};
         a.w[0] = w;
         a.total_rows = out, a.out = out, a.bpr = bpr, a.bprp = bprp;
-        a.seg_cap = p.few ? few_cap(n) : many_cap(fmt, w, w, in);
+        const int parts = (n + kSegTokens - 1) / kSegTokens;
+        a.seg_cap = few ? few_cap(n) : ((n + parts - 1) / parts + 15) / 16 * 16;
         const int nseg = (n + a.seg_cap - 1) / a.seg_cap;
-        a.strips = p.few ? choose_strips(out, bpr, nseg, false, sm_count, a.seg_cap) : 16;
+        a.strips = few ? choose_strips(out, bpr, nseg, false, sm_count, a.seg_cap) : 8;
         a.tiles = (out + 16 * a.strips - 1) / (16 * a.strips);
-        a.x = p.sliced;
+        if (few)
+            a.x = p.sliced;
+        else
+            set_halves(a, hv);
         a.rows = n;
-        a.split = split, a.split_done = p.split_done, a.split_size = split_floats(p.few, n, a.strips);
+        a.split = split, a.split_done = p.split_done, a.split_size = split_floats(few, n, a.strips);
         a.bias = ep.bias;
         a.row_scale = ep.row_scale ? ep.row_scale + r0 : nullptr;
         a.residual = ep.residual ? ep.residual + (long long)r0 * out : nullptr;
         a.act = ep.activation;
         a.y = y + (long long)r0 * out;
         a.err = err;
-        e = (p.few ? launch_few_plain : launch_many_plain)(fmt, a, sm_count, smem_per_sm, (long long)nseg * a.tiles, stream);
+        e = (few ? launch_few_plain : launch_many_plain)(fmt, a, sm_count, smem_per_sm, (long long)nseg * a.tiles, stream);
         if (e != cudaSuccess) return e;
         r0 += n;
     }
@@ -302,10 +379,14 @@ size_t experts_workspace_bytes(const MoeShape& s, int rows, int top_k) {
     auto bytes = [&](int n) {
         const int pairs = n * top_k;
         const bool few = few_rows(pairs, s.n_experts);
-        const int cap = few ? few_cap(n) : kSegTokens / 2;
-        return 256 + align256((size_t)max_segments(pairs, s.n_experts, cap) * sizeof(Segment)) +
-               align256((size_t)pairs * sizeof(int)) + sliced_bytes(n, bprp) + sliced_bytes(pairs, hp) +
-               (few && n <= kCombineRows ? 0 : align256((size_t)pairs * s.out * sizeof(float))) + split_bytes(few, n);
+        const size_t lists = 256 + align256((size_t)max_segments(pairs, s.n_experts, few ? few_cap(n) : 1) * sizeof(Segment));
+        if (few)
+            return lists + align256((size_t)pairs * sizeof(int)) + sliced_bytes(n, bprp) + sliced_bytes(pairs, hp) +
+                   (n <= kCombineRows ? 0 : align256((size_t)pairs * s.out * sizeof(float))) + split_bytes(few, n);
+        const int positions = many_positions(pairs, s.n_experts);
+        return lists + align256((size_t)positions * sizeof(int)) + halves_bytes(positions, groups_of(s.in)) +
+               halves_bytes(positions, groups_of(s.hidden)) + align256((size_t)pairs * s.out * sizeof(float)) +
+               split_bytes(few, n);
     };
     // the last pass may be smaller, and take another form
     const int last = rows % pass;
@@ -323,47 +404,56 @@ cudaError_t launch_experts(const MoeShape& s, const uint8_t* gate, const uint8_t
     for (int r0 = 0; r0 < rows; r0 += pass) {
         const int n = rows - r0 < pass ? rows - r0 : pass, pairs = n * top_k;
         const bool few = few_rows(pairs, s.n_experts);
-        int cap = few_cap(n);
-        if (!few) {
-            const int c0 = many_cap(s.fmt, gate, up, s.in), c1 = many_cap(s.fmt_down, down, down, s.hidden);
-            cap = c0 < c1 ? c0 : c1;
-        }
+        const int cap = few ? few_cap(n) : many_cap(pairs, s.n_experts);
         const bool at_once = few && n <= kCombineRows;  // the down product meets all segments of a tile in one unit
         const int nseg_max = max_segments(pairs, s.n_experts, cap);
         const int nseg_likely = pairs < s.n_experts ? pairs : nseg_max;
-        const int strips = few ? choose_strips(s.out, hb, nseg_likely, at_once, sm_count, cap) : 16;
+        const int strips = few ? choose_strips(s.out, hb, nseg_likely, at_once, sm_count, cap) : 8;
         const int tiles = (s.out + 16 * strips - 1) / (16 * strips);
         Carve c{static_cast<uint8_t*>(ws)};
         PrepArgs p{};
+        HalvesArgs hx{}, hh{};
         p.nseg = c.take<int>(1);
         p.segs = c.take<Segment>(nseg_max);
-        p.order = c.take<int>(pairs);
+        p.positions = few ? 0 : many_positions(pairs, s.n_experts);
+        p.order = c.take<int>(few ? pairs : p.positions);
         p.x = x + (long long)r0 * s.in;
-        p.rows = n, p.in = s.in, p.bpr = bpr, p.bprp = bprp, p.fmt = s.fmt;
-        p.few = few, p.seg_cap = cap;
-        p.sliced = c.take_sliced(n, bprp);
+        p.in = s.in, p.bpr = bpr, p.bprp = bprp, p.fmt = s.fmt;
+        p.seg_cap = cap;
         p.ids = ids + (long long)r0 * top_k;
         p.pairs = pairs, p.n_experts = s.n_experts;
-        p.h = c.take_sliced(pairs, hp);
-        p.h_bpr = hb, p.h_bprp = hp;
+        if (few) {
+            p.rows = n;
+            p.sliced = c.take_sliced(n, bprp);
+            p.h = c.take_sliced(pairs, hp);
+            p.h_bpr = hb, p.h_bprp = hp;
+        } else {
+            hx = halves_args(c, p.x, p.positions, s.in, s.fmt);
+            hh = halves_args(c, nullptr, p.positions, s.hidden, s.fmt_down);
+            hx.order = p.order, hx.top_k = top_k;
+        }
         float* part = c.take<float>(at_once ? 0 : (size_t)pairs * s.out);
         float* split = c.take<float>(split_floats(few, n, kImmaWarps) * split_count(few));
-        p.split_done = c.take<unsigned int>(2 * kMaxTeams);
-        cudaError_t e = launch_pdl(prep_kernel, 1 + prep_ctas((long long)n * bprp, sm_count), 256, 0, stream, p);
+        p.split_done = hx.split_done = c.take<unsigned int>(2 * kMaxTeams);
+        cudaError_t e = launch_pdl(prep_kernel, few ? 1 + prep_ctas((long long)n * bprp, sm_count) : 1, 256, 0, stream, p);
+        if (e == cudaSuccess && !few)
+            e = launch_pdl(halves_kernel, prep_ctas((long long)pairs * hx.groups, sm_count), 256, 0, stream, hx);
         if (e != cudaSuccess) return e;
 
         ImmaArgs a{};
         a.w[0] = gate, a.w[1] = up;
         a.total_rows = (long long)s.n_experts * s.hidden;
         a.out = s.hidden, a.bpr = bpr, a.bprp = bprp;
-        a.strips = few ? choose_strips(2 * s.hidden, bpr, nseg_likely, false, sm_count, 4) : 16;
+        a.strips = few ? choose_strips(2 * s.hidden, bpr, nseg_likely, false, sm_count, 4) : 8;
         a.tiles = (s.hidden + 8 * a.strips - 1) / (8 * a.strips);
         a.seg_cap = cap;
         a.x = p.sliced;
+        if (!few) set_halves(a, hx);
         a.segs = p.segs, a.nseg = p.nseg, a.order = p.order;
         a.top_k = top_k, a.rows = n;
         a.next_fmt = s.fmt_down, a.next_bprp = hp;
-        a.h = p.h;
+        a.h = few ? p.h : hh.halves;
+        a.hs = hh.scales, a.hs_pitch = hh.pitch, a.next_groups = hh.groups;
         a.split = split, a.split_done = p.split_done, a.split_size = split_floats(few, n, a.strips);
         a.err = err;
         e = (few ? launch_few_pair : launch_many_pair)(s.fmt, a, sm_count, smem_per_sm, (long long)nseg_max * a.tiles, stream);
@@ -376,6 +466,7 @@ cudaError_t launch_experts(const MoeShape& s, const uint8_t* gate, const uint8_t
         d.strips = strips, d.tiles = tiles;
         d.seg_cap = cap;
         d.x = p.h;
+        if (!few) set_halves(d, hh);
         d.segs = p.segs, d.nseg = p.nseg, d.order = p.order;
         d.top_k = top_k, d.rows = n;
         d.part = at_once ? nullptr : part;

@@ -16,14 +16,14 @@
 //   nibbles are carried 16-fold instead, and q4_0's offset of 8 is taken off by
 //   the block's sum of x, in the fold.
 // * more rows: x_i / s = hi + lo in fp16 (error <= 2^-22 |x_i|, s a power of
-//   two per block), codes as fp16, 4 m16n8k16 instructions per block and 8 rows
-//   into one fp32 accumulator.  One column per row instead of 4, and a fold
-//   of 2 instructions per value instead of 4, for ~20 conversions per block that
-//   many columns share.
+//   two per 64 values of a row), and d c too (exact: at most 19 bits; q4_1's
+//   d c + m to 22 bits), with a power of two per 64 values of a weight row.  tcgen05
+//   products hi hi + hi lo + lo hi, 64 values of K at a time into a sum that both
+//   scales then bring into an fp32 one: a product of 22 bits on both sides at 3
+//   fp16 instructions, and the chain of roundings in the tensor core is short.
 //
 // Both are bound by HBM while an expert has few rows.  The int8 instruction
-// runs at one per 2.2 cycles and SM here (1.05 POP/s measured), the fp16 one
-// too (0.52 PFLOP/s).
+// runs at one per 2.2 cycles and SM here (1.05 POP/s measured).
 #pragma once
 
 #include <limits.h>
@@ -33,10 +33,10 @@
 
 namespace mlq {
 
-constexpr int kSlicedBytes = 128;  // one sliced block of x: 4 digits, or hi and lo, of 32 values
+constexpr int kSlicedBytes = 128;  // one sliced block of x: 4 digits of 32 values
 constexpr int kChunkBlocks = 8;    // blocks of one K step of a warp
 constexpr int kImmaWarps = 8;      // warps of a CTA that compute
-constexpr int kSegTokens = 32;     // rows of x of a segment at most
+constexpr int kSegTokens = 128;    // rows of x of a segment at most
 constexpr int kFewRows = 4;        // rows of x that go by digits
 
 __host__ __device__ inline int padded_blocks(int bpr) { return (bpr + kChunkBlocks - 1) / kChunkBlocks * kChunkBlocks; }
@@ -64,15 +64,15 @@ __device__ __forceinline__ int imma_element(int fmt, int odd, int l) {
     return l;
 }
 
-// The same for the fp16 form: l = 8 t + i, i the lane's i-th value in operand order.
-__device__ __forceinline__ int half_element(int fmt, int odd, int l) {
-    const int t = l >> 3, i = l & 7;
-    const int h = fmt == kQ8_0 ? i >> 2 : (i >> 1) & 1, j = fmt == kQ8_0 ? i & 3 : 2 * (i & 1) + (i >> 2);
-    return imma_element(fmt, odd, 16 * h + 4 * t + j);
+// Element of a block at position p of the fp16 operands (many rows): the order
+// in which a block's codes are turned to fp16 pairs (mlq_imma_many.cuh).
+__device__ __forceinline__ int tile_element(int fmt, int p) {
+    if (fmt == kQ8_0) return p;
+    return (p >> 3) * 4 + ((p >> 2) & 1) + 2 * (p & 1) + 8 * (p & 2);
 }
 
 // A sliced row of x is a sequence of records, one per K step: 8 blocks of
-// digits (or halves), their scales, their sums of x.  One bulk copy brings a record to
+// digits, their scales, their sums of x.  One bulk copy brings a record to
 // shared memory.
 constexpr int kRecordBytes = kChunkBlocks * (kSlicedBytes + 8);
 constexpr int kRecordScales = kChunkBlocks * kSlicedBytes, kRecordSums = kRecordScales + kChunkBlocks * 4;
@@ -148,29 +148,18 @@ __device__ __forceinline__ void slice_digits(float x, float weight, uint8_t* row
     }
 }
 
-// Where block b of a row's records has its halves: [hi, lo][t][value].
-__host__ __device__ constexpr int half_block(int b) {
-    return (b / kChunkBlocks) * kRecordBytes + (b % kChunkBlocks) * kSlicedBytes;
-}
-
-// Slices a block into fp16 hi and lo: lane l holds the value at half_element
-// l of block b; row: the row's first record.
-__device__ __forceinline__ void slice_halves(float v, uint8_t* row, int b, int lane) {
-    const float amax = block_amax(v);
-    const bool bad = !(amax == amax);
-    const uint32_t s = block_scale(bad ? 0.0f : amax, 14, 32767.0f);
-    const float q = bad ? 0.0f : v * __uint_as_float(s);
-    const __half hi = __float2half_rn(q);
-    const __half lo = __float2half_rn(q - __half2float(hi));
-    __half* o = reinterpret_cast<__half*>(row + half_block(b));
-    o[lane] = hi;
-    o[32 + lane] = lo;
-    const float total = warp_sum(v);
-    if (lane == 0) {
-        float* at = reinterpret_cast<float*>(row + (b / kChunkBlocks) * kRecordBytes + kRecordScales) + b % kChunkBlocks;
-        at[0] = bad ? __uint_as_float(0x7fc00000u) : inverse_scale(s);
-        at[kChunkBlocks] = total;
-    }
+// Slices 64 values (positions 2 lane and 2 lane + 1) into fp16 hi and lo with
+// one power-of-two scale; to: 64 hi, then 64 lo.
+__device__ __forceinline__ void slice_64(float v0, float v1, uint8_t* to, float* scale, int lane) {
+    const float m0 = block_amax(v0), m1 = block_amax(v1);
+    const bool bad = !(m0 == m0) || !(m1 == m1);
+    const uint32_t s = block_scale(bad ? 0.0f : fmaxf(m0, m1), 14, 32767.0f);
+    const float q0 = bad ? 0.0f : v0 * __uint_as_float(s), q1 = bad ? 0.0f : v1 * __uint_as_float(s);
+    const __half2 hi = __floats2half2_rn(q0, q1);
+    const float2 h = __half22float2(hi);
+    reinterpret_cast<__half2*>(to)[lane] = hi;
+    reinterpret_cast<__half2*>(to + 128)[lane] = __floats2half2_rn(q0 - h.x, q1 - h.y);
+    if (lane == 0) *scale = bad ? __uint_as_float(0x7fc00000u) : inverse_scale(s);
 }
 
 // D = A B for 16 rows x 32 codes, signed (q8_0) or unsigned (q4), and digits.
@@ -186,13 +175,6 @@ __device__ __forceinline__ void imma(int (&c)[4], const uint32_t (&a)[4], uint2 
             "mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
             : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
             : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y), "r"(0));
-}
-
-__device__ __forceinline__ void hmma_f16(float (&c)[4], const uint32_t* a, uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
 // Facts of a warp's weight slot (16 rows x 8 blocks in shared memory).
@@ -336,43 +318,6 @@ __device__ __forceinline__ void int8_operand(const RawA& r, uint32_t (&a)[4]) {
     for (int i = 0; i < 2; ++i) {
         a[i] = F == kQ8_0 ? r.w[i][0] : r.w[i][0] & 0x0f0f0f0fu;
         a[2 + i] = F == kQ8_0 ? r.w[i][1] : r.w[i][0] & 0xf0f0f0f0u;
-    }
-}
-
-__device__ __forceinline__ uint32_t hsub2_bits(uint32_t a, uint32_t b) {
-    const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
-    return *reinterpret_cast<const uint32_t*>(&r);
-}
-
-__device__ __forceinline__ uint32_t hfma2_bits(uint32_t a, uint32_t b, uint32_t c) {
-    const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b),
-                              *reinterpret_cast<const __half2*>(&c));
-    return *reinterpret_cast<const uint32_t*>(&r);
-}
-
-// The A operands of the two fp16 instructions: the code is put under the
-// exponent of 1024 (1024 + c is exact in fp16) and the offset subtracted.
-template <int F>
-__device__ __forceinline__ void half_operand(const RawA& r, uint32_t (&a)[8]) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        if (F == kQ8_0) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const uint32_t u = r.w[i][h] ^ 0x80808080u;  // c + 128
-                a[4 * h + i] = hsub2_bits(__byte_perm(u, 0x64646464u, 0x4140), 0x64806480u);  // - 1152
-                a[4 * h + 2 + i] = hsub2_bits(__byte_perm(u, 0x64646464u, 0x4342), 0x64806480u);
-            }
-        } else {
-            const uint32_t v = r.w[i][0], v8 = v >> 8;
-            // low nibbles: 1024 + c - 1032 (q4_1, whose codes have no offset: - 1024); high ones: (1024 + 16 c) / 16 - 72
-            // (- 64)
-            constexpr uint32_t lo = F == kQ4_0 ? 0x64086408u : 0x64006400u, hi = F == kQ4_0 ? 0xd480d480u : 0xd400d400u;
-            a[i] = hsub2_bits((v & 0x000f000fu) | 0x64006400u, lo);
-            a[2 + i] = hfma2_bits((v & 0x00f000f0u) | 0x64006400u, 0x2c002c00u, hi);
-            a[4 + i] = hsub2_bits((v8 & 0x000f000fu) | 0x64006400u, lo);
-            a[6 + i] = hfma2_bits((v8 & 0x00f000f0u) | 0x64006400u, 0x2c002c00u, hi);
-        }
     }
 }
 

@@ -8,7 +8,7 @@ namespace mlq {
 enum Mode { kPlain = 0, kPair = 1, kDown = 2 };
 
 struct ImmaMaps {
-    CUtensorMap m[2];
+    CUtensorMap m[3];  // weights; [1]: the up projections (kPair); [2]: x (many rows)
 };
 
 struct ImmaArgs {
@@ -19,9 +19,15 @@ struct ImmaArgs {
     int bpr, bprp;            // blocks per row, and padded to whole steps
     int strips;               // 16-row strips of a unit (1, 2, 4 or 8); kPair: 8 gate and 8 up rows each, 4 or 8
     int tiles;                // row tiles of one matrix
-    int slots;                // ring depth of a warp
+    int slots;                // ring depth of a warp (many rows: of the CTA)
+    int x_slots;              // many rows: ring depth of x
     int seg_cap;              // rows of x of a segment at most
-    const uint8_t* x;         // records of the rows of x or h
+    const uint8_t* x;         // records of the rows of x or h; many rows: [x_rows][groups][hi, lo][64] fp16, by position
+    // many rows
+    const float* xs;          // [groups][xs_pitch] scales of x
+    int xs_pitch, x_rows, groups;
+    float* hs;                // kPair: [next_groups][hs_pitch] scales of h
+    int hs_pitch, next_groups;
     // segments (kPair, kDown); kPlain: rows in order, one matrix
     const Segment* segs;
     const int* nseg;

@@ -1,138 +1,224 @@
 // mlq_imma_many.cuh -- the streaming kernel for many rows of x per matrix
-// (halves, fp16 matrix instructions; mathematics and operand layout:
-// mlq_imma.cuh; the launches around it: mlq_imma.cu).
+// (tcgen05 with fp16 operands; mathematics: mlq_imma.cuh; the launches around
+// it: mlq_imma.cu).
 //
-// One CTA per SM: 16 computing and 4 producer warps.  A unit is a tile of 256
-// rows of one matrix (kPair: 128 gate and 128 up rows) against one segment of
-// up to 32 rows of x; a round is 8 blocks of K.  A stage holds a round's weights
-// (16 strips of 16 rows) and records of x, both fetched asynchronously, so that
-// x is read from L2 once per 256 weight rows.  A computing warp takes 2 strips
-// x 16 rows of x (one strip where the segment has at most 16): per block ~20
-// instructions turn codes to fp16 per strip and 4 matrix instructions per
-// strip and 8 rows of x use them, so the matrix unit is what bounds a full
-// segment (4 x 2.2 cycles per 16 x 8 x 32 products: 255 TFLOP/s on 148 SMs).
+// One CTA per SM.  A unit is a tile of 128 rows of one matrix (kPair: 64 gate
+// and 64 up rows) against one segment of up to 128 rows of x; a stage is 64
+// values of K (2 blocks), a round 4 stages.  Weights arrive as packed blocks
+// (TMA, or 16-byte pieces where rows are not aligned) and go through the registers
+// into tensor memory as the A operand: shared memory holds each only once, packed.
+// x (hi and lo, fp16) comes by TMA as the B operand.  12 products of 16 values
+// per stage (lo hi and hi lo first, then hi hi: the sum has its full size in 4
+// only), and a stage's sums are drained into fp32 registers with the power-of-two scales
+// of its weight row and its row of x.
+//
+//   warps 0-7    decode: warp w row 32 (w mod 4) + lane, block w / 4 of a stage
+//   warps 8-15   drain: the same rows, half of the segment's columns; the end of a unit
+//   warp 16, 19  weights; 17: x; 18: products
+//
+// Tensor memory: 2 sums of 128 columns, 4 operands of 64 (hi 32, lo 32).
 // Rounds are dealt out evenly as in mlq_imma_few.cuh.
 #pragma once
 
+#include <cuda_fp16.h>
+
 #include "mlq_imma_common.cuh"
+#include "mlq_tc.cuh"
 
 namespace mlq {
 namespace {
 
-constexpr int kStrips = 16;                       // 16-row strips of a unit
-constexpr int kUnitRows = 16 * kStrips;
-constexpr int kComputeWarps = 16, kProducers = 4;
-constexpr int kManyThreads = 32 * (kComputeWarps + kProducers);
-constexpr int kComputeThreads = 32 * kComputeWarps;
-constexpr int kSumFloats = 32 * (128 + 4);        // sums of one pass: [row of x][128 or 256 rows + 4]
-constexpr int kManyJoin = 2;                      // rounds; one takes ~2.4 us at a full segment
-// registers: as in mlq_imma_few.cuh
-constexpr int kManyLaunchRegs = 96, kManyProducerRegs = 32, kManyComputeRegs = 112;
-static_assert((kProducers * kManyProducerRegs + kComputeWarps * kManyComputeRegs) * 32 <= kManyThreads * kManyLaunchRegs,
+constexpr int kUnitRows = 128;
+constexpr int kRoleWarps = 8;                    // that decode, and that drain
+constexpr int kManyThreads = 32 * (2 * kRoleWarps + 4);
+constexpr int kDrainThreads = 32 * kRoleWarps;
+constexpr int kOperands = 4, kScaleRing = 8;
+constexpr int kMaxBStages = 6;                   // scales of x outlive the operand by two products: 8 - 2
+constexpr int kXchPitch = kUnitRows + 4;         // kPair: [32 rows of x][128 rows + 4]
+constexpr int kManyJoin = 2;                     // rounds
+// registers at launch, and after the split
+constexpr int kManyLaunchRegs = 96, kDecodeRegs = 88, kDrainRegs = 136, kOtherRegs = 32;
+static_assert((kRoleWarps * (kDecodeRegs + kDrainRegs) + 4 * kOtherRegs) * 32 <= kManyThreads * kManyLaunchRegs,
               "the shares must not exceed the launch's registers, or setmaxnreg would wait for ever");
 
-// J strips against 8 S rows of x.
-template <int F, int J, int S>
-struct ManyRows {
-    float acc[J][S][2][2];  // [.][.][row g / g + 8][row of x 2t, 2t + 1]
-
-    __device__ __forceinline__ void init() {
-#pragma unroll
-        for (int j = 0; j < J; ++j)
-#pragma unroll
-            for (int i = 0; i < S; ++i) acc[j][i][0][0] = acc[j][i][0][1] = acc[j][i][1][0] = acc[j][i][1][1] = 0.0f;
-    }
-
-    // One round; x: the lane's halves, s: the scales of its rows 2t (see run).
-    template <bool ALN>
-    __device__ __forceinline__ void step(uint32_t x, uint32_t s, int valid, const RowBase (&rows)[J]) {
-        static_for<kChunkBlocks / 2>([&](auto pc) {
-            constexpr int p = decltype(pc)::value;
-            if (2 * p >= valid) return;
-            RawA A[J][2];
-#pragma unroll
-            for (int j = 0; j < J; ++j) load_pair<F, ALN, p>(rows[j], A[j][0], A[j][1]);
-            static_for<2>([&](auto oc) {
-                constexpr int o = decltype(oc)::value, k = 2 * p + o;
-                if (k >= valid) return;
-                uint32_t op[J][8];
-#pragma unroll
-                for (int j = 0; j < J; ++j) half_operand<F>(A[j][o], op[j]);
-#pragma unroll
-                for (int i = 0; i < S; ++i) {
-                    const uint32_t xi = x + i * 8 * kRecordBytes, si = s + i * 8 * kRecordBytes;
-                    const uint4 hi = lds_u4_at<k * kSlicedBytes>(xi), lo = lds_u4_at<k * kSlicedBytes + 64>(xi);
-                    const float sx[2] = {lds_f1_at<4 * k>(si), lds_f1_at<4 * k + kRecordBytes>(si)};
-                    float mx[2] = {0.0f, 0.0f};
-                    if (F == kQ4_1)
-                        mx[0] = lds_f1_at<4 * k + 4 * kChunkBlocks>(si),
-                        mx[1] = lds_f1_at<4 * k + 4 * kChunkBlocks + kRecordBytes>(si);
-                    float c[J][4];
-#pragma unroll
-                    for (int j = 0; j < J; ++j) {
-                        c[j][0] = c[j][1] = c[j][2] = c[j][3] = 0.0f;
-                        hmma_f16(c[j], op[j], lo.x, lo.y);
-                    }
-#pragma unroll
-                    for (int j = 0; j < J; ++j) hmma_f16(c[j], op[j] + 4, lo.z, lo.w);
-#pragma unroll
-                    for (int j = 0; j < J; ++j) hmma_f16(c[j], op[j], hi.x, hi.y);
-#pragma unroll
-                    for (int j = 0; j < J; ++j) hmma_f16(c[j], op[j] + 4, hi.z, hi.w);
-#pragma unroll
-                    for (int j = 0; j < J; ++j)
-#pragma unroll
-                        for (int q = 0; q < 2; ++q)
-#pragma unroll
-                            for (int r = 0; r < 2; ++r) {
-                                acc[j][i][q][r] = fmaf(A[j][o].d[q] * sx[r], c[j][2 * q + r], acc[j][i][q][r]);
-                                if (F == kQ4_1) acc[j][i][q][r] = fmaf(A[j][o].m[q], mx[r], acc[j][i][q][r]);
-                            }
-                }
-            });
-        });
-    }
-
-    // to: [row of x][pitch], this warp's first row of x and of the tile
-    __device__ __forceinline__ void store(float* to, int pitch, int lane) const {
-        const int g = lane >> 2, t = lane & 3;
-#pragma unroll
-        for (int j = 0; j < J; ++j)
-#pragma unroll
-            for (int i = 0; i < S; ++i)
-#pragma unroll
-                for (int q = 0; q < 2; ++q)
-#pragma unroll
-                    for (int r = 0; r < 2; ++r) to[(8 * i + 2 * t + r) * pitch + 16 * j + 8 * q + g] = acc[j][i][q][r];
-    }
+// Packed blocks of 128 rows, one round.  Aligned: as TMA boxes (q4_1: two of 4
+// blocks, so that 8 rows' 16-byte pieces lie in different banks); else the 16-byte
+// windows that hold a row's blocks.
+template <int F, bool ALN>
+struct RawSlot {
+    static constexpr int kChunk = 8 * (F == kQ8_0 ? 34 : F == kQ4_0 ? 18 : 20);
+    static constexpr int kBoxes = ALN && F == kQ4_1 ? 2 : 1;
+    static constexpr int kPitch = ALN ? kChunk / kBoxes : (kChunk + 15 + 15) / 16 * 16;
+    static constexpr int kBytes = kUnitRows * kPitch * kBoxes;
 };
 
-__device__ __forceinline__ void compute_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kComputeThreads) : "memory"); }
+__device__ __forceinline__ void drain_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kDrainThreads) : "memory"); }
+
+// Whether `p` holds for any draining thread.
+__device__ __forceinline__ bool drain_any(bool p) {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                 : "=r"(r)
+                 : "r"((uint32_t)p), "n"(kDrainThreads)
+                 : "memory");
+    return r;
+}
+
+__device__ __forceinline__ uint32_t h2(__half2 v) { return *reinterpret_cast<uint32_t*>(&v); }
+__device__ __forceinline__ __half2 as_h2(uint32_t v) { return *reinterpret_cast<__half2*>(&v); }
+
+// A block's codes: W words of them, and its d (q4_1: d, m) as they are stored.
+template <int F>
+struct Block {
+    static constexpr int W = F == kQ8_0 ? 8 : 4;
+    uint32_t qs[W], dm;
+};
+
+// Block h of pair j of a round; at: the lane's row in the slot (unaligned: its first byte).
+template <int F, bool ALN, int J>
+__device__ __forceinline__ void load_block(uint32_t at, int h, Block<F>& b, uint32_t& other) {
+    constexpr int W = Block<F>::W, BB = F == kQ8_0 ? 34 : F == kQ4_0 ? 18 : 20;
+    if constexpr (ALN) {
+        // the 16-byte windows that hold it
+        constexpr int N = W / 4 + 1;
+        const uint32_t pair = at + (F == kQ4_1 ? (J >> 1) * kUnitRows * 80 + (J & 1) * 32 : J * 16 * W / 2);
+        uint32_t w[4 * N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const uint4 q = lds_u4(pair + h * 4 * W + 16 * i);
+            w[4 * i] = q.x, w[4 * i + 1] = q.y, w[4 * i + 2] = q.z, w[4 * i + 3] = q.w;
+        }
+        if constexpr (F == kQ4_1) {
+            constexpr int s = 2 * (J & 1);
+            b.dm = h ? w[s + 1] : w[s];
+#pragma unroll
+            for (int k = 0; k < W; ++k) b.qs[k] = h ? w[s + 2 + k] : w[s + 1 + k];
+            other = lds_u32(pair + 8 * (J & 1) + 20 * (1 - h));
+        } else {
+            // starts at word J of the windows, for h = 1 two bytes later
+            b.dm = (w[J] >> (16 * h)) & 0xffffu;
+#pragma unroll
+            for (int k = 0; k < W; ++k) b.qs[k] = __funnelshift_rc(w[J + k], w[J + k + 1], 16 + 16 * h);
+            other = lds_u16(pair + 4 * J + BB * (1 - h));
+        }
+    } else {
+        auto word = [](uint32_t at, uint32_t lo, uint32_t hi) { return __funnelshift_r(lo, hi, 8 * (at & 3)); };
+        const uint32_t from = at + (2 * J + h) * BB, to = at + (2 * J + 1 - h) * BB;
+        b.dm = word(from, lds_u32(from & ~3u), lds_u32((from & ~3u) + 4));
+        other = word(to, lds_u32(to & ~3u), lds_u32((to & ~3u) + 4));
+        const uint32_t qs = from + (F == kQ4_1 ? 4 : 2);
+        uint32_t last = lds_u32(qs & ~3u);
+#pragma unroll
+        for (int k = 0; k < W; ++k) {
+            const uint32_t next = lds_u32((qs & ~3u) + 4 * k + 4);
+            b.qs[k] = word(qs, last, next);
+            last = next;
+        }
+    }
+}
+
+// The power of two that brings the larger of two blocks' weights to 2^13 .. 2^14
+// (q4_1: 2^15), as float bits; *inverse undoes it.
+template <int F>
+__device__ __forceinline__ float weight_scale(uint32_t dm0, uint32_t dm1, float* inverse) {
+    uint32_t most = max(dm0 & 0x7fffu, dm1 & 0x7fffu);
+    float v = __half2float(__ushort_as_half((unsigned short)most));
+    int top = 260;  // 127 * 2^6 below 2^13, codes up to 128
+    if (F == kQ4_1) {
+        most = max((dm0 >> 16) & 0x7fffu, (dm1 >> 16) & 0x7fffu);
+        v = fmaxf(16.0f * v, __half2float(__ushort_as_half((unsigned short)most)));
+        if (most > 0x7c00u) v = NAN;
+        top = 267;
+    }
+    int f = top - (int)(__float_as_uint(v) >> 23);
+    if (f > 253) f = 253;
+    *inverse = __uint_as_float((uint32_t)(254 - f) << 23);
+    return __uint_as_float((uint32_t)f << 23);
+}
+
+// A block's weights times `scale`, as fp16 pairs hi and lo.  d * c has at most
+// 19 bits, so hi + lo is exact (q4_1: d * c + m is rounded once in fp32, and
+// hi + lo keeps 22 bits of it).
+template <int F>
+__device__ __forceinline__ void to_halves(const Block<F>& b, float scale, uint32_t (&hi)[16], uint32_t (&lo)[16]) {
+    const float d = __half2float(__ushort_as_half((unsigned short)(b.dm & 0xffffu))) * scale;
+    const float m = F == kQ4_1 ? __half2float(__ushort_as_half((unsigned short)(b.dm >> 16))) * scale : 0.0f;
+    const __half2 d2 = __float2half2_rn(d);
+    auto put = [&](int i, __half2 c) {
+        if constexpr (F == kQ4_1) {
+            const float2 q = __half22float2(c);
+            const float w0 = fmaf(q.x, d, m), w1 = fmaf(q.y, d, m);
+            const __half2 h = __floats2half2_rn(w0, w1);
+            const float2 r = __half22float2(h);
+            hi[i] = h2(h), lo[i] = h2(__floats2half2_rn(w0 - r.x, w1 - r.y));
+        } else {
+            const __half2 h = __hmul2(c, d2);
+            hi[i] = h2(h), lo[i] = h2(__hfma2(c, d2, __hneg2(h)));
+        }
+    };
+    if constexpr (F == kQ8_0) {
+        // signed bytes u - 128 as the low bits of 1024 + u
+        const __half2 off = __float2half2_rn(-1152.0f);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const uint32_t u = b.qs[k] ^ 0x80808080u;
+            put(2 * k, __hadd2(as_h2(__byte_perm(u, 0x64646464u, 0x4140)), off));
+            put(2 * k + 1, __hadd2(as_h2(__byte_perm(u, 0x64646464u, 0x4342)), off));
+        }
+    } else {
+        // 1024 + c from low nibbles; 1024 + 16 c from high ones, times 1 / 16
+        constexpr float zero = F == kQ4_0 ? 8.0f : 0.0f;
+        const __half2 low = __float2half2_rn(-1024.0f - zero), high = __float2half2_rn(-64.0f - zero),
+                      sixteenth = __float2half2_rn(0.0625f);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                const uint32_t q = b.qs[k] >> (8 * s);
+                put(4 * k + 2 * s, __hadd2(as_h2((q & 0x000f000fu) | 0x64006400u), low));
+                put(4 * k + 2 * s + 1, __hfma2(as_h2((q & 0x00f000f0u) | 0x64006400u), sixteenth, high));
+            }
+    }
+}
 
 template <int F, int MODE, bool ALN>
 __global__ void __launch_bounds__(kManyThreads, 1)
     imma_many_kernel(const __grid_constant__ ImmaMaps maps, const __grid_constant__ ImmaArgs a) {
-    extern __shared__ __align__(128) uint8_t smem[];
-    using S = Slot<F, ALN>;
-    __shared__ int s_last, s_dead, s_issued[kProducers];
+    extern __shared__ __align__(1024) uint8_t smem[];
+    using S = RawSlot<F, ALN>;
+    __shared__ int s_last, s_dead, s_raw_issued, s_b_issued;
+    __shared__ uint32_t s_tmem;
+    __shared__ __align__(16) float s_w[kScaleRing][kUnitRows], s_x[kScaleRing][128];
     const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
     const int steps = (a.bpr + kChunkBlocks - 1) / kChunkBlocks;
-    // shared memory: stages (weights, records of x), sums, the stages' barriers (full, empty)
-    const uint32_t stage_bytes = kStrips * S::kBytes + a.seg_cap * kRecordBytes;
-    float* sums = reinterpret_cast<float*>(smem + a.slots * stage_bytes);
-    const uint32_t ring = smem_u32(smem), bars = smem_u32(sums + kSumFloats);
+    const int xrows = (a.seg_cap + 31) / 32 * 32;  // of a stage of x
+    // shared memory: x, weights, (kPair) exchange, barriers
+    const uint32_t b_bytes = 256u * xrows;
+    const uint32_t b_ring = (smem_u32(smem) + 1023u) & ~1023u, raw_ring = b_ring + a.x_slots * b_bytes;
+    const uint32_t xch = raw_ring + a.slots * S::kBytes;
+    const uint32_t bars = xch + (MODE == kPair ? 32 * kXchPitch * 4 : 0);
+    const uint32_t raw_full = bars, raw_empty = raw_full + 64, b_full = raw_empty + 64, b_empty = b_full + 64,
+                   a_full = b_empty + 64, a_empty = a_full + 32, d_full = a_empty + 32, d_free = d_full + 16;
     if (threadIdx.x == 0) {
         s_dead = 0;
-        for (int i = 0; i < a.slots; ++i) {
-            mbar_init(bars + 16 * i, ALN ? kProducers : 64 + 2);
-            mbar_init(bars + 16 * i + 8, kComputeWarps);
+        for (int i = 0; i < 8; ++i) {
+            mbar_init(raw_full + 8 * i, ALN ? 1 : 64);
+            mbar_init(raw_empty + 8 * i, kRoleWarps);
+            mbar_init(b_full + 8 * i, 1);
+            mbar_init(b_empty + 8 * i, 1);
         }
+        for (int i = 0; i < kOperands; ++i) mbar_init(a_full + 8 * i, kRoleWarps), mbar_init(a_empty + 8 * i, 1);
+        for (int i = 0; i < 2; ++i) mbar_init(d_full + 8 * i, 1), mbar_init(d_free + 8 * i, kRoleWarps);
         fence_mbar_init();
     }
+    if (warp == 18) tmem_alloc(smem_u32(&s_tmem), 512);
+    tc_fence_before();
     // Segments: as in mlq_imma_few.cuh.
     if (MODE == kPair) grid_dependency_wait();
     if (MODE != kDown) launch_dependents();
     __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = s_tmem;
     const int nseg = MODE == kPlain ? (a.rows + a.seg_cap - 1) / a.seg_cap : __ldcg(a.nseg);
     const int id = blockIdx.x;
     const Deal deal(nseg * a.tiles, steps, gridDim.x, kManyJoin);
@@ -143,274 +229,380 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         first = MODE == kPlain ? seg * a.seg_cap : __ldcg(&a.segs[seg].start);
         count = MODE == kPlain ? min(a.rows - first, a.seg_cap) : __ldcg(&a.segs[seg].count);
     };
+    auto stages = [&](int c) { return min(4, (a.bpr - c * kChunkBlocks + 1) / 2); };
+    auto wait = [&](uint32_t bar, uint32_t parity, int code) {
+        if (mbar_wait(bar, parity)) return !*(volatile int*)&s_dead;
+        report_error(a.err, code);
+        *(volatile int*)&s_dead = 1;
+        return false;
+    };
+    bool alive = true;
 
-    if (warp >= kComputeWarps) {
-        // ---- producers: 0 and 1 fetch the weights of 8 strips each, 2 and 3 the records of 16 rows of x each ----
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kManyProducerRegs));
-        const int me = warp - kComputeWarps;
-        if (MODE != kPair && me >= 2) grid_dependency_wait();
-        int stage = 0, phase = 1, n = 0;
-        bool alive = true;
+    if (warp < kRoleWarps) {
+        // ---- decode ----
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kDecodeRegs));
+        const int row = 32 * (warp & 3) + lane, h = warp >> 2;
+        int slot = 0;
+        uint32_t slot_phase = 0, n = 0;  // n: stages so far
         while (alive && work.next(deal, id)) {
             int e, first, count;
             segment(work.u % nseg, e, first, count);
-            const int row0 = e * a.out + work.u / nseg * tile_rows;
-            const int token = 16 * (me - 2) + (lane & 15);
-            const int mine = me < 2 ? 8 : min(max(count - 16 * (me - 2), 0), 16);  // strips, rows of x
-            const uint8_t* x = nullptr;
-            if (me >= 2 && (lane & 15) < mine && lane < 16) {
-                const int row = MODE == kPair ? __ldcg(a.order + first + token) / a.top_k : first + token;
-                x = a.x + (size_t)row * (a.bprp / kChunkBlocks) * kRecordBytes;
+            [[maybe_unused]] uint32_t window = 0;
+            if constexpr (!ALN) {
+                // where the row starts in its 16-byte window
+                const bool up = MODE == kPair && row >= 64;
+                const long long at = (long long)e * a.out + work.u / nseg * tile_rows + (MODE == kPair ? row & 63 : row);
+                window = (uint32_t)(reinterpret_cast<uintptr_t>(a.w[up ? 1 : 0]) + at * a.row_bytes) & 15;
             }
-            for (int c = work.r0; c < work.r1; ++c, ++n) {
-                const uint32_t full = bars + 16 * stage, dst = ring + stage * stage_bytes;
-                if (!__all_sync(0xffffffffu, mbar_wait(full + 8, phase))) {
-                    if (lane == 0) report_error(a.err, 33), *(volatile int*)&s_dead = 1;
+            for (int c = work.r0; alive && c < work.r1; ++c) {
+                if (!__all_sync(0xffffffffu, wait(raw_full + 8 * slot, slot_phase, 32))) {
                     alive = false;
                     break;
                 }
-                if (__any_sync(0xffffffffu, *(volatile int*)&s_dead)) {
-                    alive = false;
-                    break;
-                }
-                if (me >= 2) {
-                    if (lane == 0) mbar_arrive_expect_tx(full, mine * kRecordBytes);
+                uint32_t at = raw_ring + slot * S::kBytes + row * S::kPitch;
+                if constexpr (!ALN) at += (window + (uint32_t)c * (S::kChunk & 15)) & 15;
+                const int valid = a.bpr - c * kChunkBlocks;
+                static_for<4>([&](auto jc) {
+                    constexpr int J = decltype(jc)::value;
+                    if (2 * J >= valid || !alive) return;
+                    Block<F> b;
+                    uint32_t other;
+                    load_block<F, ALN, J>(at, h, b, other);
+                    if (2 * J + 1 >= valid) {  // the row ends with the first block of this pair
+                        if (h == 0)
+                            other = 0;
+                        else
+                            b.dm = 0;
+                    }
+                    float inverse;
+                    const float scale = weight_scale<F>(b.dm, other, &inverse);
+                    uint32_t hi[16], lo[16];
+                    to_halves<F>(b, scale, hi, lo);
+                    const int k = n % kOperands;
+                    if (!__all_sync(0xffffffffu, wait(a_empty + 8 * k, (n / kOperands & 1) ^ 1, 33))) {
+                        alive = false;
+                        return;
+                    }
+                    tc_fence_after();
+                    const uint32_t to = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + 256 + 64 * k + 16 * h;
+                    tmem_st16(to, hi);
+                    tmem_st16(to + 32, lo);
+                    if (h == 0) s_w[n % kScaleRing][row] = inverse;
+                    tmem_wait_st();
+                    tc_fence_before();
                     __syncwarp();
-                    if (x) bulk_g2s(dst + kStrips * S::kBytes + token * kRecordBytes, x + (size_t)c * kRecordBytes, kRecordBytes, full);
-                } else if constexpr (ALN) {
-                    if (lane == 0) mbar_arrive_expect_tx(full, 8 * S::kBytes);
-                    __syncwarp();
-                    if (lane < 8) {
-                        const int strip = 8 * me + lane, row = row0 + strip * (MODE == kPair ? 8 : 16);
+                    if (lane == 0) mbar_arrive(a_full + 8 * k);
+                    ++n;
+                });
+                __syncwarp();
+                if (lane == 0) mbar_arrive(raw_empty + 8 * slot);
+                if (++slot == a.slots) slot = 0, slot_phase ^= 1;
+            }
+        }
+    } else if (warp < 2 * kRoleWarps) {
+        // ---- drain ----
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kDrainRegs));
+        if (MODE != kPair) grid_dependency_wait();
+        if (MODE == kDown) launch_dependents();
+        const int dw = warp - kRoleWarps, row = 32 * (dw & 3) + lane, half = dw >> 2;
+        uint32_t n = 0;
+        while (alive && work.next(deal, id)) {
+            const int tile = work.u / nseg;
+            int e, first, count;
+            segment(work.u % nseg, e, first, count);
+            const int cols = (count + 15) / 16 * 8;  // of this half
+            float acc[64];
 #pragma unroll
-                        for (int b = 0; b < S::kBoxes; ++b) {
-                            const int c0 = (c * chunk_bytes(F) + b * S::kPitch) / 2;
-                            const uint32_t d = dst + strip * S::kBytes + b * 16 * S::kPitch;
-                            tma_load_2d(d, &maps.m[0], c0, row, full);
-                            if (MODE == kPair) tma_load_2d(d + 8 * S::kPitch, &maps.m[1], c0, row, full);
+            for (int i = 0; i < 64; ++i) acc[i] = 0.0f;
+            int todo = 0;
+            for (int c = work.r0; c < work.r1; ++c) todo += stages(c);
+            for (; todo > 0; --todo, ++n) {
+                const int s = n & 1;
+                if (!__all_sync(0xffffffffu, wait(d_full + 8 * s, n / 2 & 1, 37))) {
+                    alive = false;
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t from = tmem + ((uint32_t)(32 * (dw & 3)) << 16) + 128 * s + half * cols;
+                const float sw = s_w[n % kScaleRing][row];
+                const float* sx = &s_x[n % kScaleRing][half * cols];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    if (16 * q >= cols) break;
+                    uint32_t v[16];
+                    tmem_ld16_issue(from + 16 * q, v);
+                    float f[16];
+#pragma unroll
+                    for (int i = 0; i < 16; i += 4) {
+                        const float4 x = *reinterpret_cast<const float4*>(sx + 16 * q + i);
+                        f[i] = x.x * sw, f[i + 1] = x.y * sw, f[i + 2] = x.z * sw, f[i + 3] = x.w * sw;
+                    }
+                    tmem_wait_ld(v);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) acc[16 * q + i] = fmaf(__uint_as_float(v[i]), f[i], acc[16 * q + i]);
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(d_free + 8 * s);
+            }
+            // together, or some would wait below for others that have gone
+            if (drain_any(!alive)) break;
+            // a unit that several CTAs share: each leaves its sums in a slot (head: the unit started before its range,
+            // tail: in it), and whoever comes last adds them up in order
+            if (work.r1 - work.r0 != deal.per) {
+                auto slot_of = [&](int c, bool tail) {
+                    return a.split + ((size_t)2 * c + (tail ? 1 : 0)) * a.split_size + (size_t)(half * cols) * kUnitRows + row;
+                };
+                const long long r = (long long)(work.u - deal.each * deal.teams) * deal.per;
+                const int j0 = deal.owner(r), j1 = deal.owner(r + deal.per - 1);
+                float* mine = slot_of(id, id == j0);
+#pragma unroll
+                for (int i = 0; i < 64; ++i)
+                    if (i < cols) mine[i * kUnitRows] = acc[i];
+                __threadfence();
+                drain_sync();
+                if (dw == 0 && lane == 0) {
+                    s_last = atomicAdd(a.split_done + j0, 1u) == (unsigned)(j1 - j0);
+                    __threadfence();
+                }
+                drain_sync();
+                if (!s_last) continue;
+#pragma unroll
+                for (int i = 0; i < 64; ++i)
+                    if (i < cols) acc[i] = __ldcg(slot_of(j0, true) + i * kUnitRows);
+                for (int c = j0 + 1; c <= j1; ++c) {
+                    const float* from = slot_of(c, false);
+#pragma unroll
+                    for (int i = 0; i < 64; ++i)
+                        if (i < cols) acc[i] += __ldcg(from + i * kUnitRows);
+                }
+            }
+            const int tok0 = half * cols;
+            if constexpr (MODE == kPair) {
+                // 32 rows of x at a time through shared memory (16 of each half): a warp takes the 64 hidden values of a
+                // row, in the order of the next product, to hi and lo
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    if (16 * q >= cols) break;
+                    drain_sync();  // the last ones have been read
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) sts_f32(xch + ((half * 16 + i) * kXchPitch + row) * 4, acc[16 * q + i]);
+                    drain_sync();
+                    for (int i = dw; i < 32; i += kRoleWarps) {
+                        const int in = 16 * q + (i & 15), tok = (i >> 4) * cols + in;
+                        if (in >= cols || tok >= count) continue;
+                        float hv[2];
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            const int at = lane * 2 + k, el = (at & 32) + tile_element(a.next_fmt, at & 31);
+                            const uint32_t g = xch + (i * kXchPitch + el) * 4;
+                            hv[k] = tile * 64 + el < a.out
+                                        ? silu_mul(__uint_as_float(lds_u32(g)), __uint_as_float(lds_u32(g + 256)))
+                                        : 0.0f;
+                        }
+                        const size_t pos = first + tok;
+                        slice_64(hv[0], hv[1], a.h + (pos * a.next_groups + tile) * 256, a.hs + (size_t)tile * a.hs_pitch + pos,
+                                 lane);
+                    }
+                }
+            } else {
+                const int o = tile * kUnitRows + row;
+                if (o < a.out) {
+                    const float bias = MODE == kPlain && a.bias ? a.bias[o] : 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 64; ++i) {
+                        if (i >= cols || tok0 + i >= count) break;
+                        const int r = first + tok0 + i;
+                        if (MODE == kDown) {
+                            a.part[(size_t)__ldcg(a.order + r) * a.out + o] = acc[i];
+                        } else {
+                            float v = activate(acc[i] + bias, a.act);
+                            if (a.row_scale) v *= a.row_scale[r];
+                            const size_t to = (size_t)r * a.out + o;
+                            a.y[to] = a.residual ? a.residual[to] + v : v;
                         }
                     }
-                } else {
-                    // lanes 2r, 2r + 1: the 16-byte windows that hold row r's blocks, strip by strip
-                    const int r = lane >> 1, sub = lane & 1;
-                    const uint8_t* base = MODE == kPair && r >= 8 ? a.w[1] : a.w[0];
-                    bool stored = false;
-#pragma unroll 1
-                    for (int k = 0; k < 8; ++k) {
-                        const int strip = 8 * me + k;
-                        const long long row = row0 + strip * (MODE == kPair ? 8 : 16) + (MODE == kPair ? (r & 7) : r);
-                        if (row >= a.total_rows) continue;
-                        long long left = a.row_bytes - (long long)c * chunk_bytes(F);
-                        if (left > chunk_bytes(F)) left = chunk_bytes(F);
-                        const uint8_t* src = base + row * a.row_bytes + (long long)c * chunk_bytes(F);
-                        const uint8_t* end = src + left;
-                        const uint8_t* q =
-                            reinterpret_cast<const uint8_t*>(reinterpret_cast<uintptr_t>(src) & ~(uintptr_t)15) + 16 * sub;
-                        uint32_t to = dst + strip * S::kBytes + r * S::kPitch + 16 * sub;
+                }
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+        if (warp == 18) {
+            // ---- products ----
+            if (lane == 0) {
+                uint32_t n = 0;
+                int k = 0;
+                uint32_t k_phase = 0;
+                while (alive && work.next(deal, id)) {
+                    int e, first, count;
+                    segment(work.u % nseg, e, first, count);
+                    const uint32_t idesc = idesc_f16kind(false, kUnitRows, 0) | (uint32_t)((count + 15) / 16 * 2) << 17;
+                    int todo = 0;
+                    for (int c = work.r0; c < work.r1; ++c) todo += stages(c);
+                    for (; todo > 0; --todo, ++n) {
+                        const int s = n & 1, o = n % kOperands;
+                        if (!wait(b_full + 8 * k, k_phase, 38) || !wait(d_free + 8 * s, (n / 2 & 1) ^ 1, 39) ||
+                            !wait(a_full + 8 * o, n / kOperands & 1, 40)) {
+                            alive = false;
+                            break;
+                        }
+                        tc_fence_after();
+                        const uint32_t at = b_ring + k * b_bytes, hi = tmem + 256 + 64 * o, lo = hi + 32, d = tmem + 128 * s;
+                        const uint64_t xhi = sw128_desc(at), xlo = sw128_desc(at + 128u * xrows);
 #pragma unroll
-                        for (int i = 0; i < (chunk_bytes(F) + 15 + 31) / 32; ++i, q += 32, to += 32) {
-                            if (q >= end) break;
-                            if (q < base) {  // the stack starts inside this window: only its own bytes are read
-                                for (int b = (int)(base - q); b < 16 && q + b < end; ++b) sts_u8(to + b, q[b]);
-                                stored = true;
-                            } else {
-                                const long long m = end - q;
-                                cp_async_16(to, q, m < 16 ? (uint32_t)m : 16u);
+                        for (int q = 0; q < 4; ++q) {
+                            mma_f16kind_ta(d, hi + 8 * q, xlo + 2 * q, idesc, q > 0);
+                            mma_f16kind_ta(d, lo + 8 * q, xhi + 2 * q, idesc, 1u);
+                        }
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) mma_f16kind_ta(d, hi + 8 * q, xhi + 2 * q, idesc, 1u);
+                        mma_commit(b_empty + 8 * k);
+                        mma_commit(a_empty + 8 * o);
+                        mma_commit(d_full + 8 * s);
+                        if (++k == a.x_slots) k = 0, k_phase ^= 1;
+                    }
+                }
+            }
+        } else if (warp == 17) {
+            // ---- x ----
+            if (MODE != kPair) grid_dependency_wait();
+            int n = 0;
+            if (lane == 0) {
+                int k = 0;
+                uint32_t k_phase = 1;
+                while (alive && work.next(deal, id)) {
+                    int e, first, count;
+                    segment(work.u % nseg, e, first, count);
+                    const int boxes = (count + 31) / 32;
+                    const uint32_t scales = (uint32_t)(count + 15) / 16 * 64;
+                    int todo = 0;
+                    for (int c = work.r0; c < work.r1; ++c) todo += stages(c);
+                    for (int g = 4 * work.r0; todo > 0; --todo, ++n, ++g) {
+                        if (!wait(b_empty + 8 * k, k_phase, 41)) {
+                            alive = false;
+                            break;
+                        }
+                        const uint32_t at = b_ring + k * b_bytes, bar = b_full + 8 * k;
+                        mbar_arrive_expect_tx(bar, boxes * 8192 + scales);
+                        bulk_g2s(smem_u32(s_x[n % kScaleRing]), a.xs + (size_t)g * a.xs_pitch + first, scales, bar);
+                        for (int i = 0; i < boxes; ++i) {
+                            tma_load_2d(at + 4096 * i, &maps.m[2], g * 128, first + 32 * i, bar);
+                            tma_load_2d(at + 128 * xrows + 4096 * i, &maps.m[2], g * 128 + 64, first + 32 * i, bar);
+                        }
+                        if (++k == a.x_slots) k = 0, k_phase ^= 1;
+                    }
+                }
+                s_b_issued = n;
+            }
+        } else if (!ALN || warp == 16) {
+            // ---- weights ----
+            int slot = 0, n = 0;
+            uint32_t slot_phase = 1;
+            const int me = 32 * (warp == 19) + lane;
+            while (alive && work.next(deal, id)) {
+                int e, first, count;
+                segment(work.u % nseg, e, first, count);
+                const int row0 = e * a.out + work.u / nseg * tile_rows;
+                for (int c = work.r0; c < work.r1; ++c, ++n) {
+                    const uint32_t full = raw_full + 8 * slot, dst = raw_ring + slot * S::kBytes;
+                    if (!__all_sync(0xffffffffu, wait(raw_empty + 8 * slot, slot_phase, 42))) {
+                        alive = false;
+                        break;
+                    }
+                    if constexpr (ALN) {
+                        if (lane == 0) {
+                            mbar_arrive_expect_tx(full, S::kBytes);
+#pragma unroll
+                            for (int b = 0; b < S::kBoxes; ++b) {
+                                const int c0 = (c * S::kChunk + b * S::kPitch) / 2;
+                                const uint32_t d = dst + b * kUnitRows * S::kPitch;
+                                tma_load_2d(d, &maps.m[0], c0, row0, full);
+                                if (MODE == kPair) tma_load_2d(d + 64 * S::kPitch, &maps.m[1], c0, row0, full);
                             }
                         }
-                    }
-                    if (stored) {  // plain stores are ordered by a plain arrival
-                        asm volatile("cp.async.wait_all;" ::: "memory");
-                        mbar_arrive(full);
                     } else {
-                        cp_async_arrive(full);
-                    }
-                }
-                __syncwarp();
-                if (++stage == a.slots) stage = 0, phase ^= 1;
-            }
-        }
-        if (!ALN) asm volatile("cp.async.wait_all;" ::: "memory");
-        if (lane == 0) s_issued[me] = n;
-        if (MODE == kDown) launch_dependents();
-        __syncthreads();
-        return;
-    }
-
-    // ---- computing warps ----
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kManyComputeRegs));
-    if (MODE != kPair) grid_dependency_wait();
-    if (MODE == kDown) launch_dependents();
-    const int tid = threadIdx.x, g = lane >> 2, t = lane & 3;
-    int stage = 0, phase = 0, taken = 0;
-    bool alive = true;
-
-    while (work.next(deal, id)) {
-        const int tile = work.u / nseg;
-        int e, first, count;
-        segment(work.u % nseg, e, first, count);
-        const bool whole = work.r1 - work.r0 == deal.per;
-        const int cap = a.seg_cap, pass_rows = cap > 16 ? 128 : 256, pitch = pass_rows + 4;
-
-        // the unit's results: get(row of x, row of the tile as the stages have it), rows [from, from + pass_rows)
-        auto epilogue = [&](int from, auto get) {
-            if (MODE == kPair) {
-                // a warp takes a block of 32 hidden values of one row of x, in the lane order of the next product
-                const int blocks = pass_rows / 64;
-                for (int i = warp; i < count * blocks; i += kComputeWarps) {
-                    const int tok = i / blocks, loc0 = from / 2 + 32 * (i % blocks), b = (tile * tile_rows + loc0) / 32;
-                    if (32 * b >= a.out) continue;
-                    const int el = half_element(a.next_fmt, b & 1, lane), loc = loc0 + el;
-                    const int row = (loc >> 3) * 16 + (loc & 7);
-                    const float h = 32 * b + el < a.out ? silu_mul(get(tok, row), get(tok, row + 8)) : 0.0f;
-                    slice_halves(h, a.h + (size_t)(first + tok) * (a.next_bprp / kChunkBlocks) * kRecordBytes, b, lane);
-                }
-            } else {
-                for (int i = tid; i < pass_rows * count; i += kComputeThreads) {
-                    const int tok = i / pass_rows, row = from + i % pass_rows;
-                    const int o = tile * tile_rows + row;
-                    if (o >= a.out) continue;
-                    float v = get(tok, row);
-                    const int r = first + tok;
-                    if (MODE == kDown) {
-                        a.part[(size_t)__ldcg(a.order + r) * a.out + o] = v;
-                    } else {
-                        if (a.bias) v += a.bias[o];
-                        v = activate(v, a.act);
-                        if (a.row_scale) v *= a.row_scale[r];
-                        const size_t to = (size_t)r * a.out + o;
-                        a.y[to] = a.residual ? a.residual[to] + v : v;
-                    }
-                }
-            }
-        };
-        // a unit that several CTAs share: each leaves its sums in a slot (head: the unit started before its range, tail: in
-        // it), and whoever comes last adds them up in order
-        auto slot_of = [&](int c, bool tail) { return a.split + ((size_t)2 * c + (tail ? 1 : 0)) * a.split_size; };
-        int j0 = 0, j1 = 0;
-        if (!whole) {
-            const long long r = (long long)(work.u - deal.each * deal.teams) * deal.per;
-            j0 = deal.owner(r), j1 = deal.owner(r + deal.per - 1);
-        }
-
-        // the rounds of this piece for J strips from `strip` against 8 SUBS rows of x from `tok0`; SUBS 0: only keep step
-        auto run = [&](auto& acc, auto jc, int strip, int tok0, bool idle) {
-            constexpr int J = decltype(jc)::value;
-            acc.init();
-            [[maybe_unused]] uint32_t window[J][2] = {};
-            if constexpr (!ALN) {
-#pragma unroll
-                for (int j = 0; j < J; ++j) {
-                    // where the lane's rows start in their windows
-                    const long long off = ((long long)e * a.out + (long long)tile * tile_rows +
-                                           (strip + j) * (MODE == kPair ? 8 : 16) + g) * a.row_bytes;
-                    window[j][0] = (uint32_t)(reinterpret_cast<uintptr_t>(a.w[0]) + off) & 15;
-                    window[j][1] = (uint32_t)(reinterpret_cast<uintptr_t>(a.w[MODE == kPair ? 1 : 0]) + off +
-                                              (MODE == kPair ? 0 : 8 * a.row_bytes)) & 15;
-                }
-            }
-            for (int c = work.r0; c < work.r1; ++c) {
-                const uint32_t full = bars + 16 * stage, at = ring + stage * stage_bytes;
-                if (!__all_sync(0xffffffffu, mbar_try_wait(full, phase)) && alive &&
-                    !__all_sync(0xffffffffu, mbar_wait(full, phase))) {
-                    alive = false;
-                    if (lane == 0) report_error(a.err, 32), *(volatile int*)&s_dead = 1;
-                }
-                if (!idle) {
-                    RowBase rows[J];
-#pragma unroll
-                    for (int j = 0; j < J; ++j) {
-                        uint32_t r0 = at + (strip + j) * S::kBytes + g * S::kPitch, r1 = r0 + 8 * S::kPitch;
-                        if constexpr (!ALN) {
-                            const uint32_t k = (uint32_t)c * (chunk_bytes(F) & 15);
-                            r0 += (window[j][0] + k) & 15;
-                            r1 += (window[j][1] + k) & 15;
+                        // two rows a thread: the 16-byte windows that hold a row's blocks
+                        bool stored = false;
+#pragma unroll 1
+                        for (int r = me; r < kUnitRows; r += 64) {
+                            const uint8_t* base = MODE == kPair && r >= 64 ? a.w[1] : a.w[0];
+                            const long long row = row0 + (MODE == kPair ? r & 63 : r);
+                            if (row >= a.total_rows) continue;
+                            long long left = a.row_bytes - (long long)c * S::kChunk;
+                            if (left > S::kChunk) left = S::kChunk;
+                            const uint8_t* src = base + row * a.row_bytes + (long long)c * S::kChunk;
+                            const uint8_t* end = src + left;
+                            const uint8_t* q =
+                                reinterpret_cast<const uint8_t*>(reinterpret_cast<uintptr_t>(src) & ~(uintptr_t)15);
+                            for (uint32_t to = dst + r * S::kPitch; q < end; q += 16, to += 16) {
+                                if (q < base) {  // the stack starts inside this window: only its own bytes are read
+                                    for (int b = (int)(base - q); b < 16 && q + b < end; ++b) sts_u8(to + b, q[b]);
+                                    stored = true;
+                                } else {
+                                    const long long m = end - q;
+                                    cp_async_16(to, q, m < 16 ? (uint32_t)m : 16u);
+                                }
+                            }
                         }
-                        rows[j] = row_base(r0, r1, t);
+                        if (stored) {  // plain stores are ordered by a plain arrival
+                            asm volatile("cp.async.wait_all;" ::: "memory");
+                            mbar_arrive(full);
+                        } else {
+                            cp_async_arrive(full);
+                        }
                     }
-                    const uint32_t x = at + kStrips * S::kBytes + tok0 * kRecordBytes;
-                    acc.template step<ALN>(x + g * kRecordBytes + t * 16, x + 2 * t * kRecordBytes + kRecordScales,
-                                           a.bpr - c * kChunkBlocks, rows);
-                }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(full + 8);
-                if (++stage == a.slots) stage = 0, phase ^= 1;
-            }
-            if (alive) taken += work.r1 - work.r0;
-            for (int from = 0; from < kUnitRows; from += pass_rows) {
-                compute_sync();  // the last pass has been read
-                if (!idle && 16 * strip >= from && 16 * strip < from + pass_rows)
-                    acc.store(sums + tok0 * pitch + 16 * strip - from, pitch, lane);
-                compute_sync();
-                auto get = [&](int tok, int row) { return sums[tok * pitch + row - from]; };
-                if (whole) {
-                    epilogue(from, get);
-                } else {
-                    float* mine = slot_of(id, id == j0);
-                    for (int i = tid; i < pass_rows * count; i += kComputeThreads)
-                        mine[(size_t)(i / pass_rows) * kUnitRows + from + i % pass_rows] = get(i / pass_rows, from + i % pass_rows);
+                    __syncwarp();
+                    if (++slot == a.slots) slot = 0, slot_phase ^= 1;
                 }
             }
-        };
-        using One = std::integral_constant<int, 1>;
-        using Two = std::integral_constant<int, 2>;
-        const bool past = tile * tile_rows + (count > 16 ? warp / 2 * 2 : warp) * (MODE == kPair ? 8 : 16) >= a.out;
-        if (count > 16) {
-            const int tok0 = 16 * (warp & 1);
-            if (count - tok0 > 8) {
-                ManyRows<F, 2, 2> acc;
-                run(acc, Two{}, warp / 2 * 2, tok0, past);
-            } else {
-                ManyRows<F, 2, 1> acc;
-                run(acc, Two{}, warp / 2 * 2, tok0, past);
-            }
-        } else if (count > 8) {
-            ManyRows<F, 1, 2> acc;
-            run(acc, One{}, warp, 0, past);
-        } else {
-            ManyRows<F, 1, 1> acc;
-            run(acc, One{}, warp, 0, past);
+            if (!ALN) asm volatile("cp.async.wait_all;" ::: "memory");
+            if (lane == 0 && warp == 16) s_raw_issued = n;
         }
-        if (!whole) {
-            compute_sync();
-            if (tid == 0) {
-                __threadfence();
-                s_last = atomicAdd(a.split_done + j0, 1u) == (unsigned)(j1 - j0);
-                __threadfence();
-            }
-            compute_sync();
-            if (s_last)
-                for (int from = 0; from < kUnitRows; from += pass_rows)
-                    epilogue(from, [&](int tok, int row) {
-                        const size_t in = (size_t)tok * kUnitRows + row;
-                        float v = __ldcg(slot_of(j0, true) + in);
-#pragma unroll 4
-                        for (int c = j0 + 1; c <= j1; ++c) v += __ldcg(slot_of(c, false) + in);
-                        return v;
-                    });
-        }
+        __syncwarp();
     }
-    __syncthreads();  // the producers have issued their last copies
-    // after a wait that ran out, copies may still be in flight: each is waited for once more, bounded
-    if (*(volatile int*)&s_dead) {
-        int n = 0;
-        for (int p = 0; p < kProducers; ++p) n = max(n, s_issued[p]);
-        for (int i = taken; i < n; ++i) mbar_wait(bars + 16 * (i % a.slots), (i / a.slots) & 1);
+    tc_fence_before();
+    __syncthreads();
+    // after a wait that ran out, copies and products may still be in flight: each is waited for once more, bounded
+    if (*(volatile int*)&s_dead && warp == 18) {
+        if (ALN)
+            for (int i = max(0, s_raw_issued - a.slots); i < s_raw_issued; ++i)
+                mbar_wait(raw_full + 8 * (i % a.slots), (i / a.slots) & 1);
+        for (int i = max(0, s_b_issued - a.x_slots); i < s_b_issued; ++i)
+            mbar_wait(b_full + 8 * (i % a.x_slots), (i / a.x_slots) & 1);
+        if (lane == 0) {
+            mma_commit(b_empty + 56);  // a barrier that no stage of x uses
+            mbar_wait(b_empty + 56, 0);
+        }
+        __syncwarp();
+    }
+    if (warp == 18) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
     }
 }
 
 template <int F, int MODE, bool ALN>
 cudaError_t launch_one(ImmaArgs a, int grid, int smem_per_sm, cudaStream_t stream) {
-    using S = Slot<F, ALN>;
+    using S = RawSlot<F, ALN>;
     auto k = imma_many_kernel<F, MODE, ALN>;
-    const int stage = kStrips * S::kBytes + a.seg_cap * kRecordBytes;
-    const int fixed = kSumFloats * 4 + 1024 + 256;  // the system's 1 KB per CTA, the static part
-    a.slots = (smem_per_sm - fixed) / (stage + 16);
+    const int xrows = (a.seg_cap + 31) / 32 * 32, stage = 256 * xrows;
+    // the system's 1 KB per CTA, the static part (up to 1 KB besides the scales), alignment, barriers
+    const int fixed = 1024 + kScaleRing * 2 * kUnitRows * 4 + 1024 + 1024 + 512 + (MODE == kPair ? 32 * kXchPitch * 4 : 0);
+    // x comes from L2, about 2 us ahead at 0.3 us a stage and 64 rows; the weights have the rest
+    a.x_slots = xrows > 64 ? 3 : xrows > 32 ? 4 : kMaxBStages;
+    a.slots = (smem_per_sm - fixed - a.x_slots * stage) / S::kBytes;
     if (a.slots > 8) a.slots = 8;
     if (a.slots < 2) return cudaErrorInvalidConfiguration;
-    const size_t smem = (size_t)a.slots * (stage + 16) + kSumFloats * 4;
+    const size_t smem = (size_t)1024 + a.x_slots * stage + a.slots * S::kBytes + (MODE == kPair ? 32 * kXchPitch * 4 : 0) + 512;
     ImmaMaps maps{};
-    if (ALN && !make_weight_maps(&maps, a, MODE == kPair, S::kPitch)) return cudaErrorInvalidValue;
+    for (int i = 0; ALN && i < (MODE == kPair ? 2 : 1); ++i)
+        if (!make_map_2d(&maps.m[i], CU_TENSOR_MAP_DATA_TYPE_UINT16, const_cast<uint8_t*>(a.w[i]),
+                         (uint64_t)a.row_bytes / 2, (uint64_t)a.total_rows, (uint64_t)a.row_bytes, S::kPitch / 2,
+                         MODE == kPair ? kUnitRows / 2 : kUnitRows, CU_TENSOR_MAP_SWIZZLE_NONE))
+            return cudaErrorInvalidValue;
+    if (!make_map_2d(&maps.m[2], CU_TENSOR_MAP_DATA_TYPE_UINT16, const_cast<uint8_t*>(a.x), (uint64_t)a.groups * 128,
+                     (uint64_t)a.x_rows, (uint64_t)a.groups * 256, 64, 32, CU_TENSOR_MAP_SWIZZLE_128B))
+        return cudaErrorInvalidValue;
     static std::atomic<uint64_t> done{0};
     cudaError_t e = ready_kernel(k, kManyLaunchRegs, done);
     if (e != cudaSuccess) return e;

@@ -5,16 +5,19 @@ with an epilogue, with elementwise error bounds of the library's arithmetic
 The bounds follow the arithmetic in include/mlq.h, not a measurement:
 * a value x in a block with largest magnitude A is carried either as 31-bit
   fixed point (half a step: below 1.01 * 2^-31 A; for q4 the block holds 16-fold
-  values too, so 2^-27 A) or as two fp16 values (each
-  rounding 2^-11 relative: 2^-22 |x|, and at most 2^-39 A where the second is
-  subnormal); the sum of both bounds covers either;
+  values too, so 2^-27 A) or, with many rows, as two fp16 values (each rounding 2^-11
+  relative: 2^-22 |x|, and at most 2^-39 of the largest of its 64 values where the
+  second is subnormal).  A weight is then two fp16 values too: 2^-22 |w| (and
+  q4_1 one fp32 rounding), 2^-39 of the largest of the row's 64; and the
+  product of both second values, below 2^-22 |x w|, is left out.  The sum of all
+  these covers either form;
 * integer sums of a block are exact.  The fp32 steps round by 2^-24 relative
   each: per block one conversion of the integer sum, one product and one sum, then a
   few for the parts of the K axis, and 5 in a block's sum of x (q4) -- counted as
   (blocks + 16) roundings of the sum of magnitudes (each sum's partial values stay
-  below it).  The fp16 form's sums
-  are made by the matrix unit, which may truncate: 4 instructions per
-  block, 2^-22 of that block's magnitudes each, 16 roundings more in all."""
+  below it).  With many rows the sums of 64 values are made by the matrix unit,
+  which may truncate: 12 instructions, 2^-22 of those magnitudes each, 48
+  roundings more in all."""
 from __future__ import annotations
 
 import math
@@ -68,22 +71,23 @@ def dequantize64(fmt, blocks, rows, cols):
     return w.reshape(rows, nb * 32)[:, :cols], mag.reshape(rows, nb * 32)[:, :cols]
 
 
-def block_max(x):
-    """Per element, the largest magnitude of its 32-value block."""
+def block_max(x, size=32):
+    """Per element, the largest magnitude of its block."""
     r, n = x.shape
-    nb = (n + 31) // 32
-    p = np.zeros((r, nb * 32))
+    nb = (n + size - 1) // size
+    p = np.zeros((r, nb * size))
     p[:, :n] = np.abs(x)
-    return np.repeat(p.reshape(r, nb, 32).max(2), 32, 1)[:, :n]
+    return np.repeat(p.reshape(r, nb, size).max(2), size, 1)[:, :n]
 
 
 def product(x, fmt, blocks, out, dx=None):
     """x W^T in float64 and its bound; dx: an elementwise error of x already there."""
     w, mag = dequantize64(fmt, blocks, out, x.shape[1])
     xa = np.abs(x) + (0 if dx is None else dx)
-    step = 2.0 ** -22 * xa + 1.01 * 2.0 ** -27 * block_max(xa)
+    step = (3 * 2.0 ** -22 + EPS) * xa + 1.01 * 2.0 ** -27 * block_max(xa) + 2.0 ** -39 * block_max(xa, 64)
     nb = (x.shape[1] + 31) // 32
-    bound = step @ np.abs(w).T + (nb + 32) * EPS * ((xa + step) @ mag.T)
+    bound = step @ np.abs(w).T + 2.0 ** -39 * (xa @ block_max(np.abs(w), 64).T)
+    bound += (nb + 64) * EPS * ((xa + step) @ mag.T)
     if dx is not None:
         bound = bound + dx @ np.abs(w).T
     return x @ w.T, bound
