@@ -64,10 +64,11 @@ __device__ __forceinline__ float silu_mul(float g, float u) {
 // mlq_device_error().  Codes: 1 = pipeline "full" wait, 2 = "empty" wait,
 // 3 = drain wait, 4 = peer flag wait, 5 = consumer rendezvous, 6 = x-tile
 // "empty" wait, 7 = resident x tiles ready wait, 8 = staged x copy wait,
-// 12-16 = GEMM waits, 20-26 = batched-decode GEMM waits, 30-33 = waits of the
-// experts' products and of the linear with an epilogue (few rows: data, free
-// stage; many rows: the same), 34-36 = waits of the router's products (free
-// stage, data, products done).
+// 12-16 = GEMM waits, 20-26 = batched-decode GEMM waits, 30-31 = waits of the
+// experts' products and of the linear with an epilogue by few rows (data, free
+// stage), 34-36 = waits of the router's products (free stage, data, products
+// done), 44-51 = waits of those products by many rows (weights, free operand, sums,
+// x, drained sums, operand, free x, free weights).
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ void report_error(int* err, int code) {
     if (err) atomicCAS(err, 0, code);
@@ -128,6 +129,13 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
         if (mbar_try_wait(bar, parity)) return true;
         if ((i & 255u) == 0 && global_ns() - t0 > kWaitLimitNs) return false;  // clock read rarely
     }
+}
+
+// True in one lane of a converged warp (the same one each time).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one != 0;
 }
 
 __device__ __forceinline__ void mbar_arrive_expect_tx(uint32_t bar, uint32_t bytes) {

@@ -32,7 +32,7 @@ constexpr int kUnitRows = 128;
 constexpr int kRoleWarps = 8;                    // that decode, and that drain
 constexpr int kManyThreads = 32 * (2 * kRoleWarps + 4);
 constexpr int kDrainThreads = 32 * kRoleWarps;
-constexpr int kOperands = 4, kScaleRing = 8;
+constexpr int kOperands = 4, kScaleRing = 8, kDone = 8;
 constexpr int kMaxBStages = 6;                   // scales of x outlive the operand by two products: 8 - 2
 constexpr int kXchPitch = kUnitRows + 4;         // kPair: [32 rows of x][128 rows + 4]
 constexpr int kManyJoin = 2;                     // rounds
@@ -197,18 +197,19 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     const uint32_t b_ring = (smem_u32(smem) + 1023u) & ~1023u, raw_ring = b_ring + a.x_slots * b_bytes;
     const uint32_t xch = raw_ring + a.slots * S::kBytes;
     const uint32_t bars = xch + (MODE == kPair ? 32 * kXchPitch * 4 : 0);
-    const uint32_t raw_full = bars, raw_empty = raw_full + 64, b_full = raw_empty + 64, b_empty = b_full + 64,
-                   a_full = b_empty + 64, a_empty = a_full + 32, d_full = a_empty + 32, d_free = d_full + 16;
+    // done: a stage's products; it frees x and the operand too
+    const uint32_t raw_full = bars, raw_empty = raw_full + 64, b_full = raw_empty + 64, done = b_full + 64,
+                   a_full = done + 8 * (kDone + 1), d_free = a_full + 32;
     if (threadIdx.x == 0) {
         s_dead = 0;
         for (int i = 0; i < 8; ++i) {
             mbar_init(raw_full + 8 * i, ALN ? 1 : 64);
             mbar_init(raw_empty + 8 * i, kRoleWarps);
             mbar_init(b_full + 8 * i, 1);
-            mbar_init(b_empty + 8 * i, 1);
         }
-        for (int i = 0; i < kOperands; ++i) mbar_init(a_full + 8 * i, kRoleWarps), mbar_init(a_empty + 8 * i, 1);
-        for (int i = 0; i < 2; ++i) mbar_init(d_full + 8 * i, 1), mbar_init(d_free + 8 * i, kRoleWarps);
+        for (int i = 0; i <= kDone; ++i) mbar_init(done + 8 * i, 1);
+        for (int i = 0; i < kOperands; ++i) mbar_init(a_full + 8 * i, kRoleWarps);
+        for (int i = 0; i < 2; ++i) mbar_init(d_free + 8 * i, kRoleWarps);
         fence_mbar_init();
     }
     if (warp == 18) tmem_alloc(smem_u32(&s_tmem), 512);
@@ -218,8 +219,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     if (MODE != kDown) launch_dependents();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = s_tmem;
-    const int nseg = MODE == kPlain ? (a.rows + a.seg_cap - 1) / a.seg_cap : __ldcg(a.nseg);
+    const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
+    const int nseg = MODE == kPlain ? (a.rows + a.seg_cap - 1) / a.seg_cap : __shfl_sync(0xffffffffu, __ldcg(a.nseg), 0);
     const int id = blockIdx.x;
     const Deal deal(nseg * a.tiles, steps, gridDim.x, kManyJoin);
     Work work(deal, id);
@@ -230,8 +231,9 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         count = MODE == kPlain ? min(a.rows - first, a.seg_cap) : __ldcg(&a.segs[seg].count);
     };
     auto stages = [&](int c) { return min(4, (a.bpr - c * kChunkBlocks + 1) / 2); };
+    // (whoever gives up lets the others run into their own limits)
     auto wait = [&](uint32_t bar, uint32_t parity, int code) {
-        if (mbar_wait(bar, parity)) return !*(volatile int*)&s_dead;
+        if (mbar_wait(bar, parity)) return true;
         report_error(a.err, code);
         *(volatile int*)&s_dead = 1;
         return false;
@@ -244,6 +246,15 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         const int row = 32 * (warp & 3) + lane, h = warp >> 2;
         int slot = 0;
         uint32_t slot_phase = 0, n = 0;  // n: stages so far
+        bool behind = false;             // the last one is on its way to tensor memory
+        auto hand_over = [&] {
+            if (!behind) return;
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(a_full + 8 * ((n - 1) % kOperands));
+            behind = false;
+        };
         while (alive && work.next(deal, id)) {
             int e, first, count;
             segment(work.u % nseg, e, first, count);
@@ -255,7 +266,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                 window = (uint32_t)(reinterpret_cast<uintptr_t>(a.w[up ? 1 : 0]) + at * a.row_bytes) & 15;
             }
             for (int c = work.r0; alive && c < work.r1; ++c) {
-                if (!__all_sync(0xffffffffu, wait(raw_full + 8 * slot, slot_phase, 32))) {
+                if (!__all_sync(0xffffffffu, wait(raw_full + 8 * slot, slot_phase, 44))) {
                     alive = false;
                     break;
                 }
@@ -278,8 +289,9 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                     const float scale = weight_scale<F>(b.dm, other, &inverse);
                     uint32_t hi[16], lo[16];
                     to_halves<F>(b, scale, hi, lo);
+                    hand_over();  // a store takes as long as a stage's conversion
                     const int k = n % kOperands;
-                    if (!__all_sync(0xffffffffu, wait(a_empty + 8 * k, (n / kOperands & 1) ^ 1, 33))) {
+                    if (!__all_sync(0xffffffffu, n >= kOperands ? wait(done + 8 * ((n - kOperands) % kDone), (n - kOperands) / kDone & 1, 45) : true)) {
                         alive = false;
                         return;
                     }
@@ -288,16 +300,13 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                     tmem_st16(to, hi);
                     tmem_st16(to + 32, lo);
                     if (h == 0) s_w[n % kScaleRing][row] = inverse;
-                    tmem_wait_st();
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(a_full + 8 * k);
-                    ++n;
+                    ++n, behind = true;
                 });
                 __syncwarp();
                 if (lane == 0) mbar_arrive(raw_empty + 8 * slot);
                 if (++slot == a.slots) slot = 0, slot_phase ^= 1;
             }
+            hand_over();
         }
     } else if (warp < 2 * kRoleWarps) {
         // ---- drain ----
@@ -318,7 +327,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             for (int c = work.r0; c < work.r1; ++c) todo += stages(c);
             for (; todo > 0; --todo, ++n) {
                 const int s = n & 1;
-                if (!__all_sync(0xffffffffu, wait(d_full + 8 * s, n / 2 & 1, 37))) {
+                if (!__all_sync(0xffffffffu, wait(done + 8 * (n % kDone), n / kDone & 1, 46))) {
                     alive = false;
                     break;
                 }
@@ -368,13 +377,16 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                 drain_sync();
                 if (!s_last) continue;
 #pragma unroll
-                for (int i = 0; i < 64; ++i)
-                    if (i < cols) acc[i] = __ldcg(slot_of(j0, true) + i * kUnitRows);
-                for (int c = j0 + 1; c <= j1; ++c) {
-                    const float* from = slot_of(c, false);
+                for (int q = 0; q < 64; q += 8) {
+                    if (q >= cols) break;
 #pragma unroll
-                    for (int i = 0; i < 64; ++i)
-                        if (i < cols) acc[i] += __ldcg(from + i * kUnitRows);
+                    for (int i = q; i < q + 8; ++i) acc[i] = __ldcg(slot_of(j0, true) + i * kUnitRows);
+#pragma unroll 4
+                    for (int c = j0 + 1; c <= j1; ++c) {
+                        const float* from = slot_of(c, false);
+#pragma unroll
+                        for (int i = q; i < q + 8; ++i) acc[i] += __ldcg(from + i * kUnitRows);
+                    }
                 }
             }
             const int tok0 = half * cols;
@@ -429,26 +441,35 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
         if (warp == 18) {
             // ---- products ----
-            if (lane == 0) {
-                uint32_t n = 0;
-                int k = 0;
-                uint32_t k_phase = 0;
-                while (alive && work.next(deal, id)) {
-                    int e, first, count;
-                    segment(work.u % nseg, e, first, count);
-                    const uint32_t idesc = idesc_f16kind(false, kUnitRows, 0) | (uint32_t)((count + 15) / 16 * 2) << 17;
-                    int todo = 0;
-                    for (int c = work.r0; c < work.r1; ++c) todo += stages(c);
-                    for (; todo > 0; --todo, ++n) {
-                        const int s = n & 1, o = n % kOperands;
-                        if (!wait(b_full + 8 * k, k_phase, 38) || !wait(d_free + 8 * s, (n / 2 & 1) ^ 1, 39) ||
-                            !wait(a_full + 8 * o, n / kOperands & 1, 40)) {
-                            alive = false;
-                            break;
-                        }
-                        tc_fence_after();
-                        const uint32_t at = b_ring + k * b_bytes, hi = tmem + 256 + 64 * o, lo = hi + 32, d = tmem + 128 * s;
-                        const uint64_t xhi = sw128_desc(at), xlo = sw128_desc(at + 128u * xrows);
+            // the whole warp goes through the loop and one lane issues, with operands that are the same in all: so they
+            // are in uniform registers (a lane on its own takes ~100 cycles per instruction)
+            uint32_t n = 0;
+            int k = 0;
+            uint32_t k_phase = 0;
+            while (alive && work.next(deal, id)) {
+                int e, first, count;
+                segment(work.u % nseg, e, first, count);
+                const uint32_t idesc = idesc_f16kind(false, kUnitRows, 0) |
+                                       (uint32_t)__shfl_sync(0xffffffffu, (count + 15) / 16 * 2, 0) << 17;
+                int todo = 0;
+                for (int c = work.r0; c < work.r1; ++c) todo += stages(c);
+                todo = __shfl_sync(0xffffffffu, todo, 0);
+                for (; todo > 0; --todo, ++n) {
+                    const uint32_t s = n & 1, o = n % kOperands;
+                    // mostly all three have come, and are looked at together
+                    const bool x_here = mbar_try_wait(b_full + 8 * k, k_phase),
+                               sum_free = mbar_try_wait(d_free + 8 * s, (n / 2 & 1) ^ 1),
+                               w_here = mbar_try_wait(a_full + 8 * o, n / kOperands & 1);
+                    if (!__all_sync(0xffffffffu, (x_here || wait(b_full + 8 * k, k_phase, 47)) &&
+                                                     (sum_free || wait(d_free + 8 * s, (n / 2 & 1) ^ 1, 48)) &&
+                                                     (w_here || wait(a_full + 8 * o, n / kOperands & 1, 49)))) {
+                        alive = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t at = b_ring + k * b_bytes, hi = tmem + 256 + 64 * o, lo = hi + 32, d = tmem + 128 * s;
+                    const uint64_t xhi = sw128_desc(at), xlo = sw128_desc(at + 128u * xrows);
+                    if (elect_one()) {
 #pragma unroll
                         for (int q = 0; q < 4; ++q) {
                             mma_f16kind_ta(d, hi + 8 * q, xlo + 2 * q, idesc, q > 0);
@@ -456,44 +477,45 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                         }
 #pragma unroll
                         for (int q = 0; q < 4; ++q) mma_f16kind_ta(d, hi + 8 * q, xhi + 2 * q, idesc, 1u);
-                        mma_commit(b_empty + 8 * k);
-                        mma_commit(a_empty + 8 * o);
-                        mma_commit(d_full + 8 * s);
-                        if (++k == a.x_slots) k = 0, k_phase ^= 1;
+                        mma_commit(done + 8 * (n % kDone));
                     }
+                    __syncwarp();
+                    if (++k == a.x_slots) k = 0, k_phase ^= 1;
                 }
             }
         } else if (warp == 17) {
             // ---- x ----
             if (MODE != kPair) grid_dependency_wait();
-            int n = 0;
-            if (lane == 0) {
-                int k = 0;
-                uint32_t k_phase = 1;
-                while (alive && work.next(deal, id)) {
-                    int e, first, count;
-                    segment(work.u % nseg, e, first, count);
-                    const int boxes = (count + 31) / 32;
-                    const uint32_t scales = (uint32_t)(count + 15) / 16 * 64;
-                    int todo = 0;
-                    for (int c = work.r0; c < work.r1; ++c) todo += stages(c);
-                    for (int g = 4 * work.r0; todo > 0; --todo, ++n, ++g) {
-                        if (!wait(b_empty + 8 * k, k_phase, 41)) {
-                            alive = false;
-                            break;
-                        }
-                        const uint32_t at = b_ring + k * b_bytes, bar = b_full + 8 * k;
+            int n = 0, k = 0;
+            while (alive && work.next(deal, id)) {
+                int e, first, count;
+                segment(work.u % nseg, e, first, count);
+                first = __shfl_sync(0xffffffffu, first, 0), count = __shfl_sync(0xffffffffu, count, 0);
+                const int boxes = (count + 31) / 32;
+                const uint32_t scales = (uint32_t)(count + 15) / 16 * 64;
+                int todo = 0;
+                for (int c = work.r0; c < work.r1; ++c) todo += stages(c);
+                todo = __shfl_sync(0xffffffffu, todo, 0);
+                for (int g = 4 * work.r0; todo > 0; --todo, ++n, ++g) {
+                    const int before = n - a.x_slots;  // had this place
+                    if (before >= 0 && !__all_sync(0xffffffffu, wait(done + 8 * (before % kDone), before / kDone & 1, 50))) {
+                        alive = false;
+                        break;
+                    }
+                    const uint32_t at = b_ring + k * b_bytes, bar = b_full + 8 * k;
+                    if (elect_one()) {
                         mbar_arrive_expect_tx(bar, boxes * 8192 + scales);
                         bulk_g2s(smem_u32(s_x[n % kScaleRing]), a.xs + (size_t)g * a.xs_pitch + first, scales, bar);
                         for (int i = 0; i < boxes; ++i) {
                             tma_load_2d(at + 4096 * i, &maps.m[2], g * 128, first + 32 * i, bar);
                             tma_load_2d(at + 128 * xrows + 4096 * i, &maps.m[2], g * 128 + 64, first + 32 * i, bar);
                         }
-                        if (++k == a.x_slots) k = 0, k_phase ^= 1;
                     }
+                    __syncwarp();
+                    if (++k == a.x_slots) k = 0;
                 }
-                s_b_issued = n;
             }
+            if (lane == 0) s_b_issued = n;
         } else if (!ALN || warp == 16) {
             // ---- weights ----
             int slot = 0, n = 0;
@@ -502,15 +524,15 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             while (alive && work.next(deal, id)) {
                 int e, first, count;
                 segment(work.u % nseg, e, first, count);
-                const int row0 = e * a.out + work.u / nseg * tile_rows;
+                const int row0 = __shfl_sync(0xffffffffu, e, 0) * a.out + work.u / nseg * tile_rows;
                 for (int c = work.r0; c < work.r1; ++c, ++n) {
                     const uint32_t full = raw_full + 8 * slot, dst = raw_ring + slot * S::kBytes;
-                    if (!__all_sync(0xffffffffu, wait(raw_empty + 8 * slot, slot_phase, 42))) {
+                    if (!__all_sync(0xffffffffu, wait(raw_empty + 8 * slot, slot_phase, 51))) {
                         alive = false;
                         break;
                     }
                     if constexpr (ALN) {
-                        if (lane == 0) {
+                        if (elect_one()) {
                             mbar_arrive_expect_tx(full, S::kBytes);
 #pragma unroll
                             for (int b = 0; b < S::kBoxes; ++b) {
@@ -569,11 +591,9 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                 mbar_wait(raw_full + 8 * (i % a.slots), (i / a.slots) & 1);
         for (int i = max(0, s_b_issued - a.x_slots); i < s_b_issued; ++i)
             mbar_wait(b_full + 8 * (i % a.x_slots), (i / a.x_slots) & 1);
-        if (lane == 0) {
-            mma_commit(b_empty + 56);  // a barrier that no stage of x uses
-            mbar_wait(b_empty + 56, 0);
-        }
+        if (elect_one()) mma_commit(done + 8 * kDone);  // a barrier of its own
         __syncwarp();
+        mbar_wait(done + 8 * kDone, 0);
     }
     if (warp == 18) {
         tc_fence_after();
