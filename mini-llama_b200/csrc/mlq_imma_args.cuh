@@ -8,7 +8,7 @@ namespace mlq {
 enum Mode { kPlain = 0, kPair = 1, kDown = 2 };
 
 struct ImmaMaps {
-    CUtensorMap m[3];  // weights; [1]: the up projections (kPair); [2]: x (many rows)
+    CUtensorMap m[2];
 };
 
 struct ImmaArgs {

@@ -41,6 +41,12 @@ constexpr int kManyLaunchRegs = 96, kDecodeRegs = 88, kDrainRegs = 136, kOtherRe
 static_assert((kRoleWarps * (kDecodeRegs + kDrainRegs) + 4 * kOtherRegs) * 32 <= kManyThreads * kManyLaunchRegs,
               "the shares must not exceed the launch's registers, or setmaxnreg would wait for ever");
 
+// Tensor maps: weights ([1]: the up projections of kPair), x in boxes of 32,
+// 64, 96 and 128 rows, hi and lo in one.
+struct ManyMaps {
+    CUtensorMap w[2], x[4];
+};
+
 // Packed blocks of 128 rows, one round.  Aligned: as TMA boxes (q4_1: two of 4
 // blocks, so that 8 rows' 16-byte pieces lie in different banks); else the 16-byte
 // windows that hold a row's blocks.
@@ -53,6 +59,28 @@ struct RawSlot {
 };
 
 __device__ __forceinline__ void drain_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kDrainThreads) : "memory"); }
+
+// Two fp32 values in one instruction.
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 unpack2(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
 
 // Whether `p` holds for any draining thread.
 __device__ __forceinline__ bool drain_any(bool p) {
@@ -183,7 +211,7 @@ __device__ __forceinline__ void to_halves(const Block<F>& b, float scale, uint32
 
 template <int F, int MODE, bool ALN>
 __global__ void __launch_bounds__(kManyThreads, 1)
-    imma_many_kernel(const __grid_constant__ ImmaMaps maps, const __grid_constant__ ImmaArgs a) {
+    imma_many_kernel(const __grid_constant__ ManyMaps maps, const __grid_constant__ ImmaArgs a) {
     extern __shared__ __align__(1024) uint8_t smem[];
     using S = RawSlot<F, ALN>;
     __shared__ int s_last, s_dead, s_raw_issued, s_b_issued;
@@ -191,7 +219,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     __shared__ __align__(16) float s_w[kScaleRing][kUnitRows], s_x[kScaleRing][128];
     const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
     const int steps = (a.bpr + kChunkBlocks - 1) / kChunkBlocks;
-    const int xrows = (a.seg_cap + 31) / 32 * 32;  // of a stage of x
+    const uint32_t xrows = (a.seg_cap + 31) / 32 * 32;  // of a stage of x
     // shared memory: x, weights, (kPair) exchange, barriers
     const uint32_t b_bytes = 256u * xrows;
     const uint32_t b_ring = (smem_u32(smem) + 1023u) & ~1023u, raw_ring = b_ring + a.x_slots * b_bytes;
@@ -320,9 +348,9 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             int e, first, count;
             segment(work.u % nseg, e, first, count);
             const int cols = (count + 15) / 16 * 8;  // of this half
-            float acc[64];
+            uint64_t acc2[32];  // pairs of columns
 #pragma unroll
-            for (int i = 0; i < 64; ++i) acc[i] = 0.0f;
+            for (int i = 0; i < 32; ++i) acc2[i] = 0;
             int todo = 0;
             for (int c = work.r0; c < work.r1; ++c) todo += stages(c);
             for (; todo > 0; --todo, ++n) {
@@ -335,24 +363,32 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                 const uint32_t from = tmem + ((uint32_t)(32 * (dw & 3)) << 16) + 128 * s + half * cols;
                 const float sw = s_w[n % kScaleRing][row];
                 const float* sx = &s_x[n % kScaleRing][half * cols];
+                const uint64_t sw2 = pack2(sw, sw);
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                     if (16 * q >= cols) break;
                     uint32_t v[16];
                     tmem_ld16_issue(from + 16 * q, v);
-                    float f[16];
+                    uint64_t f[8];
 #pragma unroll
                     for (int i = 0; i < 16; i += 4) {
                         const float4 x = *reinterpret_cast<const float4*>(sx + 16 * q + i);
-                        f[i] = x.x * sw, f[i + 1] = x.y * sw, f[i + 2] = x.z * sw, f[i + 3] = x.w * sw;
+                        f[i / 2] = mul2(pack2(x.x, x.y), sw2), f[i / 2 + 1] = mul2(pack2(x.z, x.w), sw2);
                     }
                     tmem_wait_ld(v);
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) acc[16 * q + i] = fmaf(__uint_as_float(v[i]), f[i], acc[16 * q + i]);
+                    for (int i = 0; i < 8; ++i)
+                        acc2[8 * q + i] = fma2(pack2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), f[i], acc2[8 * q + i]);
                 }
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(d_free + 8 * s);
+            }
+            float acc[64];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+                const float2 p = unpack2(acc2[i]);
+                acc[2 * i] = p.x, acc[2 * i + 1] = p.y;
             }
             // together, or some would wait below for others that have gone
             if (drain_any(!alive)) break;
@@ -454,6 +490,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                 int todo = 0;
                 for (int c = work.r0; c < work.r1; ++c) todo += stages(c);
                 todo = __shfl_sync(0xffffffffu, todo, 0);
+                const uint32_t plane = (uint32_t)__shfl_sync(0xffffffffu, (count + 31) / 32, 0) * 4096;
                 for (; todo > 0; --todo, ++n) {
                     const uint32_t s = n & 1, o = n % kOperands;
                     // mostly all three have come, and are looked at together
@@ -468,7 +505,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                     }
                     tc_fence_after();
                     const uint32_t at = b_ring + k * b_bytes, hi = tmem + 256 + 64 * o, lo = hi + 32, d = tmem + 128 * s;
-                    const uint64_t xhi = sw128_desc(at), xlo = sw128_desc(at + 128u * xrows);
+                    const uint64_t xhi = sw128_desc(at), xlo = sw128_desc(at + plane);
                     if (elect_one()) {
 #pragma unroll
                         for (int q = 0; q < 4; ++q) {
@@ -490,9 +527,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             while (alive && work.next(deal, id)) {
                 int e, first, count;
                 segment(work.u % nseg, e, first, count);
-                first = __shfl_sync(0xffffffffu, first, 0), count = __shfl_sync(0xffffffffu, count, 0);
-                const int boxes = (count + 31) / 32;
-                const uint32_t scales = (uint32_t)(count + 15) / 16 * 64;
+                first = __shfl_sync(0xffffffffu, first, 0);
+                const int boxes = __shfl_sync(0xffffffffu, (count + 31) / 32, 0);
                 int todo = 0;
                 for (int c = work.r0; c < work.r1; ++c) todo += stages(c);
                 todo = __shfl_sync(0xffffffffu, todo, 0);
@@ -504,12 +540,9 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                     }
                     const uint32_t at = b_ring + k * b_bytes, bar = b_full + 8 * k;
                     if (elect_one()) {
-                        mbar_arrive_expect_tx(bar, boxes * 8192 + scales);
-                        bulk_g2s(smem_u32(s_x[n % kScaleRing]), a.xs + (size_t)g * a.xs_pitch + first, scales, bar);
-                        for (int i = 0; i < boxes; ++i) {
-                            tma_load_2d(at + 4096 * i, &maps.m[2], g * 128, first + 32 * i, bar);
-                            tma_load_2d(at + 128 * xrows + 4096 * i, &maps.m[2], g * 128 + 64, first + 32 * i, bar);
-                        }
+                        mbar_arrive_expect_tx(bar, boxes * (8192 + 128));
+                        bulk_g2s(smem_u32(s_x[n % kScaleRing]), a.xs + (size_t)g * a.xs_pitch + first, boxes * 128, bar);
+                        tma_load_3d(at, &maps.x[boxes - 1], 0, first, 2 * g, bar);
                     }
                     __syncwarp();
                     if (++k == a.x_slots) k = 0;
@@ -538,8 +571,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                             for (int b = 0; b < S::kBoxes; ++b) {
                                 const int c0 = (c * S::kChunk + b * S::kPitch) / 2;
                                 const uint32_t d = dst + b * kUnitRows * S::kPitch;
-                                tma_load_2d(d, &maps.m[0], c0, row0, full);
-                                if (MODE == kPair) tma_load_2d(d + 64 * S::kPitch, &maps.m[1], c0, row0, full);
+                                tma_load_2d(d, &maps.w[0], c0, row0, full);
+                                if (MODE == kPair) tma_load_2d(d + 64 * S::kPitch, &maps.w[1], c0, row0, full);
                             }
                         }
                     } else {
@@ -601,6 +634,18 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     }
 }
 
+// x as [plane: group and hi or lo][row][64], boxes of both planes of a group.
+inline bool make_map_x(CUtensorMap* m, const ImmaArgs& a, int rows) {
+    const EncodeTiledFn fn = encode_fn();
+    if (!fn) return false;
+    const cuuint64_t dims[3] = {64, (cuuint64_t)a.x_rows, (cuuint64_t)a.groups * 2};
+    const cuuint64_t strides[2] = {(cuuint64_t)a.groups * 256, 128};
+    const cuuint32_t box[3] = {64, (cuuint32_t)rows, 2}, one[3] = {1, 1, 1};
+    return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<uint8_t*>(a.x), dims, strides, box, one,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <int F, int MODE, bool ALN>
 cudaError_t launch_one(ImmaArgs a, int grid, int smem_per_sm, cudaStream_t stream) {
     using S = RawSlot<F, ALN>;
@@ -614,15 +659,14 @@ cudaError_t launch_one(ImmaArgs a, int grid, int smem_per_sm, cudaStream_t strea
     if (a.slots > 8) a.slots = 8;
     if (a.slots < 2) return cudaErrorInvalidConfiguration;
     const size_t smem = (size_t)1024 + a.x_slots * stage + a.slots * S::kBytes + (MODE == kPair ? 32 * kXchPitch * 4 : 0) + 512;
-    ImmaMaps maps{};
+    ManyMaps maps{};
     for (int i = 0; ALN && i < (MODE == kPair ? 2 : 1); ++i)
-        if (!make_map_2d(&maps.m[i], CU_TENSOR_MAP_DATA_TYPE_UINT16, const_cast<uint8_t*>(a.w[i]),
+        if (!make_map_2d(&maps.w[i], CU_TENSOR_MAP_DATA_TYPE_UINT16, const_cast<uint8_t*>(a.w[i]),
                          (uint64_t)a.row_bytes / 2, (uint64_t)a.total_rows, (uint64_t)a.row_bytes, S::kPitch / 2,
                          MODE == kPair ? kUnitRows / 2 : kUnitRows, CU_TENSOR_MAP_SWIZZLE_NONE))
             return cudaErrorInvalidValue;
-    if (!make_map_2d(&maps.m[2], CU_TENSOR_MAP_DATA_TYPE_UINT16, const_cast<uint8_t*>(a.x), (uint64_t)a.groups * 128,
-                     (uint64_t)a.x_rows, (uint64_t)a.groups * 256, 64, 32, CU_TENSOR_MAP_SWIZZLE_128B))
-        return cudaErrorInvalidValue;
+    for (int i = 0; i < xrows / 32; ++i)
+        if (!make_map_x(&maps.x[i], a, 32 * (i + 1))) return cudaErrorInvalidValue;
     static std::atomic<uint64_t> done{0};
     cudaError_t e = ready_kernel(k, kManyLaunchRegs, done);
     if (e != cudaSuccess) return e;
