@@ -16,7 +16,7 @@
 //   warps 8-15   drain: the same rows, half of the segment's columns; the end of a unit
 //   warp 16, 19  weights; 17: x; 18: products
 //
-// Tensor memory: 2 sums of 128 columns, 4 operands of 64 (hi 32, lo 32).
+// Tensor memory: 2 sums of 128 columns (4 of 64 where a segment has no more), 4 operands of 64 (hi 32, lo 32).
 // Rounds are dealt out evenly as in mlq_imma_few.cuh.
 #pragma once
 
@@ -32,8 +32,8 @@ constexpr int kUnitRows = 128;
 constexpr int kRoleWarps = 8;                    // that decode, and that drain
 constexpr int kManyThreads = 32 * (2 * kRoleWarps + 4);
 constexpr int kDrainThreads = 32 * kRoleWarps;
-constexpr int kOperands = 4, kScaleRing = 8, kDone = 8;
-constexpr int kMaxBStages = 6;                   // scales of x outlive the operand by two products: 8 - 2
+constexpr int kOperands = 4, kScaleRing = 8, kXRing = 16, kDone = 8;
+constexpr int kMaxBStages = 6;                   // + 4 sums: scales of x outlive the operand by as many products
 constexpr int kXchPitch = kUnitRows + 4;         // kPair: [32 rows of x][128 rows + 4]
 constexpr int kManyJoin = 2;                     // rounds
 // registers at launch, and after the split
@@ -216,7 +216,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     using S = RawSlot<F, ALN>;
     __shared__ int s_last, s_dead, s_raw_issued, s_b_issued;
     __shared__ uint32_t s_tmem;
-    __shared__ __align__(16) float s_w[kScaleRing][kUnitRows], s_x[kScaleRing][128];
+    __shared__ __align__(16) float s_w[kScaleRing][kUnitRows], s_x[kXRing][128];
     const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
     const int steps = (a.bpr + kChunkBlocks - 1) / kChunkBlocks;
     const uint32_t xrows = (a.seg_cap + 31) / 32 * 32;  // of a stage of x
@@ -237,7 +237,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         }
         for (int i = 0; i <= kDone; ++i) mbar_init(done + 8 * i, 1);
         for (int i = 0; i < kOperands; ++i) mbar_init(a_full + 8 * i, kRoleWarps);
-        for (int i = 0; i < 2; ++i) mbar_init(d_free + 8 * i, kRoleWarps);
+        for (int i = 0; i < 4; ++i) mbar_init(d_free + 8 * i, kRoleWarps);
         fence_mbar_init();
     }
     if (warp == 18) tmem_alloc(smem_u32(&s_tmem), 512);
@@ -258,6 +258,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         first = MODE == kPlain ? seg * a.seg_cap : __ldcg(&a.segs[seg].start);
         count = MODE == kPlain ? min(a.rows - first, a.seg_cap) : __ldcg(&a.segs[seg].count);
     };
+    // sums in tensor memory: 4 of 64 columns or 2 of 128
+    const uint32_t sums = xrows <= 64 ? 4 : 2, sum_shift = xrows <= 64 ? 2 : 1, sum_cols = 256 / sums;
     auto stages = [&](int c) { return min(4, (a.bpr - c * kChunkBlocks + 1) / 2); };
     // (whoever gives up lets the others run into their own limits)
     auto wait = [&](uint32_t bar, uint32_t parity, int code) {
@@ -354,15 +356,15 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             int todo = 0;
             for (int c = work.r0; c < work.r1; ++c) todo += stages(c);
             for (; todo > 0; --todo, ++n) {
-                const int s = n & 1;
+                const uint32_t s = n & (sums - 1);
                 if (!__all_sync(0xffffffffu, wait(done + 8 * (n % kDone), n / kDone & 1, 46))) {
                     alive = false;
                     break;
                 }
                 tc_fence_after();
-                const uint32_t from = tmem + ((uint32_t)(32 * (dw & 3)) << 16) + 128 * s + half * cols;
+                const uint32_t from = tmem + ((uint32_t)(32 * (dw & 3)) << 16) + sum_cols * s + half * cols;
                 const float sw = s_w[n % kScaleRing][row];
-                const float* sx = &s_x[n % kScaleRing][half * cols];
+                const float* sx = &s_x[n % kXRing][half * cols];
                 const uint64_t sw2 = pack2(sw, sw);
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
@@ -492,19 +494,19 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                 todo = __shfl_sync(0xffffffffu, todo, 0);
                 const uint32_t plane = (uint32_t)__shfl_sync(0xffffffffu, (count + 31) / 32, 0) * 4096;
                 for (; todo > 0; --todo, ++n) {
-                    const uint32_t s = n & 1, o = n % kOperands;
+                    const uint32_t s = n & (sums - 1), o = n % kOperands;
                     // mostly all three have come, and are looked at together
                     const bool x_here = mbar_try_wait(b_full + 8 * k, k_phase),
-                               sum_free = mbar_try_wait(d_free + 8 * s, (n / 2 & 1) ^ 1),
+                               sum_free = mbar_try_wait(d_free + 8 * s, (n >> sum_shift & 1) ^ 1),
                                w_here = mbar_try_wait(a_full + 8 * o, n / kOperands & 1);
                     if (!__all_sync(0xffffffffu, (x_here || wait(b_full + 8 * k, k_phase, 47)) &&
-                                                     (sum_free || wait(d_free + 8 * s, (n / 2 & 1) ^ 1, 48)) &&
+                                                     (sum_free || wait(d_free + 8 * s, (n >> sum_shift & 1) ^ 1, 48)) &&
                                                      (w_here || wait(a_full + 8 * o, n / kOperands & 1, 49)))) {
                         alive = false;
                         break;
                     }
                     tc_fence_after();
-                    const uint32_t at = b_ring + k * b_bytes, hi = tmem + 256 + 64 * o, lo = hi + 32, d = tmem + 128 * s;
+                    const uint32_t at = b_ring + k * b_bytes, hi = tmem + 256 + 64 * o, lo = hi + 32, d = tmem + sum_cols * s;
                     const uint64_t xhi = sw128_desc(at), xlo = sw128_desc(at + plane);
                     if (elect_one()) {
 #pragma unroll
@@ -541,7 +543,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                     const uint32_t at = b_ring + k * b_bytes, bar = b_full + 8 * k;
                     if (elect_one()) {
                         mbar_arrive_expect_tx(bar, boxes * (8192 + 128));
-                        bulk_g2s(smem_u32(s_x[n % kScaleRing]), a.xs + (size_t)g * a.xs_pitch + first, boxes * 128, bar);
+                        bulk_g2s(smem_u32(s_x[n % kXRing]), a.xs + (size_t)g * a.xs_pitch + first, boxes * 128, bar);
                         tma_load_3d(at, &maps.x[boxes - 1], 0, first, 2 * g, bar);
                     }
                     __syncwarp();
@@ -652,7 +654,7 @@ cudaError_t launch_one(ImmaArgs a, int grid, int smem_per_sm, cudaStream_t strea
     auto k = imma_many_kernel<F, MODE, ALN>;
     const int xrows = (a.seg_cap + 31) / 32 * 32, stage = 256 * xrows;
     // the system's 1 KB per CTA, the static part (up to 1 KB besides the scales), alignment, barriers
-    const int fixed = 1024 + kScaleRing * 2 * kUnitRows * 4 + 1024 + 1024 + 512 + (MODE == kPair ? 32 * kXchPitch * 4 : 0);
+    const int fixed = 1024 + (kScaleRing * kUnitRows + kXRing * 128) * 4 + 1024 + 1024 + 512 + (MODE == kPair ? 32 * kXchPitch * 4 : 0);
     // x comes from L2, about 2 us ahead at 0.3 us a stage and 64 rows; the weights have the rest
     a.x_slots = xrows > 64 ? 3 : xrows > 32 ? 4 : kMaxBStages;
     a.slots = (smem_per_sm - fixed - a.x_slots * stage) / S::kBytes;
