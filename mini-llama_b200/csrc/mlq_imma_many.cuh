@@ -102,36 +102,33 @@ struct Block {
     uint32_t qs[W], dm;
 };
 
-// Block h of pair j of a round; at: the lane's row in the slot (unaligned: its first byte).
-template <int F, bool ALN, int J>
-__device__ __forceinline__ void load_block(uint32_t at, int h, Block<F>& b, uint32_t& other) {
+// Block h of pair j of a round, and the d (q4_1: d, m) of the pair's other one;
+// at: the lane's row in the slot (unaligned: its first byte).
+template <int F, bool ALN>
+__device__ __forceinline__ void load_block(uint32_t at, int j, int h, Block<F>& b, uint32_t& other) {
     constexpr int W = Block<F>::W, BB = F == kQ8_0 ? 34 : F == kQ4_0 ? 18 : 20;
     if constexpr (ALN) {
-        // the 16-byte windows that hold it
-        constexpr int N = W / 4 + 1;
-        const uint32_t pair = at + (F == kQ4_1 ? (J >> 1) * kUnitRows * 80 + (J & 1) * 32 : J * 16 * W / 2);
-        uint32_t w[4 * N];
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const uint4 q = lds_u4(pair + h * 4 * W + 16 * i);
-            w[4 * i] = q.x, w[4 * i + 1] = q.y, w[4 * i + 2] = q.z, w[4 * i + 3] = q.w;
-        }
+        const uint32_t pair = at + (F == kQ4_1 ? (j >> 1) * kUnitRows * 80 + (j & 1) * 40 : j * 2 * BB);
         if constexpr (F == kQ4_1) {
-            constexpr int s = 2 * (J & 1);
-            b.dm = h ? w[s + 1] : w[s];
+            const uint32_t from = pair + BB * h;
+            b.dm = lds_u32(from);
 #pragma unroll
-            for (int k = 0; k < W; ++k) b.qs[k] = h ? w[s + 2 + k] : w[s + 1 + k];
-            other = lds_u32(pair + 8 * (J & 1) + 20 * (1 - h));
+            for (int k = 0; k < W; ++k) b.qs[k] = lds_u32(from + 4 + 4 * k);
+            other = lds_u32(pair + BB * (1 - h));
         } else {
-            // starts at word J of the windows, for h = 1 two bytes later
-            b.dm = (w[J] >> (16 * h)) & 0xffffu;
+            // starts at a word, for h = 1 two bytes later
+            const uint32_t from = pair + (BB - 2) * h;
+            uint32_t w[W + 1];
 #pragma unroll
-            for (int k = 0; k < W; ++k) b.qs[k] = __funnelshift_rc(w[J + k], w[J + k + 1], 16 + 16 * h);
-            other = lds_u16(pair + 4 * J + BB * (1 - h));
+            for (int k = 0; k <= W; ++k) w[k] = lds_u32(from + 4 * k);
+            b.dm = (w[0] >> (16 * h)) & 0xffffu;
+#pragma unroll
+            for (int k = 0; k < W; ++k) b.qs[k] = __funnelshift_rc(w[k], w[k + 1], 16 + 16 * h);
+            other = lds_u16(pair + BB * (1 - h));
         }
     } else {
         auto word = [](uint32_t at, uint32_t lo, uint32_t hi) { return __funnelshift_r(lo, hi, 8 * (at & 3)); };
-        const uint32_t from = at + (2 * J + h) * BB, to = at + (2 * J + 1 - h) * BB;
+        const uint32_t from = at + (2 * j + h) * BB, to = at + (2 * j + 1 - h) * BB;
         b.dm = word(from, lds_u32(from & ~3u), lds_u32((from & ~3u) + 4));
         other = word(to, lds_u32(to & ~3u), lds_u32((to & ~3u) + 4));
         const uint32_t qs = from + (F == kQ4_1 ? 4 : 2);
@@ -303,13 +300,12 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                 uint32_t at = raw_ring + slot * S::kBytes + row * S::kPitch;
                 if constexpr (!ALN) at += (window + (uint32_t)c * (S::kChunk & 15)) & 15;
                 const int valid = a.bpr - c * kChunkBlocks;
-                static_for<4>([&](auto jc) {
-                    constexpr int J = decltype(jc)::value;
-                    if (2 * J >= valid || !alive) return;
+#pragma unroll 1
+                for (int j = 0; j < 4 && 2 * j < valid; ++j) {
                     Block<F> b;
                     uint32_t other;
-                    load_block<F, ALN, J>(at, h, b, other);
-                    if (2 * J + 1 >= valid) {  // the row ends with the first block of this pair
+                    load_block<F, ALN>(at, j, h, b, other);
+                    if (2 * j + 1 >= valid) {  // the row ends with the first block of this pair
                         if (h == 0)
                             other = 0;
                         else
@@ -323,7 +319,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                     const int k = n % kOperands;
                     if (!__all_sync(0xffffffffu, n >= kOperands ? wait(done + 8 * ((n - kOperands) % kDone), (n - kOperands) / kDone & 1, 45) : true)) {
                         alive = false;
-                        return;
+                        break;
                     }
                     tc_fence_after();
                     const uint32_t to = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + 256 + 64 * k + 16 * h;
@@ -331,7 +327,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                     tmem_st16(to + 32, lo);
                     if (h == 0) s_w[n % kScaleRing][row] = inverse;
                     ++n, behind = true;
-                });
+                }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(raw_empty + 8 * slot);
                 if (++slot == a.slots) slot = 0, slot_phase ^= 1;
