@@ -188,7 +188,7 @@ double deal_cost(long long units, long long per, double end, int teams) {
 
 // 16-row strips of a unit (at least `least`): the K axis is then split in 8 /
 // strips parts.  all_segs: a unit meets every segment.
-int choose_strips(int out, int bpr, int nseg, bool all_segs, int sm_count, int least) {
+int choose_strips(int out, int bpr, int nseg, bool all_segs, int sm_count, int least, double* cost = nullptr) {
     const int steps = (bpr + kChunkBlocks - 1) / kChunkBlocks;
     int best = kImmaWarps;
     double best_cost = 1e300;
@@ -199,7 +199,18 @@ int choose_strips(int out, int bpr, int nseg, bool all_segs, int sm_count, int l
                                   : deal_cost(tiles * nseg, per, 0.7, 2 * sm_count);
         if (c < best_cost) best_cost = c, best = n;
     }
+    if (cost) *cost = best_cost;
     return best;
+}
+
+// Rows of x of a segment of a linear that goes by digits: 2 while that ends sooner by the count of rounds, mostly for
+// small matrices (4 rows of q4_0, 2048 x 2048: 8.3 us with one segment and 5.5 with two; 4096 x 4096: 14.2 and 8.5).
+int linear_cap(int rows, int out, int bpr, int sm_count) {
+    if (rows < 3) return rows;
+    double two, four;
+    choose_strips(out, bpr, (rows + 1) / 2, false, sm_count, 2, &two);
+    choose_strips(out, bpr, (rows + kFewRows - 1) / kFewRows, false, sm_count, kFewRows, &four);
+    return two < four ? 2 : kFewRows;
 }
 
 struct Carve {
@@ -219,10 +230,15 @@ constexpr int kMaxPairs = 8192;           // pairs of one pass at most
 constexpr size_t kMaxSliced = 1u << 30;   // sliced bytes of one pass at most (offsets are 32 bits)
 constexpr size_t kMaxParts = 1u << 30;    // bytes of the pairs' outputs of one pass at most
 constexpr int kMaxPassRows = 16384;       // rows of one pass of a linear at most
+// Rows of a linear that go by digits, in segments of 4 whose weights come from L2 after the first.  3584 x 18944, us by
+// digits and by halves: q4_0 5 rows 27 and 39, 12 rows 36 and 41, 16 rows 43 and 41; q8_0 31 and 42, 41 and 44, 50 and 45.
+constexpr int kLinearFewRows = 12;
 constexpr int kCombineRows = 32;          // more rows: the sum over slots is a launch of its own
 
-// Rows of x of a segment at most in the form of few rows.
-int few_cap(int rows) { return rows < 3 ? rows : kFewRows; }
+// Rows of x of a segment at most in the form of few rows.  A stage holds 8
+// records of x, so a unit of fewer rows may have its K axis split further: with about a
+// row per expert, 2 (an expert with more has several segments).
+int few_cap(int rows, int pairs, int n_experts) { return rows < 3 ? rows : pairs <= n_experts ? 2 : kFewRows; }
 
 // And in that of many: half as many again as an expert has on average, so
 // that most experts are one segment.
@@ -313,9 +329,9 @@ void set_halves(ImmaArgs& a, const HalvesArgs& h) {
 size_t epilogue_workspace_bytes(int in, int rows) {
     const int n = linear_pass_rows(in, rows);
     // more rows never need less
-    const size_t few = sliced_bytes(n < kFewRows ? n : kFewRows, padded_blocks((in + kQK - 1) / kQK)) +
-                       split_bytes(true, n < kFewRows ? n : kFewRows);
-    const size_t many = n <= kFewRows ? 0 : halves_bytes(n, groups_of(in)) + split_bytes(false, n);
+    const int few_rows = n < kLinearFewRows ? n : kLinearFewRows;
+    const size_t few = sliced_bytes(few_rows, padded_blocks((in + kQK - 1) / kQK)) + split_bytes(true, few_rows);
+    const size_t many = n <= kLinearFewRows ? 0 : halves_bytes(n, groups_of(in)) + split_bytes(false, n);
     return few > many ? few : many;
 }
 
@@ -330,7 +346,7 @@ cudaError_t launch_linear_epilogue(int fmt, const uint8_t* w, int out, int in, c
         PrepArgs p{};
         p.x = x + (long long)r0 * in;
         p.rows = n, p.in = in, p.bpr = bpr, p.bprp = bprp, p.fmt = fmt;
-        const bool few = n <= kFewRows;
+        const bool few = n <= kLinearFewRows;
         HalvesArgs hv{};
         float* split;
         cudaError_t e;
@@ -350,7 +366,7 @@ cudaError_t launch_linear_epilogue(int fmt, const uint8_t* w, int out, int in, c
         a.w[0] = w;
         a.total_rows = out, a.out = out, a.bpr = bpr, a.bprp = bprp;
         const int parts = (n + kSegTokens - 1) / kSegTokens;
-        a.seg_cap = few ? few_cap(n) : ((n + parts - 1) / parts + 15) / 16 * 16;
+        a.seg_cap = few ? linear_cap(n, out, bpr, sm_count) : ((n + parts - 1) / parts + 15) / 16 * 16;
         const int nseg = (n + a.seg_cap - 1) / a.seg_cap;
         a.strips = few ? choose_strips(out, bpr, nseg, false, sm_count, a.seg_cap) : 8;
         a.tiles = (out + 16 * a.strips - 1) / (16 * a.strips);
@@ -379,7 +395,7 @@ size_t experts_workspace_bytes(const MoeShape& s, int rows, int top_k) {
     auto bytes = [&](int n) {
         const int pairs = n * top_k;
         const bool few = few_rows(pairs, s.n_experts);
-        const size_t lists = 256 + align256((size_t)max_segments(pairs, s.n_experts, few ? few_cap(n) : 1) * sizeof(Segment));
+        const size_t lists = 256 + align256((size_t)max_segments(pairs, s.n_experts, few ? few_cap(n, pairs, s.n_experts) : 1) * sizeof(Segment));
         if (few)
             return lists + align256((size_t)pairs * sizeof(int)) + sliced_bytes(n, bprp) + sliced_bytes(pairs, hp) +
                    (n <= kCombineRows ? 0 : align256((size_t)pairs * s.out * sizeof(float))) + split_bytes(few, n);
@@ -404,7 +420,7 @@ cudaError_t launch_experts(const MoeShape& s, const uint8_t* gate, const uint8_t
     for (int r0 = 0; r0 < rows; r0 += pass) {
         const int n = rows - r0 < pass ? rows - r0 : pass, pairs = n * top_k;
         const bool few = few_rows(pairs, s.n_experts);
-        const int cap = few ? few_cap(n) : many_cap(pairs, s.n_experts);
+        const int cap = few ? few_cap(n, pairs, s.n_experts) : many_cap(pairs, s.n_experts);
         const bool at_once = few && n <= kCombineRows;  // the down product meets all segments of a tile in one unit
         const int nseg_max = max_segments(pairs, s.n_experts, cap);
         const int nseg_likely = pairs < s.n_experts ? pairs : nseg_max;
