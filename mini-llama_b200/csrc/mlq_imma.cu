@@ -13,14 +13,39 @@
 namespace mlq {
 namespace {
 
-// y from the parts of every pair, for calls with many rows.
-__global__ void combine_kernel(const ImmaArgs a) {
+// y from the parts of every pair, for calls with many rows; V consecutive
+// values per thread.
+template <int V>
+__global__ void __launch_bounds__(256) combine_kernel(const ImmaArgs a) {
     launch_dependents();
     grid_dependency_wait();
-    const size_t n = (size_t)a.rows * a.out;
-    for (size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (size_t)gridDim.x * blockDim.x)
-        a.y[i] = combine(a, (int)(i / a.out), (int)(i % a.out));
+    const int per = a.out / V;
+    const size_t n = (size_t)a.rows * per;
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) {
+        const int r = (int)(i / per), o = (int)(i % per) * V;
+        if constexpr (V == 1) {
+            a.y[i] = combine(a, r, o);
+        } else {
+            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+            for (int j = 0; j < a.top_k; ++j) {  // as combine() does it
+                const int p = r * a.top_k + j, e = a.ids[p];
+                if (e < 0 || e >= a.n_experts) continue;
+                const float w = a.weights[p];
+                const float4 q = __ldcg(reinterpret_cast<const float4*>(a.part + (size_t)p * a.out + o));
+                v.x = fmaf(w, q.x, v.x), v.y = fmaf(w, q.y, v.y), v.z = fmaf(w, q.z, v.z), v.w = fmaf(w, q.w, v.w);
+            }
+            const size_t at = (size_t)r * a.out + o;
+            if (a.residual) {
+                const float4 q = *reinterpret_cast<const float4*>(a.residual + at);
+                v.x = q.x + v.x, v.y = q.y + v.y, v.z = q.z + v.z, v.w = q.w + v.w;
+            }
+            *reinterpret_cast<float4*>(a.y + at) = v;
+        }
+    }
 }
+
+constexpr int kMaxPairs = 8192;  // pairs of one pass at most
 
 struct PrepArgs {
     const float* x;
@@ -31,10 +56,11 @@ struct PrepArgs {
     // experts only (ids not null)
     const int32_t* ids;
     int pairs, n_experts;
-    int positions;    // many rows: of order, an expert's first one a multiple of 8 (the others: -1); else 0
+    int positions;    // many rows: of order, an expert's first one a multiple of 8; else 0
     Segment* segs;
     int* nseg;
-    int* order;
+    int* order;       // position -> pair
+    int* place;       // many rows: pair -> position, -1: no expert
     // padding blocks of the sliced h
     uint8_t* h;
     int h_bpr, h_bprp;
@@ -54,9 +80,9 @@ __global__ void __launch_bounds__(256) prep_kernel(const PrepArgs a) {
             __shared__ int cnt[MLQ_MOE_MAX_EXPERTS];
             __shared__ int wsum[2][8];
             __shared__ unsigned char in_warp[8][MLQ_MOE_MAX_EXPERTS];
+            __shared__ short s_ids[kMaxPairs];  // -1: none of the experts
             for (int e = threadIdx.x; e < a.n_experts; e += 256) cnt[e] = 0;
             const int pad = a.h ? a.h_bprp - a.h_bpr : 0;
-            for (int i = threadIdx.x; i < a.positions; i += 256) a.order[i] = -1;
             const int align = a.positions ? 8 : 1;
             for (int i = threadIdx.x; i < a.pairs * pad; i += 256) {
                 const int b = a.h_bpr + i % pad;
@@ -65,9 +91,12 @@ __global__ void __launch_bounds__(256) prep_kernel(const PrepArgs a) {
                 at[0] = at[kChunkBlocks] = 0.0f;
             }
             __syncthreads();
+#pragma unroll 8
             for (int p = threadIdx.x; p < a.pairs; p += 256) {
                 const int e = a.ids[p];
-                if (e >= 0 && e < a.n_experts) atomicAdd(&cnt[e], 1);
+                const bool is = e >= 0 && e < a.n_experts;
+                s_ids[p] = (short)(is ? e : -1);
+                if (is) atomicAdd(&cnt[e], 1);
             }
             __syncthreads();
             // each thread: 4 consecutive experts; exclusive sums of pairs and of segments
@@ -106,8 +135,7 @@ __global__ void __launch_bounds__(256) prep_kernel(const PrepArgs a) {
             __syncthreads();
             for (int p0 = 0; p0 < a.pairs; p0 += 256) {
                 const int p = p0 + threadIdx.x;
-                int e = p < a.pairs ? a.ids[p] : -1;
-                if (e >= a.n_experts) e = -1;
+                const int e = p < a.pairs ? s_ids[p] : -1;
                 const unsigned same = __match_any_sync(0xffffffffu, e);
                 const int rank = __popc(same & ((1u << lane) - 1));
                 if (e >= 0 && rank == 0) in_warp[warp][e] = (unsigned char)__popc(same);
@@ -116,6 +144,9 @@ __global__ void __launch_bounds__(256) prep_kernel(const PrepArgs a) {
                     int at = cnt[e] + rank;
                     for (int w = 0; w < warp; ++w) at += in_warp[w][e];
                     a.order[at] = p;
+                    if (a.place) a.place[p] = at;
+                } else if (a.place && p < a.pairs) {
+                    a.place[p] = -1;
                 }
                 __syncthreads();
                 if (e >= 0 && rank == 0) {
@@ -141,34 +172,41 @@ __global__ void __launch_bounds__(256) prep_kernel(const PrepArgs a) {
 
 struct HalvesArgs {
     const float* x;
-    const int* order;  // position -> pair; null: positions are rows
-    int positions, top_k, in, groups, fmt;
+    const int* place;  // [rows][top_k] positions of a row's pairs, -1: none; null: rows are positions
+    int rows, positions, top_k, in, groups, fmt;
     uint8_t* halves;   // [position][groups][hi, lo][64]
     float* scales;     // [groups][pitch]
     int pitch;
     unsigned int* split_done;
 };
 
-// x by position for many rows: a warp per 64 values.
+// x by position for many rows: a warp per 64 values, sliced once for all of
+// the row's experts.
 __global__ void __launch_bounds__(256) halves_kernel(const HalvesArgs a) {
     launch_dependents();
     grid_dependency_wait();
     const int lane = threadIdx.x & 31;
     if (blockIdx.x == 0)
         for (int i = threadIdx.x; i < 2 * kMaxTeams; i += 256) a.split_done[i] = 0;
-    const long long n = (long long)a.positions * a.groups, step = (long long)gridDim.x * 8;
+    const long long n = (long long)a.rows * a.groups, step = (long long)gridDim.x * 8;
     for (long long i = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); i < n; i += step) {
-        const int pos = (int)(i / a.groups), g = (int)(i % a.groups);
-        const int pair = a.order ? a.order[pos] : pos;
-        if (pair < 0) continue;
-        const float* x = a.x + (long long)(a.order ? pair / a.top_k : pair) * a.in;
+        const int r = (int)(i / a.groups), g = (int)(i % a.groups);
+        const float* x = a.x + (long long)r * a.in;
         float v[2];
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
             const int p = 2 * lane + k, at = 64 * g + (p & 32) + tile_element(a.fmt, p & 31);
             v[k] = at < a.in ? x[at] : 0.0f;
         }
-        slice_64(v[0], v[1], a.halves + (size_t)i * 256, a.scales + (size_t)g * a.pitch + pos, lane);
+        const Sliced64 s = slice_64(v[0], v[1]);
+        if (!a.place) {
+            s.store(a.halves + (size_t)i * 256, a.scales + (size_t)g * a.pitch + r, lane);
+            continue;
+        }
+        for (int j = 0; j < a.top_k; ++j) {
+            const int pos = a.place[r * a.top_k + j];
+            if (pos >= 0) s.store(a.halves + ((size_t)pos * a.groups + g) * 256, a.scales + (size_t)g * a.pitch + pos, lane);
+        }
     }
 }
 
@@ -226,7 +264,6 @@ struct Carve {
 
 size_t sliced_bytes(size_t rows, int bprp) { return align256(rows * (bprp / kChunkBlocks) * kRecordBytes); }
 
-constexpr int kMaxPairs = 8192;           // pairs of one pass at most
 constexpr size_t kMaxSliced = 1u << 30;   // sliced bytes of one pass at most (offsets are 32 bits)
 constexpr size_t kMaxParts = 1u << 30;    // bytes of the pairs' outputs of one pass at most
 constexpr int kMaxPassRows = 16384;       // rows of one pass of a linear at most
@@ -310,10 +347,10 @@ int prep_ctas(long long blocks, int sm_count) {
     return (int)(n < 8LL * sm_count ? n : 8LL * sm_count);
 }
 
-// x of `positions` rows (or positions of `order`, to be set) as halves.
-HalvesArgs halves_args(Carve& c, const float* x, int positions, int in, int fmt) {
+// `rows` rows of x (null: made by a product) as halves in `positions` places.
+HalvesArgs halves_args(Carve& c, const float* x, int rows, int positions, int in, int fmt) {
     HalvesArgs h{};
-    h.x = x, h.positions = positions, h.in = in, h.fmt = fmt;
+    h.x = x, h.rows = rows, h.positions = positions, h.in = in, h.fmt = fmt;
     h.groups = groups_of(in), h.pitch = scale_pitch(positions);
     h.halves = c.take<uint8_t>((size_t)positions * h.groups * 256);
     h.scales = c.take<float>((size_t)h.groups * h.pitch);
@@ -356,7 +393,7 @@ cudaError_t launch_linear_epilogue(int fmt, const uint8_t* w, int out, int in, c
             p.split_done = c.take<unsigned int>(2 * kMaxTeams);
             e = launch_pdl(prep_kernel, prep_ctas((long long)n * bprp, sm_count), 256, 0, stream, p);
         } else {
-            hv = halves_args(c, p.x, n, in, fmt);
+            hv = halves_args(c, p.x, n, n, in, fmt);
             split = c.take<float>(split_floats(few, n, kImmaWarps) * split_count(few));
             p.split_done = hv.split_done = c.take<unsigned int>(2 * kMaxTeams);
             e = launch_pdl(halves_kernel, prep_ctas((long long)n * hv.groups, sm_count), 256, 0, stream, hv);
@@ -400,7 +437,7 @@ size_t experts_workspace_bytes(const MoeShape& s, int rows, int top_k) {
             return lists + align256((size_t)pairs * sizeof(int)) + sliced_bytes(n, bprp) + sliced_bytes(pairs, hp) +
                    (n <= kCombineRows ? 0 : align256((size_t)pairs * s.out * sizeof(float))) + split_bytes(few, n);
         const int positions = many_positions(pairs, s.n_experts);
-        return lists + align256((size_t)positions * sizeof(int)) + halves_bytes(positions, groups_of(s.in)) +
+        return lists + align256((size_t)positions * sizeof(int)) + align256((size_t)pairs * sizeof(int)) + halves_bytes(positions, groups_of(s.in)) +
                halves_bytes(positions, groups_of(s.hidden)) + align256((size_t)pairs * s.out * sizeof(float)) +
                split_bytes(few, n);
     };
@@ -444,16 +481,17 @@ cudaError_t launch_experts(const MoeShape& s, const uint8_t* gate, const uint8_t
             p.h = c.take_sliced(pairs, hp);
             p.h_bpr = hb, p.h_bprp = hp;
         } else {
-            hx = halves_args(c, p.x, p.positions, s.in, s.fmt);
-            hh = halves_args(c, nullptr, p.positions, s.hidden, s.fmt_down);
-            hx.order = p.order, hx.top_k = top_k;
+            p.place = c.take<int>(pairs);
+            hx = halves_args(c, p.x, n, p.positions, s.in, s.fmt);
+            hh = halves_args(c, nullptr, n, p.positions, s.hidden, s.fmt_down);
+            hx.place = p.place, hx.top_k = top_k;
         }
         float* part = c.take<float>(at_once ? 0 : (size_t)pairs * s.out);
         float* split = c.take<float>(split_floats(few, n, kImmaWarps) * split_count(few));
         p.split_done = hx.split_done = c.take<unsigned int>(2 * kMaxTeams);
         cudaError_t e = launch_pdl(prep_kernel, few ? 1 + prep_ctas((long long)n * bprp, sm_count) : 1, 256, 0, stream, p);
         if (e == cudaSuccess && !few)
-            e = launch_pdl(halves_kernel, prep_ctas((long long)pairs * hx.groups, sm_count), 256, 0, stream, hx);
+            e = launch_pdl(halves_kernel, prep_ctas((long long)n * hx.groups, sm_count), 256, 0, stream, hx);
         if (e != cudaSuccess) return e;
 
         ImmaArgs a{};
@@ -497,8 +535,10 @@ cudaError_t launch_experts(const MoeShape& s, const uint8_t* gate, const uint8_t
         e = (few ? launch_few_down : launch_many_down)(s.fmt_down, d, sm_count, smem_per_sm, (long long)nseg_max * tiles, stream);
         if (e != cudaSuccess) return e;
         if (d.part) {
-            const long long vals = (long long)n * s.out;
-            e = launch_pdl(combine_kernel, (int)((vals + 255) / 256 < 16 * sm_count ? (vals + 255) / 256 : 16 * sm_count),
+            const bool four = s.out % 4 == 0 && reinterpret_cast<uintptr_t>(d.y) % 16 == 0 &&
+                              reinterpret_cast<uintptr_t>(d.residual) % 16 == 0;
+            const long long ctas = ((long long)n * s.out / (four ? 4 : 1) + 255) / 256;
+            e = launch_pdl(four ? combine_kernel<4> : combine_kernel<1>, (int)(ctas < 16 * sm_count ? ctas : 16 * sm_count),
                            256, 0, stream, d);
             if (e != cudaSuccess) return e;
         }

@@ -148,18 +148,31 @@ __device__ __forceinline__ void slice_digits(float x, float weight, uint8_t* row
     }
 }
 
-// Slices 64 values (positions 2 lane and 2 lane + 1) into fp16 hi and lo with
-// one power-of-two scale; to: 64 hi, then 64 lo.
-__device__ __forceinline__ void slice_64(float v0, float v1, uint8_t* to, float* scale, int lane) {
-    const float m0 = block_amax(v0), m1 = block_amax(v1);
-    const bool bad = !(m0 == m0) || !(m1 == m1);
-    const uint32_t s = block_scale(bad ? 0.0f : fmaxf(m0, m1), 14, 32767.0f);
+// 64 values (positions 2 lane and 2 lane + 1) as fp16 hi and lo with one
+// power-of-two scale.
+struct Sliced64 {
+    __half2 hi, lo;
+    float scale;
+    // to: 64 hi, then 64 lo
+    __device__ __forceinline__ void store(uint8_t* to, float* to_scale, int lane) const {
+        reinterpret_cast<__half2*>(to)[lane] = hi;
+        reinterpret_cast<__half2*>(to + 128)[lane] = lo;
+        if (lane == 0) *to_scale = scale;
+    }
+};
+
+__device__ __forceinline__ Sliced64 slice_64(float v0, float v1) {
+    const float most = fmaxf(fabsf(v0), fabsf(v1));
+    const float m = block_amax(v0 == v0 && v1 == v1 ? most : __uint_as_float(0x7fc00000u));
+    const bool bad = !(m == m);
+    const uint32_t s = block_scale(bad ? 0.0f : m, 14, 32767.0f);
     const float q0 = bad ? 0.0f : v0 * __uint_as_float(s), q1 = bad ? 0.0f : v1 * __uint_as_float(s);
-    const __half2 hi = __floats2half2_rn(q0, q1);
-    const float2 h = __half22float2(hi);
-    reinterpret_cast<__half2*>(to)[lane] = hi;
-    reinterpret_cast<__half2*>(to + 128)[lane] = __floats2half2_rn(q0 - h.x, q1 - h.y);
-    if (lane == 0) *scale = bad ? __uint_as_float(0x7fc00000u) : inverse_scale(s);
+    Sliced64 r;
+    r.hi = __floats2half2_rn(q0, q1);
+    const float2 h = __half22float2(r.hi);
+    r.lo = __floats2half2_rn(q0 - h.x, q1 - h.y);
+    r.scale = bad ? __uint_as_float(0x7fc00000u) : inverse_scale(s);
+    return r;
 }
 
 // D = A B for 16 rows x 32 codes, signed (q8_0) or unsigned (q4), and digits.

@@ -447,8 +447,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                                         : 0.0f;
                         }
                         const size_t pos = first + tok;
-                        slice_64(hv[0], hv[1], a.h + (pos * a.next_groups + tile) * 256, a.hs + (size_t)tile * a.hs_pitch + pos,
-                                 lane);
+                        slice_64(hv[0], hv[1])
+                            .store(a.h + (pos * a.next_groups + tile) * 256, a.hs + (size_t)tile * a.hs_pitch + pos, lane);
                     }
                 }
             } else {
