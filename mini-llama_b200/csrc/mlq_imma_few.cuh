@@ -25,7 +25,7 @@ namespace {
 template <int F, int NT>
 struct FewRows {
     uint32_t xo[NT], so[NT];  // a lane's digits and scales in the step's records
-    float acc[NT][2], accm[F == kQ4_1 ? NT : 1][2];
+    float acc[NT][2];
 
     __device__ __forceinline__ void init(int count, int lane) {
         const int g = lane >> 2, t = lane & 3;
@@ -36,7 +36,6 @@ struct FewRows {
             xo[i] = (r < count ? r : 0) * kRecordBytes + (g & 3) * 64 + t * 16;
             so[i] = (rs < count ? rs : 0) * kRecordBytes + kRecordScales;
             acc[i][0] = acc[i][1] = 0.0f;
-            if (F == kQ4_1) accm[i][0] = accm[i][1] = 0.0f;
         }
     }
 
@@ -44,7 +43,7 @@ struct FewRows {
     template <bool ALN>
     __device__ __forceinline__ void step(uint32_t x, int valid, uint32_t r0, uint32_t r1, int lane) {
         const RowBase rows = row_base(r0, r1, lane & 3);
-        const float offset = lane & 1 ? 0.0f : -8.0f * 16.0f / 65536.0f;
+        const float offset = lane & 1 ? 0.0f : (F == kQ4_0 ? -8.0f : 1.0f) * 16.0f / 65536.0f;
         static_for<kChunkBlocks / 2>([&](auto pc) {
             constexpr int p = decltype(pc)::value;
             if (!ALN && 2 * p >= valid) return;
@@ -72,10 +71,13 @@ struct FewRows {
                     const float v[2] = {(float)(c[0] * 256 + c[1]), (float)(c[2] * 256 + c[3])};
 #pragma unroll
                     for (int q = 0; q < 2; ++q) {
-                        // q4_0: sum of (c - 8) x, in the unit of digits 3 and 2 (see store); lanes of digits 1, 0 take none
+                        // q4_0: sum of (c - 8) x, in the unit of digits 3 and 2 (see store); lanes of digits 1, 0 take none.
+                        // q4_1: the block's d c x and m x cancel each other for the most part, so they meet here
                         const float u = F == kQ4_0 ? fmaf(v[q], sx, mx * offset) : v[q] * sx;
-                        acc[i][q] = fmaf(A[o].d[q], u, acc[i][q]);
-                        if (F == kQ4_1) accm[i][q] = fmaf(A[o].m[q], mx, accm[i][q]);
+                        if (F == kQ4_1)
+                            acc[i][q] += fmaf(A[o].d[q], u, A[o].m[q] * (mx * offset));
+                        else
+                            acc[i][q] = fmaf(A[o].d[q], u, acc[i][q]);
                     }
                 }
             }
@@ -93,7 +95,6 @@ struct FewRows {
             for (int q = 0; q < 2; ++q) {
                 float v = acc[i][q] * f;
                 v += __shfl_xor_sync(0xffffffffu, v, 1);
-                if (F == kQ4_1) v += accm[i][q];
                 if (!(t & 1)) red[(2 * i + (t >> 1)) * 16 + 8 * q + (lane >> 2)] = v;
             }
     }
