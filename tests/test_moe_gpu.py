@@ -83,6 +83,19 @@ CASES = [
 ]
 
 
+# more than 5 rows per expert on average: the form of many rows.  Segments of up to 128 rows and experts with more,
+# hidden widths and outputs that end inside a tile of 64 and of 128, an odd number of blocks, rows that are not aligned, K
+# axes that several CTAs share, one row above and exactly at the border to the form of few rows, two passes
+CASES += [
+    ("q8_0", "q8_0", 70, 256, 192, 384, 2, 1), ("q4_0", "q4_0", 300, 512, 96, 130, 2, 2),
+    ("q4_1", "q8_0", 129, 2080, 65, 256, 1, 1), ("q8_0", "q4_1", 64, 3104, 128, 129, 4, 2),
+    ("q4_0", "q8_0", 25, 4096, 64, 64, 4, 1), ("q8_0", "q4_0", 513, 64, 2048, 1024, 3, 1),
+    ("q4_1", "q4_1", 1000, 96, 33, 40, 16, 3), ("q4_0", "q4_1", 25, 288, 160, 96, 5, 1),
+    ("q4_0", "q4_1", 26, 288, 160, 96, 5, 1), ("q4_0", "q8_0", 3000, 64, 64, 32, 8, 3),
+    ("q8_0", "q8_0", 128, 1024, 64, 1, 1, 1), ("q4_0", "q4_0", 2000, 1, 1, 1, 2, 1),
+]
+
+
 @pytest.mark.parametrize("c", CASES, ids=lambda c: "-".join(map(str, c)))
 def test_experts(pkg, c):
     t = Case(pkg, *c, residual=c[2] % 2 == 1)
@@ -93,8 +106,35 @@ def test_experts(pkg, c):
 @pytest.mark.parametrize("offset", [2, 1, 16, 30])
 def test_experts_at_any_address(pkg, fmt, offset):
     """Stacks that start inside a 16-byte window, at even and odd addresses."""
-    t = Case(pkg, fmt, fmt, 3, 256, 288, 256, 4, 2, offset=offset)
-    check(t.run(), *t.want(), pkg)
+    for rows, n in ((3, 4), (48, 2)):
+        t = Case(pkg, fmt, fmt, rows, 256, 288, 256, n, 2, offset=offset)
+        check(t.run(), *t.want(), pkg)
+
+
+def test_many_rows_guarded_replayed_and_not_finite(pkg):
+    """A workspace of the stated size, full of NaN bits, with nothing written
+    behind it; the same bits from a replayed graph; a NaN and an infinity stay
+    in their rows."""
+    t = Case(pkg, "q4_0", "q8_0", 150, 544, 224, 200, 3, 2)
+    size = t.mlq.experts_workspace_bytes(t.experts, 150, 2)
+    ws = torch.full((size + 512,), 255, dtype=torch.uint8, device="cuda")
+    x, ids, w, res = dev(t.x), dev(t.ids), dev(t.w), dev(t.res)
+    y = t.mlq.moe_experts(t.experts, x, ids, w, residual=res, workspace=ws[:size])
+    check(y, *t.want(), pkg)
+    assert (ws[size:] == 255).all()
+    z = torch.empty_like(y)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        t.mlq.moe_experts(t.experts, x, ids, w, residual=res, y=z, workspace=ws[:size])
+    for _ in range(2):
+        z.fill_(float("nan"))
+        g.replay()
+        assert torch.equal(y, z)
+    x[17, 3], x[90, 500] = float("nan"), float("inf")
+    g.replay()
+    rest = [i for i in range(150) if i not in (17, 90)]
+    assert torch.equal(y[rest], z[rest]) and z[17].isnan().all() and z[90].isnan().all()
+    assert pkg.mlq.device_error(0) == 0
 
 
 @pytest.mark.parametrize("rows", [5, 40])
@@ -563,6 +603,12 @@ LINEARS = [
     ("q4_0", 33, 512, 1, True, "gelu_tanh", False, True), ("q4_1", 301, 64, 96, True, "sigmoid", False, True),
     ("q8_0", 65, 1, 5, True, "none", False, False), ("q4_0", 1, 32, 1, False, "none", False, False),
     ("q4_1", 1, 18944, 64, False, "none", False, True), ("q8_0", 17, 272, 77, False, "relu", True, True),
+    # segments of 2 and of 4 rows, the borders between the forms and between one segment and two, K axes shared by CTAs
+    ("q4_0", 3, 2048, 512, False, "none", False, True), ("q8_0", 4, 2048, 6000, True, "silu", True, False),
+    ("q8_0", 12, 4096, 256, False, "none", True, True), ("q4_0", 12, 704, 300, True, "gelu", False, False),
+    ("q4_1", 13, 4096, 130, False, "none", True, True), ("q8_0", 40, 18944, 64, False, "none", False, True),
+    ("q4_0", 128, 1312, 256, True, "relu", False, False), ("q4_1", 129, 352, 200, False, "none", True, True),
+    ("q8_0", 1000, 2080, 40, True, "sigmoid", False, False), ("q4_0", 257, 5000, 129, False, "none", False, False),
 ]
 
 
