@@ -438,10 +438,12 @@ MLQ_API mlq_status mlq_peer_free(void* ptr);
  * after the previous kernel on the stream has completed, and may stream
  * the quantized weights before.  They can be captured into a graph.
  *
- * Arithmetic: weights are exact; each row of x (and of an expert's hidden
- * vector) is carried, per 32-value block, as 31-bit fixed point or as the sum
- * of two fp16 values (to 2^-22 of each value) against a power of two; sums
- * are integers or fp32 per block and fp32 across blocks.  Outputs are within
+ * Arithmetic: with few rows per matrix (a linear: up to 12) weights are exact and
+ * each row of x (and of an expert's hidden vector) is carried, per 32-value block,
+ * as 31-bit fixed point; sums are integers per block and fp32 across blocks.
+ * With more, values of x and weights are each the sum of two fp16 values (to
+ * 2^-22 of the value) against a power of two per 64 values; sums are the
+ * tensor cores' fp32 over 64 values and fp32 across them.  Outputs are within
  * ~1e-6 relative L2 of the 64-bit result.  A value of x that is not finite
  * makes every output that reads it NaN.  Results do not
  * depend on the other rows of the call or on their order beyond rounding,
@@ -502,7 +504,9 @@ typedef struct mlq_experts {
  * [rows][top_k].  A slot whose id is outside [0, n_experts) adds nothing (-1:
  * a padded row, or an expert that another GPU holds); a row of only such slots
  * gives y = residual (0 without one).  The same expert may appear in several
- * slots.  Up to 32 rows every chosen expert's weights are read once. */
+ * slots.  With up to 5 rows per expert on average (rows x top_k against
+ * n_experts) x goes by digits, in segments of up to 4 rows of one expert; beyond, as
+ * pairs of fp16 values, in segments of up to 128. */
 MLQ_API mlq_status mlq_moe_experts(const mlq_experts* experts, const float* x, int rows, int top_k,
                                    const int32_t* ids, const float* weights, const float* residual,
                                    float* y, void* workspace, size_t workspace_bytes,

@@ -1,16 +1,16 @@
-// mlq_imma.cuh -- quantized products on the int8 matrix instructions, shared
-// by the experts' products and the linear with an epilogue (sm_100a).
+// mlq_imma.cuh -- quantized products on the matrix instructions: the
+// arithmetic that the experts' products and the linear with an epilogue share (sm_100a).
 //
 // The mathematics.  A weight block is d * c (+ m) with integer codes c, so
 // the sum over one 32-value block is d * sum_i c_i x_i (+ m * sum_i x_i).
-// c_i is exact in 8 bits, x is cut into pieces whose products with c are
-// exact, and one fp32 fold per block applies d and the block's scale of x:
+// c_i is exact in 8 bits, and x is cut into pieces:
 //
-// * up to 4 rows of x: 4 signed base-256 digits of x_i / s, s a power of two
+// * few rows of x (segments of up to 4): 4 signed base-256 digits of x_i / s, s a power of two
 //   per 32-value block of a row (31-bit fixed point, error <= 2^-31
 //   max|x_block|).  The codes meet the digits in m16n8k32 int8 matrix
 //   instructions: one covers exactly one block of 16 weight rows, its 8 columns are
-//   the digits of 2 rows of x, and every integer sum is exact.  q8_0 codes are
+//   the digits of 2 rows of x, every integer sum is exact, and one fp32 fold per
+//   block applies d and the block's scale of x.  q8_0 codes are
 //   the operand as they are.  q4 codes are unsigned bytes, c from the low nibble
 //   and 16 c from the high one (one mask each); the values of x that meet low
 //   nibbles are carried 16-fold instead, and q4_0's offset of 8 is taken off by

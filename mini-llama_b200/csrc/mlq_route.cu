@@ -571,7 +571,12 @@ constexpr long long kDigitWork = 64ll << 20;
 
 size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 
-bool by_digits(int n_experts, int in, int rows) { return rows >= 32 && (long long)rows * n_experts * in >= kDigitWork; }
+// a product of two 31-bit values is below 2^62, in units of 2^16 2^46: the 64-bit sum takes 2^17 of them
+constexpr int kDigitFeatures = 1 << 17;
+
+bool by_digits(int n_experts, int in, int rows) {
+    return rows >= 32 && in <= kDigitFeatures && (long long)rows * n_experts * in >= kDigitWork;
+}
 
 // The digits' part of the arguments, with the arrays at `ws`; their bytes.
 size_t lay_out(RouteArgs& a, char* ws) {

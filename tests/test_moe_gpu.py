@@ -507,6 +507,16 @@ def test_route_many_rows_ties_outliers_masks(pkg, scoring):
         assert np.array_equal(ids.cpu().numpy(), want_ids) and (wt[ids < 0] == 0).all()
 
 
+@pytest.mark.parametrize("cin", [131072, 131104])
+def test_route_many_rows_largest_sums(pkg, cin):
+    """Every value near its row's largest, all products of one sign: the sums come
+    as near to 64 bits as they can; from 131072 columns on the fp64 form takes over."""
+    x = np.full((70, cin), 1.99 * 2.0 ** -10, np.float32) * np.linspace(0.9, 1, 70, dtype=np.float32)[:, None]
+    w = np.full((8, cin), 1.99 * 2.0 ** -10, np.float32) * (1 - np.array([3, 1, 0, 2, 7, 5, 4, 6], np.float32) / 16)[:, None]
+    _, ids, _ = big_route(pkg, x, w, 3, None, "softmax", True, 1.0)
+    assert (ids.cpu().numpy() == [2, 1, 3]).all()
+
+
 def test_route_many_rows_not_finite(pkg):
     """NaN or infinite rows of x take the first experts or infinite logits' order, as in
     few rows; the other rows keep their bits.  An infinite weight makes every row uncertain."""
