@@ -249,11 +249,10 @@ __global__ void __launch_bounds__(256) route_digits_kernel(const RouteArgs a, in
 // One CTA: 128 rows x `tile` experts over one range of K steps.  Warp 0 fetches
 // (a stage is two copies: the images are laid out for it), warp 1 issues the
 // products, all four then add up the five sums of an element as one 64-bit number.
-// 2048 x 256 x 4096: 24 us, 1.2 Pmac/s of int8 over its 28 Tmac (12 us of it are the
-// matrix unit's at 8192 per clock and multiprocessor, the rest two loads ahead of
-// the first product, the last stage and the sums' way out); with the digits' kernel (13 us,
-// 67 MB in and out), the choice (12 us) and two nearly empty launches 52 us, where
-// fp64 matrix instructions took 316.
+// 2048 x 256 x 4096: 24 us, 1.2 Pmac/s of int8 over its 28 Tmac; the matrix unit is
+// busy for 64 % of that, the rest is the first loads, the last stage and the sums' way
+// out.  With the digits' kernel (13 us, 76 MB in and out), the choice (12 us) and two
+// nearly empty launches 52 us, where fp64 matrix instructions took 316.
 __global__ void __launch_bounds__(128) route_product_kernel(const RouteArgs a) {
     extern __shared__ __align__(1024) uint8_t smem[];
     __shared__ __align__(8) uint64_t s_full[kStages], s_empty[kStages], s_done;
