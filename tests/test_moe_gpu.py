@@ -137,6 +137,44 @@ def test_many_rows_guarded_replayed_and_not_finite(pkg):
     assert pkg.mlq.device_error(0) == 0
 
 
+def test_forms_side_by_side_on_streams(pkg):
+    """Routers, experts and linears of both forms at once on three streams, each
+    with a workspace of its own, while the next one's launches already wait
+    for the last: the bits of every call are those of the call alone."""
+    mlq = pkg.mlq
+    rng = np.random.default_rng(21)
+    few = Case(pkg, "q4_0", "q8_0", 6, 1024, 512, 768, 8, 2)
+    many = Case(pkg, "q8_0", "q4_1", 200, 512, 320, 256, 4, 2)
+    router = mlq.Router(dev(rng.standard_normal((64, 2048)).astype(np.float32) / 45), 4)
+    xr = dev(rng.standard_normal((1024, 2048)).astype(np.float32))
+    blocks = dev(ref.random_blocks(rng, "q4_0", 2048, 2048))
+    xl = dev(rng.standard_normal((100, 2048)).astype(np.float32))
+    on = {k: (dev(t.x), dev(t.ids), dev(t.w)) for k, t in (("few", few), ("many", many))}
+    calls = [
+        lambda ws: mlq.moe_experts(few.experts, *on["few"], workspace=ws),
+        lambda ws: mlq.moe_experts(many.experts, *on["many"], workspace=ws),
+        lambda ws: mlq.moe_route(router, xr, workspace=ws)[1],
+        lambda ws: mlq.linear_epilogue("q4_0", blocks, 2048, 2048, xl, workspace=ws),
+        lambda ws: mlq.linear_epilogue("q4_0", blocks, 2048, 2048, xl[:4], workspace=ws),
+    ]
+    size = max(mlq.experts_workspace_bytes(few.experts, 6, 2), mlq.experts_workspace_bytes(many.experts, 200, 2),
+               mlq.route_workspace_bytes(router, 1024), mlq.epilogue_workspace_bytes("q4_0", 2048, 2048, 100))
+    spaces = [torch.full((size,), 255, dtype=torch.uint8, device="cuda") for _ in range(3)]
+    want = [c(spaces[0]) for c in calls]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    got = []
+    for turn in range(12):
+        for k, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                n = (turn * (k + 1) + 2 * k) % len(calls)
+                got.append((n, calls[n](spaces[k])))
+    torch.cuda.synchronize()
+    assert mlq.device_error(0) == 0
+    for n, y in got:
+        assert torch.equal(y, want[n])
+
+
 @pytest.mark.parametrize("rows", [5, 40])
 def test_slots_without_an_expert(pkg, rows):
     """-1 and ids past the stack add nothing; a row of only such slots is its
