@@ -422,10 +422,11 @@ MLQ_API mlq_status mlq_peer_free(void* ptr);
  *
  * Workspace: these calls keep nothing between calls and allocate nothing.
  * The caller passes a device buffer of at least the bytes the matching
- * *_workspace_bytes function returns, 256-byte aligned; its contents need
- * not be initialised and mean nothing afterwards.  One call at a time may use a
- * workspace: calls ordered on one stream may share it, calls (or captured
- * graphs) that may run at the same time need one each.
+ * *_workspace_bytes function returns, 256-byte aligned (a workspace for more
+ * rows serves fewer); its contents need not be initialised and mean nothing
+ * afterwards.  One call at a time may use a workspace: calls ordered on one
+ * stream may share it, calls (or captured graphs) that may run at the same
+ * time need one each.
  *
  * x, y, ids, weights and residual are dense row-major device arrays with
  * the alignment of their type.  y may be residual itself.  y may be x itself

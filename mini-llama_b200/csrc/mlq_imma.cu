@@ -289,7 +289,7 @@ int many_positions(int pairs, int n_experts) { return (pairs + 7 * (pairs < n_ex
 
 int groups_of(int in) { return (in + 63) / 64; }
 
-// A copy of 16 scales may start at the last position.
+// A copy of up to 128 scales may start at the last position.
 int scale_pitch(int positions) { return (positions + 7) / 8 * 8 + kSegTokens; }
 
 size_t halves_bytes(int positions, int groups) {
@@ -432,19 +432,25 @@ size_t experts_workspace_bytes(const MoeShape& s, int rows, int top_k) {
     auto bytes = [&](int n) {
         const int pairs = n * top_k;
         const bool few = few_rows(pairs, s.n_experts);
-        const size_t lists = 256 + align256((size_t)max_segments(pairs, s.n_experts, few ? few_cap(n, pairs, s.n_experts) : 1) * sizeof(Segment));
+        const int cap = few ? few_cap(n, pairs, s.n_experts) : many_cap(pairs, s.n_experts);
+        const size_t lists = 256 + align256((size_t)max_segments(pairs, s.n_experts, cap) * sizeof(Segment));
         if (few)
             return lists + align256((size_t)pairs * sizeof(int)) + sliced_bytes(n, bprp) + sliced_bytes(pairs, hp) +
                    (n <= kCombineRows ? 0 : align256((size_t)pairs * s.out * sizeof(float))) + split_bytes(few, n);
         const int positions = many_positions(pairs, s.n_experts);
-        return lists + align256((size_t)positions * sizeof(int)) + align256((size_t)pairs * sizeof(int)) + halves_bytes(positions, groups_of(s.in)) +
-               halves_bytes(positions, groups_of(s.hidden)) + align256((size_t)pairs * s.out * sizeof(float)) +
+        return lists + align256((size_t)positions * sizeof(int)) + align256((size_t)pairs * sizeof(int)) +
+               halves_bytes(positions, groups_of(s.in)) + halves_bytes(positions, groups_of(s.hidden)) +
+               align256((size_t)pairs * s.out * sizeof(float)) +
                split_bytes(few, n);
     };
-    // the last pass may be smaller, and take another form
-    const int last = rows % pass;
-    const size_t whole = bytes(pass), rest = last ? bytes(last) : 0;
-    return whole > rest ? whole : rest;
+    // never less than for fewer rows (the last pass is one of those): each form needs most at its largest
+    size_t most = 0;
+    for (const long long n : {(long long)pass, (long long)kCombineRows, 5LL * s.n_experts / top_k})
+        if (n >= 1 && n <= pass) {
+            const size_t b = bytes((int)n);
+            if (b > most) most = b;
+        }
+    return most;
 }
 
 cudaError_t launch_experts(const MoeShape& s, const uint8_t* gate, const uint8_t* up, const uint8_t* down,

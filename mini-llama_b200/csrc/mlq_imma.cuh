@@ -112,9 +112,9 @@ __device__ __forceinline__ float warp_sum(float v) {
 __device__ __forceinline__ float digit_weight(int fmt, int l) { return fmt != kQ8_0 && l < 16 ? 16.0f : 1.0f; }
 
 // Slices a block into digits: lane l holds the value at imma_element l, times
-// `weight` in the digits (digit_weight).  Two
-// blocks share 256 bytes, [digit][t][block of the pair][word h].  A block with a value that is not finite gets the scale NaN: every output that
-// reads it is NaN.
+// `weight` in the digits (digit_weight).  Two blocks share 256 bytes, [digit]
+// [t][block of the pair][word h].  A block with a value that is not finite gets
+// the scale NaN: every output that reads it is NaN.
 // row: the row's first record, b the block.
 __device__ __forceinline__ void slice_digits(float x, float weight, uint8_t* row, int b, int lane) {
     const float v = x * weight;

@@ -200,7 +200,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int kws = kImmaWarps / a.strips;
     const int steps = (a.bpr + kChunkBlocks - 1) / kChunkBlocks;
     const int per_seg = (steps + kws - 1) / kws;  // rounds of a tile against a segment
-    // shared memory: stages [team][stage] of the warps' weights and the rounds' records of x, sums [team], (all_segs) y [team], the stages' barriers [team][stage] (full, empty)
+    // shared memory: stages [team][stage] of the warps' weights and the rounds' records of x, sums [team], (all_segs) y
+    // [team], the stages' barriers [team][stage] (full, empty)
     constexpr uint32_t kStage = kImmaWarps * S::kBytes + kXStage;
     const uint32_t red0 = kTeams * a.slots * kStage;
     const uint32_t y_floats = MODE == kDown && !a.part ? a.rows * 16 * a.strips : 0;

@@ -325,7 +325,9 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                     to_halves<F>(b, scale, hi, lo);
                     hand_over();  // a store takes as long as a stage's conversion
                     const int k = n % kOperands;
-                    if (!__all_sync(0xffffffffu, n >= kOperands ? wait(done + 8 * ((n - kOperands) % kDone), (n - kOperands) / kDone & 1, 45) : true)) {
+                    const uint32_t before = n - kOperands;  // had this place
+                    if (n >= kOperands &&
+                        !__all_sync(0xffffffffu, wait(done + 8 * (before % kDone), before / kDone & 1, 45))) {
                         alive = false;
                         break;
                     }
@@ -384,7 +386,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                     tmem_wait_ld(v);
 #pragma unroll
                     for (int i = 0; i < 8; ++i)
-                        acc2[8 * q + i] = fma2(pack2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), f[i], acc2[8 * q + i]);
+                        acc2[8 * q + i] = fma2(pack2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), f[i],
+                                               acc2[8 * q + i]);
                 }
                 tc_fence_before();
                 __syncwarp();

@@ -57,6 +57,20 @@ def experts(mlq, fmt=8, fmt_down=2, n=8, cin=64, hid=32, out=64, gate=0x1000, up
                              n * out * ((hid + 31) // 32) if nbd is None else nbd)
 
 
+def test_workspace_of_more_rows_serves_fewer(pkg):
+    mlq = pkg.mlq
+    L = mlq._moe_lib()
+    rows = sorted({*range(1, 140), *range(140, 9000, 61), 2047, 2048, 2049, 4096, 4097, 16384, 16385, 20000})
+    for n, cin, hid, out, k in ((8, 64, 32, 64, 2), (60, 3584, 2560, 3584, 4), (128, 2048, 768, 2048, 8),
+                                (1024, 7168, 96, 64, 64), (1, 1, 1, 1, 1), (3, 40000, 500, 100, 1)):
+        r, m = router(mlq, n=n, cin=cin, k=k), experts(mlq, n=n, cin=cin, hid=hid, out=out)
+        for size in (lambda i: L.mlq_moe_route_workspace_bytes(r, i), lambda i: L.mlq_moe_experts_workspace_bytes(m, i, k),
+                     lambda i: L.mlq_moe_layer_workspace_bytes(r, m, i),
+                     lambda i: L.mlq_linear_epilogue_workspace_bytes(8, out, cin, i)):
+            sizes = [size(i) for i in rows]
+            assert sizes[0] > 0 and sizes == sorted(sizes)
+
+
 BIG = 1 << 40  # a workspace size that is never too small
 
 
