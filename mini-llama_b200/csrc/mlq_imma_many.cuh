@@ -42,7 +42,8 @@ constexpr int kManyThreads = 32 * (2 * kRoleWarps + 4);
 constexpr int kDrainThreads = 32 * kRoleWarps;
 constexpr int kOperands = 4, kScaleRing = 8, kXRing = 16, kDone = 8;
 constexpr int kMaxBStages = 6;                   // + 4 sums: scales of x outlive the operand by as many products
-constexpr int kXchPitch = kUnitRows + 4;         // kPair: [32 rows of x][128 rows + 4]
+constexpr int kXchPitch = kUnitRows + 4;         // exchange of a unit's results: [32 rows of x][128 rows + 4]
+constexpr int kXchBytes = 32 * kXchPitch * 4;
 constexpr int kManyJoin = 2;                     // rounds
 // registers at launch, and after the split
 constexpr int kManyLaunchRegs = 96, kDecodeRegs = 88, kDrainRegs = 136, kOtherRegs = 32;
@@ -225,11 +226,11 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
     const int steps = (a.bpr + kChunkBlocks - 1) / kChunkBlocks;
     const uint32_t xrows = (a.seg_cap + 31) / 32 * 32;  // of a stage of x
-    // shared memory: x, weights, (kPair) exchange, barriers
+    // shared memory: x, weights, (not kDown) exchange, barriers
     const uint32_t b_bytes = 256u * xrows;
     const uint32_t b_ring = (smem_u32(smem) + 1023u) & ~1023u, raw_ring = b_ring + a.x_slots * b_bytes;
     const uint32_t xch = raw_ring + a.slots * S::kBytes;
-    const uint32_t bars = xch + (MODE == kPair ? 32 * kXchPitch * 4 : 0);
+    const uint32_t bars = xch + (MODE == kDown ? 0 : kXchBytes);
     // done: a stage's products; it frees x and the operand too
     const uint32_t raw_full = bars, raw_empty = raw_full + 64, b_full = raw_empty + 64, done = b_full + 64,
                    a_full = done + 8 * (kDone + 1), d_free = a_full + 32;
@@ -356,6 +357,14 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             int e, first, count;
             segment(work.u % nseg, e, first, count);
             const int cols = (count + 15) / 16 * 8;  // of this half
+            // for the end of the unit: lane l has rows of x l and l + 32 of this half
+            [[maybe_unused]] int pair[2];
+            if (MODE == kDown)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const int tok = half * cols + lane + 32 * k;
+                    pair[k] = tok < count ? __ldcg(a.order + first + tok) : 0;
+                }
             uint64_t acc2[32];  // pairs of columns
 #pragma unroll
             for (int i = 0; i < 32; ++i) acc2[i] = 0;
@@ -462,22 +471,35 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                             .store(a.h + (pos * a.next_groups + tile) * 256, a.hs + (size_t)tile * a.hs_pitch + pos, lane);
                     }
                 }
-            } else {
+            } else if constexpr (MODE == kDown) {
                 const int o = tile * kUnitRows + row;
-                if (o < a.out) {
-                    const float bias = MODE == kPlain && a.bias ? a.bias[o] : 0.0f;
 #pragma unroll
-                    for (int i = 0; i < 64; ++i) {
-                        if (i >= cols || tok0 + i >= count) break;
-                        const int r = first + tok0 + i;
-                        if (MODE == kDown) {
-                            a.part[(size_t)__ldcg(a.order + r) * a.out + o] = acc[i];
-                        } else {
-                            float v = activate(acc[i] + bias, a.act);
-                            if (a.row_scale) v *= a.row_scale[r];
-                            const size_t to = (size_t)r * a.out + o;
-                            a.y[to] = a.residual ? a.residual[to] + v : v;
-                        }
+                for (int i = 0; i < 64; ++i) {
+                    if (i >= cols || tok0 + i >= count) break;
+                    const int to = __shfl_sync(0xffffffffu, pair[i / 32], i % 32);
+                    if (o < a.out) a.part[(size_t)to * a.out + o] = acc[i];
+                }
+            } else {
+                // as above, then a loop of few instructions: 64 copies of it would come from memory each time
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    if (16 * q >= cols) break;
+                    drain_sync();
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) sts_f32(xch + ((half * 16 + i) * kXchPitch + row) * 4, acc[16 * q + i]);
+                    drain_sync();
+                    const int loc = threadIdx.x & 127, o = tile * kUnitRows + loc;
+                    const float bias = a.bias && o < a.out ? a.bias[o] : 0.0f;
+#pragma unroll 4
+                    for (int i = dw >> 2; i < 32; i += 2) {
+                        const int in = 16 * q + (i & 15), tok = (i >> 4) * cols + in;
+                        if (in >= cols || tok >= count || o >= a.out) continue;
+                        const int r = first + tok;
+                        const size_t to = (size_t)r * a.out + o;
+                        const float add = a.residual ? a.residual[to] : 0.0f;
+                        float v = activate(__uint_as_float(lds_u32(xch + (i * kXchPitch + loc) * 4)) + bias, a.act);
+                        if (a.row_scale) v *= a.row_scale[r];
+                        a.y[to] = a.residual ? add + v : v;
                     }
                 }
             }
@@ -661,13 +683,13 @@ cudaError_t launch_one(ImmaArgs a, int grid, int smem_per_sm, cudaStream_t strea
     auto k = imma_many_kernel<F, MODE, ALN>;
     const int xrows = (a.seg_cap + 31) / 32 * 32, stage = 256 * xrows;
     // the system's 1 KB per CTA, the static part (up to 1 KB besides the scales), alignment, barriers
-    const int fixed = 1024 + (kScaleRing * kUnitRows + kXRing * 128) * 4 + 1024 + 1024 + 512 + (MODE == kPair ? 32 * kXchPitch * 4 : 0);
+    const int fixed = 1024 + (kScaleRing * kUnitRows + kXRing * 128) * 4 + 1024 + 1024 + 512 + (MODE == kDown ? 0 : kXchBytes);
     // x comes from L2, about 2 us ahead at 0.3 us a stage and 64 rows; the weights have the rest
     a.x_slots = xrows > 64 ? 3 : xrows > 32 ? 4 : kMaxBStages;
     a.slots = (smem_per_sm - fixed - a.x_slots * stage) / S::kBytes;
     if (a.slots > 8) a.slots = 8;
     if (a.slots < 2) return cudaErrorInvalidConfiguration;
-    const size_t smem = (size_t)1024 + a.x_slots * stage + a.slots * S::kBytes + (MODE == kPair ? 32 * kXchPitch * 4 : 0) + 512;
+    const size_t smem = (size_t)1024 + a.x_slots * stage + a.slots * S::kBytes + (MODE == kDown ? 0 : kXchBytes) + 512;
     ManyMaps maps{};
     for (int i = 0; ALN && i < (MODE == kPair ? 2 : 1); ++i)
         if (!make_map_2d(&maps.w[i], CU_TENSOR_MAP_DATA_TYPE_UINT16, const_cast<uint8_t*>(a.w[i]),
