@@ -454,6 +454,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) sts_f32(xch + ((half * 16 + i) * kXchPitch + row) * 4, acc[16 * q + i]);
                     drain_sync();
+#pragma unroll 1
                     for (int i = dw; i < 32; i += kRoleWarps) {
                         const int in = 16 * q + (i & 15), tok = (i >> 4) * cols + in;
                         if (in >= cols || tok >= count) continue;
@@ -490,7 +491,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                     drain_sync();
                     const int loc = threadIdx.x & 127, o = tile * kUnitRows + loc;
                     const float bias = a.bias && o < a.out ? a.bias[o] : 0.0f;
-#pragma unroll 4
+#pragma unroll 1
                     for (int i = dw >> 2; i < 32; i += 2) {
                         const int in = 16 * q + (i & 15), tok = (i >> 4) * cols + in;
                         if (in >= cols || tok >= count || o >= a.out) continue;
