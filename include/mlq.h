@@ -505,7 +505,7 @@ typedef struct mlq_experts {
  * [rows][top_k].  A slot whose id is outside [0, n_experts) adds nothing (-1:
  * a padded row, or an expert that another GPU holds); a row of only such slots
  * gives y = residual (0 without one).  The same expert may appear in several
- * slots.  With up to 5 rows per expert on average (rows x top_k against
+ * slots.  With up to 11 rows per expert on average (rows x top_k against
  * n_experts) x goes by digits, in segments of up to 4 rows of one expert; beyond, as
  * pairs of fp16 values, in segments of up to 128. */
 MLQ_API mlq_status mlq_moe_experts(const mlq_experts* experts, const float* x, int rows, int top_k,

@@ -337,10 +337,12 @@ int max_segments(int pairs, int n_experts, int cap) {
 
 // Whether a call's rows of x go by digits, in segments of at most 4: an
 // expert with more rows has several segments, whose weights come from L2 after the
-// first.  60 experts of 3584 x 2560, q4_0 (q8_0), us by digits and by halves: 2 rows
-// per expert 224 and 300 (302 and 338), 4 rows 281 and 364 (343 and 400), 6 rows
-// 388 and 399 (457 and 430), 12 rows 698 and 592 (802 and 604).
-bool few_rows(int pairs, int n_experts) { return pairs <= 5 * n_experts; }
+// first, so the time grows with the rows, while that of the other form hardly does below
+// 16 rows per expert.  60 experts of 3584 x 2560, us by digits and by halves: q4_0 6 rows
+// per expert 389 and 701, 10 rows 591 and 704, 11 rows 641 and 705; q8_0 450 and 709, 686
+// and 713, 736 and 714; q4_1 462 and 988, 708 and 990, 772 and 991.
+constexpr int kFewPerExpert = 11;
+bool few_rows(int pairs, int n_experts) { return pairs <= kFewPerExpert * n_experts; }
 
 int prep_ctas(long long blocks, int sm_count) {
     const long long n = (blocks + 7) / 8;
@@ -445,7 +447,7 @@ size_t experts_workspace_bytes(const MoeShape& s, int rows, int top_k) {
     };
     // never less than for fewer rows (the last pass is one of those): each form needs most at its largest
     size_t most = 0;
-    for (const long long n : {(long long)pass, (long long)kCombineRows, 5LL * s.n_experts / top_k})
+    for (const long long n : {(long long)pass, (long long)kCombineRows, (long long)kFewPerExpert * s.n_experts / top_k})
         if (n >= 1 && n <= pass) {
             const size_t b = bytes((int)n);
             if (b > most) most = b;

@@ -83,7 +83,7 @@ CASES = [
 ]
 
 
-# more than 5 rows per expert on average: the form of many rows.  Segments of up to 128 rows and experts with more,
+# more rows per expert: mostly the form of many rows.  Segments of up to 128 rows and experts with more,
 # hidden widths and outputs that end inside a tile of 64 and of 128, an odd number of blocks, rows that are not aligned, K
 # axes that several CTAs share, one row above and exactly at the border to the form of few rows, two passes
 CASES += [
@@ -94,6 +94,11 @@ CASES += [
     ("q4_0", "q4_1", 26, 288, 160, 96, 5, 1), ("q4_0", "q8_0", 3000, 64, 64, 32, 8, 3),
     ("q8_0", "q8_0", 128, 1024, 64, 1, 1, 1), ("q4_0", "q4_0", 2000, 1, 1, 1, 2, 1),
 ]
+
+
+# the border itself: 11 rows per expert, and one more
+CASES += [("q4_0", "q4_1", 55, 288, 160, 96, 5, 1), ("q4_0", "q4_1", 56, 288, 160, 96, 5, 1),
+          ("q8_0", "q8_0", 44, 1024, 96, 200, 8, 2), ("q4_1", "q4_0", 45, 1024, 96, 200, 8, 2)]
 
 
 @pytest.mark.parametrize("c", CASES, ids=lambda c: "-".join(map(str, c)))
