@@ -260,6 +260,8 @@ struct Carve {
         return r;
     }
     uint8_t* take_sliced(size_t rows, int bprp) { return take<uint8_t>(rows * (bprp / kChunkBlocks) * kRecordBytes); }
+    // Whether what was taken lies within `bytes` bytes from `ws` on.
+    bool within(const void* ws, size_t bytes) const { return (size_t)(p - static_cast<const uint8_t*>(ws)) <= bytes; }
 };
 
 size_t sliced_bytes(size_t rows, int bprp) { return align256(rows * (bprp / kChunkBlocks) * kRecordBytes); }
@@ -279,8 +281,9 @@ int few_cap(int rows, int pairs, int n_experts) { return rows < 3 ? rows : pairs
 
 // And in that of many: half as many again as an expert has on average, so
 // that most experts are one segment.
+constexpr int kManyCapStep = 32;
 int many_cap(int pairs, int n_experts) {
-    const int n = (pairs / n_experts * 3 / 2 + 8 + 31) / 32 * 32;
+    const int n = (pairs / n_experts * 3 / 2 + 8 + kManyCapStep - 1) / kManyCapStep * kManyCapStep;
     return n < kSegTokens ? n : kSegTokens;
 }
 
@@ -335,6 +338,13 @@ int max_segments(int pairs, int n_experts, int cap) {
     return full < pairs ? full : pairs;
 }
 
+// Places in the segment list: as many as the form's smallest cap gives.  The
+// cap in use grows with the rows, and a list of just its segments would get shorter
+// where it does: a pass of fewer rows would then need more than a full one.
+int segment_places(bool few, int pairs, int n_experts) {
+    return max_segments(pairs, n_experts, few ? 1 : kManyCapStep);
+}
+
 // Whether a call's rows of x go by digits, in segments of at most 4: an
 // expert with more rows has several segments, whose weights come from L2 after the
 // first, so the time grows with the rows, while that of the other form hardly does below
@@ -375,8 +385,8 @@ size_t epilogue_workspace_bytes(int in, int rows) {
 }
 
 cudaError_t launch_linear_epilogue(int fmt, const uint8_t* w, int out, int in, const float* x, int rows,
-                                   const mlq_epilogue& ep, float* y, void* ws, int sm_count, int smem_per_sm, int* err,
-                                   cudaStream_t stream) {
+                                   const mlq_epilogue& ep, float* y, void* ws, size_t ws_bytes, int sm_count,
+                                   int smem_per_sm, int* err, cudaStream_t stream) {
     const int bpr = (in + kQK - 1) / kQK, bprp = padded_blocks(bpr);
     const int pass = linear_pass_rows(in, rows);
     for (int r0 = 0; r0 < rows;) {
@@ -387,19 +397,15 @@ cudaError_t launch_linear_epilogue(int fmt, const uint8_t* w, int out, int in, c
         p.rows = n, p.in = in, p.bpr = bpr, p.bprp = bprp, p.fmt = fmt;
         const bool few = n <= kLinearFewRows;
         HalvesArgs hv{};
-        float* split;
-        cudaError_t e;
-        if (few) {
+        if (few)
             p.sliced = c.take_sliced(n, bprp);
-            split = c.take<float>(split_floats(few, n, kImmaWarps) * split_count(few));
-            p.split_done = c.take<unsigned int>(2 * kMaxTeams);
-            e = launch_pdl(prep_kernel, prep_ctas((long long)n * bprp, sm_count), 256, 0, stream, p);
-        } else {
+        else
             hv = halves_args(c, p.x, n, n, in, fmt);
-            split = c.take<float>(split_floats(few, n, kImmaWarps) * split_count(few));
-            p.split_done = hv.split_done = c.take<unsigned int>(2 * kMaxTeams);
-            e = launch_pdl(halves_kernel, prep_ctas((long long)n * hv.groups, sm_count), 256, 0, stream, hv);
-        }
+        float* split = c.take<float>(split_floats(few, n, kImmaWarps) * split_count(few));
+        p.split_done = hv.split_done = c.take<unsigned int>(2 * kMaxTeams);
+        if (!c.within(ws, ws_bytes)) return cudaErrorInvalidValue;
+        cudaError_t e = few ? launch_pdl(prep_kernel, prep_ctas((long long)n * bprp, sm_count), 256, 0, stream, p)
+                            : launch_pdl(halves_kernel, prep_ctas((long long)n * hv.groups, sm_count), 256, 0, stream, hv);
         if (e != cudaSuccess) return e;
         ImmaArgs a{};
         a.w[0] = w;
@@ -434,8 +440,7 @@ size_t experts_workspace_bytes(const MoeShape& s, int rows, int top_k) {
     auto bytes = [&](int n) {
         const int pairs = n * top_k;
         const bool few = few_rows(pairs, s.n_experts);
-        const int cap = few ? few_cap(n, pairs, s.n_experts) : many_cap(pairs, s.n_experts);
-        const size_t lists = 256 + align256((size_t)max_segments(pairs, s.n_experts, cap) * sizeof(Segment));
+        const size_t lists = 256 + align256((size_t)segment_places(few, pairs, s.n_experts) * sizeof(Segment));
         if (few)
             return lists + align256((size_t)pairs * sizeof(int)) + sliced_bytes(n, bprp) + sliced_bytes(pairs, hp) +
                    (n <= kCombineRows ? 0 : align256((size_t)pairs * s.out * sizeof(float))) + split_bytes(few, n);
@@ -445,7 +450,8 @@ size_t experts_workspace_bytes(const MoeShape& s, int rows, int top_k) {
                align256((size_t)pairs * s.out * sizeof(float)) +
                split_bytes(few, n);
     };
-    // never less than for fewer rows (the last pass is one of those): each form needs most at its largest
+    // never less than for fewer rows (the last pass is one of those): within a form, and on either side of kCombineRows,
+    // every array grows with the rows, so the most is at one of these
     size_t most = 0;
     for (const long long n : {(long long)pass, (long long)kCombineRows, (long long)kFewPerExpert * s.n_experts / top_k})
         if (n >= 1 && n <= pass) {
@@ -457,8 +463,8 @@ size_t experts_workspace_bytes(const MoeShape& s, int rows, int top_k) {
 
 cudaError_t launch_experts(const MoeShape& s, const uint8_t* gate, const uint8_t* up, const uint8_t* down,
                            const float* x, int rows, int top_k, const int32_t* ids, const float* weights,
-                           const float* residual, float* y, void* ws, int sm_count, int smem_per_sm, int* err,
-                           cudaStream_t stream) {
+                           const float* residual, float* y, void* ws, size_t ws_bytes, int sm_count, int smem_per_sm,
+                           int* err, cudaStream_t stream) {
     const int pass = experts_pass_rows(s, rows, top_k);
     const int bpr = (s.in + kQK - 1) / kQK, bprp = padded_blocks(bpr);
     const int hb = (s.hidden + kQK - 1) / kQK, hp = padded_blocks(hb);
@@ -475,7 +481,7 @@ cudaError_t launch_experts(const MoeShape& s, const uint8_t* gate, const uint8_t
         PrepArgs p{};
         HalvesArgs hx{}, hh{};
         p.nseg = c.take<int>(1);
-        p.segs = c.take<Segment>(nseg_max);
+        p.segs = c.take<Segment>(segment_places(few, pairs, s.n_experts));
         p.positions = few ? 0 : many_positions(pairs, s.n_experts);
         p.order = c.take<int>(few ? pairs : p.positions);
         p.x = x + (long long)r0 * s.in;
@@ -497,6 +503,7 @@ cudaError_t launch_experts(const MoeShape& s, const uint8_t* gate, const uint8_t
         float* part = c.take<float>(at_once ? 0 : (size_t)pairs * s.out);
         float* split = c.take<float>(split_floats(few, n, kImmaWarps) * split_count(few));
         p.split_done = hx.split_done = c.take<unsigned int>(2 * kMaxTeams);
+        if (!c.within(ws, ws_bytes)) return cudaErrorInvalidValue;
         cudaError_t e = launch_pdl(prep_kernel, few ? 1 + prep_ctas((long long)n * bprp, sm_count) : 1, 256, 0, stream, p);
         if (e == cudaSuccess && !few)
             e = launch_pdl(halves_kernel, prep_ctas((long long)n * hx.groups, sm_count), 256, 0, stream, hx);

@@ -218,24 +218,25 @@ struct DeviceFacts {
 };
 mlq_status current_device_facts(DeviceFacts* f);
 
-// Experts' products and the linear with an epilogue (mlq_imma.cu).
+// Experts' products and the linear with an epilogue (mlq_imma.cu).  The launches lay a workspace of ws_bytes out per
+// pass and refuse (cudaErrorInvalidValue) a pass that would not fit in it.
 struct MoeShape {
     int fmt, fmt_down, n_experts, in, hidden, out;
 };
 size_t experts_workspace_bytes(const MoeShape& s, int rows, int top_k);
 cudaError_t launch_experts(const MoeShape& s, const uint8_t* gate, const uint8_t* up, const uint8_t* down,
                            const float* x, int rows, int top_k, const int32_t* ids, const float* weights,
-                           const float* residual, float* y, void* ws, int sm_count, int smem_per_sm, int* err,
-                           cudaStream_t stream);
+                           const float* residual, float* y, void* ws, size_t ws_bytes, int sm_count, int smem_per_sm,
+                           int* err, cudaStream_t stream);
 size_t epilogue_workspace_bytes(int in, int rows);
 cudaError_t launch_linear_epilogue(int fmt, const uint8_t* w, int out, int in, const float* x, int rows,
-                                   const mlq_epilogue& ep, float* y, void* ws, int sm_count, int smem_per_sm, int* err,
-                                   cudaStream_t stream);
+                                   const mlq_epilogue& ep, float* y, void* ws, size_t ws_bytes, int sm_count,
+                                   int smem_per_sm, int* err, cudaStream_t stream);
 
 // The router (mlq_route.cu).
 size_t route_workspace_bytes(int n_experts, int in, int rows);
 cudaError_t launch_route(const mlq_router& r, const float* x, int rows, int32_t* ids, float* weights, float* logits,
-                         void* ws, int* err, cudaStream_t stream);
+                         void* ws, size_t ws_bytes, int* err, cudaStream_t stream);
 
 // Quantize fp32 [rows][cols] -> blocks, reference rules (mlq_convert.cu).
 cudaError_t launch_quantize(int fmt, const float* src, long long rows, int cols, uint8_t* blocks,

@@ -86,23 +86,24 @@ mlq::MoeShape shape_of(const mlq_experts& m) {
 }
 
 mlq_status run_route(const char* who, const mlq_router& r, const float* x, int rows, int32_t* ids, float* weights,
-                     float* logits, void* ws, mlq_stream stream) {
+                     float* logits, void* ws, size_t ws_bytes, mlq_stream stream) {
     mlq::DeviceFacts f{};
     mlq_status st = mlq::current_device_facts(&f);
     if (st != MLQ_OK) return st;
-    cudaError_t e = mlq::launch_route(r, x, rows, ids, weights, logits, ws, f.err, stream);
+    cudaError_t e = mlq::launch_route(r, x, rows, ids, weights, logits, ws, ws_bytes, f.err, stream);
     return e == cudaSuccess ? MLQ_OK : fail_cuda(std::string(who) + " launch", e);
 }
 
 mlq_status run_experts(const char* who, const mlq_experts& m, const float* x, int rows, int top_k, const int32_t* ids,
-                       const float* weights, const float* residual, float* y, void* ws, mlq_stream stream) {
+                       const float* weights, const float* residual, float* y, void* ws, size_t ws_bytes,
+                       mlq_stream stream) {
     mlq::DeviceFacts f{};
     mlq_status st = mlq::current_device_facts(&f);
     if (st != MLQ_OK) return st;
     cudaError_t e = mlq::launch_experts(shape_of(m), static_cast<const uint8_t*>(m.w_gate),
                                         static_cast<const uint8_t*>(m.w_up), static_cast<const uint8_t*>(m.w_down), x,
-                                        rows, top_k, ids, weights, residual, y, ws, f.sm_count, f.smem_per_sm, f.err,
-                                        stream);
+                                        rows, top_k, ids, weights, residual, y, ws, ws_bytes, f.sm_count,
+                                        f.smem_per_sm, f.err, stream);
     return e == cudaSuccess ? MLQ_OK : fail_cuda(std::string(who) + " launch", e);
 }
 
@@ -131,7 +132,7 @@ MLQ_API mlq_status mlq_moe_route(const mlq_router* router, const float* x, int r
         if (!x || !ids || !weights) return fail(MLQ_ERR_NULL, std::string(who) + ": null input/output pointer");
         st = check_workspace(who, workspace, workspace_bytes, mlq::route_workspace_bytes(router->n_experts, router->in_features, rows));
         if (st != MLQ_OK) return st;
-        return run_route(who, *router, x, rows, ids, weights, logits, workspace, stream);
+        return run_route(who, *router, x, rows, ids, weights, logits, workspace, workspace_bytes, stream);
     } catch (...) {
         return fail(MLQ_ERR_CUDA, "mlq_moe_route: host exception");
     }
@@ -164,7 +165,7 @@ MLQ_API mlq_status mlq_moe_experts(const mlq_experts* experts, const float* x, i
         st = check_workspace(who, workspace, workspace_bytes,
                              mlq::experts_workspace_bytes(shape_of(*experts), rows, top_k));
         if (st != MLQ_OK) return st;
-        return run_experts(who, *experts, x, rows, top_k, ids, weights, residual, y, workspace, stream);
+        return run_experts(who, *experts, x, rows, top_k, ids, weights, residual, y, workspace, workspace_bytes, stream);
     } catch (...) {
         return fail(MLQ_ERR_CUDA, "mlq_moe_experts: host exception");
     }
@@ -197,10 +198,10 @@ MLQ_API mlq_status mlq_moe_layer(const mlq_router* router, const mlq_experts* ex
         st = check_workspace(who, workspace, workspace_bytes,
                              rb + mlq::experts_workspace_bytes(shape_of(*experts), rows, router->top_k));
         if (st != MLQ_OK) return st;
-        st = run_route(who, *router, x, rows, ids, weights, nullptr, workspace, stream);
+        st = run_route(who, *router, x, rows, ids, weights, nullptr, workspace, rb, stream);
         if (st != MLQ_OK) return st;
         return run_experts(who, *experts, x, rows, router->top_k, ids, weights, residual, y,
-                           static_cast<char*>(workspace) + rb, stream);
+                           static_cast<char*>(workspace) + rb, workspace_bytes - rb, stream);
     } catch (...) {
         return fail(MLQ_ERR_CUDA, "mlq_moe_layer: host exception");
     }
@@ -235,8 +236,8 @@ MLQ_API mlq_status mlq_linear_epilogue(mlq_format fmt, const void* w, size_t blo
         st = mlq::current_device_facts(&f);
         if (st != MLQ_OK) return st;
         cudaError_t e = mlq::launch_linear_epilogue(fmt, static_cast<const uint8_t*>(w), out_features, in_features, x,
-                                                    rows, *epilogue, y, workspace, f.sm_count, f.smem_per_sm, f.err,
-                                                    stream);
+                                                    rows, *epilogue, y, workspace, workspace_bytes, f.sm_count,
+                                                    f.smem_per_sm, f.err, stream);
         return e == cudaSuccess ? MLQ_OK : fail_cuda(who + " launch", e);
     } catch (...) {
         return fail(MLQ_ERR_CUDA, "mlq_linear_epilogue: host exception");

@@ -635,7 +635,7 @@ size_t route_workspace_bytes(int n_experts, int in, int rows) {
 }
 
 cudaError_t launch_route(const mlq_router& r, const float* x, int rows, int32_t* ids, float* weights, float* logits,
-                         void* ws, int* err, cudaStream_t stream) {
+                         void* ws, size_t ws_bytes, int* err, cudaStream_t stream) {
     for (int r0 = 0; r0 < rows; r0 += kPassRows) {
         RouteArgs a{};
         a.w = r.w, a.bias = r.bias;
@@ -647,7 +647,7 @@ cudaError_t launch_route(const mlq_router& r, const float* x, int rows, int32_t*
         a.weights = weights + (size_t)r0 * r.top_k;
         a.logits = logits ? logits + (size_t)r0 * r.n_experts : nullptr;
         a.err = err;
-        lay_out(a, static_cast<char*>(ws));
+        if (lay_out(a, static_cast<char*>(ws)) > ws_bytes) return cudaErrorInvalidValue;
         const int vec = a.in % 4 == 0 && reinterpret_cast<uintptr_t>(a.w) % 16 == 0 && reinterpret_cast<uintptr_t>(a.x) % 16 == 0;
         auto up = [](int n, int d) { return (unsigned)((n + d - 1) / d); };
         // at most 64 KB (1024 experts); the default limit of 48 KB is raised only for calls that need it
