@@ -731,14 +731,17 @@ def moe_route(router: Router, x, ids=None, weights=None, logits=None, workspace=
 
 def moe_experts(experts: Experts, x, ids, weights, residual=None, y=None, workspace=None, stream=None):
     """mlq_moe_experts: y = residual + sum over slots of weights * expert(x),
-    ids int32 / weights float32 [rows, top_k]; ids outside [0, n_experts) add
-    nothing."""
+    ids int32 / weights float32 [rows, top_k] (of a single row also [top_k]);
+    ids outside [0, n_experts) add nothing."""
     torch = _the_torch()
     dev, f32 = experts.device, torch.float32
     rows = _rows_of(x, experts.in_features)
     xp = _need(x, f32, x.shape, dev, "x")
+    if ids.dim() == 0 or ids.numel() == 0:
+        raise ValueError(f"ids: expected [{rows}, top_k], got {tuple(ids.shape)}")
     top_k = ids.shape[-1]
-    shape = (rows, top_k) if ids.dim() == 2 else (top_k,)
+    # the library reads rows x top_k of them: [top_k] is the form of a single row
+    shape = (top_k,) if ids.dim() == 1 and rows == 1 else (rows, top_k)
     yshape = (*x.shape[:-1], experts.out_features)
     if y is None:
         y = x.new_empty(yshape)

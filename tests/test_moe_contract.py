@@ -57,3 +57,22 @@ def test_two_passes_of_unequal_length(pkg):
     are one of 1326 and one of 1325."""
     whole, first, last = sizes(pkg.mlq, (468, 31744, 32, 64), 6, [2651, 1326, 1325])
     assert whole == first >= last
+
+
+def test_ids_of_one_row_serve_one_row_only(pkg):
+    """The C call reads rows x top_k ids and weights: 1-D ones belong to a single
+    row of x (CPU tensors: a call that passes the shapes is refused for its device)."""
+    torch = pytest.importorskip("torch")
+    mlq = pkg.mlq
+    stack, down = (torch.zeros(4 * r * nb * 34, dtype=torch.uint8) for r, nb in ((32, 2), (64, 1)))
+    m = mlq.Experts("q8_0", stack, stack, down, 4, 64, 32)
+    ids, w = torch.zeros(2, dtype=torch.int32), torch.zeros(2)
+    for x, i, v, text in [(torch.zeros(3, 64), ids, w, "ids: expected"), (torch.zeros(2, 64), ids, w, "ids: expected"),
+                          (torch.zeros(3, 64), ids.expand(3, 2).contiguous(), w, "weights: expected"),
+                          (torch.zeros(64), ids, w.view(1, 2), "weights: expected"),
+                          (torch.zeros(64), ids[0], w, "ids: expected"), (torch.zeros(1, 64), ids[:0], w[:0], "ids: expected"),
+                          (torch.zeros(64), ids, w, "CUDA"), (torch.zeros(1, 64), ids, w, "CUDA"),
+                          (torch.zeros(64), ids.view(1, 2), w.view(1, 2), "CUDA"),
+                          (torch.zeros(3, 64), ids.expand(3, 2).contiguous(), w.expand(3, 2).contiguous(), "CUDA")]:
+        with pytest.raises(ValueError, match=text):
+            mlq.moe_experts(m, x, i, v)
