@@ -737,7 +737,7 @@ def moe_experts(experts: Experts, x, ids, weights, residual=None, y=None, worksp
     dev, f32 = experts.device, torch.float32
     rows = _rows_of(x, experts.in_features)
     xp = _need(x, f32, x.shape, dev, "x")
-    if ids.dim() == 0 or ids.numel() == 0:
+    if ids.dim() == 0:
         raise ValueError(f"ids: expected [{rows}, top_k], got {tuple(ids.shape)}")
     top_k = ids.shape[-1]
     # the library reads rows x top_k of them: [top_k] is the form of a single row
