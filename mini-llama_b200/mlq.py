@@ -615,6 +615,27 @@ def _blocks_need(w, fmt, rows: int, cols: int, device, what: str) -> int:
     return w.data_ptr()
 
 
+def _on_stream(device, stream, call, *given):
+    """call() with `stream` current, so that what it allocates belongs to that
+    stream: no earlier work of another stream may still use the memory, and once
+    dropped it is reused after the call's kernels only.  Results that are not among
+    `given` may be used on the caller's stream, and be dropped there."""
+    torch = _the_torch()
+    handle = stream if isinstance(stream, int) else stream.cuda_stream
+    if device.type != "cuda" or handle == torch._C._cuda_getCurrentRawStream(device.index):
+        return call()
+    if isinstance(stream, int):
+        # 0 and 1 both name the default stream
+        stream = torch.cuda.ExternalStream(handle, device=device) if handle > 1 else torch.cuda.default_stream(device)
+    caller = torch.cuda.current_stream(device)
+    with torch.cuda.stream(stream):
+        out = call()
+    for t in out if isinstance(out, tuple) else (out,):
+        if not any(t is g for g in given):
+            t.record_stream(caller)
+    return out
+
+
 def _on_device(device, stream, fn, *args) -> None:
     """fn(*args, stream handle) with `device` current (the library runs on the
     current device); stream: the caller's, or that device's current one."""
@@ -637,8 +658,8 @@ def _on_device(device, stream, fn, *args) -> None:
 
 def _workspace(ws, need, device):
     """(address, bytes) of the caller's workspace, or of a fresh one of need()
-    bytes from torch's allocator (which keeps it alive in stream order, and
-    per graph under capture), and the tensor."""
+    bytes from torch's allocator (which keeps it alive in the order of the
+    current stream, the call's, and per graph under capture), and the tensor."""
     uint8 = _the_torch().uint8
     if ws is None:
         ws = _the_torch().empty(need(), dtype=uint8, device=device)
@@ -712,7 +733,11 @@ def epilogue_workspace_bytes(fmt, out_features: int, in_features: int, rows: int
 def moe_route(router: Router, x, ids=None, weights=None, logits=None, workspace=None, stream=None):
     """mlq_moe_route: (ids int32 [rows, top_k], weights float32 [rows, top_k])
     of x float32 [rows, in] (or [in]).  logits: float32 [rows, n_experts] to
-    fill, or None.  Without `workspace` one is allocated for the call."""
+    fill, or None.  Without `workspace` one is allocated for the call.  What a
+    call allocates belongs to the stream it runs on (`stream`, or the current one);
+    x and the other tensors given must be ready there."""
+    if stream is not None and (ids is None or weights is None or workspace is None):
+        return _on_stream(router.device, stream, lambda: moe_route(router, x, ids, weights, logits, workspace), ids, weights)
     torch = _the_torch()
     dev, f32 = router.device, torch.float32
     rows = _rows_of(x, router.in_features)
@@ -733,6 +758,8 @@ def moe_experts(experts: Experts, x, ids, weights, residual=None, y=None, worksp
     """mlq_moe_experts: y = residual + sum over slots of weights * expert(x),
     ids int32 / weights float32 [rows, top_k] (of a single row also [top_k]);
     ids outside [0, n_experts) add nothing."""
+    if stream is not None and (y is None or workspace is None):
+        return _on_stream(experts.device, stream, lambda: moe_experts(experts, x, ids, weights, residual, y, workspace), y)
     torch = _the_torch()
     dev, f32 = experts.device, torch.float32
     rows = _rows_of(x, experts.in_features)
@@ -756,6 +783,9 @@ def moe_layer(router: Router, experts: Experts, x, residual=None, y=None, ids=No
               stream=None):
     """mlq_moe_layer: the router's choice, then the experts; returns
     (y, ids, weights)."""
+    if stream is not None and (y is None or ids is None or weights is None or workspace is None):
+        return _on_stream(experts.device, stream,
+                          lambda: moe_layer(router, experts, x, residual, y, ids, weights, workspace), y, ids, weights)
     torch = _the_torch()
     dev, f32 = experts.device, torch.float32
     rows = _rows_of(x, experts.in_features)
@@ -781,6 +811,9 @@ def linear_epilogue(fmt, w, out_features: int, in_features: int, x, bias=None, a
                     residual=None, y=None, workspace=None, stream=None):
     """mlq_linear_epilogue: y = residual + row_scale[:, None] * act(x @ W^T + bias);
     activation: None / "none", "silu", "gelu", "gelu_tanh", "relu", "sigmoid"."""
+    if stream is not None and (y is None or workspace is None):
+        return _on_stream(x.device, stream, lambda: linear_epilogue(fmt, w, out_features, in_features, x, bias, activation,
+                                                                    row_scale, residual, y, workspace), y)
     torch = _the_torch()
     act = ACTIVATIONS.get(activation)
     if act is None:

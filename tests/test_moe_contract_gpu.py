@@ -52,3 +52,66 @@ def test_two_passes_stay_in_their_workspace(pkg, c):
     some = [0, first - 1, first, rows - 1]
     want, bound = ref.experts(x[some], ids[some] % 4, w[some], None, "q4_0", "q4_0", gate, up, down, 4, hid, out)
     check(y[some], want, bound, pkg)
+
+
+def test_stream_given_and_nothing_else(pkg):
+    """Outputs and workspace that a call on another stream allocates are not what
+    the current stream has just let go of and still writes, and what that stream is
+    given next is not the call's workspace."""
+    mlq = pkg.mlq
+    rng = np.random.default_rng(4)
+    rows, cin, hid, n, k = 40, 512, 256, 8, 2
+    m = mlq.Experts("q4_0", *(dev(ref.random_blocks(rng, "q4_0", n * r, c)) for r, c in ((hid, cin), (hid, cin), (cin, hid))),
+                    n, cin, hid)
+    router = mlq.Router(dev(rng.standard_normal((n, cin)).astype(np.float32) / 23), k)
+    x = dev(rng.standard_normal((rows, cin)).astype(np.float32))
+    want = [t.clone() for t in mlq.moe_layer(router, m, x)]
+    size = mlq.layer_workspace_bytes(router, m, rows)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    for stream in (side, side.cuda_stream):
+        # blocks of the sizes that the call needs, let go with a write of theirs still to come
+        left = [torch.empty(size, dtype=torch.uint8, device="cuda"), torch.empty(rows, cin, device="cuda"),
+                torch.empty(rows, k, dtype=torch.int32, device="cuda"), torch.empty(rows, k, device="cuda")]
+        torch.cuda._sleep(100_000_000)
+        for t in left:
+            t.view(torch.uint8).fill_(255)
+        gone = {t.data_ptr() for t in left}
+        del left, t
+        got = mlq.moe_layer(router, m, x, stream=stream)
+        assert not gone & {t.data_ptr() for t in got}
+        after = torch.full((size,), 255, dtype=torch.uint8, device="cuda")
+        torch.cuda.synchronize()
+        assert mlq.device_error(0) == 0
+        for a, b in zip(want, (got[0], got[1], got[2])):
+            assert torch.equal(a, b)
+        del got, after
+    # the default stream by its handle, while another one is current
+    with torch.cuda.stream(side):
+        got = mlq.moe_layer(router, m, x, stream=0)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+def test_stream_given_under_capture(pkg):
+    """A captured fork: the call runs on a second stream that joins the capture by
+    events, and takes its workspace from the graph's pool."""
+    mlq = pkg.mlq
+    rng = np.random.default_rng(5)
+    w = dev(ref.random_blocks(rng, "q4_0", 256, 512))
+    x = dev(rng.standard_normal((3, 512)).astype(np.float32))
+    want = mlq.linear_epilogue("q4_0", w, 256, 512, x).clone()
+    torch.cuda.synchronize()
+    side, z = torch.cuda.Stream(), torch.empty(3, 256, device="cuda")
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        side.wait_stream(torch.cuda.current_stream())
+        y = mlq.linear_epilogue("q4_0", w, 256, 512, x, stream=side)
+        torch.cuda.current_stream().wait_stream(side)
+        z.copy_(y)
+    for _ in range(2):
+        z.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(z, want)
+    assert mlq.device_error(0) == 0
