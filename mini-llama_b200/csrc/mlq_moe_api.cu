@@ -75,6 +75,21 @@ mlq_status check_experts(const std::string& who, const mlq_experts* m) {
     return MLQ_OK;
 }
 
+mlq_status check_top_k(const std::string& who, int top_k) {
+    if (top_k <= 0) return fail(MLQ_ERR_EMPTY, who + ": empty tensors are not supported");
+    if (top_k > MLQ_MOE_MAX_TOP_K)
+        return fail(MLQ_ERR_RANGE, who + ": top_k must be at most " + std::to_string(MLQ_MOE_MAX_TOP_K));
+    return MLQ_OK;
+}
+
+// Everything but the block count and the pointers.
+mlq_status check_linear(const std::string& who, int fmt, int out, int in, int rows) {
+    if (!known_format(fmt)) return fail(MLQ_ERR_FORMAT, who + ": unknown block format");
+    if (in <= 0 || out <= 0 || rows <= 0) return fail(MLQ_ERR_EMPTY, who + ": empty tensors are not supported");
+    if (in > kMaxFeatures || out > kMaxOut) return fail(MLQ_ERR_RANGE, who + ": a dimension is too large");
+    return MLQ_OK;
+}
+
 mlq_status check_rows(const std::string& who, int rows, long long per_row) {
     if (rows <= 0) return fail(MLQ_ERR_EMPTY, who + ": empty tensors are not supported");
     if ((long long)rows * per_row > 0x7fffffffLL) return fail(MLQ_ERR_RANGE, who + ": too many rows");
@@ -107,15 +122,14 @@ mlq_status run_experts(const char* who, const mlq_experts& m, const float* x, in
     return e == cudaSuccess ? MLQ_OK : fail_cuda(std::string(who) + " launch", e);
 }
 
-bool valid_router(const mlq_router* r) { return check_router("", r) == MLQ_OK; }
-
 }  // namespace
 
 extern "C" {
 
 MLQ_API size_t mlq_moe_route_workspace_bytes(const mlq_router* router, int rows) {
     try {
-        if (check_router("mlq_moe_route_workspace_bytes", router) != MLQ_OK || rows <= 0) return 0;
+        const char* who = "mlq_moe_route_workspace_bytes";
+        if (check_router(who, router) != MLQ_OK || check_rows(who, rows, router->top_k) != MLQ_OK) return 0;
         return mlq::route_workspace_bytes(router->n_experts, router->in_features, rows);
     } catch (...) {
         return 0;
@@ -140,8 +154,9 @@ MLQ_API mlq_status mlq_moe_route(const mlq_router* router, const float* x, int r
 
 MLQ_API size_t mlq_moe_experts_workspace_bytes(const mlq_experts* experts, int rows, int top_k) {
     try {
-        if (check_experts("mlq_moe_experts_workspace_bytes", experts) != MLQ_OK || rows <= 0 || top_k <= 0 ||
-            top_k > MLQ_MOE_MAX_TOP_K)
+        const char* who = "mlq_moe_experts_workspace_bytes";
+        if (check_experts(who, experts) != MLQ_OK || check_top_k(who, top_k) != MLQ_OK ||
+            check_rows(who, rows, top_k) != MLQ_OK)
             return 0;
         return mlq::experts_workspace_bytes(shape_of(*experts), rows, top_k);
     } catch (...) {
@@ -156,10 +171,8 @@ MLQ_API mlq_status mlq_moe_experts(const mlq_experts* experts, const float* x, i
         const char* who = "mlq_moe_experts";
         mlq_status st = check_experts(who, experts);
         if (st != MLQ_OK) return st;
-        if (top_k <= 0) return fail(MLQ_ERR_EMPTY, std::string(who) + ": empty tensors are not supported");
-        if (top_k > MLQ_MOE_MAX_TOP_K)
-            return fail(MLQ_ERR_RANGE, std::string(who) + ": top_k must be at most " + std::to_string(MLQ_MOE_MAX_TOP_K));
-        st = check_rows(who, rows, top_k);
+        st = check_top_k(who, top_k);
+        if (st == MLQ_OK) st = check_rows(who, rows, top_k);
         if (st != MLQ_OK) return st;
         if (!x || !ids || !weights || !y) return fail(MLQ_ERR_NULL, std::string(who) + ": null input/output pointer");
         st = check_workspace(who, workspace, workspace_bytes,
@@ -173,7 +186,9 @@ MLQ_API mlq_status mlq_moe_experts(const mlq_experts* experts, const float* x, i
 
 MLQ_API size_t mlq_moe_layer_workspace_bytes(const mlq_router* router, const mlq_experts* experts, int rows) {
     try {
-        if (!valid_router(router) || check_experts("mlq_moe_layer_workspace_bytes", experts) != MLQ_OK || rows <= 0)
+        const char* who = "mlq_moe_layer_workspace_bytes";
+        if (check_router(who, router) != MLQ_OK || check_experts(who, experts) != MLQ_OK ||
+            check_rows(who, rows, router->top_k) != MLQ_OK)
             return 0;
         return mlq::route_workspace_bytes(router->n_experts, router->in_features, rows) +
                mlq::experts_workspace_bytes(shape_of(*experts), rows, router->top_k);
@@ -208,8 +223,12 @@ MLQ_API mlq_status mlq_moe_layer(const mlq_router* router, const mlq_experts* ex
 }
 
 MLQ_API size_t mlq_linear_epilogue_workspace_bytes(mlq_format fmt, int out_features, int in_features, int rows) {
-    if (!known_format(fmt) || out_features <= 0 || in_features <= 0 || rows <= 0 || in_features > kMaxFeatures) return 0;
-    return mlq::epilogue_workspace_bytes(in_features, rows);
+    try {
+        if (check_linear("mlq_linear_epilogue_workspace_bytes", fmt, out_features, in_features, rows) != MLQ_OK) return 0;
+        return mlq::epilogue_workspace_bytes(in_features, rows);
+    } catch (...) {
+        return 0;
+    }
 }
 
 MLQ_API mlq_status mlq_linear_epilogue(mlq_format fmt, const void* w, size_t block_count, int out_features,
@@ -217,20 +236,17 @@ MLQ_API mlq_status mlq_linear_epilogue(mlq_format fmt, const void* w, size_t blo
                                        float* y, void* workspace, size_t workspace_bytes, mlq_stream stream) {
     try {
         const std::string who = "mlq_linear_epilogue";
-        if (!known_format(fmt)) return fail(MLQ_ERR_FORMAT, who + ": unknown block format");
+        mlq_status st = check_linear(who, fmt, out_features, in_features, rows);
+        if (st != MLQ_OK) return st;
         if (w == nullptr) return fail(MLQ_ERR_NULL, who + ": null weight pointer");
-        if (in_features <= 0 || out_features <= 0 || rows <= 0)
-            return fail(MLQ_ERR_EMPTY, who + ": empty tensors are not supported");
         if (!x || !y || !epilogue) return fail(MLQ_ERR_NULL, who + ": null input/output pointer");
-        if (in_features > kMaxFeatures || out_features > kMaxOut)
-            return fail(MLQ_ERR_RANGE, who + ": a dimension is too large");
         const size_t expected = mlq_block_count(out_features, in_features);
         if (block_count != expected)
             return fail(MLQ_ERR_BLOCK_COUNT, who + ": block count mismatch: expected " + std::to_string(expected) +
                                                  ", got " + std::to_string(block_count));
         if (epilogue->activation < MLQ_ACT_NONE || epilogue->activation > MLQ_ACT_SIGMOID)
             return fail(MLQ_ERR_RANGE, who + ": unknown activation");
-        mlq_status st = check_workspace(who, workspace, workspace_bytes, mlq::epilogue_workspace_bytes(in_features, rows));
+        st = check_workspace(who, workspace, workspace_bytes, mlq::epilogue_workspace_bytes(in_features, rows));
         if (st != MLQ_OK) return st;
         mlq::DeviceFacts f{};
         st = mlq::current_device_facts(&f);

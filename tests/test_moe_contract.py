@@ -80,3 +80,22 @@ def test_ids_of_one_row_serve_one_row_only(pkg):
     for x, i, v in [(torch.zeros(0, 64), ids.view(1, 2)[:0], w.view(1, 2)[:0]), (torch.zeros(1, 64), ids[:0], w[:0])]:
         with pytest.raises(mlq.MLQError):
             mlq.moe_experts(m, x, i, v)
+
+
+def test_a_refused_size_leaves_its_own_message(pkg):
+    """Every size that is 0 says why, whatever failed before on this thread."""
+    mlq, L = pkg.mlq, pkg.mlq._moe_lib()
+    for args, text in [((7, 4, 64, 2), b"format"), ((8, 0, 64, 2), b"empty"), ((8, 4, 0, 2), b"empty"), ((8, 4, 64, 0), b"empty"),
+                       ((8, 4, (1 << 20) + 1, 2), b"too large"), ((8, (1 << 24) + 1, 64, 2), b"too large")]:
+        assert L.mlq_moe_route_workspace_bytes(None, 1) == 0 and b"null router" in L.mlq_last_error()
+        assert L.mlq_linear_epilogue_workspace_bytes(*args) == 0
+        assert b"mlq_linear_epilogue_workspace_bytes" in L.mlq_last_error() and text in L.mlq_last_error()
+    m = experts_struct(mlq, 4, 64, 32, 64)
+    r = mlq.RouterStruct(0x1000, None, 4, 64, 2, 0, 1, 1.0)
+    for call in (lambda: L.mlq_moe_experts_workspace_bytes(m, 0, 2), lambda: L.mlq_moe_experts_workspace_bytes(m, 3, 0),
+                 lambda: L.mlq_moe_experts_workspace_bytes(m, 3, 65), lambda: L.mlq_moe_route_workspace_bytes(r, 0),
+                 lambda: L.mlq_moe_layer_workspace_bytes(r, m, -1)):
+        assert L.mlq_linear_epilogue_workspace_bytes(7, 4, 64, 2) == 0
+        assert call() == 0 and b"format" not in L.mlq_last_error()
+    assert L.mlq_moe_layer_workspace_bytes(None, m, 3) == 0
+    assert b"mlq_moe_layer_workspace_bytes: null router" in L.mlq_last_error()
