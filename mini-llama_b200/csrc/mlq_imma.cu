@@ -166,7 +166,7 @@ __global__ void __launch_bounds__(256) prep_kernel(const PrepArgs a) {
         const float* x = a.x + (long long)r * a.in;
         uint8_t* row = a.sliced + (size_t)r * (a.bprp / kChunkBlocks) * kRecordBytes;
         const int at = b * kQK + imma_element(a.fmt, b & 1, lane);
-        slice_digits(at < a.in ? x[at] : 0.0f, digit_weight(a.fmt, lane), row, b, lane);
+        slice_digits(at < a.in ? x[at] : 0.0f, row, b, lane);
     }
 }
 

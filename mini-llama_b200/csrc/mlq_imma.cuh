@@ -11,10 +11,9 @@
 //   instructions: one covers exactly one block of 16 weight rows, its 8 columns are
 //   the digits of 2 rows of x, every integer sum is exact, and one fp32 fold per
 //   block applies d and the block's scale of x.  q8_0 codes are
-//   the operand as they are.  q4 codes are unsigned bytes, c from the low nibble
-//   and 16 c from the high one (one mask each); the values of x that meet low
-//   nibbles are carried 16-fold instead, and q4_0's offset of 8 is taken off by
-//   the block's sum of x, in the fold.
+//   the operand as they are.  q4 codes are unsigned bytes 16 c (a mask for the high
+//   nibbles, a shift and a mask for the low ones), and q4_0's offset of 8 is taken off
+//   by the block's sum of x, in the fold.
 // * more rows: x_i / s = hi + lo in fp16 (error <= 2^-22 |x_i|, s a power of
 //   two per 64 values of a row), and d c too (exact: at most 19 bits; q4_1's
 //   d c + m to 22 bits), with a power of two per 64 values of a weight row.  tcgen05
@@ -72,10 +71,10 @@ __device__ __forceinline__ int tile_element(int fmt, int p) {
 }
 
 // A sliced row of x is a sequence of records, one per K step: 8 blocks of
-// digits, their scales, their sums of x.  One bulk copy brings a record to
+// digits, their scales, their means of x.  One bulk copy brings a record to
 // shared memory.
 constexpr int kRecordBytes = kChunkBlocks * (kSlicedBytes + 8);
-constexpr int kRecordScales = kChunkBlocks * kSlicedBytes, kRecordSums = kRecordScales + kChunkBlocks * 4;
+constexpr int kRecordScales = kChunkBlocks * kSlicedBytes, kRecordMeans = kRecordScales + kChunkBlocks * 4;
 
 // Where block b of a row's records has its digits (see slice_digits).
 __host__ __device__ constexpr int digit_block(int b) {
@@ -107,21 +106,15 @@ __device__ __forceinline__ float warp_sum(float v) {
     return v;
 }
 
-// What the value at position l of a sliced q4 block is multiplied with: low
-// nibbles (the first 16 positions) meet 16 x, high ones, which count 16, x.
-__device__ __forceinline__ float digit_weight(int fmt, int l) { return fmt != kQ8_0 && l < 16 ? 16.0f : 1.0f; }
-
-// Slices a block into digits: lane l holds the value at imma_element l, times
-// `weight` in the digits (digit_weight).  Two blocks share 256 bytes, [digit]
-// [t][block of the pair][word h].  A block with a value that is not finite gets
+// Slices a block into digits: lane l holds the value at imma_element l.  Two
+// blocks share 256 bytes, [digit][t][block of the pair][word h].  A block with a value that is not finite gets
 // the scale NaN: every output that reads it is NaN.
 // row: the row's first record, b the block.
-__device__ __forceinline__ void slice_digits(float x, float weight, uint8_t* row, int b, int lane) {
-    const float v = x * weight;
-    const float amax = block_amax(v);
+__device__ __forceinline__ void slice_digits(float x, uint8_t* row, int b, int lane) {
+    const float amax = block_amax(x);
     const bool bad = !(amax == amax);
     const uint32_t s = block_scale(bad ? 0.0f : amax, 30, 2139062016.0f);  // below 127 * 16843009: four digits hold it
-    const int q = bad ? 0 : __float2int_rn(v * __uint_as_float(s));
+    const int q = bad ? 0 : __float2int_rn(x * __uint_as_float(s));
     const int d0 = (int)(int8_t)(q & 0xff);
     const int q1 = (q - d0) >> 8;
     const int d1 = (int)(int8_t)(q1 & 0xff);
@@ -140,7 +133,7 @@ __device__ __forceinline__ void slice_digits(float x, float weight, uint8_t* row
     }
     const int h = lane >> 4, t = (lane >> 2) & 3;
     *reinterpret_cast<uint32_t*>(row + digit_block(b) + j * 64 + t * 16 + h * 4) = out;
-    const float total = warp_sum(x);
+    const float total = warp_sum(x * (1.0f / kQK));  // the mean: 32 finite values may have a sum that is not
     if (lane == 0) {
         float* at = reinterpret_cast<float*>(row + (b / kChunkBlocks) * kRecordBytes + kRecordScales) + b % kChunkBlocks;
         at[0] = bad ? __uint_as_float(0x7fc00000u) : inverse_scale(s);
@@ -329,7 +322,7 @@ template <int F>
 __device__ __forceinline__ void int8_operand(const RawA& r, uint32_t (&a)[4]) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        a[i] = F == kQ8_0 ? r.w[i][0] : r.w[i][0] & 0x0f0f0f0fu;
+        a[i] = F == kQ8_0 ? r.w[i][0] : r.w[i][0] << 4 & 0xf0f0f0f0u;
         a[2 + i] = F == kQ8_0 ? r.w[i][1] : r.w[i][0] & 0xf0f0f0f0u;
     }
 }

@@ -50,7 +50,7 @@ struct FewRows {
     template <bool ALN>
     __device__ __forceinline__ void step(uint32_t x, int valid, uint32_t r0, uint32_t r1, int lane) {
         const RowBase rows = row_base(r0, r1, lane & 3);
-        const float offset = lane & 1 ? 0.0f : (F == kQ4_0 ? -8.0f : 1.0f) * 16.0f / 65536.0f;
+        const float offset = lane & 1 ? 0.0f : (F == kQ4_0 ? -8.0f : 1.0f) * kQK * 16.0f / 65536.0f;
         static_for<kChunkBlocks / 2>([&](auto pc) {
             constexpr int p = decltype(pc)::value;
             if (!ALN && 2 * p >= valid) return;
@@ -474,8 +474,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         const int loc = 32 * (i % blocks) + el;
                         const int row = (loc >> 3) * 16 + (loc & 7);
                         const float h = 32 * b + el < a.out ? silu_mul(get(tok, row), get(tok, row + 8)) : 0.0f;
-                        slice_digits(h, digit_weight(a.next_fmt, lane),
-                                     a.h + (size_t)(first + tok) * (a.next_bprp / kChunkBlocks) * kRecordBytes, b, lane);
+                        slice_digits(h, a.h + (size_t)(first + tok) * (a.next_bprp / kChunkBlocks) * kRecordBytes, b, lane);
                     }
                 } else {
                     for (int i = tid; i < unit_rows * count; i += kTeamThreads) {
