@@ -11,9 +11,10 @@
 //   instructions: one covers exactly one block of 16 weight rows, its 8 columns are
 //   the digits of 2 rows of x, every integer sum is exact, and one fp32 fold per
 //   block applies d and the block's scale of x.  q8_0 codes are
-//   the operand as they are.  q4 codes are unsigned bytes 16 c (a mask for the high
-//   nibbles, a shift and a mask for the low ones), and q4_0's offset of 8 is taken off
-//   by the block's sum of x, in the fold.
+//   the operand as they are.  q4 codes are bytes 16 c (a mask for the high
+//   nibbles, a shift and a mask for the low ones): unsigned in q4_1, in q4_0 signed 16 (c - 8),
+//   which is the same byte with its highest bit changed, so that a weight of 0 adds
+//   exactly nothing however large its x is.
 // * more rows: x_i / s = hi + lo in fp16 (error <= 2^-22 |x_i|, s a power of
 //   two per 64 values of a row), and d c too (exact: at most 19 bits; q4_1's
 //   d c + m to 22 bits), with a power of two per 64 values of a weight row.  tcgen05
@@ -168,10 +169,10 @@ __device__ __forceinline__ Sliced64 slice_64(float v0, float v1) {
     return r;
 }
 
-// D = A B for 16 rows x 32 codes, signed (q8_0) or unsigned (q4), and digits.
+// D = A B for 16 rows x 32 codes, signed or unsigned (q4_1), and digits.
 template <int F>
 __device__ __forceinline__ void imma(int (&c)[4], const uint32_t (&a)[4], uint2 b) {
-    if constexpr (F == kQ8_0)
+    if constexpr (F != kQ4_1)
         asm volatile(
             "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
             : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
@@ -322,8 +323,9 @@ template <int F>
 __device__ __forceinline__ void int8_operand(const RawA& r, uint32_t (&a)[4]) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        a[i] = F == kQ8_0 ? r.w[i][0] : r.w[i][0] << 4 & 0xf0f0f0f0u;
-        a[2 + i] = F == kQ8_0 ? r.w[i][1] : r.w[i][0] & 0xf0f0f0f0u;
+        constexpr uint32_t sign = F == kQ4_0 ? 0x80808080u : 0u;
+        a[i] = F == kQ8_0 ? r.w[i][0] : (r.w[i][0] << 4 & 0xf0f0f0f0u) ^ sign;
+        a[2 + i] = F == kQ8_0 ? r.w[i][1] : (r.w[i][0] & 0xf0f0f0f0u) ^ sign;
     }
 }
 

@@ -50,7 +50,8 @@ struct FewRows {
     template <bool ALN>
     __device__ __forceinline__ void step(uint32_t x, int valid, uint32_t r0, uint32_t r1, int lane) {
         const RowBase rows = row_base(r0, r1, lane & 3);
-        const float offset = lane & 1 ? 0.0f : (F == kQ4_0 ? -8.0f : 1.0f) * kQK * 16.0f / 65536.0f;
+        // q4_1: a block's sum of x from its mean, in the unit of digits 3 and 2 (see store); lanes of digits 1, 0 take none
+        const float to_sum = lane & 1 ? 0.0f : kQK * 16.0f / 65536.0f;
         static_for<kChunkBlocks / 2>([&](auto pc) {
             constexpr int p = decltype(pc)::value;
             if (!ALN && 2 * p >= valid) return;
@@ -60,7 +61,7 @@ struct FewRows {
             for (int i = 0; i < NT; ++i) {
                 b[i] = lds_u4_at<256 * p>(x + xo[i]);
                 s[i] = lds_f2_at<8 * p>(x + so[i]);
-                if (F != kQ8_0) m[i] = lds_f2_at<8 * p + 4 * kChunkBlocks>(x + so[i]);
+                if (F == kQ4_1) m[i] = lds_f2_at<8 * p + 4 * kChunkBlocks>(x + so[i]);
             }
             RawA A[2];
             load_pair<F, ALN, p>(rows, A[0], A[1]);
@@ -72,17 +73,15 @@ struct FewRows {
 #pragma unroll
                 for (int i = 0; i < NT; ++i) {
                     const float sx = o ? s[i].y : s[i].x;
-                    const float mx = F == kQ8_0 ? 0.0f : (o ? m[i].y : m[i].x);
+                    const float mx = F == kQ4_1 ? (o ? m[i].y : m[i].x) : 0.0f;
                     int c[4];
                     imma<F>(c, op, o ? make_uint2(b[i].z, b[i].w) : make_uint2(b[i].x, b[i].y));
                     const float v[2] = {(float)(c[0] * 256 + c[1]), (float)(c[2] * 256 + c[3])};
 #pragma unroll
                     for (int q = 0; q < 2; ++q) {
-                        // q4_0: sum of (c - 8) x, in the unit of digits 3 and 2 (see store); lanes of digits 1, 0 take none.
                         // q4_1: the block's d c x and m x cancel each other for the most part, so they meet in one sum
-                        const float u = F == kQ4_0 ? fmaf(v[q], sx, mx * offset) : v[q] * sx;
-                        acc[i][q] = fmaf(A[o].d[q], u, acc[i][q]);
-                        if (F == kQ4_1) acc[i][q] = fmaf(A[o].m[q], mx * offset, acc[i][q]);
+                        acc[i][q] = fmaf(A[o].d[q], v[q] * sx, acc[i][q]);
+                        if (F == kQ4_1) acc[i][q] = fmaf(A[o].m[q], mx * to_sum, acc[i][q]);
                     }
                 }
             }

@@ -68,3 +68,56 @@ def test_largest_finite_hidden_values(pkg, fmt, rows):
     assert 2.0 ** 124 < hidden(x.astype(np.float64)) < 3e38 and np.abs(want).max() < 3e38
     m = pkg.mlq.Experts(fmt, dev(gate), dev(up), dev(down), 2, cin, hid, out_features=out)
     check(pkg.mlq.moe_experts(m, dev(x), dev(ids), dev(w)), want, bound, pkg)
+
+
+def with_codes(fmt, blocks, rows, cols, channels, code):
+    """`blocks` with `code` at these columns of every row."""
+    nb = (cols + 31) // 32
+    raw = blocks.reshape(rows, nb, ref.BLOCK[fmt]).copy()
+    if fmt == "q8_0":
+        for c in channels:
+            raw[:, c // 32, 2 + c % 32] = code & 255
+        return raw.reshape(-1)
+    at = ref.BLOCK[fmt] - 16
+    for c in channels:
+        b, i = c // 32, c % 32
+        old = raw[:, b, at + i % 16]
+        raw[:, b, at + i % 16] = (old & 0xf0) | code if i < 16 else (old & 0x0f) | (code << 4)
+    return raw.reshape(-1)
+
+
+def tight(x, fmt, blocks, out):
+    """x W^T and the bound of the form of few rows as the header states it:
+    * a value is off by half a step, 1.01 * 2^-31 of its block's largest;
+    * it goes in two parts of 16 bits, together at most |x| + 2^-15 of the block's largest
+      (twice the second part); a block's sum of a part is rounded as it becomes fp32, in the product with
+      the block's scale and in the sum over blocks, and with the parts of the K axis and the store there are at most
+      blocks + 68 roundings of the sum of magnitudes."""
+    w, _ = ref.dequantize64(fmt, blocks, out, x.shape[1])
+    x = x.astype(np.float64)
+    most = ref.block_max(x)
+    parts = np.abs(x) + 2.0 ** -15 * most
+    nb = (x.shape[1] + 31) // 32
+    bound = 1.01 * 2.0 ** -31 * (most @ np.abs(w).T) + (nb + 68) * EPS * (parts @ np.abs(w).T)
+    return x @ w.T, bound + 1e-37
+
+
+
+@pytest.mark.parametrize("strong", [1.0, 1e3, 1e4, 1e5, 1e7])
+@pytest.mark.parametrize("fmt,code", [("q8_0", 0), ("q4_0", 8)])
+def test_a_strong_channel_with_weights_of_zero(pkg, fmt, code, strong):
+    """A channel whose weights are all exactly 0 costs the others only what the
+    fixed point of its own block cannot hold: any place of a block, one row to 12."""
+    rng = np.random.default_rng(int(strong))
+    cin, out = 2048, 256
+    for rows in (1, 2, 4, 7, 12):
+        for channel in (5, 640 + 21, 2047):
+            blocks = with_codes(fmt, ref.random_blocks(rng, fmt, out, cin), out, cin, [channel], code)
+            x = rng.standard_normal((rows, cin)).astype(np.float32)
+            x[:, channel] = strong * rng.choice([-1, 1], rows) * rng.uniform(0.5, 1, rows)
+            want, bound = tight(x, fmt, blocks, out)
+            y = pkg.mlq.linear_epilogue(fmt, dev(blocks), out, cin, dev(x))
+            check(y, want, bound, pkg)
+            if strong <= 1e4:  # half a step of the strong channel's block: below 2e-6 of an ordinary value
+                err = np.linalg.norm(y.cpu().numpy() - want, axis=1) / np.linalg.norm(want, axis=1)
+                assert err.max() <= 1e-6
