@@ -63,7 +63,7 @@ struct PrepArgs {
     int* place;       // many rows: pair -> position, -1: no expert
     // padding blocks of the sliced h
     uint8_t* h;
-    int h_bpr, h_bprp;
+    int h_bpr, h_bprp, h_fmt;
 };
 
 // Pairs by expert (CTA 0), x sliced (one warp per block).  Latency-bound:
@@ -86,9 +86,11 @@ __global__ void __launch_bounds__(256) prep_kernel(const PrepArgs a) {
             const int align = a.positions ? 8 : 1;
             for (int i = threadIdx.x; i < a.pairs * pad; i += 256) {
                 const int b = a.h_bpr + i % pad;
-                float* at = reinterpret_cast<float*>(a.h + ((size_t)(i / pad) * (a.h_bprp / kChunkBlocks) + b / kChunkBlocks) *
-                                                                    kRecordBytes + kRecordScales) + b % kChunkBlocks;
-                at[0] = at[kChunkBlocks] = 0.0f;
+                uint8_t* record = a.h + ((size_t)(i / pad) * (a.h_bprp / kChunkBlocks) + b / kChunkBlocks) * record_bytes(a.h_fmt);
+                reinterpret_cast<float*>(record + kRecordScales)[b % kChunkBlocks] = 0.0f;
+                if (a.h_fmt == kQ4_1)
+                    for (int odd = 0; odd < 2; ++odd)
+                        *reinterpret_cast<float2*>(record + block_sums(b % kChunkBlocks, odd)) = make_float2(0.0f, 0.0f);
             }
             __syncthreads();
 #pragma unroll 8
@@ -164,9 +166,9 @@ __global__ void __launch_bounds__(256) prep_kernel(const PrepArgs a) {
     for (long long i = (long long)first * 8 + warp; i < n; i += (long long)ctas * 8) {
         const int r = (int)(i / a.bprp), b = (int)(i % a.bprp);
         const float* x = a.x + (long long)r * a.in;
-        uint8_t* row = a.sliced + (size_t)r * (a.bprp / kChunkBlocks) * kRecordBytes;
+        uint8_t* row = a.sliced + (size_t)r * (a.bprp / kChunkBlocks) * record_bytes(a.fmt);
         const int at = b * kQK + imma_element(a.fmt, b & 1, lane);
-        slice_digits(at < a.in ? x[at] : 0.0f, row, b, lane);
+        slice_digits(at < a.in ? x[at] : 0.0f, a.fmt, row, b, lane);
     }
 }
 
@@ -259,12 +261,14 @@ struct Carve {
         p += align256(n * sizeof(T));
         return r;
     }
-    uint8_t* take_sliced(size_t rows, int bprp) { return take<uint8_t>(rows * (bprp / kChunkBlocks) * kRecordBytes); }
+    uint8_t* take_sliced(size_t rows, int bprp, int fmt) {
+        return take<uint8_t>(rows * (bprp / kChunkBlocks) * record_bytes(fmt));
+    }
     // Whether what was taken lies within `bytes` bytes from `ws` on.
     bool within(const void* ws, size_t bytes) const { return (size_t)(p - static_cast<const uint8_t*>(ws)) <= bytes; }
 };
 
-size_t sliced_bytes(size_t rows, int bprp) { return align256(rows * (bprp / kChunkBlocks) * kRecordBytes); }
+size_t sliced_bytes(size_t rows, int bprp, int fmt) { return align256(rows * (bprp / kChunkBlocks) * record_bytes(fmt)); }
 
 constexpr size_t kMaxSliced = 1u << 30;   // sliced bytes of one pass at most (offsets are 32 bits)
 constexpr size_t kMaxParts = 1u << 30;    // bytes of the pairs' outputs of one pass at most
@@ -375,11 +379,11 @@ void set_halves(ImmaArgs& a, const HalvesArgs& h) {
 
 }  // namespace
 
-size_t epilogue_workspace_bytes(int in, int rows) {
+size_t epilogue_workspace_bytes(int fmt, int in, int rows) {
     const int n = linear_pass_rows(in, rows);
     // more rows never need less
     const int few_rows = n < kLinearFewRows ? n : kLinearFewRows;
-    const size_t few = sliced_bytes(few_rows, padded_blocks((in + kQK - 1) / kQK)) + split_bytes(true, few_rows);
+    const size_t few = sliced_bytes(few_rows, padded_blocks((in + kQK - 1) / kQK), fmt) + split_bytes(true, few_rows);
     const size_t many = n <= kLinearFewRows ? 0 : halves_bytes(n, groups_of(in)) + split_bytes(false, n);
     return few > many ? few : many;
 }
@@ -398,7 +402,7 @@ cudaError_t launch_linear_epilogue(int fmt, const uint8_t* w, int out, int in, c
         const bool few = n <= kLinearFewRows;
         HalvesArgs hv{};
         if (few)
-            p.sliced = c.take_sliced(n, bprp);
+            p.sliced = c.take_sliced(n, bprp, fmt);
         else
             hv = halves_args(c, p.x, n, n, in, fmt);
         float* split = c.take<float>(split_floats(few, n, kImmaWarps) * split_count(few));
@@ -442,7 +446,8 @@ size_t experts_workspace_bytes(const MoeShape& s, int rows, int top_k) {
         const bool few = few_rows(pairs, s.n_experts);
         const size_t lists = 256 + align256((size_t)segment_places(few, pairs, s.n_experts) * sizeof(Segment));
         if (few)
-            return lists + align256((size_t)pairs * sizeof(int)) + sliced_bytes(n, bprp) + sliced_bytes(pairs, hp) +
+            return lists + align256((size_t)pairs * sizeof(int)) + sliced_bytes(n, bprp, s.fmt) +
+                   sliced_bytes(pairs, hp, s.fmt_down) +
                    (n <= kCombineRows ? 0 : align256((size_t)pairs * s.out * sizeof(float))) + split_bytes(few, n);
         const int positions = many_positions(pairs, s.n_experts);
         return lists + align256((size_t)positions * sizeof(int)) + align256((size_t)pairs * sizeof(int)) +
@@ -491,9 +496,9 @@ cudaError_t launch_experts(const MoeShape& s, const uint8_t* gate, const uint8_t
         p.pairs = pairs, p.n_experts = s.n_experts;
         if (few) {
             p.rows = n;
-            p.sliced = c.take_sliced(n, bprp);
-            p.h = c.take_sliced(pairs, hp);
-            p.h_bpr = hb, p.h_bprp = hp;
+            p.sliced = c.take_sliced(n, bprp, s.fmt);
+            p.h = c.take_sliced(pairs, hp, s.fmt_down);
+            p.h_bpr = hb, p.h_bprp = hp, p.h_fmt = s.fmt_down;
         } else {
             p.place = c.take<int>(pairs);
             hx = halves_args(c, p.x, n, p.positions, s.in, s.fmt);

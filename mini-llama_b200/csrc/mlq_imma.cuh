@@ -14,7 +14,9 @@
 //   the operand as they are.  q4 codes are bytes 16 c (a mask for the high
 //   nibbles, a shift and a mask for the low ones): unsigned in q4_1, in q4_0 signed 16 (c - 8),
 //   which is the same byte with its highest bit changed, so that a weight of 0 adds
-//   exactly nothing however large its x is.
+//   exactly nothing however large its x is.  q4_1's two parts, d sum(c x) and m sum(x), cancel
+//   each other where a weight is near 0, so the sums of x's digits are integers too and meet
+//   the other part in fused steps that round only what is left (FewRows::step).
 // * more rows: x_i / s = hi + lo in fp16 (error <= 2^-22 |x_i|, s a power of
 //   two per 64 values of a row), and d c too (exact: at most 19 bits; q4_1's
 //   d c + m to 22 bits), with a power of two per 64 values of a weight row.  tcgen05
@@ -72,15 +74,18 @@ __device__ __forceinline__ int tile_element(int fmt, int p) {
 }
 
 // A sliced row of x is a sequence of records, one per K step: 8 blocks of
-// digits, their scales, their means of x.  One bulk copy brings a record to
-// shared memory.
-constexpr int kRecordBytes = kChunkBlocks * (kSlicedBytes + 8);
-constexpr int kRecordScales = kChunkBlocks * kSlicedBytes, kRecordMeans = kRecordScales + kChunkBlocks * 4;
+// digits, their scales and, for q4_1, their sums of digits (block_sums).  One bulk
+// copy brings a record to shared memory.
+__host__ __device__ constexpr int record_bytes(int fmt) { return kChunkBlocks * (kSlicedBytes + (fmt == kQ4_1 ? 20 : 4)); }
+constexpr int kRecordScales = kChunkBlocks * kSlicedBytes, kRecordSums = kRecordScales + kChunkBlocks * 4;
 
-// Where block b of a row's records has its digits (see slice_digits).
-__host__ __device__ constexpr int digit_block(int b) {
-    return (b / kChunkBlocks) * kRecordBytes + (b % kChunkBlocks / 2) * 2 * kSlicedBytes + (b & 1) * 8;
-}
+// Where block b of a record has its digits (see slice_digits).
+__host__ __device__ constexpr int digit_block(int b) { return (b / 2) * 2 * kSlicedBytes + (b & 1) * 8; }
+
+// And its sums of digits, for digits 3, 2 or 1, 0 (odd): two floats, of the
+// higher digit and of the lower one, in the unit of a sum of codes 16 c with
+// digits.  Two blocks share 32 bytes, [odd][block of the pair].
+__host__ __device__ constexpr int block_sums(int b, int odd) { return kRecordSums + (b / 2) * 32 + odd * 16 + (b & 1) * 8; }
 
 // The power of two 2^k whose product with amax is in (limit / 2, limit], as
 // bits; top: floor(log2 limit).  Clamped so that 2^-k is a normal number.
@@ -102,16 +107,13 @@ __device__ __forceinline__ float block_amax(float v) {
     return bad ? __uint_as_float(0x7fc00000u) : amax;
 }
 
-__device__ __forceinline__ float warp_sum(float v) {
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
-}
-
 // Slices a block into digits: lane l holds the value at imma_element l.  Two
-// blocks share 256 bytes, [digit][t][block of the pair][word h].  A block with a value that is not finite gets
-// the scale NaN: every output that reads it is NaN.
-// row: the row's first record, b the block.
-__device__ __forceinline__ void slice_digits(float x, uint8_t* row, int b, int lane) {
+// blocks share 256 bytes, [digit][t][block of the pair][word h].  A block with a
+// value that is not finite gets the scale NaN: every output that reads it is NaN.
+// row: the row's first record, of format fmt; b: the block.
+__device__ __forceinline__ void slice_digits(float x, int fmt, uint8_t* row, int b, int lane) {
+    row += (size_t)(b / kChunkBlocks) * record_bytes(fmt);
+    b %= kChunkBlocks;
     const float amax = block_amax(x);
     const bool bad = !(amax == amax);
     const uint32_t s = block_scale(bad ? 0.0f : amax, 30, 2139062016.0f);  // below 127 * 16843009: four digits hold it
@@ -134,11 +136,15 @@ __device__ __forceinline__ void slice_digits(float x, uint8_t* row, int b, int l
     }
     const int h = lane >> 4, t = (lane >> 2) & 3;
     *reinterpret_cast<uint32_t*>(row + digit_block(b) + j * 64 + t * 16 + h * 4) = out;
-    const float total = warp_sum(x * (1.0f / kQK));  // the mean: 32 finite values may have a sum that is not
-    if (lane == 0) {
-        float* at = reinterpret_cast<float*>(row + (b / kChunkBlocks) * kRecordBytes + kRecordScales) + b % kChunkBlocks;
-        at[0] = bad ? __uint_as_float(0x7fc00000u) : inverse_scale(s);
-        at[kChunkBlocks] = total;
+    if (lane == 0) reinterpret_cast<float*>(row + kRecordScales)[b] = bad ? __uint_as_float(0x7fc00000u) : inverse_scale(s);
+    if (fmt == kQ4_1) {
+        // |sum of 32 digits| <= 4096: two sums in a word
+        const int high = __reduce_add_sync(0xffffffffu, d3 * 65536 + d2), low = __reduce_add_sync(0xffffffffu, d1 * 65536 + d0);
+        if (lane < 2) {
+            const int both = lane == 0 ? high : low, second = (int)(int16_t)(both & 0xffff), first = (both - second) >> 16;
+            float* at = reinterpret_cast<float*>(row + block_sums(b, lane));
+            at[0] = (float)first * 4096.0f, at[1] = (float)second * 16.0f;
+        }
     }
 }
 
@@ -247,6 +253,15 @@ template <int OFF>
 __device__ __forceinline__ float lds_f1_at(uint32_t a) {
     float v;
     asm volatile("ld.shared.f32 %0, [%1+%2];" : "=f"(v) : "r"(a), "n"(OFF));
+    return v;
+}
+
+template <int OFF>
+__device__ __forceinline__ float4 lds_f4_at(uint32_t a) {
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4+%5];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(a), "n"(OFF));
     return v;
 }
 

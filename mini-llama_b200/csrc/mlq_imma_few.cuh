@@ -32,7 +32,7 @@ namespace {
 template <int F, int NT>
 struct FewRows {
     uint32_t xo[NT], so[NT];  // a lane's digits and scales in the step's records
-    float acc[NT][2];
+    uint64_t acc[NT];         // of the lane's two weight rows
 
     __device__ __forceinline__ void init(int count, int lane) {
         const int g = lane >> 2, t = lane & 3;
@@ -40,9 +40,9 @@ struct FewRows {
         for (int i = 0; i < NT; ++i) {
             // columns without a row of x repeat the first one's; nothing reads them
             const int r = 2 * i + (g >> 2), rs = 2 * i + (t >> 1);
-            xo[i] = (r < count ? r : 0) * kRecordBytes + (g & 3) * 64 + t * 16;
-            so[i] = (rs < count ? rs : 0) * kRecordBytes + kRecordScales;
-            acc[i][0] = acc[i][1] = 0.0f;
+            xo[i] = (r < count ? r : 0) * record_bytes(F) + (g & 3) * 64 + t * 16;
+            so[i] = (rs < count ? rs : 0) * record_bytes(F);
+            acc[i] = 0;
         }
     }
 
@@ -50,18 +50,18 @@ struct FewRows {
     template <bool ALN>
     __device__ __forceinline__ void step(uint32_t x, int valid, uint32_t r0, uint32_t r1, int lane) {
         const RowBase rows = row_base(r0, r1, lane & 3);
-        // q4_1: a block's sum of x from its mean, in the unit of digits 3 and 2 (see store); lanes of digits 1, 0 take none
-        const float to_sum = lane & 1 ? 0.0f : kQK * 16.0f / 65536.0f;
+        [[maybe_unused]] const uint32_t sums = x + block_sums(0, lane & 1);
         static_for<kChunkBlocks / 2>([&](auto pc) {
             constexpr int p = decltype(pc)::value;
             if (!ALN && 2 * p >= valid) return;
             uint4 b[NT];
-            float2 s[NT], m[NT];
+            float2 s[NT];
+            [[maybe_unused]] float4 sum[NT];  // q4_1: the pair's sums of the lane's digits
 #pragma unroll
             for (int i = 0; i < NT; ++i) {
                 b[i] = lds_u4_at<256 * p>(x + xo[i]);
-                s[i] = lds_f2_at<8 * p>(x + so[i]);
-                if (F == kQ4_1) m[i] = lds_f2_at<8 * p + 4 * kChunkBlocks>(x + so[i]);
+                s[i] = lds_f2_at<8 * p + kRecordScales>(x + so[i]);
+                if (F == kQ4_1) sum[i] = lds_f4_at<32 * p>(sums + so[i]);
             }
             RawA A[2];
             load_pair<F, ALN, p>(rows, A[0], A[1]);
@@ -70,18 +70,22 @@ struct FewRows {
             for (int o = 0; o < 2; ++o) {
                 uint32_t op[4];
                 int8_operand<F>(A[o], op);
+                const uint64_t d = pack2(A[o].d[0], A[o].d[1]);
+                [[maybe_unused]] const uint64_t m = F == kQ4_1 ? pack2(A[o].m[0], A[o].m[1]) : 0;
 #pragma unroll
                 for (int i = 0; i < NT; ++i) {
                     const float sx = o ? s[i].y : s[i].x;
-                    const float mx = F == kQ4_1 ? (o ? m[i].y : m[i].x) : 0.0f;
                     int c[4];
                     imma<F>(c, op, o ? make_uint2(b[i].z, b[i].w) : make_uint2(b[i].x, b[i].y));
-                    const float v[2] = {(float)(c[0] * 256 + c[1]), (float)(c[2] * 256 + c[3])};
-#pragma unroll
-                    for (int q = 0; q < 2; ++q) {
-                        // q4_1: the block's d c x and m x cancel each other for the most part, so they meet in one sum
-                        acc[i][q] = fmaf(A[o].d[q], v[q] * sx, acc[i][q]);
-                        if (F == kQ4_1) acc[i][q] = fmaf(A[o].m[q], mx * to_sum, acc[i][q]);
+                    const uint64_t v = pack2((float)(c[0] * 256 + c[1]), (float)(c[2] * 256 + c[3])), sx2 = pack2(sx, sx);
+                    if constexpr (F == kQ4_1) {
+                        // d v + m sum: m times the higher digits' sum is exact (11 and 12 bits), so the first step
+                        // rounds what the parts leave of each other, and the second adds the lower digits' share
+                        const float2 t = o ? make_float2(sum[i].z, sum[i].w) : make_float2(sum[i].x, sum[i].y);
+                        const uint64_t left = fma2(d, v, mul2(m, pack2(t.x, t.x)));
+                        acc[i] = fma2(fma2(m, pack2(t.y, t.y), left), sx2, acc[i]);
+                    } else {
+                        acc[i] = fma2(d, mul2(v, sx2), acc[i]);
                     }
                 }
             }
@@ -94,19 +98,21 @@ struct FewRows {
         // digits 3 and 2 count 2^16 times digits 1 and 0; q4 codes count 16
         const float f = (t & 1 ? 1.0f : 65536.0f) * (F == kQ8_0 ? 1.0f : 0.0625f);
 #pragma unroll
-        for (int i = 0; i < NT; ++i)
+        for (int i = 0; i < NT; ++i) {
+            const float2 both = unpack2(acc[i]);
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
-                float v = acc[i][q] * f;
+                float v = (q ? both.y : both.x) * f;
                 v += __shfl_xor_sync(0xffffffffu, v, 1);
                 if (!(t & 1)) red[(2 * i + (t >> 1)) * 16 + 8 * q + (lane >> 2)] = v;
             }
+        }
     }
 };
 
 constexpr int kTeams = 2;
 // Records of a round: (K parts) x (rows of x of a segment) <= 8, see choose_strips.
-constexpr int kXStage = 8 * kRecordBytes;
+constexpr int x_stage(int fmt) { return 8 * record_bytes(fmt); }
 constexpr int kThreads = 32 * kTeams * (kImmaWarps + 2);  // computing warps, then two producer warps per team
 constexpr int kTeamThreads = 32 * kImmaWarps;
 // Registers: the launch has 96 per thread (65536 / 640, in eights); the
@@ -201,7 +207,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int per_seg = (steps + kws - 1) / kws;  // rounds of a tile against a segment
     // shared memory: stages [team][stage] of the warps' weights and the rounds' records of x, sums [team], (all_segs) y
     // [team], the stages' barriers [team][stage] (full, empty)
-    constexpr uint32_t kStage = kImmaWarps * S::kBytes + kXStage;
+    constexpr uint32_t kRecord = record_bytes(F), kStage = kImmaWarps * S::kBytes + x_stage(F);
     const uint32_t red0 = kTeams * a.slots * kStage;
     const uint32_t y_floats = MODE == kDown && !a.part ? a.rows * 16 * a.strips : 0;
     const uint32_t bars0 = smem_u32(smem) + red0 + kTeams * (2 * kRedFloats + y_floats) * 4;
@@ -269,7 +275,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint32_t full = bars + 16 * c.stage, dst = ring + c.stage * kStage;
             if constexpr (ALN) {
                 if (lane == 0)
-                    mbar_arrive_expect_tx(full, active(c) * (a.strips * S::kBytes + c.count * kRecordBytes));
+                    mbar_arrive_expect_tx(full, active(c) * (a.strips * S::kBytes + c.count * kRecord));
                 __syncwarp();
                 const int kw = lane / a.strips;
                 if (kw < active(c)) {
@@ -284,7 +290,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 __syncwarp();
             } else {
-                if (half == 0 && lane == 0) mbar_expect_tx(full, active(c) * c.count * kRecordBytes);
+                if (half == 0 && lane == 0) mbar_expect_tx(full, active(c) * c.count * kRecord);
                 // lanes 2r, 2r + 1: the windows that hold row r's blocks
                 const int r = lane >> 1, sub = lane & 1;
                 const uint8_t* base = MODE == kPair && r >= 8 ? a.w[1] : a.w[0];
@@ -329,8 +335,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int kw = lane / a.seg_cap, r = lane % a.seg_cap;
             if (kw < active(c) && r < c.count) {
                 const int row = MODE == kPair ? __ldcg(a.order + c.first + r) / a.top_k : c.first + r;
-                bulk_g2s(ring + c.stage * kStage + kImmaWarps * S::kBytes + lane * kRecordBytes,
-                         a.x + ((size_t)row * (a.bprp / kChunkBlocks) + c.round * kws + kw) * kRecordBytes, kRecordBytes,
+                bulk_g2s(ring + c.stage * kStage + kImmaWarps * S::kBytes + lane * kRecord,
+                         a.x + ((size_t)row * (a.bprp / kChunkBlocks) + c.round * kws + kw) * kRecord, kRecord,
                          bars + 16 * c.stage);
             }
             __syncwarp();
@@ -423,7 +429,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             UnitArgs u{};
             u.red = rb + warp * kFewRows * 16;
             u.full = bars, u.slots = ring + warp * S::kBytes, u.stages = a.slots, u.stage_bytes = kStage;
-            u.to_x = (kImmaWarps - warp) * S::kBytes + kw * a.seg_cap * kRecordBytes;
+            u.to_x = (kImmaWarps - warp) * S::kBytes + kw * a.seg_cap * kRecord;
             u.count = count;
             u.c0 = r0 * kws + kw, u.kws = kws, u.rounds = r1 - r0, u.blocks = a.bpr;
             u.c_end = r1 * kws < steps ? r1 * kws : steps;
@@ -473,7 +479,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                         const int loc = 32 * (i % blocks) + el;
                         const int row = (loc >> 3) * 16 + (loc & 7);
                         const float h = 32 * b + el < a.out ? silu_mul(get(tok, row), get(tok, row + 8)) : 0.0f;
-                        slice_digits(h, a.h + (size_t)(first + tok) * (a.next_bprp / kChunkBlocks) * kRecordBytes, b, lane);
+                        slice_digits(h, a.next_fmt,
+                                     a.h + (size_t)(first + tok) * (a.next_bprp / kChunkBlocks) * record_bytes(a.next_fmt), b,
+                                     lane);
                     }
                 } else {
                     for (int i = tid; i < unit_rows * count; i += kTeamThreads) {
@@ -543,7 +551,7 @@ cudaError_t launch_one(ImmaArgs a, int grid, int smem_per_sm, cudaStream_t strea
     auto k = imma_few_kernel<F, MODE, ALN>;
     const int sums = kTeams * (2 * kRedFloats + (MODE == kDown && !a.part ? a.rows * 16 * a.strips : 0)) * 4;
     const int fixed = sums + 1024 + 256;  // the system's 1 KB per CTA, the static part
-    constexpr int stage = kImmaWarps * S::kBytes + kXStage;
+    constexpr int stage = kImmaWarps * S::kBytes + x_stage(F);
     a.slots = (smem_per_sm - fixed) / (kTeams * (stage + 16));
     if (a.slots > 8) a.slots = 8;
     if (a.slots < 2) return cudaErrorInvalidConfiguration;

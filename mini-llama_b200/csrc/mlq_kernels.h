@@ -228,7 +228,7 @@ cudaError_t launch_experts(const MoeShape& s, const uint8_t* gate, const uint8_t
                            const float* x, int rows, int top_k, const int32_t* ids, const float* weights,
                            const float* residual, float* y, void* ws, size_t ws_bytes, int sm_count, int smem_per_sm,
                            int* err, cudaStream_t stream);
-size_t epilogue_workspace_bytes(int in, int rows);
+size_t epilogue_workspace_bytes(int fmt, int in, int rows);
 cudaError_t launch_linear_epilogue(int fmt, const uint8_t* w, int out, int in, const float* x, int rows,
                                    const mlq_epilogue& ep, float* y, void* ws, size_t ws_bytes, int sm_count,
                                    int smem_per_sm, int* err, cudaStream_t stream);

@@ -225,7 +225,7 @@ MLQ_API mlq_status mlq_moe_layer(const mlq_router* router, const mlq_experts* ex
 MLQ_API size_t mlq_linear_epilogue_workspace_bytes(mlq_format fmt, int out_features, int in_features, int rows) {
     try {
         if (check_linear("mlq_linear_epilogue_workspace_bytes", fmt, out_features, in_features, rows) != MLQ_OK) return 0;
-        return mlq::epilogue_workspace_bytes(in_features, rows);
+        return mlq::epilogue_workspace_bytes(fmt, in_features, rows);
     } catch (...) {
         return 0;
     }
@@ -246,7 +246,7 @@ MLQ_API mlq_status mlq_linear_epilogue(mlq_format fmt, const void* w, size_t blo
                                                  ", got " + std::to_string(block_count));
         if (epilogue->activation < MLQ_ACT_NONE || epilogue->activation > MLQ_ACT_SIGMOID)
             return fail(MLQ_ERR_RANGE, who + ": unknown activation");
-        st = check_workspace(who, workspace, workspace_bytes, mlq::epilogue_workspace_bytes(in_features, rows));
+        st = check_workspace(who, workspace, workspace_bytes, mlq::epilogue_workspace_bytes(fmt, in_features, rows));
         if (st != MLQ_OK) return st;
         mlq::DeviceFacts f{};
         st = mlq::current_device_facts(&f);

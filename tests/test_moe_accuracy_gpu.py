@@ -70,14 +70,19 @@ def test_largest_finite_hidden_values(pkg, fmt, rows):
     check(pkg.mlq.moe_experts(m, dev(x), dev(ids), dev(w)), want, bound, pkg)
 
 
-def with_codes(fmt, blocks, rows, cols, channels, code):
-    """`blocks` with `code` at these columns of every row."""
+def with_codes(fmt, blocks, rows, cols, channels, code, m_of_d=None):
+    """`blocks` with `code` at these columns of every row; m_of_d: q4_1's m as that
+    multiple of d (exact in fp16: d gets 7 bits first)."""
     nb = (cols + 31) // 32
     raw = blocks.reshape(rows, nb, ref.BLOCK[fmt]).copy()
     if fmt == "q8_0":
         for c in channels:
             raw[:, c // 32, 2 + c % 32] = code & 255
         return raw.reshape(-1)
+    if m_of_d is not None:
+        d = raw[:, :, 0:2].copy().view(np.uint16) & 0xfff0
+        raw[:, :, 0:2] = d.view(np.uint8)
+        raw[:, :, 2:4] = (d.view(np.float16) * np.float16(m_of_d)).view(np.uint8)
     at = ref.BLOCK[fmt] - 16
     for c in channels:
         b, i = c // 32, c % 32
@@ -92,27 +97,39 @@ def tight(x, fmt, blocks, out):
     * it goes in two parts of 16 bits, together at most |x| + 2^-15 of the block's largest
       (twice the second part); a block's sum of a part is rounded as it becomes fp32, in the product with
       the block's scale and in the sum over blocks, and with the parts of the K axis and the store there are at most
-      blocks + 68 roundings of the sum of magnitudes."""
+      blocks + 68 roundings of the sum of magnitudes;
+    * q4_1: d times the codes' sum and m times the higher digits' sum of x meet in one rounding of what
+      they leave, and the lower digits' share joins in the next.  Until then the first lacks that share, |m| times at
+      most 2^-7 of the block's largest per value (and no more than the value has): a magnitude too, at most twice."""
     w, _ = ref.dequantize64(fmt, blocks, out, x.shape[1])
     x = x.astype(np.float64)
     most = ref.block_max(x)
     parts = np.abs(x) + 2.0 ** -15 * most
     nb = (x.shape[1] + 31) // 32
     bound = 1.01 * 2.0 ** -31 * (most @ np.abs(w).T) + (nb + 68) * EPS * (parts @ np.abs(w).T)
+    if fmt == "q4_1":
+        raw = np.ascontiguousarray(blocks).reshape(out, nb, 20)
+        m = np.abs(raw[:, :, 2:4].copy().view(np.float16).astype(np.float64)).reshape(out, nb)
+        m = np.repeat(m, 32, 1)[:, :x.shape[1]]
+        bound += 2 * EPS * (np.minimum(parts, 2.0 ** -7 * most) @ m.T)
     return x @ w.T, bound + 1e-37
+
+
+# (format, the code of a strong channel, q4_1's m as a multiple of d)
+ZEROS = [("q8_0", 0, None), ("q4_0", 8, None), ("q4_1", 8, -8), ("q4_1", 3, -3), ("q4_1", 15, -15), ("q4_1", 0, 0)]
 
 
 
 @pytest.mark.parametrize("strong", [1.0, 1e3, 1e4, 1e5, 1e7])
-@pytest.mark.parametrize("fmt,code", [("q8_0", 0), ("q4_0", 8)])
-def test_a_strong_channel_with_weights_of_zero(pkg, fmt, code, strong):
+@pytest.mark.parametrize("fmt,code,m_of_d", ZEROS)
+def test_a_strong_channel_with_weights_of_zero(pkg, fmt, code, m_of_d, strong):
     """A channel whose weights are all exactly 0 costs the others only what the
     fixed point of its own block cannot hold: any place of a block, one row to 12."""
     rng = np.random.default_rng(int(strong))
     cin, out = 2048, 256
     for rows in (1, 2, 4, 7, 12):
         for channel in (5, 640 + 21, 2047):
-            blocks = with_codes(fmt, ref.random_blocks(rng, fmt, out, cin), out, cin, [channel], code)
+            blocks = with_codes(fmt, ref.random_blocks(rng, fmt, out, cin), out, cin, [channel], code, m_of_d)
             x = rng.standard_normal((rows, cin)).astype(np.float32)
             x[:, channel] = strong * rng.choice([-1, 1], rows) * rng.uniform(0.5, 1, rows)
             want, bound = tight(x, fmt, blocks, out)
