@@ -51,6 +51,7 @@ struct FewRows {
     __device__ __forceinline__ void step(uint32_t x, int valid, uint32_t r0, uint32_t r1, int lane) {
         const RowBase rows = row_base(r0, r1, lane & 3);
         [[maybe_unused]] const uint32_t sums = x + block_sums(0, lane & 1);
+        uint64_t part[NT] = {};  // of this step: a row of n blocks is a chain of n / 8 + 8 roundings, not of n
         static_for<kChunkBlocks / 2>([&](auto pc) {
             constexpr int p = decltype(pc)::value;
             if (!ALN && 2 * p >= valid) return;
@@ -83,13 +84,15 @@ struct FewRows {
                         // rounds what the parts leave of each other, and the second adds the lower digits' share
                         const float2 t = o ? make_float2(sum[i].z, sum[i].w) : make_float2(sum[i].x, sum[i].y);
                         const uint64_t left = fma2(d, v, mul2(m, pack2(t.x, t.x)));
-                        acc[i] = fma2(fma2(m, pack2(t.y, t.y), left), sx2, acc[i]);
+                        part[i] = fma2(fma2(m, pack2(t.y, t.y), left), sx2, part[i]);
                     } else {
-                        acc[i] = fma2(d, mul2(v, sx2), acc[i]);
+                        part[i] = fma2(d, mul2(v, sx2), part[i]);
                     }
                 }
             }
         });
+#pragma unroll
+        for (int i = 0; i < NT; ++i) acc[i] = add2(acc[i], part[i]);
     }
 
     // red: [row of x][weight row 0..15] of this warp
