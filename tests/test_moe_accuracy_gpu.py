@@ -138,3 +138,48 @@ def test_a_strong_channel_with_weights_of_zero(pkg, fmt, code, m_of_d, strong):
             if strong <= 1e4:  # half a step of the strong channel's block: below 2e-6 of an ordinary value
                 err = np.linalg.norm(y.cpu().numpy() - want, axis=1) / np.linalg.norm(want, axis=1)
                 assert err.max() <= 1e-6
+
+
+@pytest.mark.parametrize("rows", [13, 40, 130])
+@pytest.mark.parametrize("fmt,code,m_of_d", ZEROS)
+def test_a_strong_channel_among_many_rows(pkg, fmt, code, m_of_d, rows):
+    """The form of many rows, to the header's 1e-6 (its terms: 2^-22 of x, of w and of
+    their second values' product, the sums 1e-7 as in test_moe_gpu.py)."""
+    rng = np.random.default_rng(rows)
+    cin, out = 2048, 256
+    for strong in (1.0, 1e3, 1e4):
+        blocks = with_codes(fmt, ref.random_blocks(rng, fmt, out, cin), out, cin, [700], code, m_of_d)
+        x = rng.standard_normal((rows, cin)).astype(np.float32)
+        x[:, 700] = strong
+        want, bound = ref.product(x.astype(np.float64), fmt, blocks, out)
+        y = pkg.mlq.linear_epilogue(fmt, dev(blocks), out, cin, dev(x))
+        check(y, want, bound, pkg)
+        err = np.linalg.norm(y.cpu().numpy() - want, axis=1) / np.linalg.norm(want, axis=1)
+        assert err.max() <= 1e-6
+
+
+@pytest.mark.parametrize("fmt", ["q8_0", "q4_0", "q4_1"])
+@pytest.mark.parametrize("cin", [1, 31, 33, 96, 257, 300])
+def test_padding_blocks_of_a_row_and_of_the_hidden_vector(pkg, fmt, cin):
+    """Rows that end inside a step of 8 blocks, aligned and not, in a workspace full
+    of NaN bits: what lies behind the last block reaches no sum."""
+    rng = np.random.default_rng(cin)
+    hid, out, n = cin + 5, 48, 3
+    gate, up = (ref.random_blocks(rng, fmt, n * hid, cin) for _ in range(2))
+    down = ref.random_blocks(rng, fmt, n * out, hid)
+    for rows, offset in ((1, 0), (4, 0), (5, 2)):
+        x = rng.standard_normal((rows, cin)).astype(np.float32)
+        ids = rng.integers(0, n, (rows, 2)).astype(np.int32)
+        w = rng.uniform(0.1, 1, (rows, 2)).astype(np.float32)
+        on = []
+        for b in (gate, up, down):
+            buf = torch.zeros(b.size + 64, dtype=torch.uint8, device="cuda")
+            buf[offset:offset + b.size].copy_(dev(b))
+            on.append(buf[offset:offset + b.size])
+        m = pkg.mlq.Experts(fmt, *on, n, cin, hid, out_features=out)
+        ws = torch.full((pkg.mlq.experts_workspace_bytes(m, rows, 2),), 255, dtype=torch.uint8, device="cuda")
+        want, bound = ref.experts(x, ids, w, None, fmt, fmt, gate, up, down, n, hid, out)
+        check(pkg.mlq.moe_experts(m, dev(x), dev(ids), dev(w), workspace=ws), want, bound, pkg)
+        ws = torch.full((pkg.mlq.epilogue_workspace_bytes(fmt, hid, cin, rows),), 255, dtype=torch.uint8, device="cuda")
+        y = pkg.mlq.linear_epilogue(fmt, on[0][:gate.size // n], hid, cin, dev(x), workspace=ws)
+        check(y, *ref.product(x.astype(np.float64), fmt, gate[:gate.size // n], hid), pkg)
