@@ -244,7 +244,7 @@ int choose_strips(int out, int bpr, int nseg, bool all_segs, int sm_count, int l
 }
 
 // Rows of x of a segment of a linear that goes by digits: 2 while that ends sooner by the count of rounds, mostly for
-// small matrices (4 rows of q4_0, 2048 x 2048: 8.3 us with one segment and 5.5 with two; 4096 x 4096: 14.2 and 8.5).
+// small matrices (4 rows of q4_0, 2048 x 2048: 8.1 us with one segment and 5.6 with two; 4096 x 4096: 14.0 and 8.4).
 int linear_cap(int rows, int out, int bpr, int sm_count) {
     if (rows < 3) return rows;
     double two, four;
@@ -274,7 +274,7 @@ constexpr size_t kMaxSliced = 1u << 30;   // sliced bytes of one pass at most (o
 constexpr size_t kMaxParts = 1u << 30;    // bytes of the pairs' outputs of one pass at most
 constexpr int kMaxPassRows = 16384;       // rows of one pass of a linear at most
 // Rows of a linear that go by digits, in segments of 4 whose weights come from L2 after the first.  3584 x 18944, us by
-// digits and by halves: q4_0 5 rows 27 and 39, 12 rows 36 and 41, 16 rows 43 and 41; q8_0 31 and 42, 41 and 44, 50 and 45.
+// digits and by halves: q4_0 5 rows 26 and 38, 12 rows 35 and 40, 16 rows 42 and 41; q8_0 31 and 40, 40 and 43, 50 and 45.
 constexpr int kLinearFewRows = 12;
 constexpr int kCombineRows = 32;          // more rows: the sum over slots is a launch of its own
 
@@ -353,8 +353,11 @@ int segment_places(bool few, int pairs, int n_experts) {
 // expert with more rows has several segments, whose weights come from L2 after the
 // first, so the time grows with the rows, while that of the other form hardly does below
 // 16 rows per expert.  60 experts of 3584 x 2560, us by digits and by halves: q4_0 6 rows
-// per expert 389 and 701, 10 rows 591 and 704, 11 rows 641 and 705; q8_0 450 and 709, 686
-// and 713, 736 and 714; q4_1 462 and 988, 708 and 990, 772 and 991.
+// per expert 386 and 701, 10 rows 588 and 704, 11 rows 639 and 705, 12 rows 689 and 706; q8_0 447 and
+// 708, 664 and 713, 727 and 715, 774 and 721; q4_1 453 and 987, 691 and 991, 750 and 991, 811 and 991, and 14
+// rows 920 and 993.  One border for all: q8_0's own is 10 rows, q4_0's 12, q4_1's 14 (whose calls of
+// 12 to 14 rows take up to a fifth longer than they need).  The ids are on the device, so the average decides: where
+// most rows go to few experts, those are unpacked again for each 4 rows although their number would call for the other form.
 constexpr int kFewPerExpert = 11;
 bool few_rows(int pairs, int n_experts) { return pairs <= kFewPerExpert * n_experts; }
 

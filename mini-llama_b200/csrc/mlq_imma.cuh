@@ -7,10 +7,11 @@
 //
 // * few rows of x (segments of up to 4): 4 signed base-256 digits of x_i / s, s a power of two
 //   per 32-value block of a row (31-bit fixed point, error <= 2^-31
-//   max|x_block|).  The codes meet the digits in m16n8k32 int8 matrix
+//   max|x_block|; below 2^-96 a fixed step of 2^-126).  The codes meet the digits in m16n8k32 int8 matrix
 //   instructions: one covers exactly one block of 16 weight rows, its 8 columns are
 //   the digits of 2 rows of x, every integer sum is exact, and one fp32 fold per
-//   block applies d and the block's scale of x.  q8_0 codes are
+//   block (its sum rounded to fp32) applies d and the block's scale of x.  fp32 sums go over
+//   8 blocks, then over those.  q8_0 codes are
 //   the operand as they are.  q4 codes are bytes 16 c (a mask for the high
 //   nibbles, a shift and a mask for the low ones): unsigned in q4_1, in q4_0 signed 16 (c - 8),
 //   which is the same byte with its highest bit changed, so that a weight of 0 adds
@@ -24,7 +25,7 @@
 //   scales then bring into an fp32 one: a product of 22 bits on both sides at 3
 //   fp16 instructions, and the chain of roundings in the tensor core is short.
 //
-// Both are bound by HBM while an expert has few rows.  The int8 instruction
+// Both are bound by HBM, past a launch's start and end, while an expert has few rows.  The int8 instruction
 // runs at one per 2.2 cycles and SM here (1.05 POP/s measured).
 #pragma once
 
@@ -193,8 +194,8 @@ __device__ __forceinline__ void imma(int (&c)[4], const uint32_t (&a)[4], uint2 
 // Facts of a warp's weight slot (16 rows x 8 blocks in shared memory).
 // Aligned rows come by 2-D TMA boxes; the row pitch is 4 mod 8 words, so the
 // 8 rows x 4 words that a warp reads at a time touch 32 banks (q4_1 takes two
-// boxes of 4 blocks for that).  Other rows come one by one, by 1-D copies of
-// the 16-byte aligned window around each, in a pitch with the same property.
+// boxes of 4 blocks for that).  Other rows come one by one, as the 16-byte
+// aligned pieces (cp.async) of the window around each, in a pitch with the same property.
 template <int F, bool ALN>
 struct Slot;
 template <>

@@ -14,11 +14,12 @@
 // shared memory in a fixed order; a unit whose rounds fall to several teams is
 // added up (in order) by the last of them to finish.
 //
-// One row, 28672 x 8192, with the slicing launch (us, and the matrix's bytes
-// as a share of a copy's 6.56 TB/s): q8_0 46 and 0.82, q4_0 31 and 0.65, q4_1 35
-// and 0.64; 4 rows of q4_1 43.  q8_0 is bound by HBM, the q4 formats by the instructions
-// that unpack a block and fold its sums; small matrices by latency (4096 x 4096 q4_0,
-// one row: 6.1 us, 1.5 us of HBM time).
+// One row of 8192 values, with the slicing launch (us): 14336, 28672, 57344 and
+// 114688 outputs take 26, 47, 82 and 153 in q8_0, 18, 32, 54 and 95 in q4_0, 20, 36, 59 and 105 in
+// q4_1.  Past ~12 us for the slicing launch, the ramp and the last units, every
+// format runs at 0.97 or more of a copy's 6.56 TB/s.  With 4 rows 28672 outputs take 51, 38 and 44:
+// there the products and folds of the second pair of rows show.  Small matrices are
+// bound by latency (4096 x 4096 q4_0, one row: 6.1 us, 1.4 us of HBM time).
 #pragma once
 
 #include "mlq_imma_common.cuh"

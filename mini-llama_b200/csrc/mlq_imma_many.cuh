@@ -19,8 +19,8 @@
 // Tensor memory: 2 sums of 128 columns (4 of 64 where a segment has no more), 4 operands of 64 (hi 32, lo 32).
 // Rounds are dealt out evenly as in mlq_imma_few.cuh.
 //
-// 18944 x 16384, q4_0: 16 rows 133 us, 64 rows 160 us (250 TFLOP/s), 128 rows
-// 241 us (330).  A stage takes ~1200 cycles at 64 rows, of which the products are
+// 18944 x 16384, q4_0: 16 rows 134 us, 64 rows 159 us (250 TFLOP/s), 128 rows
+// 234 us (340).  A stage takes ~1200 cycles at 64 rows, of which the products are
 // 400 to 550; decoding (~500 and ~300 of handing over) and draining (~650) run beside
 // them but on the same schedulers, which issue 0.55 instructions a cycle, and each
 // stage passes three barriers.  Twice the decoding warps, two stages at a time and more

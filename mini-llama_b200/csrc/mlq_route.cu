@@ -133,7 +133,9 @@ __global__ void __launch_bounds__(256) route_logits_kernel(const RouteArgs a, in
     logits_of<E, R>(a, vec, blockIdx.x * E, blockIdx.y * R, blockIdx.y * R);
 }
 
-// The rows on the list, 4 experts at a time (mostly there are none).
+// The rows on the list, 4 experts at a time (mostly there are none).  x and w are
+// read again for every 4 logits: 2048 x 256 x 4096 takes 49 us without such rows, 108 us with 64 of them, and
+// 1.75 ms where every row has an element of 1e5 times the others.
 __global__ void __launch_bounds__(256) route_again_kernel(const RouteArgs a, int vec) {
     launch_dependents();
     grid_dependency_wait();
