@@ -624,9 +624,12 @@ def _on_stream(device, stream, call, *given):
     handle = stream if isinstance(stream, int) else stream.cuda_stream
     if device.type != "cuda" or handle == torch._C._cuda_getCurrentRawStream(device.index):
         return call()
-    if isinstance(stream, int):
+    where = getattr(stream, "device", None)  # an integer, or another library's stream, has none
+    if where is None:
         # 0 and 1 both name the default stream
         stream = torch.cuda.ExternalStream(handle, device=device) if handle > 1 else torch.cuda.default_stream(device)
+    elif where != device:
+        raise ValueError(f"stream: expected one of {device}, got one of {where}")
     caller = torch.cuda.current_stream(device)
     with torch.cuda.stream(stream):
         out = call()

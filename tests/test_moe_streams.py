@@ -115,3 +115,16 @@ def test_a_call_allocates_for_its_stream(pkg, monkeypatch, name, given, stream):
     # what the caller gets may be used on its own stream, and be dropped there
     for t in out if isinstance(out, tuple) else (out,):
         assert t.used_on == ([] if stream == CURRENT or name == "all given" else [CURRENT])
+
+
+@pytest.mark.parametrize("name", [c for c in CALLS if c != "all given"])
+def test_a_stream_of_another_device_is_refused(pkg, monkeypatch, name):
+    """Under such a stream the tensors' device would have another current stream."""
+    mlq, world = pkg.mlq, World()
+    monkeypatch.setattr(mlq, "_torch", world)
+    monkeypatch.setattr(mlq, "_moe_lib", lambda: world)
+    with pytest.raises(ValueError, match="stream"):
+        CALLS[name](mlq, world, stream=types.SimpleNamespace(cuda_stream=OTHER, device="cuda:1"))
+    assert world.calls == [] and world.allocated == []
+    CALLS[name](mlq, world, stream=types.SimpleNamespace(cuda_stream=OTHER, device=world.device))
+    assert world.calls == [OTHER]
