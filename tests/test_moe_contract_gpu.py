@@ -115,3 +115,31 @@ def test_stream_given_under_capture(pkg):
         torch.cuda.synchronize()
         assert torch.equal(z, want)
     assert mlq.device_error(0) == 0
+
+
+@pytest.mark.parametrize("rows", [300, 3000])
+def test_layer_of_a_prompt(pkg, rows):
+    """More rows than a pass of either half holds (2048 of the router, 2730 of the
+    experts with 3 slots): the bits of the halves, also written over x and over the residual."""
+    mlq = pkg.mlq
+    rng = np.random.default_rng(rows)
+    n, cin, hid, k = 16, 256, 96, 3
+    stacks = [ref.random_blocks(rng, f, n * r, c) for f, r, c in (("q4_0", hid, cin), ("q4_0", hid, cin), ("q4_1", cin, hid))]
+    m = mlq.Experts("q4_0", *(dev(b) for b in stacks), n, cin, hid, fmt_down="q4_1")
+    w = (rng.standard_normal((n, cin)) / 16).astype(np.float32)
+    router = mlq.Router(dev(w), k)
+    host = rng.standard_normal((rows, cin)).astype(np.float32)
+    x = dev(host)
+    y, ids, wt = mlq.moe_layer(router, m, x, residual=x)
+    want_ids, _, _ = ref.route(host, w, k)
+    assert np.array_equal(ids.cpu().numpy(), want_ids)
+    ids2, wt2 = mlq.moe_route(router, x)
+    assert torch.equal(ids, ids2) and torch.equal(wt, wt2)
+    assert torch.equal(y, mlq.moe_experts(m, x, ids, wt, residual=x))
+    into = x.clone()
+    mlq.moe_layer(router, m, into, residual=into, y=into)
+    assert torch.equal(y, into)
+    some = [0, 1, rows // 2, 2047 % rows, 2048 % rows, 2729 % rows, 2730 % rows, rows - 1]
+    want, bound = ref.experts(host[some], want_ids[some], wt.cpu().numpy()[some], host[some], "q4_0", "q4_1", *stacks, n,
+                              hid, cin)
+    check(y[some], want, bound, pkg)
