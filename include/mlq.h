@@ -446,7 +446,7 @@ MLQ_API mlq_status mlq_peer_free(void* ptr);
  * With more, values of x and weights are each the sum of two fp16 values (to
  * 2^-22 of the value) against a power of two per 64 values; sums are the
  * tensor cores' fp32 over 64 values and fp32 across them.  Outputs are within
- * ~1e-6 relative L2 of the 64-bit result (1e-7 to 2e-7 on ordinary data; by few rows a value
+ * ~1e-6 relative L2 of the 64-bit result (1e-7 to 2e-7 on ordinary data; with few rows a value
  * 1e5 times its block's others costs these more than that where its own weights are 0).
  * Every finite x is a value.  One that is not finite makes every output that reads it NaN.  Results do not
  * depend on the other rows of the call or on their order beyond rounding,
